@@ -38,6 +38,7 @@
 
 #include "common.h"
 #include "few_rows_rule.h"
+#include "gemm_util.h"
 #include "ktile.h"
 
 // Element type of this build of the file: bf16, or fp16 with -DPMX_ELT_F16
@@ -106,13 +107,9 @@ constexpr int kTileTab = PMX_TILE_TAB;
 static_assert(kTileTab >= 1 && kTileTab <= 1024, "tile table: 1 .. 1024 entries (16 KB of LDS)");
 // A table entry packs the group id in 12 bits and the n-tile above it.
 static_assert(kMaxGroups <= (1 << 12), "group ids must fit the tile table's 12 bits");
-constexpr uint32_t kOOB = 0x80000000u;  // buffer offset that always fails the range check
-constexpr uint32_t kRsrcWord3 = 0x00020000u;
-
 enum Kind { KIND_FC1 = 0, KIND_NT = 1, KIND_NN = 2, KIND_NNS = 3, KIND_TN = 4 };
 
 typedef __bf16 bf16x4_t __attribute__((ext_vector_type(4)));
-#define LDS_PTR(p) ((__attribute__((address_space(3))) void*)(p))
 #define LDS_TR_PTR(p) ((__attribute__((address_space(3))) bf16x4_t*)(p))
 
 // Row-major bf16 operand whose rows may come from two tensors: rows below
@@ -150,16 +147,6 @@ template <int KIND>
 constexpr bool a_is_mn() { return KIND == KIND_TN; }
 template <int KIND>
 constexpr bool b_is_mn() { return KIND == KIND_NN || KIND == KIND_NNS || KIND == KIND_TN; }
-
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t make_rsrc(const void* base, uint64_t bytes) {
-  const uint32_t n = bytes > 0x7fffffffull ? 0x7fffffffu : (uint32_t)bytes;
-  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), (short)0, (int)n, (int)kRsrcWord3);
-}
-
-// 16-byte chunk swizzle of the 128-byte rows of K-contiguous tiles: 16
-// consecutive rows read at one logical chunk hit 16 distinct (row parity,
-// chunk) bank groups.
-__device__ __forceinline__ int kc_swz(int row) { return (row >> 1) & 7; }
 
 // Per-tile operand description.  Each DMA instruction of this wave has a
 // tile-invariant per-lane byte offset `voff[q0]` (kOOB where the lane's chunk
@@ -199,28 +186,6 @@ struct Tile {
   TileInfo i;
   Operand A, B;
 };
-
-// Wave-uniform copies (SGPRs) of values every lane holds alike: tile
-// bookkeeping read from LDS or memory would otherwise stay in VGPRs, and
-// descriptor selections on it would become branches around each load.
-__device__ __forceinline__ int32_t uni(int32_t v) { return __builtin_amdgcn_readfirstlane(v); }
-__device__ __forceinline__ int64_t uni64(int64_t v) {
-  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v);
-  const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)((uint64_t)v >> 32));
-  return (int64_t)(((uint64_t)hi << 32) | lo);
-}
-
-// One buffer->LDS instruction: 64 lanes x 16 bytes land contiguously at `dst`
-// (M0 holds the wave's LDS address).  Written as inline asm so that the
-// compiler does not track it: its own LDS-DMA bookkeeping cannot tell the
-// pipeline stages apart and would wait for younger stages before every LDS
-// read.  Completion is tracked by hand (wait_loads) and published to the
-// other waves by block_barrier, both of which clobber memory; this asm does
-// not, so LDS reads of other stages may be scheduled across it.
-__device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t r, char* dst, uint32_t voff, uint32_t soff) {
-  const uint32_t m0 = (uint32_t)(uintptr_t)LDS_PTR(dst);
-  asm volatile("buffer_load_dwordx4 %0, %1, %2 offen lds" ::"v"(voff), "s"(r), "s"(soff), "{m0}"(m0));
-}
 
 // An empty descriptor: every offset fails its range check and loads zeros.
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t empty_rsrc(const void* base) { return make_rsrc(base, 0); }
@@ -478,20 +443,6 @@ __device__ __forceinline__ void mma_frags(const Frags<BM>& f, f32x16_t (&acc)[MT
 #pragma unroll
     for (int nt = 0; nt < NTT; ++nt)
       acc[mt][nt] = mfma32(f.b[nt], f.a[mt], acc[mt][nt]);
-}
-
-// Compile-time loop: f(Int<I>{}) for I = B .. E-1, so that accumulator
-// indices stay constants however large the unrolled body grows.
-template <int V>
-struct Int {
-  static constexpr int value = V;
-};
-template <int B, int E, typename F>
-__device__ __forceinline__ void static_for(F&& f) {
-  if constexpr (B < E) {
-    f(Int<B>{});
-    static_for<B + 1, E>(f);
-  }
 }
 
 // The MFMAs take the B fragment as their first operand, so each accumulator
@@ -973,36 +924,6 @@ __device__ __forceinline__ TileInfo decode_tile(const GemmParams& P, int64_t til
   return ti;
 }
 
-// Wait until at most PENDING of this wave's vector memory operations (its
-// buffer->LDS loads, and any stores since) are in flight.
-template <int PENDING>
-__device__ __forceinline__ void wait_loads() {
-  static_assert(PENDING >= 0 && PENDING <= 63, "vmcnt is 6 bits");
-  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PENDING) : "memory");
-}
-
-// Same, and this wave's LDS reads and writes have completed.
-template <int PENDING>
-__device__ __forceinline__ void wait_loads_lds() {
-  static_assert(PENDING >= 0 && PENDING <= 63, "vmcnt is 6 bits");
-  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(PENDING) : "memory");
-}
-
-// Wait until this wave's LDS reads and writes have completed.
-__device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
-
-// Workgroup barrier that neither the compiler's memory model nor its
-// scheduler moves anything across: memory operations stay on their side (the
-// asm clobbers memory), and so do the MFMAs, so that every LDS read consumed
-// before the barrier has returned by the time the wave reaches it.
-__device__ __forceinline__ void block_barrier() {
-  __builtin_amdgcn_sched_barrier(0);
-  asm volatile("" ::: "memory");
-  __builtin_amdgcn_s_barrier();
-  asm volatile("" ::: "memory");
-  __builtin_amdgcn_sched_barrier(0);
-}
-
 // Weight-gradient schedule.  A wgrad tile of copy g costs ceil(rows_g / 64)
 // K-tiles, so copies of very different sizes make the round-robin deal of
 // tiles to blocks uneven.  The schedule keeps the deal's structure - the
@@ -1024,7 +945,7 @@ __device__ __forceinline__ void block_barrier() {
 // grid of whole XCDs and G <= NT (the block's threads); otherwise (false) the plain order
 // is used.  Rounds past what the LDS holds alternate direction.
 constexpr int kBandTiles = 32;
-constexpr int kNumXcd = 8;
+
 
 // `order[r]` = the copy of rank r (more K-tiles first, ties by copy index);
 // `deal[r]` (bytes after nk[G]) = the band of round r, 0..7 within the round,
