@@ -462,6 +462,77 @@ int pmx_ep_combine_aggregate_i64(const void* Y, const int64_t* pos, const void* 
                              pmx_stream_t stream);
 
 /* ------------------------------------------------------------------------ */
+/* Rows in 8 bits: activation checkpoints and products                       */
+/* ------------------------------------------------------------------------ */
+/* Blocks of 32 neighbouring columns share a power of two 2^e, and each value
+ * is held beside it as an e4m3 float or an int8:
+ *   e    = the smallest integer in [-127, 127] with most <= room * 2^e, `most`
+ *          the block's largest finite magnitude and room = 448 (e4m3) or 127
+ *          (int8); 0 for a block of zeros
+ *   code = x / 2^e rounded to nearest even.
+ * A value that is not finite is held as NaN (int8: code -128).  Reading back
+ * code * 2^e is exact, except that values beyond the output type's range
+ * become its largest finite one.
+ *   codes:  [.., R, N] one byte each, row-major.
+ *   scales: [.., B, R, 16] bytes, B = ceil(N / 512): byte [b, r, j] = e + 127
+ *           of row r's columns 512 b + 32 j .. + 31; 127 past the last column.
+ * The row functions take any N and any alignment; the two products e4m3 only.
+ * No counterpart in the reference, whose expert layer is 16-bit throughout. */
+#define PMX_ROWS8_E4M3 0
+#define PMX_ROWS8_INT8 1
+
+/* x: G groups of R rows of N bf16, row r of group g at x + g*gsx + r*ldx
+ * elements (ldx >= N) -> codes [G, R, N], scales [G, B, R, 16]. */
+int pmx_rows8_quantize(const void* x, int64_t ldx, int64_t gsx, int64_t G, int64_t R, int64_t N,
+                       int32_t format, void* codes, void* scales, pmx_stream_t stream);
+
+/* The same (e4m3) for the T contiguous token rows x [T, H] of a routing, and for each
+ * assignment its row's token and weight: row_token[pos[t,k]] = t and
+ * row_w[pos[t,k]] = w[t,k].  pos, row_token int32, w and row_w bf16 [T*K].  A
+ * position outside [0, T*K) is skipped. */
+int pmx_rows8_quantize_routed(const void* x, const int32_t* pos, const void* w, int64_t T, int32_t K,
+                              int64_t H, void* codes, void* scales, int32_t* row_token, void* row_w,
+                              pmx_stream_t stream);
+
+/* Rows back in bf16: out[r] (pos NULL), or out[pos[r,k]] for every k (pos
+ * int32 [R, K]; positions outside [0, R*K) are skipped). */
+int pmx_rows8_dequantize(const void* codes, const void* scales, const int32_t* pos, int64_t R, int32_t K,
+                         int64_t N, int32_t format, void* out, pmx_stream_t stream);
+
+/* SwiGLU backward from gate and up rows (gate | up) [R, 2I] in 8 bits, in fp32
+ * with one rounding at the end.  With s = gate * sigmoid(gate), d = d_act * row_w:
+ *   dG1[r]   = (d * up * (sigmoid(gate) + s * (1 - sigmoid(gate))) | d * s)   [R, 2I]
+ *   act_w[r] = row_w * s * up                                                  [R, I]
+ *   dw[row_src[r]] = sum_j d_act * s * up                                      [A]
+ * d_act bf16 [R, I]: gradient of the weighted activations.  row_w NULL: 1.
+ * dw and row_src both NULL: no dw; entries that no row names are not written,
+ * rows naming one outside [0, A) are skipped. */
+int pmx_rows8_swiglu_bwd(const void* d_act, const void* codes, const void* scales, const void* row_w,
+                         const int32_t* row_src, int64_t R, int64_t I, int64_t A, int32_t format, void* dG1,
+                         void* act_w, void* dw, pmx_stream_t stream);
+
+/* C[rows of g] = A[rows of g] B[g]^T over 8-bit rows (e4m3), fp32 sums, C bf16
+ * [M, N]; rows of g: offsets[g] .. offsets[g+1]-1 (offsets outside [0, M] are
+ * clamped).  A: codes [M, K]; B: codes [G, N, K], each with its scales.  K a
+ * multiple of 16, N of 8, pointers 16-byte aligned, N*K and the scales of all
+ * rows below 2 GiB, else PMX_ERR_SHAPE. */
+int pmx_rows8_group_gemm_nt(const void* a, const void* a_scales, const void* b, const void* b_scales,
+                            const int32_t* offsets, int32_t G, int64_t M, int64_t N, int64_t K, void* c,
+                            pmx_stream_t stream);
+
+/* fc1 + SwiGLU over 8-bit rows, into 8-bit rows:
+ *   (gate | up) = X[row_token[r]] w[g]^T,  act[r] = silu(gate) * up * row_w[r]
+ * X: T rows of H (codes and scales); row_token int32 [A], NULL: row r is X's
+ * row r (T = A); a token outside [0, T) reads as zeros.  w [G, 2I, H], gate
+ * rows first.  row_w bf16 [A], NULL: 1.  act: codes [A, I]; of its scales the
+ * bytes of the columns' multiple of 128 are written.  H and I multiples of
+ * 16; T*H below 2 GiB with row_token. */
+int pmx_rows8_gemm_fc1_swiglu(const void* x, const void* x_scales, int64_t T, const int32_t* row_token,
+                              const void* w, const void* w_scales, const int32_t* offsets, int32_t G,
+                              int64_t A, int64_t H, int64_t I, const void* row_w, void* act, void* act_scales,
+                              pmx_stream_t stream);
+
+/* ------------------------------------------------------------------------ */
 /* fp16 tensors                                                              */
 /* ------------------------------------------------------------------------ */
 /* The reference's fused MoE op takes bf16 or fp16 hidden states and router
@@ -530,6 +601,24 @@ int pmx_ep_combine_aggregate_i64_f16(const void* Y, const int64_t* pos, const vo
                                  int32_t* run_offsets, int32_t* rank_runs, int32_t* num_runs,
                                  int32_t* status, void* workspace, size_t workspace_bytes,
                                  pmx_stream_t stream);
+
+int pmx_rows8_quantize_f16(const void* x, int64_t ldx, int64_t gsx, int64_t G, int64_t R, int64_t N,
+                           int32_t format, void* codes, void* scales, pmx_stream_t stream);
+int pmx_rows8_quantize_routed_f16(const void* x, const int32_t* pos, const void* w, int64_t T, int32_t K,
+                                  int64_t H, void* codes, void* scales, int32_t* row_token, void* row_w,
+                                  pmx_stream_t stream);
+int pmx_rows8_dequantize_f16(const void* codes, const void* scales, const int32_t* pos, int64_t R, int32_t K,
+                             int64_t N, int32_t format, void* out, pmx_stream_t stream);
+int pmx_rows8_swiglu_bwd_f16(const void* d_act, const void* codes, const void* scales, const void* row_w,
+                             const int32_t* row_src, int64_t R, int64_t I, int64_t A, int32_t format, void* dG1,
+                             void* act_w, void* dw, pmx_stream_t stream);
+int pmx_rows8_group_gemm_nt_f16(const void* a, const void* a_scales, const void* b, const void* b_scales,
+                                const int32_t* offsets, int32_t G, int64_t M, int64_t N, int64_t K, void* c,
+                                pmx_stream_t stream);
+int pmx_rows8_gemm_fc1_swiglu_f16(const void* x, const void* x_scales, int64_t T, const int32_t* row_token,
+                                  const void* w, const void* w_scales, const int32_t* offsets, int32_t G,
+                                  int64_t A, int64_t H, int64_t I, const void* row_w, void* act, void* act_scales,
+                                  pmx_stream_t stream);
 
 #ifdef __cplusplus
 }

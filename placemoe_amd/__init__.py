@@ -11,11 +11,13 @@ from .fused_moe import (  # noqa: F401
     apply_veomni_fused_moe_patch,
     fused_moe_forward,
     hip_fused_moe_forward,
+    set_activation_checkpoint,
     set_router_weight_point,
 )
 from .kernel_registry import KERNEL_REGISTRY, HardwareRequirement, KernelSpec  # noqa: F401
 from .placement import PLACEMENTS, LayerPlacement, LayerPlan, PlaceMoETopology, mirrored_r2_plan  # noqa: F401
 from .replica import OverlappedReplicaSync, fold_replica_gradients, sync_redundant_gradients  # noqa: F401
+from .rows8 import Experts8, Rows8, dequantize_rows, expert_layer_rows8, quantize_rows  # noqa: F401
 from .statistics import ProfileStatistics, RouteStatisticsRecorder, profile_route_statistics  # noqa: F401
 
 __version__ = "0.1.0"

@@ -140,6 +140,32 @@ SIGNATURES = {
         [c_void_p, c_void_p, c_void_p, c_int64, c_int32, c_int64, c_int32, c_int32, c_void_p, c_void_p, c_void_p,
          c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p],
     ),
+    "pmx_rows8_quantize": (
+        c_int,
+        [c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64, c_int32, c_void_p, c_void_p, c_void_p],
+    ),
+    "pmx_rows8_quantize_routed": (
+        c_int,
+        [c_void_p, c_void_p, c_void_p, c_int64, c_int32, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p],
+    ),
+    "pmx_rows8_dequantize": (
+        c_int,
+        [c_void_p, c_void_p, c_void_p, c_int64, c_int32, c_int64, c_int32, c_void_p, c_void_p],
+    ),
+    "pmx_rows8_swiglu_bwd": (
+        c_int,
+        [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int32, c_void_p, c_void_p,
+         c_void_p, c_void_p],
+    ),
+    "pmx_rows8_group_gemm_nt": (
+        c_int,
+        [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int64, c_int64, c_int64, c_void_p, c_void_p],
+    ),
+    "pmx_rows8_gemm_fc1_swiglu": (
+        c_int,
+        [c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int64, c_int64, c_int64,
+         c_void_p, c_void_p, c_void_p, c_void_p],
+    ),
     "pmx_ep_combine_workspace_bytes": (c_size_t, [c_int64]),
     "pmx_ep_combine_aggregate": (
         c_int,
@@ -160,6 +186,8 @@ F16_TWINS = (
     "pmx_group_gemm_nn_unpermute_top1", "pmx_gemm_fc2_dgrad_swiglu_bwd", "pmx_group_gemm_tn", "pmx_weight_rows",
     "pmx_swiglu_bwd_weighted", "pmx_gemm_fc1_swiglu_weighted_fwd", "pmx_swiglu_bwd_weighted_gu",
     "pmx_replica_fold", "pmx_ep_combine_aggregate", "pmx_ep_combine_aggregate_i64",
+    "pmx_rows8_quantize", "pmx_rows8_quantize_routed", "pmx_rows8_dequantize", "pmx_rows8_swiglu_bwd",
+    "pmx_rows8_group_gemm_nt", "pmx_rows8_gemm_fc1_swiglu",
 )
 SIGNATURES.update({name + "_f16": SIGNATURES[name] for name in F16_TWINS})
 

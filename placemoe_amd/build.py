@@ -5,12 +5,13 @@ object file (in parallel), and the objects are linked into
 ``placemoe_amd/_lib/libplacemoe_amd.so``.  Runs without a GPU: hipcc
 cross-compiles.  Usage: ``python -m placemoe_amd.build``.
 
-The grouped GEMM's main loop issues its buffer->LDS loads as inline asm and
-counts their completion by hand (``s_waitcnt vmcnt``), out of the compiler's
-sight; compiler-generated scratch traffic (register spills) inside that loop
-would share the memory counter with them.  The build therefore compiles that
-file with the compiler's per-kernel resource report and fails if any of its
-kernels uses scratch memory or spills vector registers
+The grouped GEMMs' main loops (16-bit and 8-bit operands) issue their
+buffer->LDS loads as inline asm and count their completion by hand
+(``s_waitcnt vmcnt``), out of the compiler's sight; compiler-generated scratch
+traffic (register spills) inside such a loop would share the memory counter
+with them.  The build therefore compiles those files with the compiler's
+per-kernel resource report and fails if any of their kernels uses scratch
+memory or spills vector registers
 (``resource_usage.json`` beside the library keeps the report).
 
 The grouped GEMM source is compiled twice into the library: once for bf16
@@ -57,7 +58,7 @@ HIP_FLAGS = [
 
 # Sources whose kernels must run without scratch memory (see the module
 # docstring), and the kernel-name pattern the check applies to.
-RESOURCE_CHECKED = {"grouped_gemm.hip": re.compile(r"grouped_gemm")}
+RESOURCE_CHECKED = {"grouped_gemm.hip": re.compile(r"grouped_gemm"), "rows8_gemm.hip": re.compile(r"rows8_grouped_gemm")}
 RESOURCE_FLAG = "-Rpass-analysis=kernel-resource-usage"
 
 # name -> (source, extra flags): further objects of the library, built from a

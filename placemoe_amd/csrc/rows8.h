@@ -1,0 +1,75 @@
+// Rows in 8 bits: what their kernels share.
+//
+// Blocks of 32 neighbouring columns of a row share a power of two; each value
+// is held beside it as an e4m3 float or as an int8.  With `most` the block's
+// largest finite magnitude and room = 448 (e4m3's largest) or 127,
+//   e    = the smallest integer with most <= room * 2^e, within [-127, 127]; 0 for a block of zeros
+//   code = x / 2^e rounded to nearest even
+// so nothing saturates, and both the division and, in fp32 and bf16, the value
+// code * 2^e that is read back are exact; the rounding to 8 bits is the only
+// one.  (The floor of log2(most), as the microscaling formats' usual recipe
+// has it, would cut the top eighth of a block's range to 448.)  A code that is
+// not finite stands for NaN: e4m3's NaN, -128 for int8; infinities become NaN.
+//
+// codes:  [.., R, N] one byte each, row-major.
+// scales: [.., B, R, 16] with B = ceil(N / 512), byte [b, r, j] = e + 127 of
+//   row r's columns 512 b + 32 j .. + 31 (127 past the last column).  The
+//   16 bytes of 512 columns lie together and those of neighbouring rows next to
+//   each other, so that a GEMM brings in the exponents of four K-tiles of 64
+//   rows with one 1 KB load.
+#pragma once
+
+#include "common.h"
+
+namespace {
+
+constexpr int kFmtE4M3 = 0, kFmtInt8 = 1;
+constexpr int kScaleBlock = 32, kScaleGroup = 512, kScaleBytes = 16;
+
+// The exponent byte of a block whose largest finite magnitude has the fp32
+// bits `most`: 448 = 1.75 * 2^8 and 127 = 1.984375 * 2^6.  (A subnormal fp32
+// has exponent field 0 and ends at the lower clamp with the small normals.)
+template <int FMT>
+__device__ __forceinline__ uint32_t scale_byte(uint32_t most) {
+  const int e = (int)(most >> 23);
+  const uint32_t m = most & 0x7fffffu;
+  const int b = FMT == kFmtE4M3 ? e - 8 + (m > 0x600000u ? 1 : 0) : e - 6 + (m > 0x7e0000u ? 1 : 0);
+  return most == 0 ? 127u : (uint32_t)(b < 0 ? 0 : b);
+}
+// 2^(127 - b), b <= 248: a normal fp32.
+__device__ __forceinline__ float inv_scale(uint32_t b) { return __uint_as_float((254u - b) << 23); }
+// 2^(b - 127); 2^-127 is subnormal.
+__device__ __forceinline__ float scale_of(uint32_t b) { return __uint_as_float(b == 0 ? 0x400000u : b << 23); }
+
+// Four values (already divided by the block's power of two) -> four codes.
+template <int FMT>
+__device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d) {
+  if constexpr (FMT == kFmtE4M3) {
+    // infinities come out as NaN
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+    w = __builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
+    return (uint32_t)w;
+  } else {
+    const auto one = [](float v) -> uint32_t {
+      return __builtin_fabsf(v) <= 127.0f ? (uint32_t)(int)__builtin_rintf(v) & 0xffu : 0x80u;  // NaN: false
+    };
+    return one(a) | one(b) << 8 | one(c) << 16 | one(d) << 24;
+  }
+}
+
+// Four codes -> the values that they stand for beside 2^0 (exact).
+template <int FMT>
+__device__ __forceinline__ void values4(uint32_t w, float* v) {
+  if constexpr (FMT == kFmtE4M3) {
+    const f32x2_t lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
+    v[0] = lo[0], v[1] = lo[1], v[2] = hi[0], v[3] = hi[1];
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int c = (int)(w << (24 - 8 * j)) >> 24;
+      v[j] = c == -128 ? __uint_as_float(0x7fc00000u) : (float)c;
+    }
+  }
+}
+
+}  // namespace

@@ -1,0 +1,575 @@
+// Grouped GEMM over ragged row groups, both operands rows in 8 bits (rows8.h,
+// e4m3):
+//   NT   C[rows of g] = A[rows of g] B[g]^T                          (bf16 or fp16)
+//   FC1  (gate | up) = A[rows of g] B[g]^T, act = silu(gate) * up * row_w, written
+//        as rows in 8 bits again, ready to be fc2's A
+// with fp32 accumulation on v_mfma_scale_f32_32x32x64_f8f6f4, which takes the
+// two operands' powers of two per 32 columns with the codes: no value is ever
+// scaled outside of the matrix core.  (Within one such instruction the 64
+// products are added to about 2^-12 of the largest one, as measured: 1.3e-5 of
+// a random sum, a hundredth of the bf16 result's half step.  Sums over K are
+// fp32.)  A row map lets A's rows come from anywhere: fc1 reads each token's
+// row where it lies, once per copy it is routed to, and the permuted copy of
+// the hidden states is never made.
+//
+// Bound: MFMA from some hundred rows per group on (twice the rate of bf16 at
+// half the bytes), the weights' bytes below.
+//
+// Tiles of BM x BN, K in steps of 128 through a ring of NST stages filled by
+// buffer->LDS loads NST - 1 K-tiles ahead; 128-byte rows with 16-byte chunk c
+// at c ^ ((row >> 1) & 7), as in the bf16 kernels, whose K-tiles are as many
+// bytes.  The exponents of four K-tiles are 16 bytes per row (rows8.h): they
+// come with the first of the four, 64 rows per load, into a ring of their
+// own, and each wave picks a K-tile's word per row from there.
+
+#include <atomic>
+
+#include "gemm_util.h"
+#include "rows8.h"
+
+namespace {
+
+typedef int32_t i32x8_t __attribute__((ext_vector_type(8)));
+typedef int32_t i32x4_t __attribute__((ext_vector_type(4)));
+
+constexpr int kMaxGroups = 2048;  // groups (the m-tile prefix in LDS)
+constexpr int KT = 128;           // depth of a K-tile
+constexpr int kScaleTiles = kScaleGroup / KT;
+
+enum Kind8 { NT8 = 0, FC18 = 1 };
+
+struct Params8 {
+  const uint8_t *a, *as;     // A's codes [a_rows, K] and exponents
+  const int32_t* row_token;  // row r of the groups is row row_token[r] of A; null: row r
+  int64_t a_rows;
+  const uint8_t *b, *bs;     // [G, N, K]
+  const int32_t* offsets;    // [G + 1]
+  int32_t G;
+  int64_t M, N, K;           // M rows over all groups; N: rows of a B[g] (FC1: 2 I)
+  int64_t I;
+  bf16_t* c;                 // NT: [M, N]
+  uint8_t *q, *qs;           // FC1: act's codes [M, I] and exponents
+  const bf16_t* row_w;       // FC1: [M], null: 1
+};
+
+// WM x WN waves, each FM x FN tiles of 32 x 32; NST stages; BPC blocks per CU.
+template <int WM_, int WN_, int FM_, int FN_, int NST_, int BPC_>
+struct Cfg8 {
+  static constexpr int WM = WM_, WN = WN_, FM = FM_, FN = FN_, NST = NST_, BPC = BPC_;
+  static constexpr int NW = WM * WN, NTH = 64 * NW;
+  static constexpr int BM = WM * FM * 32, BN = WN * FN * 32;
+  static constexpr int A_BYTES = BM * KT, STAGE = (BM + BN) * KT;
+  static constexpr int QA = BM / 8 / NW, QB = BN / 8 / NW;  // 1 KB loads (8 rows) of one wave per K-tile
+  static constexpr int SA = (BM + 63) / 64, SB = BN / 64;   // 1 KB loads of exponents (64 rows), all waves
+  static constexpr int QS = (SA + SB + NW - 1) / NW;
+  static constexpr int SLOT = (SA + SB) * 1024;
+  static constexpr int LDS = NST * (STAGE + SLOT);
+  static_assert(BM / 8 % NW == 0 && BN / 8 % NW == 0 && BN % 64 == 0, "whole loads per wave");
+  static_assert(FN % 2 == 0 || WN % 2 == 0, "gate and up tiles alternate");
+  static_assert(NST >= 2 && (NST - 2) * (QA + QB) <= 63, "vmcnt is 6 bits");
+};
+
+// Where one output tile lies.
+struct Place {
+  int32_t g, ntile, row0, row_end;
+};
+
+// The issue cursor's loads for one output tile.
+template <class CF>
+struct Loads {
+  __amdgpu_buffer_rsrc_t a, b, as, bs;
+  uint32_t off[CF::QA + CF::QB];  // a lane's byte offset (kOOB: outside of the operand)
+  uint32_t soff[CF::QS];
+  uint32_t past;                  // bit j: load j's lane lies past K in the last K-tile
+};
+
+// Row of B for the tile's virtual row: FC1 alternates 32 gate rows and the
+// matching 32 up rows.
+template <int KIND, class CF>
+__device__ __forceinline__ int32_t b_row(const Params8& P, int32_t ntile, int row) {
+  if constexpr (KIND == FC18) {
+    const int32_t I = (int32_t)P.I, j = ntile * (CF::BN / 2) + (row >> 6) * 32 + (row & 31);
+    return j < I ? (row & 32 ? I : 0) + j : -1;
+  } else {
+    const int32_t j = ntile * CF::BN + row;
+    return j < (int32_t)P.N ? j : -1;
+  }
+}
+
+template <int KIND, class CF>
+__device__ __forceinline__ void setup(const Params8& P, const Place& at, Loads<CF>& ld, int wave, int lane) {
+  asm volatile("" : "+v"(lane));  // keep the per-lane arithmetic here
+  const int krem = (int)(P.K - (P.K - 1) / KT * KT);
+  const int64_t kgroups = (P.K + kScaleGroup - 1) / kScaleGroup;
+  const bool mapped = KIND == FC18 && P.row_token != nullptr;
+  const int64_t base = mapped ? 0 : at.row0;
+  // A's row behind the tile's row, relative to `base`; -1: none
+  const auto a_row = [&](int row) -> int32_t {
+    if (row >= at.row_end - at.row0) return -1;
+    if (!mapped) return row;
+    const int32_t t = P.row_token[at.row0 + row];
+    return t < (int32_t)P.a_rows ? t : -1;
+  };
+  const uint32_t K = (uint32_t)P.K;
+  ld.a = make_rsrc(P.a + base * P.K, (uint64_t)(P.a_rows - base) * P.K);
+  ld.b = make_rsrc(P.b + (int64_t)at.g * P.N * P.K, (uint64_t)P.N * P.K);
+  ld.as = make_rsrc(P.as + base * kScaleBytes, (uint64_t)(kgroups * P.a_rows - base) * kScaleBytes);
+  ld.bs = make_rsrc(P.bs + (int64_t)at.g * kgroups * P.N * kScaleBytes, (uint64_t)kgroups * P.N * kScaleBytes);
+  ld.past = 0;
+#pragma unroll
+  for (int j = 0; j < CF::QA + CF::QB; ++j) {
+    const bool is_a = j < CF::QA;
+    const int row = ((is_a ? j : j - CF::QA) * CF::NW + wave) * 8 + lane / 8;
+    const int c = (lane % 8) ^ kc_swz(row);
+    const int32_t r = is_a ? a_row(row) : b_row<KIND, CF>(P, at.ntile, row);
+    ld.off[j] = r >= 0 ? (uint32_t)r * K + (uint32_t)c * 16u : kOOB;
+    ld.past |= (c * 16 < krem ? 0u : 1u) << j;
+    asm volatile("" : "+v"(ld.off[j]));  // one register, worked out here
+  }
+#pragma unroll
+  for (int j = 0; j < CF::QS; ++j) {
+    const int s = j * CF::NW + wave;
+    const int row = (s < CF::SA ? s : s - CF::SA) * 64 + lane;
+    const int32_t r = s < CF::SA ? (row < CF::BM ? a_row(row) : -1) : b_row<KIND, CF>(P, at.ntile, row);
+    ld.soff[j] = r >= 0 ? (uint32_t)r * kScaleBytes : kOOB;
+    asm volatile("" : "+v"(ld.soff[j]));
+  }
+}
+
+template <class CF>
+struct Frags8 {
+  i32x8_t a[CF::FM], b[CF::FN];
+  // the lane's exponents, two fragments to a word: byte 2 (f & 1) + ks is fragment f's in half ks of the K-tile
+  int32_t sa[(CF::FM + 1) / 2], sb[(CF::FN + 1) / 2];
+};
+
+// The I-th fragment read of a k-step, in the order its (m-major) MFMAs use
+// them: A0, B0 .. B(FN-1), A1 .. ; ids as in the reads (A first, then B).
+template <class CF>
+constexpr int order8(int i) { return i == 0 ? 0 : i <= CF::FN ? CF::FM + i - 1 : i - CF::FN; }
+
+// Exchanges the upper half-wave's `lo` with the lower half-wave's `hi`.
+__device__ __forceinline__ void swap_halves(uint32_t& lo, uint32_t& hi) {
+  const auto v = __builtin_amdgcn_permlane32_swap(lo, hi, false, false);
+  lo = v[0];
+  hi = v[1];
+}
+
+// An accumulator holds its 32 x 32 output tile transposed (B is the MFMA's
+// first operand): lane l has row l%32, columns 8*(i/4) + 4*(l/32) + i%4.
+template <class E, int KIND, class CF>
+__device__ __forceinline__ void epilogue(const Params8& P, const Place& at, int wm, int wn, int lane,
+                                         f32x16_t (&acc)[CF::FM][CF::FN]) {
+  // Each accumulator leaves the accumulation registers where it is used: read
+  // right behind their last MFMAs, they would need as many vector registers.
+  const auto here = [](f32x16_t& v) __attribute__((always_inline)) { asm volatile("" : "+a"(v)); };
+  asm volatile("" : "+v"(lane));
+  const int h = lane >> 5;
+#pragma unroll
+  for (int m = 0; m < CF::FM; ++m) {
+    const int64_t r = (int64_t)at.row0 + (wm * CF::FM + m) * 32 + (lane & 31);
+    const bool in = r < at.row_end;
+    if constexpr (KIND == NT8) {
+#pragma unroll
+      for (int n = 0; n < CF::FN; ++n) {
+        here(acc[m][n]);
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {  // 16 columns: the half-waves exchange, and each lane has 8 of them
+          const f32x16_t& v = acc[m][n];
+          uint32_t w0 = E::pack2(v[8 * p], v[8 * p + 1]), w1 = E::pack2(v[8 * p + 2], v[8 * p + 3]);
+          uint32_t w2 = E::pack2(v[8 * p + 4], v[8 * p + 5]), w3 = E::pack2(v[8 * p + 6], v[8 * p + 7]);
+          swap_halves(w0, w2);
+          swap_halves(w1, w3);
+          const int64_t col = (int64_t)at.ntile * CF::BN + (wn * CF::FN + n) * 32 + p * 16 + h * 8;
+          if (in && col < P.N) *reinterpret_cast<uint4*>(P.c + r * P.N + col) = make_uint4(w0, w1, w2, w3);
+        }
+        __builtin_amdgcn_sched_barrier(0);  // one tile's registers at a time
+      }
+    } else {
+      const float w = in && P.row_w != nullptr ? E::to_f32(P.row_w[r]) : 1.0f;
+#pragma unroll
+      for (int n = 0; n < CF::FN; n += 2) {
+        here(acc[m][n]);
+        here(acc[m][n + 1]);
+        float f[16];
+        float most = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          f[i] = silu_f32(acc[m][n][i]) * acc[m][n + 1][i] * w;
+          const float v = __builtin_fabsf(f[i]);
+          most = v > most && v < __builtin_inff() ? v : most;
+        }
+        most = fmaxf(most, __shfl_xor(most, 32, 64));
+        const uint32_t byte = scale_byte<kFmtE4M3>(__float_as_uint(most));
+        const float inv = inv_scale(byte);
+        uint32_t c[4];  // columns 8 i + 4 h .. + 3
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          c[i] = codes4<kFmtE4M3>(f[4 * i] * inv, f[4 * i + 1] * inv, f[4 * i + 2] * inv, f[4 * i + 3] * inv);
+        // ... and after the exchange each lane has columns 16 h .. + 15
+        swap_halves(c[0], c[2]);
+        swap_halves(c[1], c[3]);
+        const int64_t j = (int64_t)at.ntile * (CF::BN / 2) + (wn * CF::FN + n) * 16;
+        if (in) {
+          if (j + h * 16 < P.I) *reinterpret_cast<uint4*>(P.q + r * P.I + j + h * 16) = make_uint4(c[0], c[2], c[1], c[3]);
+          // also the blocks past I within the last 128 columns, which fc2's last K-tile takes along (zeros)
+          if (h == 0) P.qs[(j / kScaleGroup * P.M + r) * kScaleBytes + j / kScaleBlock % 16] = (uint8_t)byte;
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+  }
+}
+
+template <class E, int KIND, class CF>
+__global__ __launch_bounds__(CF::NTH, CF::NW * CF::BPC / 4) void rows8_grouped_gemm_kernel(Params8 P) {
+  constexpr int NW = CF::NW, L = CF::QA + CF::QB;
+  __shared__ __attribute__((aligned(1024))) char lds[CF::LDS];
+  __shared__ int32_t tpre[kMaxGroups + 1];
+  __shared__ int32_t wsum[NW];
+  char* const slots = lds + CF::NST * CF::STAGE;
+  const int t = threadIdx.x;
+  const int lane = t & 63;
+  const int wave = uni(t >> 6);
+  const int wm = wave / CF::WN, wn = wave % CF::WN;
+  const int G = P.G;
+  // offsets as they are used: within [0, M], whatever the tensor holds
+  const auto offset = [&](int g) {
+    const int32_t o = P.offsets[g];
+    return o < 0 ? 0 : o > P.M ? (int32_t)P.M : o;
+  };
+  const auto m_tiles = [&](int g) {
+    const int32_t n = offset(g + 1) - offset(g);
+    return n > 0 ? (n + CF::BM - 1) / CF::BM : 0;
+  };
+
+  // Exclusive prefix of the groups' m-tiles in tpre[0..G]: consecutive groups
+  // per thread, a wave scan of the threads' sums, then the waves' sums.
+  {
+    const int per = (G + CF::NTH - 1) / CF::NTH;
+    const int g0 = t * per, g1 = g0 + per < G ? g0 + per : G;
+    int32_t sum = 0;
+    for (int g = g0; g < g1; ++g) sum += m_tiles(g);
+    int32_t inc = sum;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const int32_t v = __shfl_up(inc, off, 64);
+      if (lane >= off) inc += v;
+    }
+    if (lane == 63) wsum[wave] = inc;
+    __syncthreads();
+    int32_t run = inc - sum;
+    for (int w = 0; w < wave; ++w) run += wsum[w];
+    for (int g = g0; g < g1; ++g) {
+      tpre[g] = run;
+      run += m_tiles(g);
+    }
+    if (t == CF::NTH - 1) tpre[G] = run;
+    __syncthreads();
+  }
+  const int32_t ntn = (int32_t)(KIND == FC18 ? (P.I + CF::BN / 2 - 1) / (CF::BN / 2) : (P.N + CF::BN - 1) / CF::BN);
+  const int64_t total = (int64_t)uni(tpre[G]) * ntn;
+  const int32_t nk = (int32_t)((P.K + KT - 1) / KT);
+  // Blocks go round-robin over the XCDs: each XCD walks its own eighth of the
+  // tile list, its blocks round-robin within it.
+  int64_t first = blockIdx.x, step = gridDim.x, end = total;
+  if (gridDim.x % kNumXcd == 0) {
+    const int64_t x = blockIdx.x % kNumXcd;
+    step = gridDim.x / kNumXcd;
+    end = total * (x + 1) / kNumXcd;
+    first = total * x / kNumXcd + blockIdx.x / kNumXcd;
+  }
+  if (first >= end) return;
+
+  // Tile order: group by group, in bands of 8 m-tiles walked n-tile by n-tile:
+  // neighbouring tiles share a strip of B, and a band of A.
+  auto decode = [&](int64_t tile, Place& at) {
+    constexpr int kBand = 8;
+    const int32_t m = (int32_t)(tile / ntn);
+    int lo = 0, hi = G - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (uni(tpre[mid]) <= m) lo = mid;
+      else hi = mid - 1;
+    }
+    const int32_t m0 = uni(tpre[lo]), gm = uni(tpre[lo + 1]) - m0;
+    const int64_t local = tile - (int64_t)m0 * ntn;
+    const int32_t band = (int32_t)(local / ((int64_t)kBand * ntn)) * kBand;
+    const int32_t rest = (int32_t)(local - (int64_t)band * ntn);
+    const int32_t high = gm - band < kBand ? gm - band : kBand;
+    at.g = lo;
+    at.ntile = rest / high;
+    const int32_t row0 = uni(offset(lo)) + (band + rest % high) * CF::BM;
+    at.row0 = row0;
+    at.row_end = uni(offset(lo + 1));
+  };
+
+  // Issue cursor: NST - 1 K-tiles in front of the one being multiplied.
+  Loads<CF> ld;
+  int64_t i_tile = first;
+  int32_t i_kt = 0, i_stage = 0, i_slot = 0;
+  bool i_live = true;
+  auto set_tile = [&]() {
+    Place at;
+    decode(i_tile, at);
+    setup<KIND, CF>(P, at, ld, wave, lane);
+  };
+  set_tile();
+  // The K-tile's exponents, where it is the first of four; ahead of its other
+  // loads, so that whoever waits for those has these too.
+  auto issue_scales = [&]() {
+    if (i_kt % kScaleTiles != 0 || !i_live) return;
+    const uint32_t kg = (uint32_t)(i_kt / kScaleTiles);
+#pragma unroll
+    for (int j = 0; j < CF::QS; ++j) {
+      const int s = j * NW + wave;
+      if (s >= CF::SA + CF::SB) continue;
+      char* dst = slots + i_slot * CF::SLOT + s * 1024;
+      if (s < CF::SA) dma16(ld.as, dst, ld.soff[j], kg * (uint32_t)(P.a_rows * kScaleBytes));
+      else dma16(ld.bs, dst, ld.soff[j], kg * (uint32_t)(P.N * kScaleBytes));
+    }
+  };
+  auto issue = [&](auto jj) __attribute__((always_inline)) {
+    constexpr int J = decltype(jj)::value;
+    // kOOB's bit on top of the offset where the lane lies past K
+    const uint32_t past = i_kt == nk - 1 ? ld.past : 0u;
+    const uint32_t off = ld.off[J] | ((past >> J) << 31);
+    char* stage = lds + i_stage * CF::STAGE;
+    if constexpr (J < CF::QA) dma16(ld.a, stage + (J * NW + wave) * 1024, off, (uint32_t)i_kt * KT);
+    else dma16(ld.b, stage + CF::A_BYTES + ((J - CF::QA) * NW + wave) * 1024, off, (uint32_t)i_kt * KT);
+  };
+  auto advance_issue = [&]() {
+    i_stage = i_stage + 1 == CF::NST ? 0 : i_stage + 1;
+    if (!i_live) return;
+    ++i_kt;
+    if (i_kt < nk) {
+      if (i_kt % kScaleTiles == 0) i_slot = i_slot + 1 == CF::NST ? 0 : i_slot + 1;
+      return;
+    }
+    i_kt = 0;
+    i_slot = i_slot + 1 == CF::NST ? 0 : i_slot + 1;
+    i_tile += step;
+    if (i_tile < end) {
+      set_tile();
+    } else {
+      // past the block's last K-tile: loads out of range, so that every K-tile issues the same number
+      i_live = false;
+#pragma unroll
+      for (int q = 0; q < L; ++q) ld.off[q] = kOOB;
+    }
+  };
+#pragma unroll
+  for (int s = 0; s < CF::NST - 1; ++s) {
+    issue_scales();
+    static_for<0, L>(issue);
+    advance_issue();
+  }
+
+  // Fragments: in half ks of the K-tile lane l holds row l%32, columns 16 h ..
+  // + 15 and 32 + 16 h .. + 15 of the half's 64 (h = l/32), and the exponent
+  // of its block h.
+  const int h = lane >> 5, r32 = lane & 31;
+  int32_t at[2][2];
+#pragma unroll
+  for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) at[ks][e] = r32 * KT + (((ks * 4 + e * 2 + h) ^ kc_swz(r32)) << 4);
+  const uint32_t pick = 0x06040200u + 0x01010101u * h;  // bytes h and 2 + h of two words
+  const int32_t arow = wm * CF::FM * 32, brow = wn * CF::FN * 32;
+  auto read = [&](auto jj, auto kk, const char* stage, const char* slot, const Frags8<CF>& fm, Frags8<CF>& fr)
+      __attribute__((always_inline)) {
+    constexpr int J = decltype(jj)::value, ks = decltype(kk)::value;
+    constexpr bool is_a = J < CF::FM;
+    const int row = is_a ? arow + J * 32 : brow + (J - CF::FM) * 32;
+    const char* p = stage + (is_a ? 0 : CF::A_BYTES) + row * KT;
+    const i32x4_t lo = *reinterpret_cast<const i32x4_t*>(p + at[ks][0]);
+    const i32x4_t hi = *reinterpret_cast<const i32x4_t*>(p + at[ks][1]);
+    const i32x8_t v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+    if constexpr (is_a) fr.a[J] = v;
+    else fr.b[J - CF::FM] = v;
+    constexpr int F = is_a ? J : J - CF::FM, last = (is_a ? CF::FM : CF::FN) - 1;
+    if constexpr (F % 2 == 0) {
+      int32_t& out = is_a ? fr.sa[F / 2] : fr.sb[F / 2];
+      if constexpr (ks == 0) {
+        const char* w = slot + (is_a ? 0 : CF::SA * 1024) + (row + r32) * kScaleBytes;
+        const uint32_t w0 = *reinterpret_cast<const uint32_t*>(w);
+        const uint32_t w1 = F < last ? *reinterpret_cast<const uint32_t*>(w + 32 * kScaleBytes) : w0;
+        out = (int32_t)__builtin_amdgcn_perm(w1, w0, pick);
+      } else {
+        out = is_a ? fm.sa[F / 2] : fm.sb[F / 2];
+      }
+    }
+  };
+
+  f32x16_t acc[CF::FM][CF::FN];
+  Frags8<CF> f0, f1;
+  constexpr int NM = CF::FM * CF::FN, NR = CF::FM + CF::FN;
+  auto mfma = [&](auto xx, auto kk, auto zero, const Frags8<CF>& f) __attribute__((always_inline)) {
+    constexpr int x = decltype(xx)::value, m = x / CF::FN, n = x % CF::FN, ks = decltype(kk)::value;
+    acc[m][n] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(f.b[n], f.a[m], decltype(zero)::value ? f32x16_t{} : acc[m][n],
+                                                                0, 0, n % 2 * 2 + ks, f.sb[n / 2], m % 2 * 2 + ks, f.sa[m / 2]);
+  };
+  // The MFMAs of half `km` from `fm`, in NR groups: each reads one fragment of
+  // the other half into `fr` and (loads) issues its share of the loads of the
+  // K-tile NST - 1 ahead.
+  auto kstep = [&](auto zero, auto km, auto loads, const Frags8<CF>& fm, const char* stage, const char* slot, Frags8<CF>& fr)
+      __attribute__((always_inline)) {
+    if constexpr (decltype(loads)::value) issue_scales();
+    static_for<0, NR>([&](auto jj) __attribute__((always_inline)) {
+      constexpr int j = decltype(jj)::value;
+      if constexpr (decltype(loads)::value) static_for<j * L / NR, (j + 1) * L / NR>(issue);
+      read(Int<order8<CF>(j)>{}, Int<1 - decltype(km)::value>{}, stage, slot, fm, fr);
+      static_for<j * NM / NR, (j + 1) * NM / NR>([&](auto xx) __attribute__((always_inline)) { mfma(xx, km, zero, fm); });
+      __builtin_amdgcn_sched_barrier(0);
+    });
+  };
+  // The end of a K-tile: the next one has landed (at most the loads of the
+  // NST - 2 K-tiles issued after it are outstanding), and every wave has read
+  // this one.
+  auto turn = [&]() __attribute__((always_inline)) {
+    wait_loads_lds<(CF::NST - 2) * L>();
+    block_barrier();
+  };
+
+  turn();
+  int c_stage = 0, c_slot = 0;
+  for (int64_t tile = first; tile < end; tile += step) {
+    // The tile's first K-tile: no MFMAs of this tile to read its first half behind.
+    {
+      const char* stage = lds + c_stage * CF::STAGE;
+      const char* slot = slots + c_slot * CF::SLOT;
+      static_for<0, NR>([&](auto j) __attribute__((always_inline)) {
+        read(Int<order8<CF>(decltype(j)::value)>{}, Int<0>{}, stage, slot, f0, f0);
+      });
+      kstep(Int<1>{}, Int<0>{}, Int<1>{}, f0, stage, slot, f1);
+      advance_issue();
+      turn();
+      c_stage = c_stage + 1 == CF::NST ? 0 : c_stage + 1;
+    }
+    for (int32_t kt = 1; kt < nk; ++kt) {
+      if (kt % kScaleTiles == 0) c_slot = c_slot + 1 == CF::NST ? 0 : c_slot + 1;
+      const char* stage = lds + c_stage * CF::STAGE;
+      const char* slot = slots + c_slot * CF::SLOT + kt % kScaleTiles * 4;
+      kstep(Int<0>{}, Int<1>{}, Int<1>{}, f1, stage, slot, f0);
+      kstep(Int<0>{}, Int<0>{}, Int<0>{}, f0, stage, slot, f1);
+      advance_issue();
+      turn();
+      c_stage = c_stage + 1 == CF::NST ? 0 : c_stage + 1;
+    }
+    static_for<0, NM>([&](auto x) __attribute__((always_inline)) { mfma(x, Int<1>{}, Int<0>{}, f1); });
+    c_slot = c_slot + 1 == CF::NST ? 0 : c_slot + 1;
+    Place place;
+    decode(tile, place);
+    epilogue<E, KIND, CF>(P, place, wm, wn, lane, acc);
+  }
+  wait_loads<0>();
+}
+
+// ---------------------------------------------------------------------------
+// Launches
+// ---------------------------------------------------------------------------
+
+int cu_count() {
+  static std::atomic<int> cached{0};
+  int cus = cached.load(std::memory_order_relaxed);
+  if (cus == 0) {
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess) return -1;
+    if (hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || cus <= 0) return -1;
+    cached.store(cus, std::memory_order_relaxed);
+  }
+  return cus;
+}
+
+using Rows32 = Cfg8<1, 4, 1, 2, 3, 1>;   // 32 x 256 tiles
+using Rows128 = Cfg8<2, 2, 2, 4, 2, 1>;  // 128 x 256
+using Rows256 = Cfg8<2, 2, 4, 4, 2, 1>;  // 256 x 256
+
+template <class E, int KIND, class CF>
+int launch_cfg(const Params8& P, int cus, pmx_stream_t stream) {
+  rows8_grouped_gemm_kernel<E, KIND, CF><<<cus * CF::BPC, CF::NTH, 0, stream>>>(P);
+  PMX_LAUNCH_CHECK();
+  return PMX_OK;
+}
+
+template <class E, int KIND>
+int launch(const Params8& P, pmx_stream_t stream) {
+  const int cus = cu_count();
+  if (cus <= 0) return PMX_ERR_HIP;
+  if (P.M <= 32 * (int64_t)P.G) return launch_cfg<E, KIND, Rows32>(P, cus, stream);
+  if (P.M <= 160 * (int64_t)P.G) return launch_cfg<E, KIND, Rows128>(P, cus, stream);
+  return launch_cfg<E, KIND, Rows256>(P, cus, stream);
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+// What one buffer descriptor covers: offsets are 32 bits, the top one marks
+// what lies outside.
+bool one_window(int64_t rows, int64_t bytes) { return rows <= (int64_t)0x7fffffff / bytes; }
+
+// The checks that both kinds share; PMX_OK to go on.
+int check(const Params8& P) {
+  if (P.G <= 0 || P.G > kMaxGroups || P.M < 0 || P.N <= 0 || P.K <= 0 || P.a_rows < 0) return PMX_ERR_ARG;
+  if (P.K % 16 || P.M > INT32_MAX - 256 || P.a_rows > INT32_MAX) return PMX_ERR_SHAPE;
+  const int64_t kgroups = (P.K + kScaleGroup - 1) / kScaleGroup;
+  if (!one_window(P.N, P.K) || !one_window(P.N, kgroups * kScaleBytes) || !one_window(P.a_rows, kgroups * kScaleBytes) ||
+      !one_window(P.row_token != nullptr ? P.a_rows : 256, P.K))
+    return PMX_ERR_SHAPE;
+  return PMX_OK;
+}
+
+template <class E>
+int nt_t(const void* a, const void* as, const void* b, const void* bs, const int32_t* offsets, int32_t G, int64_t M, int64_t N,
+         int64_t K, void* c, pmx_stream_t stream) {
+  Params8 P = {};
+  P.a = (const uint8_t*)a, P.as = (const uint8_t*)as, P.a_rows = M;
+  P.b = (const uint8_t*)b, P.bs = (const uint8_t*)bs;
+  P.offsets = offsets, P.G = G, P.M = M, P.N = N, P.K = K, P.c = (bf16_t*)c;
+  if (const int rc = check(P)) return rc;
+  if (N % 8) return PMX_ERR_SHAPE;
+  if (M == 0) return PMX_OK;
+  if (!a || !as || !b || !bs || !offsets || !c) return PMX_ERR_ARG;
+  if (!aligned16(a) || !aligned16(as) || !aligned16(b) || !aligned16(bs) || !aligned16(c)) return PMX_ERR_SHAPE;
+  return launch<E, NT8>(P, stream);
+}
+
+template <class E>
+int fc1_t(const void* x, const void* xs, int64_t T, const int32_t* row_token, const void* w, const void* ws,
+          const int32_t* offsets, int32_t G, int64_t A, int64_t H, int64_t I, const void* row_w, void* act, void* act_s,
+          pmx_stream_t stream) {
+  if (I <= 0 || I > INT32_MAX / 2) return PMX_ERR_ARG;
+  Params8 P = {};
+  P.a = (const uint8_t*)x, P.as = (const uint8_t*)xs, P.a_rows = T, P.row_token = row_token;
+  P.b = (const uint8_t*)w, P.bs = (const uint8_t*)ws;
+  P.offsets = offsets, P.G = G, P.M = A, P.N = 2 * I, P.K = H, P.I = I;
+  P.q = (uint8_t*)act, P.qs = (uint8_t*)act_s, P.row_w = (const bf16_t*)row_w;
+  if (const int rc = check(P)) return rc;
+  if (I % 16) return PMX_ERR_SHAPE;
+  if (A == 0) return PMX_OK;
+  if (!x || !xs || !w || !ws || !offsets || !act || !act_s || (row_token == nullptr && T != A)) return PMX_ERR_ARG;
+  if (!aligned16(x) || !aligned16(xs) || !aligned16(w) || !aligned16(ws) || !aligned16(act) || !aligned16(act_s))
+    return PMX_ERR_SHAPE;
+  return launch<E, FC18>(P, stream);
+}
+
+}  // namespace
+
+extern "C" {
+
+#define PMX_ROWS8_GEMM_ENTRIES(SUFFIX, E)                                                                                   \
+  int pmx_rows8_group_gemm_nt##SUFFIX(const void* a, const void* a_scales, const void* b, const void* b_scales,             \
+                                      const int32_t* offsets, int32_t G, int64_t M, int64_t N, int64_t K, void* c,          \
+                                      pmx_stream_t stream) {                                                                \
+    return nt_t<E>(a, a_scales, b, b_scales, offsets, G, M, N, K, c, stream);                                               \
+  }                                                                                                                         \
+  int pmx_rows8_gemm_fc1_swiglu##SUFFIX(const void* x, const void* x_scales, int64_t T, const int32_t* row_token,           \
+                                        const void* w, const void* w_scales, const int32_t* offsets, int32_t G, int64_t A,  \
+                                        int64_t H, int64_t I, const void* row_w, void* act, void* act_scales,               \
+                                        pmx_stream_t stream) {                                                              \
+    return fc1_t<E>(x, x_scales, T, row_token, w, w_scales, offsets, G, A, H, I, row_w, act, act_scales, stream);           \
+  }
+
+PMX_ROWS8_GEMM_ENTRIES(, EltBF16)
+PMX_ROWS8_GEMM_ENTRIES(_f16, EltF16)
+
+}  // extern "C"

@@ -23,6 +23,14 @@ SwiGLU output is multiplied by its router weight before fc2, the top-k rows
 of a token are summed unweighted (``moe_gather``), and the backward takes the
 router-weight gradient from the fc2 input side.  The two agree in exact
 arithmetic and differ in bf16 rounding.
+
+``activation_checkpoint="e4m3"`` (or ``"int8"``) leaves the output as it is, bit
+for bit, and keeps for the backward the hidden states [T, H] and the gate/up
+rows [A, 2I] in 8 bits instead of the permuted rows [A, H], the gate/up rows,
+the activations [A, I] and the expert outputs [A, H] in 16: H + 2I instead of
+4H + 6I bytes per row of a top-1 layer, less still with more experts per
+token.  Its backward takes the weights' gradient on the fc2 input side in both
+arithmetics, where it needs no expert outputs.
 """
 
 from __future__ import annotations
@@ -31,7 +39,7 @@ import os
 
 import torch
 
-from . import kernels
+from . import kernels, rows8
 
 # Route checks whose status has not been looked at yet.  The op never
 # waits for one: each forward and backward polls them (a read of a host word)
@@ -134,12 +142,29 @@ def _poll_pending_checks() -> None:
         failed.raise_if_failed()
 
 
+def route_checked(selected, num_slots: int, mapping, sources, source: int) -> kernels.Routing:
+    """Route one batch; its status is looked at without a host sync."""
+    _poll_pending_checks()
+    # Invalid expert or source ids are clamped on the device and flagged in
+    # the routing status word, which the routing stores to pinned host
+    # memory.  It is looked at without a host sync: by the backward if it
+    # has landed by then, else by a later forward or backward (or
+    # check_pending_routes).
+    check = kernels.RouteCheck()
+    r = kernels.route(selected, num_slots, mapping=mapping, sources=sources, source=source, check=check)
+    if _sync_route_checks():
+        check.raise_if_failed()
+    elif not check.checked:
+        _PENDING_CHECKS.append(check)
+    return r
+
+
 class _ExpertLayerBase(torch.autograd.Function):
     """Shared forward/backward; subclasses fix how fc1 weights are passed."""
 
     @staticmethod
     def _forward(ctx, hidden, routing_weights, selected, mapping, sources, source, w_gate, w_up, copy_stride,
-                 fc2_weight, split, recorder, weighted_input):
+                 fc2_weight, split, recorder, weighted_input, checkpoint):
         T, H = hidden.shape
         C, H2, inter = fc2_weight.shape
         assert H2 == H, f"down_proj hidden size {H2} != hidden size {H}"
@@ -157,24 +182,17 @@ class _ExpertLayerBase(torch.autograd.Function):
             f"fc1 weight shape {tuple(w_gate.shape)} does not match fc2 {tuple(fc2_weight.shape)} "
             f"and hidden size {H} (expected {fc1_shape})"
         )
-        _poll_pending_checks()
-        # Invalid expert or source ids are clamped on the device and flagged in
-        # the routing status word, which the routing stores to pinned host
-        # memory.  It is looked at without a host sync: by the backward if it
-        # has landed by then, else by a later forward or backward (or
-        # check_pending_routes).
-        check = kernels.RouteCheck()
-        r = kernels.route(selected, C, mapping=mapping, sources=sources, source=source, check=check)
-        if _sync_route_checks():
-            check.raise_if_failed()
-        elif not check.checked:
-            _PENDING_CHECKS.append(check)
+        r = route_checked(selected, C, mapping, sources, source)
         if recorder is not None:
             recorder(r.counts)
         ctx.split = split
         ctx.inter = inter
         ctx.routing = r
         ctx.weighted_input = weighted_input
+        ctx.checkpoint = checkpoint
+        if checkpoint is not None:
+            return _ExpertLayerBase._forward_checkpointed(ctx, r, hidden, routing_weights, w_gate, w_up, copy_stride,
+                                                          fc2_weight)
         if weighted_input:
             # group_gemm.py:473-511: fc1_weighted_output = fc1_activation *
             # scattered_gate_weight feeds fc2; moe_gather sums a token's rows.
@@ -202,8 +220,30 @@ class _ExpertLayerBase(torch.autograd.Function):
         return out
 
     @staticmethod
+    def _forward_checkpointed(ctx, r, hidden, routing_weights, w_gate, w_up, copy_stride, fc2_weight):
+        """The same kernels as without checkpoints; what is kept differs."""
+        C, _, inter = fc2_weight.shape
+        fmt = ctx.checkpoint
+        xp, row_src, row_w = kernels.moe_scatter_src(hidden, r.pos, routing_weights)
+        top1 = r.pos.shape[1] == 1 and _TOP1_FUSION
+        gu, act = kernels.gemm_fc1_swiglu(xp, w_gate, w_up, copy_stride, r.offsets, C, inter,
+                                          row_w=row_w if ctx.weighted_input else None)
+        if ctx.weighted_input:
+            out = kernels.moe_gather(kernels.group_gemm_nt(act, fc2_weight, r.offsets), r.pos)
+        elif top1:
+            _, out = kernels.group_gemm_nt_combine_top1(act, fc2_weight, r.offsets, row_src, row_w)
+        else:
+            out = kernels.combine_fwd(kernels.group_gemm_nt(act, fc2_weight, r.offsets), r.pos, routing_weights)
+        x8, gu8 = rows8.quantize_rows(hidden, fmt), rows8.quantize_rows(gu, fmt)
+        ctx.save_for_backward(x8.codes, x8.scales, gu8.codes, gu8.scales, r.pos, r.offsets, routing_weights, w_gate,
+                              w_up, fc2_weight, row_src, row_w)
+        return out
+
+    @staticmethod
     def _backward(ctx, grad_out):
         _poll_pending_checks()
+        if ctx.checkpoint is not None:
+            return _ExpertLayerBase._backward_checkpointed(ctx, grad_out)
         if ctx.weighted_input:
             return _ExpertLayerBase._backward_weighted_input(ctx, grad_out)
         xp, gu, act, y, pos, offsets, w, w_gate, w_up, fc2_weight, row_src = ctx.saved_tensors
@@ -286,12 +326,50 @@ class _ExpertLayerBase(torch.autograd.Function):
         return dx, (dw.view(w.shape) if need_w else None), d_fc1, d_fc2
 
 
+    @staticmethod
+    def _backward_checkpointed(ctx, grad_out):
+        """As ``_backward_weighted_input``, from the 8-bit hidden states and
+        gate/up rows: the weighted activations, fc2's weight gradient's other
+        operand, come out of the SwiGLU backward, and the permuted rows, fc1's,
+        are read back into place when its weight gradient needs them."""
+        x_codes, x_scales, gu_codes, gu_scales, pos, offsets, w, w_gate, w_up, fc2_weight, row_src, row_w = ctx.saved_tensors
+        gu8 = rows8.Rows8(gu_codes, gu_scales, w.dtype)
+        grad_out = grad_out.contiguous()
+        need_w, need_x = ctx.needs_input_grad[1], ctx.needs_input_grad[0]
+        dyp = kernels.moe_scatter(grad_out, pos)
+        main = torch.cuda.current_stream(dyp.device)
+        side = _side_stream(dyp.device) if uses_backward_overlap(dyp.shape[0], dyp.shape[1], ctx.inter) else main
+        d_fc2 = d_fc1 = None
+        d_act_w = kernels.group_gemm_nn(dyp, fc2_weight, offsets)
+        dg1, act_w, dw = rows8.swiglu_bwd_rows8(d_act_w, gu8, row_w, row_src, pos.numel())
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            if ctx.fc2_needs_grad:
+                d_fc2 = kernels.group_gemm_tn(dyp, act_w, offsets)
+            if ctx.fc1_needs_grad:
+                xp = rows8.dequantize_rows(rows8.Rows8(x_codes, x_scales, w.dtype), pos)
+                d_fc1 = kernels.group_gemm_tn(dg1, xp, offsets, split=ctx.inter if ctx.split else None)
+        dx = None
+        if need_x:
+            b_second = w_up if ctx.split else None
+            if pos.shape[1] == 1 and _TOP1_FUSION:
+                dx = kernels.group_gemm_nn_unpermute_top1(dg1, w_gate, offsets, row_src, b_second=b_second)
+            else:
+                dx = kernels.moe_gather(kernels.group_gemm_nn(dg1, w_gate, offsets, b_second=b_second), pos)
+        if side is not main:
+            main.wait_stream(side)
+            for t in (d_fc2, *(d_fc1 if isinstance(d_fc1, tuple) else (d_fc1,))):
+                if t is not None:
+                    t.record_stream(main)
+        return dx, (dw.view(w.shape) if need_w else None), d_fc1, d_fc2
+
+
 class HipMergedFc1ExpertLayer(_ExpertLayerBase):
     """Merged ``gate_up_proj`` [C, 2I, H] (``EPMergedFc1GroupGemm`` layout)."""
 
     @staticmethod
     def forward(ctx, hidden, routing_weights, selected, mapping, sources, source, fc1_1_2_weight, fc2_weight,
-                recorder=None, weighted_input=False):
+                recorder=None, weighted_input=False, checkpoint=None):
         C, two_i, H = fc1_1_2_weight.shape
         assert two_i % 2 == 0, f"Merged fc1_1_2_weight dim 1 must be even, got {two_i}"
         inter = two_i // 2
@@ -301,13 +379,13 @@ class HipMergedFc1ExpertLayer(_ExpertLayerBase):
         ctx.fc2_needs_grad = ctx.needs_input_grad[7]
         return _ExpertLayerBase._forward(
             ctx, hidden, routing_weights, selected, mapping, sources, source, fc1_1_2_weight, w_up,
-            2 * inter * H, fc2_weight, False, recorder, weighted_input,
+            2 * inter * H, fc2_weight, False, recorder, weighted_input, checkpoint,
         )
 
     @staticmethod
     def backward(ctx, grad_out):
         dx, dw, d_fc1, d_fc2 = _ExpertLayerBase._backward(ctx, grad_out)
-        return dx, dw, None, None, None, None, d_fc1, d_fc2, None, None
+        return dx, dw, None, None, None, None, d_fc1, d_fc2, None, None, None
 
 
 class HipSplitFc1ExpertLayer(_ExpertLayerBase):
@@ -315,7 +393,7 @@ class HipSplitFc1ExpertLayer(_ExpertLayerBase):
 
     @staticmethod
     def forward(ctx, hidden, routing_weights, selected, mapping, sources, source, fc1_1_weight, fc1_2_weight,
-                fc2_weight, recorder=None, weighted_input=False):
+                fc2_weight, recorder=None, weighted_input=False, checkpoint=None):
         C, inter, H = fc1_1_weight.shape
         assert fc1_2_weight.shape == fc1_1_weight.shape, "fc1_1 and fc1_2 shapes differ"
         assert fc1_1_weight.is_contiguous() and fc1_2_weight.is_contiguous() and fc2_weight.is_contiguous(), (
@@ -325,14 +403,14 @@ class HipSplitFc1ExpertLayer(_ExpertLayerBase):
         ctx.fc2_needs_grad = ctx.needs_input_grad[8]
         return _ExpertLayerBase._forward(
             ctx, hidden, routing_weights, selected, mapping, sources, source, fc1_1_weight, fc1_2_weight,
-            inter * H, fc2_weight, True, recorder, weighted_input,
+            inter * H, fc2_weight, True, recorder, weighted_input, checkpoint,
         )
 
     @staticmethod
     def backward(ctx, grad_out):
         dx, dw, d_fc1, d_fc2 = _ExpertLayerBase._backward(ctx, grad_out)
         d_gate, d_up = d_fc1 if d_fc1 is not None else (None, None)
-        return dx, dw, None, None, None, None, d_gate, d_up, d_fc2, None, None
+        return dx, dw, None, None, None, None, d_gate, d_up, d_fc2, None, None, None
 
 
 def expert_layer(
@@ -348,6 +426,7 @@ def expert_layer(
     source: int = 0,
     recorder=None,
     weighted_input: bool = False,
+    activation_checkpoint: str | None = None,
 ) -> torch.Tensor:
     """The full layer on one GPU: [T, H] -> [T, H], differentiable in hidden,
     routing weights and the expert weights.
@@ -357,17 +436,27 @@ def expert_layer(
     ``recorder(counts)`` receives the int32 per-copy token counts (on the device).
     ``weighted_input``: apply the router weights to the fc2 input (the
     reference's non-EP arithmetic) instead of in the combine (EP).
+    ``activation_checkpoint``: keep for the backward only the hidden states and
+    the gate/up rows, in 8 bits (``"e4m3"`` or ``"int8"``); None keeps them, the
+    activations and the expert outputs in 16.
     """
+    if activation_checkpoint is not None and activation_checkpoint not in rows8.FORMATS:
+        raise ValueError(f"activation checkpoint must be None or one of {sorted(rows8.FORMATS)}, "
+                         f"got {activation_checkpoint!r}")
+    if not (torch.is_grad_enabled() and any(
+            t is not None and t.requires_grad
+            for t in (hidden, routing_weights, fc2_weight, fc1_1_2_weight, fc1_1_weight, fc1_2_weight))):
+        activation_checkpoint = None  # no backward will read it
     if fc1_1_2_weight is not None:
         if fc1_1_weight is not None or fc1_2_weight is not None:
             raise ValueError("Provide either split fc1 weights or merged fc1_1_2_weight, not both.")
         return HipMergedFc1ExpertLayer.apply(
             hidden, routing_weights, selected_experts, mapping, sources, source, fc1_1_2_weight, fc2_weight,
-            recorder, bool(weighted_input),
+            recorder, bool(weighted_input), activation_checkpoint,
         )
     if fc1_1_weight is None or fc1_2_weight is None:
         raise ValueError("Split fc1 mode requires both fc1_1_weight and fc1_2_weight.")
     return HipSplitFc1ExpertLayer.apply(
         hidden, routing_weights, selected_experts, mapping, sources, source, fc1_1_weight, fc1_2_weight, fc2_weight,
-        recorder, bool(weighted_input),
+        recorder, bool(weighted_input), activation_checkpoint,
     )

@@ -29,6 +29,7 @@ from __future__ import annotations
 
 import torch
 
+from . import rows8
 from .experts import expert_layer
 from .kernel_registry import KERNEL_REGISTRY, HardwareRequirement, KernelSpec
 from .placement import PLACEMENTS
@@ -51,6 +52,23 @@ def set_router_weight_point(point: str) -> str:
     if point not in _ROUTER_WEIGHT_POINTS:
         raise ValueError(f"router weight point must be one of {_ROUTER_WEIGHT_POINTS}, got {point!r}")
     prev, _ROUTER_WEIGHT_POINT = _ROUTER_WEIGHT_POINT, point
+    return prev
+
+
+# None (16-bit activations are kept for the backward) or an 8-bit format.
+_ACTIVATION_CHECKPOINT: str | None = None
+
+
+def set_activation_checkpoint(fmt: str | None) -> str | None:
+    """What the hip backend keeps of a layer's forward for its backward: with
+    ``"e4m3"`` or ``"int8"`` the hidden states and the gate/up rows in 8 bits
+    (outputs stay the same bit for bit, gradients carry the rounding of what was
+    kept), with None (the default) everything in 16 bits.  A layer uses the
+    setting of its forward.  Returns the previous setting."""
+    global _ACTIVATION_CHECKPOINT
+    if fmt is not None and fmt not in rows8.FORMATS:
+        raise ValueError(f"activation checkpoint must be None or one of {sorted(rows8.FORMATS)}, got {fmt!r}")
+    prev, _ACTIVATION_CHECKPOINT = _ACTIVATION_CHECKPOINT, fmt
     return prev
 
 
@@ -132,7 +150,7 @@ def hip_fused_moe_forward(
     out = expert_layer(
         hidden, w, sel, fc2_weight, fc1_1_2_weight=fc1_1_2_weight, fc1_1_weight=fc1_1_weight,
         fc1_2_weight=fc1_2_weight, mapping=mapping, sources=sources, source=source, recorder=recorder,
-        weighted_input=point == "fc2_input",
+        weighted_input=point == "fc2_input", activation_checkpoint=_ACTIVATION_CHECKPOINT,
     )
     return out.reshape(shape)
 

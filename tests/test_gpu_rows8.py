@@ -1,0 +1,714 @@
+"""Rows in 8 bits on the GPU against the 64-bit oracle.
+
+Tolerances, from the arithmetic:
+
+* writing and reading back are exact by definition (one rounding to nearest
+  even, powers of two): codes, exponents and values must be equal;
+* SwiGLU backward: one rounding of each result (half a step, eps / 2), beside
+  fp32 arithmetic whose sigmoid is good to 2^-18 for |gate| <= 32 (the
+  exponential's argument, up to 46 in base 2, is rounded to 2^-19);
+* products of small integers, whose every sum is exact in fp32, must be equal
+  after the one rounding; products of arbitrary values carry up to 2^-11 of
+  the largest product of each 64 columns (a matrix instruction adds its 64
+  products to about 2^-12 of the largest, measured) and the result's half step.
+"""
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import placemoe_amd
+from oracle import moe_oracle
+from oracle import rows8_oracle as O
+from placemoe_amd import _capi, experts, kernels, rows8
+from placemoe_amd.workloads import make_workload
+from tests.helpers import BF16_REL, assert_bf16_close, assert_exact
+
+pytestmark = pytest.mark.gpu
+
+BF, F16 = torch.bfloat16, torch.float16
+SUBNORMAL = {BF: 2.0**-133, F16: 2.0**-24}
+
+
+def _randn(shape, seed, dtype=BF, std=1.0):
+    return (torch.randn(shape, generator=torch.Generator().manual_seed(seed)) * std).to(dtype)
+
+
+def _same(got, want, name):
+    """Equal as 64-bit values, NaN where NaN."""
+    got = got.detach().double().cpu().numpy() if isinstance(got, torch.Tensor) else got
+    bad = np.argwhere(~((got == want) | (np.isnan(got) & np.isnan(want))))
+    assert bad.size == 0, f"{name}: {len(bad)} differ, first at {bad[0]}: {got[tuple(bad[0])]} for {want[tuple(bad[0])]}"
+
+
+def _check_written(q, x, fmt, name):
+    v, scales = O.quantize(x, fmt)
+    assert torch.equal(q.scales.cpu(), scales), f"{name}: exponents"
+    _same(O.values(q.codes.cpu(), q.scales.cpu()), v, name)
+    return v
+
+
+def _spiky(shape, seed, dtype):
+    """Blocks of every size, zeros, one loud column, values at the edges of the type."""
+    R, N = shape
+    x = _randn(shape, seed, torch.float32) * torch.logspace(-7 if dtype == F16 else -30, 4, R).unsqueeze(1)
+    if N > 3:
+        x[:, 3] *= 100
+    x[R // 2] = 0
+    x = x.to(dtype)
+    info = torch.finfo(dtype)
+    x[0, N // 2] = info.max
+    x[-1, :] = info.smallest_normal
+    x[-1, N - 1] = info.smallest_normal * 2.0 ** (-7 if dtype == BF else -10)  # the smallest subnormal
+    return x
+
+
+@pytest.mark.parametrize("dtype", [BF, F16])
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("R,N", [(1, 1), (1, 8), (3, 31), (5, 33), (33, 512), (31, 513), (65, 1411), (4, 2048), (40, 100)])
+def test_written_and_read_back_exactly(cuda, R, N, fmt, dtype):
+    print(f"rows8 {R}x{N} {fmt} {dtype}", flush=True)
+    x = _spiky((R, N), R * 31 + N, dtype)
+    q = rows8.quantize_rows(x.to(cuda), fmt)
+    assert q.shape == (R, N) and q.dtype == dtype and q.codes.dtype == rows8.FORMATS[fmt]
+    v = _check_written(q, x, fmt, f"{R}x{N}")
+    most = float(torch.finfo(dtype).max)
+    _same(rows8.dequantize_rows(q), np.clip(v, -most, most), "read back")
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("dtype", [BF, F16])
+def test_values_that_are_not_finite(cuda, fmt, dtype):
+    x = _randn((6, 96), 5, dtype)
+    x[0, 3], x[1, 40], x[2, 95] = math.inf, -math.inf, math.nan
+    x[3, 32:64] = math.inf  # a block with nothing finite
+    x[4] = math.nan
+    q = rows8.quantize_rows(x.to(cuda), fmt)
+    _check_written(q, x, fmt, "not finite")
+    back = rows8.dequantize_rows(q).cpu()
+    assert torch.equal(back.isnan(), ~x.isfinite())
+
+
+def test_ties_round_to_even(cuda):
+    # beside 2^0 (the block holds 448): 17 and 19 lie halfway between multiples of 2
+    x = torch.zeros((1, 32), dtype=BF)
+    x[0, :6] = torch.tensor([448.0, 17.0, 19.0, -17.0, 2.0**-10, 3 * 2.0**-10])
+    back = rows8.dequantize_rows(rows8.quantize_rows(x.to(cuda))).cpu()[0, :6]
+    assert back.tolist() == [448.0, 16.0, 20.0, -16.0, 0.0, 2.0**-8]
+    x[0, :6] = torch.tensor([127.0, 0.5, 1.5, 2.5, -0.5, -1.5])
+    back = rows8.dequantize_rows(rows8.quantize_rows(x.to(cuda), "int8")).cpu()[0, :6]
+    assert back.tolist() == [127.0, 0.0, 2.0, 2.0, 0.0, -2.0]
+
+
+def test_strided_unaligned_and_grouped_rows(cuda):
+    big = _randn((70, 1500), 6)
+    dev = big.to(cuda)
+    for part in (slice(0, 700), slice(1, 702), slice(3, 4)):
+        _check_written(rows8.quantize_rows(dev[:, part]), big[:, part], "e4m3", f"columns {part}")
+    _check_written(rows8.quantize_rows(dev[::3, 5:600]), big[::3, 5:600], "e4m3", "every third row")
+    one = rows8.quantize_rows(dev.view(-1)[7: 7 + 2 * 515].view(2, 515))
+    _check_written(one, big.view(-1)[7: 7 + 2 * 515].view(2, 515), "e4m3", "odd address")
+    w = _randn((3, 37, 130), 7)
+    q = rows8.quantize_rows(w.to(cuda))
+    assert q.scales.shape == (3, 1, 37, 16)
+    for g in range(3):
+        v, s = O.quantize(w[g], "e4m3")
+        assert torch.equal(q.scales[g].cpu(), s)
+        _same(O.values(q.codes[g].cpu(), q.scales[g].cpu()), v, f"group {g}")
+    for bad in (dev.t(), dev[:, ::2], dev[0].expand(4, 1500), w.to(cuda).transpose(1, 2)):
+        with pytest.raises(AssertionError):
+            rows8.quantize_rows(bad)
+    with pytest.raises(AssertionError):
+        rows8.quantize_rows(dev.float())
+
+
+def test_nothing_to_write(cuda):
+    for shape in ((0, 64), (5, 0), (0, 0), (0, 4, 64), (2, 0, 64)):
+        q = rows8.quantize_rows(torch.empty(shape, dtype=BF, device=cuda))
+        assert q.shape == shape and tuple(q.scales.shape) == rows8.scales_shape(shape)
+        if len(shape) == 2:
+            assert rows8.dequantize_rows(q).shape == shape
+
+
+@pytest.mark.parametrize("dtype", [BF, F16])
+@pytest.mark.parametrize("T,K,N", [(1, 1, 40), (37, 2, 1000), (50, 8, 515), (7, 4, 16)])
+def test_read_back_into_copies_rows(cuda, T, K, N, dtype):
+    print(f"read back T={T} K={K} N={N}", flush=True)
+    q = rows8.quantize_rows(_randn((T, N), T, dtype).to(cuda), "int8")
+    pos = torch.randperm(T * K, generator=torch.Generator().manual_seed(T)).to(torch.int32).view(T, K).to(cuda)
+    assert_exact(rows8.dequantize_rows(q, pos), kernels.moe_scatter(rows8.dequantize_rows(q), pos), "rows")
+
+
+def test_positions_outside_are_skipped(cuda):
+    q = rows8.quantize_rows(_randn((4, 64), 1).to(cuda))
+    pos = torch.tensor([[0], [9], [-1], [3]], dtype=torch.int32, device=cuda)
+    out = torch.full((4, 64), 7.0, dtype=BF, device=cuda)
+    _capi.call("pmx_rows8_dequantize", q.codes.data_ptr(), q.scales.data_ptr(), pos.data_ptr(), 4, 1, 64, 0, out.data_ptr(),
+               torch.cuda.current_stream().cuda_stream)
+    want = rows8.dequantize_rows(q)
+    assert_exact(out[[0, 3]], want[[0, 3]], "named rows")
+    assert (out[[1, 2]] == 7.0).all()
+
+
+def test_routed_rows(cuda):
+    T, K, H = 75, 3, 528
+    x, w = _randn((T, H), 8), torch.rand((T, K), generator=torch.Generator().manual_seed(9)).to(BF)
+    pos = torch.randperm(T * K, generator=torch.Generator().manual_seed(10)).to(torch.int32).view(T, K)
+    q, row_token, row_w = rows8.quantize_rows_routed(x.to(cuda), pos.to(cuda), w.to(cuda))
+    _check_written(q, x, "e4m3", "tokens")
+    want = torch.empty(T * K, dtype=torch.int64)
+    want[pos.view(-1).long()] = torch.arange(T * K)
+    assert_exact(row_token, want // K, "row_token")
+    assert_exact(row_w, w.view(-1)[want], "row_w")
+
+
+# ---------------------------------------------------------------------------
+# SwiGLU backward
+# ---------------------------------------------------------------------------
+
+
+def _near(got, exact, slack, dtype, name):
+    """Within half a step of the exact value and the slack."""
+    got = got.detach().double().cpu().numpy()
+    tol = np.abs(exact) * torch.finfo(dtype).eps / 2 + slack + SUBNORMAL[dtype]
+    off = np.abs(got - exact) - tol * 1.0001
+    assert np.isfinite(got).all(), name
+    assert (off <= 0).all(), f"{name}: {np.abs(got - exact).max()} off, {off.max()} over its tolerance"
+
+
+@pytest.mark.parametrize("dtype", [BF, F16])
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("R,I", [(1, 1), (2, 16), (5, 33), (64, 96), (33, 513), (130, 1411), (7, 2048), (300, 100)])
+def test_swiglu_backward_from_8_bits(cuda, R, I, fmt, dtype):
+    print(f"swiglu_bwd_rows8 {R}x{I} {fmt} {dtype}", flush=True)
+    gu = _randn((R, 2 * I), R + I, torch.float32, 3.0).clamp(-30, 30).to(dtype)
+    d = _randn((R, I), R + I + 1, dtype)
+    w = (0.05 + torch.rand(R, generator=torch.Generator().manual_seed(I))).to(dtype)
+    src = torch.randperm(R, generator=torch.Generator().manual_seed(R)).to(torch.int32)
+    q = rows8.quantize_rows(gu.to(cuda), fmt)
+    dg1, act_w, dw = rows8.swiglu_bwd_rows8(d.to(cuda), q, w.to(cuda), src.to(cuda), R)
+    v = O.values(q.codes.cpu(), q.scales.cpu())
+    dn, wn = d.double().numpy(), w.double().numpy()
+    e_dg1, e_act, e_dw = O.swiglu_backward(dn, v, wn)
+    g, u = v[:, :I], v[:, I:]
+    sig = 1 / (1 + np.exp(-g))
+    size = np.abs(np.concatenate([dn * wn[:, None] * u * (sig + np.abs(g) * sig), dn * wn[:, None] * g * sig], 1))
+    _near(dg1, e_dg1, size * 2.0**-17, dtype, "dG1")
+    _near(act_w, e_act, np.abs(e_act) * 2.0**-17, dtype, "act_w")
+    terms = np.abs(dn * g * sig * u).sum(1)
+    got_dw = torch.empty(R, dtype=dtype)
+    got_dw = dw.cpu()[src.long()]
+    _near(got_dw, e_dw, terms * (2.0**-17 + (I + 8) * 2.0**-24), dtype, "dw")
+    # without weights: ones
+    dg1, act, none = rows8.swiglu_bwd_rows8(d.to(cuda), q)
+    e_dg1, e_act, _ = O.swiglu_backward(dn, v, np.ones(R))
+    assert none is None
+    _near(dg1, e_dg1, size / wn[:, None] * 2.0**-17, dtype, "dG1 unweighted")
+    _near(act, e_act, np.abs(e_act) * 2.0**-17, dtype, "act")
+
+
+def test_swiglu_gradient_against_differences(cuda):
+    """d/dg and d/du of sum(d * silu(g) * u) in 64 bits, by central differences."""
+    R, I = 6, 40
+    q = rows8.quantize_rows(_randn((R, 2 * I), 1).to(cuda))
+    d = _randn((R, I), 2).to(cuda)
+    dg1, _, _ = rows8.swiglu_bwd_rows8(d, q)
+    v, dn = O.values(q.codes.cpu(), q.scales.cpu()), d.double().cpu().numpy()
+
+    def f(x):  # per element of (g | u), only its own term changes
+        g, u = x[:, :I], x[:, I:]
+        return dn * g / (1 + np.exp(-g)) * u
+
+    h = 1e-5
+    num = np.empty_like(v)
+    for half in (slice(0, I), slice(I, 2 * I)):
+        up, down = v.copy(), v.copy()
+        up[:, half] += h
+        down[:, half] -= h
+        num[:, half] = (f(up) - f(down)) / (2 * h)
+    # differences are good to h^2 times a third derivative of a few units, and 1e-16 / h
+    _near(dg1, num, np.abs(np.concatenate([dn, dn], 1)) * (2.0**-16 + 1e-8) * (1 + np.abs(v).max()), BF, "gradient")
+
+
+def test_swiglu_extreme_gates(cuda):
+    """Saturated gates: silu -> 0 or g, no NaN from infinities on the way; a NaN stays in its row."""
+    gu = torch.zeros((3, 64), dtype=BF)
+    gu[0, :32] = torch.tensor([-3e38, -1e4, -100.0, -90.0, 100.0, 1e4] + [0.0] * 26)
+    gu[0, 32:] = 1.0
+    gu[1, :] = 2.0
+    gu[1, 5] = math.nan
+    gu[2, :] = 0.5
+    q = rows8.quantize_rows(gu.to(cuda))
+    d = torch.ones((3, 32), dtype=BF, device=cuda)
+    dg1, act, _ = rows8.swiglu_bwd_rows8(d, q)
+    assert dg1[0].isfinite().all() and act[0].isfinite().all() and dg1[2].isfinite().all()
+    v = rows8.dequantize_rows(q)[0, :6].float()
+    assert torch.equal(act[0, :6].float()[v <= -1e4], torch.zeros_like(v[v <= -1e4]))
+    assert torch.equal(act[0, 5:6].float(), v[5:6])
+    assert dg1[1].isnan().nonzero().view(-1).tolist() == [5, 37] and act[1].isnan().nonzero().view(-1).tolist() == [5]
+
+
+def test_swiglu_skips_unnamed_weights(cuda):
+    R, I, A = 8, 40, 12
+    q = rows8.quantize_rows(_randn((R, 2 * I), 3).to(cuda))
+    d, w = _randn((R, I), 4).to(cuda), torch.ones(R, dtype=BF, device=cuda)
+    src = torch.tensor([0, 2, 4, 6, 8, 10, 12, -1], dtype=torch.int32, device=cuda)
+    dg1, act = torch.empty((R, 2 * I), dtype=BF, device=cuda), torch.empty((R, I), dtype=BF, device=cuda)
+    dw = torch.full((A,), 7.0, dtype=BF, device=cuda)
+    _capi.call("pmx_rows8_swiglu_bwd", d.data_ptr(), q.codes.data_ptr(), q.scales.data_ptr(), w.data_ptr(), src.data_ptr(), R, I,
+               A, 0, dg1.data_ptr(), act.data_ptr(), dw.data_ptr(), torch.cuda.current_stream().cuda_stream)
+    assert (dw.cpu()[1::2] == 7.0).all() and (dw.cpu()[::2] != 7.0).all()
+
+
+# ---------------------------------------------------------------------------
+# Products
+# ---------------------------------------------------------------------------
+
+
+def _offsets(counts):
+    return torch.tensor([0, *np.cumsum(counts)], dtype=torch.int32)
+
+
+def _ints(shape, seed, dtype=BF):
+    """Small integers times a power of two per block of 32 columns: exact in 8 bits."""
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randint(-3, 4, shape, generator=g).float()
+    nb = -(-shape[-1] // 32)
+    p = torch.exp2(torch.randint(0, 3, (*shape[:-1], nb), generator=g).float()).repeat_interleave(32, -1)[..., : shape[-1]]
+    return (x * p).to(dtype)
+
+
+LAYOUTS = {
+    "one row": ([1], 8, 16),
+    "one row each": ([1] * 5, 40, 48),
+    "empty groups": ([0, 3, 0, 0, 17, 0], 64, 128),
+    "only the last": ([0, 0, 0, 33], 256, 512),
+    "ragged": ([5, 31, 32, 33, 64, 1, 0, 70], 200, 1104),
+    "long K": ([9, 40], 72, 2320),
+    "mid": ([130, 61, 0, 255, 128], 328, 144),
+    "mid wide": ([100, 90], 1000, 656),
+    "large": ([256, 257, 511, 300], 264, 272),
+    "large odd": ([700, 0, 301], 520, 1040),
+    "many groups": ([2, 0, 1] * 400, 16, 32),
+}
+
+
+@pytest.mark.parametrize("dtype", [BF, F16])
+@pytest.mark.parametrize("name", LAYOUTS)
+def test_products_of_integers_are_exact(cuda, name, dtype):
+    counts, N, K = LAYOUTS[name]
+    print(f"rows8 gemm {name} {dtype}", flush=True)
+    M, G = sum(counts), len(counts)
+    a, b = _ints((M, K), 1, dtype), _ints((G, N, K), 2, dtype)
+    off = _offsets(counts)
+    qa, qb = rows8.quantize_rows(a.to(cuda)), rows8.quantize_rows(b.to(cuda))
+    got = rows8.group_gemm_nt_rows8(qa, qb, off.to(cuda))
+    want = torch.cat([a[off[g]:off[g + 1]].double() @ b[g].double().t() for g in range(G)])
+    # |sum| <= K * (3 * 4)^2 < 2^24: fp32 holds it, and one rounding follows
+    assert_exact(got, want.float().to(dtype), name)
+
+
+@pytest.mark.parametrize("dtype", [BF, F16])
+@pytest.mark.parametrize("counts,N,K", [([7, 0, 40], 48, 400), ([150, 170], 136, 1008), ([300, 260], 264, 528)])
+def test_products_of_activations(cuda, counts, N, K, dtype):
+    M, G = sum(counts), len(counts)
+    a, b = _randn((M, K), 11, dtype), _randn((G, N, K), 12, dtype, 0.05)
+    a[:, 5] *= 30
+    off = _offsets(counts)
+    print(f"rows8 gemm {counts} {N} {K} {dtype}", flush=True)
+    qa, qb = rows8.quantize_rows(a.to(cuda)), rows8.quantize_rows(b.to(cuda))
+    got = rows8.group_gemm_nt_rows8(qa, qb, off.to(cuda))
+    va = O.values(qa.codes.cpu(), qa.scales.cpu())
+    vb = np.stack([O.values(qb.codes[g].cpu(), qb.scales[g].cpu()) for g in range(G)])
+    c, big = O.grouped_nt(va, vb, off.numpy())
+    _near(got, c, big * 2.0**-11, dtype, "C")
+
+
+def test_rows_of_no_group_are_left_alone(cuda):
+    a, b = rows8.quantize_rows(_ints((300, 64), 1).to(cuda)), rows8.quantize_rows(_ints((2, 32, 64), 2).to(cuda))
+    for offsets in ([3, 20, 290], [0, 300, 300], [5, 5, 5]):
+        c = torch.full((300, 32), 7.0, dtype=BF, device=cuda)
+        off = torch.tensor(offsets, dtype=torch.int32, device=cuda)
+        _capi.call("pmx_rows8_group_gemm_nt", a.codes.data_ptr(), a.scales.data_ptr(), b.codes.data_ptr(), b.scales.data_ptr(),
+                   off.data_ptr(), 2, 300, 32, 64, c.data_ptr(), torch.cuda.current_stream().cuda_stream)
+        out = torch.ones(300, dtype=torch.bool)
+        out[offsets[0]:offsets[2]] = False
+        assert (c.cpu()[out] == 7.0).all()
+        full = rows8.dequantize_rows(a).float()
+        w = rows8.dequantize_rows(rows8.Rows8(b.codes.view(64, 64), b.scales.permute(1, 0, 2, 3).reshape(1, 64, 16).contiguous(), BF))
+        for g in range(2):
+            rows = slice(offsets[g], offsets[g + 1])
+            assert_exact(c[rows], (full[rows].double() @ w.view(2, 32, 64)[g].double().t()).to(BF), f"group {g}")
+
+
+def test_offsets_past_the_rows_are_clamped(cuda):
+    """Offsets that leave [0, M] or descend reach no memory outside the operands."""
+    a, b = rows8.quantize_rows(_ints((40, 64), 1).to(cuda)), rows8.quantize_rows(_ints((3, 32, 64), 2).to(cuda))
+    want = rows8.group_gemm_nt_rows8(a, b, torch.tensor([0, 10, 10, 40], dtype=torch.int32, device=cuda))
+    got = rows8.group_gemm_nt_rows8(a, b, torch.tensor([-7, 10, 10, 1 << 30], dtype=torch.int32, device=cuda))
+    assert_exact(got, want, "clamped")
+    rows8.group_gemm_nt_rows8(a, b, torch.tensor([40, 30, 20, 10], dtype=torch.int32, device=cuda))
+    torch.cuda.synchronize()
+
+
+def test_a_row_depends_on_itself_and_its_copy_alone(cuda):
+    """The same row in calls of one, a few, and many rows, in any slot: the same bits."""
+    K, N = 1104, 264
+    a, w = _randn((2000, K), 1).to(cuda), _randn((1, N, K), 2, std=0.05).to(cuda)
+    q = rows8.quantize_rows(a)
+    ref = rows8.group_gemm_nt_rows8(q, rows8.quantize_rows(w), torch.tensor([0, 2000], dtype=torch.int32, device=cuda))
+    for rows, slots in ((1, 1), (20, 3), (130, 2), (300, 5)):
+        part = rows8.quantize_rows(a[:rows])
+        counts = [0] * slots
+        counts[slots // 2] = rows
+        ww = torch.randn((slots, N, K), device=cuda).to(BF)
+        ww[slots // 2] = w[0]
+        got = rows8.group_gemm_nt_rows8(part, rows8.quantize_rows(ww), _offsets(counts).to(cuda))
+        assert_exact(got, ref[:rows], f"{rows} rows in slot {slots // 2}")
+
+
+@pytest.mark.parametrize("dtype", [BF, F16])
+@pytest.mark.parametrize("counts,I,H,T", [([1], 16, 16, 1), ([3, 0, 30, 7], 48, 144, 20), ([130, 90, 61], 144, 528, 100),
+                                          ([300, 280], 208, 272, 290), ([40] * 3, 640, 64, 50)])
+def test_fc1_swiglu_in_8_bits(cuda, counts, I, H, T, dtype):
+    G, A = len(counts), sum(counts)
+    print(f"rows8 fc1 {counts} I={I} H={H} {dtype}", flush=True)
+    g = torch.Generator().manual_seed(A + I)
+    x, w = _randn((T, H), 1, dtype), _randn((G, 2 * I, H), 2, dtype, 1.5 / math.sqrt(H))
+    token = torch.randint(0, T, (A,), generator=g).to(torch.int32)
+    row_w = (0.05 + torch.rand(A, generator=g)).to(dtype)
+    off = _offsets(counts)
+    qx, qw = rows8.quantize_rows(x.to(cuda)), rows8.quantize_rows(w.to(cuda))
+    act = rows8.gemm_fc1_swiglu_rows8(qx, qw, off.to(cuda), token.to(cuda), row_w.to(cuda))
+    assert act.shape == (A, I) and act.codes.dtype == torch.float8_e4m3fn
+    vx = O.values(qx.codes.cpu(), qx.scales.cpu())[token.numpy()]
+    vw = np.stack([O.values(qw.codes[k].cpu(), qw.scales[k].cpu()) for k in range(G)])
+    gu, big = O.grouped_nt(vx, vw, off.numpy())
+    gate, up = gu[:, :I], gu[:, I:]
+    rw = row_w.double().numpy()[:, None]
+    exact = gate / (1 + np.exp(-gate)) * up * rw
+    slack = rw * (1.1 * big[:, :I] * np.abs(up) + np.abs(gate) * big[:, I:]) * 2.0**-11 + np.abs(exact) * 2.0**-17
+    # the block's power of two: that of the exact values, or of values that differ by the slack
+    low, high = np.abs(exact) - slack, np.abs(exact) + slack
+    e_low, e_high = O.block_exponents(np.maximum(low, 0), "e4m3"), O.block_exponents(high, "e4m3")
+    nb = e_low.shape[1]
+    e = act.scales.cpu().permute(1, 0, 2).reshape(A, -1)[:, :nb].numpy().astype(np.int64) - 127
+    assert ((e >= e_low) & (e <= e_high)).all(), "exponents"
+    got = O.values(act.codes.cpu(), act.scales.cpu())
+    unit = np.repeat(2.0**e, 32, axis=1)[:, :I]
+    # e4m3: half a step is 2^-4 of the value, at least 2^-10 of the unit
+    tol = slack + np.maximum((np.abs(exact) + slack) * 2.0**-4, unit * 2.0**-10)
+    assert (np.abs(got - exact) <= tol * 1.0001).all(), f"codes: {(np.abs(got - exact) - tol).max()}"
+    # the blocks that fc2's last K-tile takes along stand beside 2^0
+    tail = act.scales.cpu().permute(1, 0, 2).reshape(A, -1)[:, nb: -(-I // 128) * 4]
+    assert (tail == 127).all()
+    plain = rows8.gemm_fc1_swiglu_rows8(rows8.Rows8(qx.codes[token.long()].contiguous(), qx.scales[:, token.long()].contiguous(), dtype),
+                                        qw, off.to(cuda), None, row_w.to(cuda))
+    assert torch.equal(plain.codes.view(torch.uint8), act.codes.view(torch.uint8)), "rows in place"
+
+
+def test_token_outside_reads_as_zeros(cuda):
+    qx, qw = rows8.quantize_rows(_randn((4, 64), 1).to(cuda)), rows8.quantize_rows(_randn((1, 64, 64), 2).to(cuda))
+    off = torch.tensor([0, 3], dtype=torch.int32, device=cuda)
+    act = rows8.gemm_fc1_swiglu_rows8(qx, qw, off, torch.tensor([1, 4, -5], dtype=torch.int32, device=cuda))
+    v = rows8.dequantize_rows(act)
+    assert v[0].abs().max() > 0 and (v[1:] == 0).all()
+
+
+def test_product_refusals(cuda):
+    a, b = rows8.quantize_rows(_randn((8, 64), 1).to(cuda)), rows8.quantize_rows(_randn((2, 32, 64), 2).to(cuda))
+    off = torch.tensor([0, 4, 8], dtype=torch.int32, device=cuda)
+    with pytest.raises(AssertionError, match="e4m3 for a product"):
+        rows8.group_gemm_nt_rows8(rows8.quantize_rows(_randn((8, 64), 1).to(cuda), "int8"), b, off)
+    with pytest.raises(AssertionError, match="stand for"):
+        rows8.group_gemm_nt_rows8(rows8.quantize_rows(_randn((8, 64), 1, F16).to(cuda)), b, off)
+    with pytest.raises(AssertionError, match="disagree on K"):
+        rows8.group_gemm_nt_rows8(rows8.quantize_rows(_randn((8, 48), 1).to(cuda)), b, off)
+    with pytest.raises(AssertionError, match="offsets"):
+        rows8.group_gemm_nt_rows8(a, b, off[:2])
+    with pytest.raises(ValueError, match="unsupported shape"):
+        rows8.group_gemm_nt_rows8(rows8.quantize_rows(_randn((8, 40), 1).to(cuda)),
+                                  rows8.quantize_rows(_randn((2, 32, 40), 2).to(cuda)), off)
+    with pytest.raises(ValueError, match="unsupported shape"):
+        rows8.group_gemm_nt_rows8(a, rows8.quantize_rows(_randn((2, 12, 64), 2).to(cuda)), off)
+    empty = rows8.quantize_rows(torch.empty((0, 64), dtype=BF, device=cuda))
+    assert rows8.group_gemm_nt_rows8(empty, b, torch.zeros(3, dtype=torch.int32, device=cuda)).shape == (0, 32)
+
+
+# ---------------------------------------------------------------------------
+# The serving layer
+# ---------------------------------------------------------------------------
+
+
+def _layer_oracle(hidden, w, phys, experts8, eps):
+    """(out, tolerance) of the 8-bit layer in 64 bits, from the weights' 8-bit values.
+
+    The kernel's activations, before they are rounded to 8 bits, lie within
+    `slack` of the exact ones (products to 2^-11 of the largest of each 64,
+    the sigmoid to 2^-17).  Rounding is monotonic, so each one's 8-bit value lies
+    between those of act - slack and act + slack at the block's power of two:
+    where these agree it is exact, where a border lies between them it may be
+    either, off by at most their distance (a block whose power of two itself may
+    differ: both powers are tried).  fc2 carries these distances on, adds its
+    own 2^-11, and rounds each row once; the rows' sum is rounded once more.
+    """
+    C = experts8.down.shape[0]
+    T, K = phys.shape
+    x, _ = O.quantize(hidden, "e4m3")
+    H = hidden.shape[1]
+    out, tol = np.zeros((T, H)), np.zeros((T, H))
+
+    def rounded(v, e):
+        unit = np.repeat(2.0 ** e.astype(np.float64), 32, axis=1)[:, : v.shape[1]]
+        y = np.clip(v / unit, -448, 448)
+        _, k = np.frexp(y)
+        step = 2.0 ** np.maximum(k - 4, -9)
+        return np.rint(y / step) * step * unit
+
+    for c in range(C):
+        at = np.argwhere(phys == c)
+        if not len(at):
+            continue
+        up = O.values(experts8.gate_up.codes[c].cpu(), experts8.gate_up.scales[c].cpu())
+        down = O.values(experts8.down.codes[c].cpu(), experts8.down.scales[c].cpu())
+        I = down.shape[1]
+        one = np.array([0, len(at)])
+        gu, big = O.grouped_nt(x[at[:, 0]], up[None], one)
+        g, u = gu[:, :I], gu[:, I:]
+        wr = w.double().numpy()[at[:, 0], at[:, 1]][:, None]
+        act = g / (1 + np.exp(-g)) * u * wr
+        # |d silu / dg| <= 1.1
+        slack = wr * (1.1 * big[:, :I] * np.abs(u) + np.abs(g) * big[:, I:]) * 2.0**-11 + np.abs(act) * 2.0**-17
+        e = O.block_exponents(act, "e4m3")
+        held = rounded(act, e)
+        far = np.zeros_like(act)
+        for e2 in {"low": O.block_exponents(np.maximum(np.abs(act) - slack, 0), "e4m3"),
+                   "high": O.block_exponents(np.abs(act) + slack, "e4m3")}.values():
+            for v in (act - slack, act + slack):
+                far = np.maximum(far, np.abs(rounded(v, e2) - held))
+        y, big2 = O.grouped_nt(held, down[None], one)
+        off = far @ np.abs(down).T + big2 * 2.0**-11
+        np.add.at(out, at[:, 0], y)
+        np.add.at(tol, at[:, 0], off + (np.abs(y) + off) * eps / 2)
+    return out, tol + (np.abs(out) + tol) * eps / 2
+
+
+@pytest.mark.parametrize("T", [1, 5, 64, 700])
+@pytest.mark.parametrize("dtype", [BF, F16])
+def test_layer_over_8_bit_weights(cuda, T, dtype):
+    H, I, E, C, K, S = 272, 144, 12, 17, 3, 4
+    g = torch.Generator().manual_seed(T)
+    hidden = _randn((T, H), T, dtype)
+    sel = torch.stack([torch.randperm(E, generator=g)[:K] for _ in range(T)])
+    w = torch.softmax(torch.randn((T, K), generator=g), -1).to(dtype)
+    src = torch.randint(0, S, (T,), generator=g)
+    e, s = torch.arange(E), torch.arange(S).unsqueeze(1)
+    mapping = torch.where((e < C - E) & (s % 2 == 1), E + e, e).contiguous()
+    q = rows8.Experts8.quantize(_randn((C, 2 * I, H), 1, dtype, 0.1).to(cuda), _randn((C, H, I), 2, dtype, 0.1).to(cuda))
+    print(f"layer rows8 T={T} {dtype}", flush=True)
+    seen = []
+    got = placemoe_amd.expert_layer_rows8(hidden.to(cuda), w.to(cuda), sel.to(cuda), q, mapping=mapping.to(cuda),
+                                          sources=src.to(cuda), recorder=lambda c: seen.append(c.clone()))
+    phys = moe_oracle.map_logical_to_physical(mapping.numpy(), src.numpy(), sel.numpy())
+    exact, tol = _layer_oracle(hidden, w, np.asarray(phys), q, torch.finfo(dtype).eps)
+    assert int(seen[0].sum()) == T * K
+    off = np.abs(got.double().cpu().numpy() - exact)
+    assert (off <= tol * 1.0001 + SUBNORMAL[dtype]).all(), (off - tol).max()
+    # the tolerance itself stays small beside the outputs
+    assert np.linalg.norm(tol) <= 0.1 * np.linalg.norm(exact), np.linalg.norm(tol) / np.linalg.norm(exact)
+    assert_bf16_close(got, torch.from_numpy(exact), name="out")
+
+
+def test_layer_refusals_and_edges(cuda):
+    H, I, C = 64, 32, 4
+    gate_up, down = _randn((C, 2 * I, H), 1).to(cuda), _randn((C, H, I), 2).to(cuda)
+    q = rows8.Experts8.quantize(gate_up, down)
+    x, w = _randn((5, H), 3).to(cuda), torch.ones((5, 1), dtype=BF, device=cuda)
+    sel = torch.zeros((5, 1), dtype=torch.int64, device=cuda)
+    assert placemoe_amd.expert_layer_rows8(x, w, sel, q).shape == (5, H)
+    assert placemoe_amd.expert_layer_rows8(x[:0], w[:0], sel[:0], q).shape == (0, H)
+    with pytest.raises(ValueError, match="no backward"):
+        placemoe_amd.expert_layer_rows8(x.clone().requires_grad_(), w, sel, q)
+    with torch.no_grad():
+        placemoe_amd.expert_layer_rows8(x.clone().requires_grad_(), w, sel, q)
+    with pytest.raises(AssertionError):
+        placemoe_amd.expert_layer_rows8(x.to(F16), w.to(F16), sel, q)
+    with pytest.raises(AssertionError):
+        placemoe_amd.expert_layer_rows8(x, w, sel, (gate_up, down))
+    with pytest.raises(AssertionError):
+        placemoe_amd.expert_layer_rows8(x[:, :32].contiguous(), w, sel, q)
+    with pytest.raises(AssertionError):
+        rows8.Experts8.quantize(gate_up, down[:, :32].contiguous())
+    bad = rows8.Experts8.quantize(_randn((C, 48, H), 1).to(cuda), _randn((C, H, 24), 2).to(cuda))
+    with pytest.raises(ValueError, match="multiples of 16"):
+        placemoe_amd.expert_layer_rows8(x, w, sel, bad)
+    placemoe_amd.expert_layer_rows8(x, w, sel + 99, q)
+    with pytest.raises(ValueError, match="expert id outside"):
+        experts.check_pending_routes(block=True)
+
+
+def test_layer_on_another_stream_and_in_a_graph(cuda):
+    wl = make_workload("qwen3", device=cuda, tokens=24)
+    q = rows8.Experts8.quantize(wl.fc1, wl.fc2)
+
+    def step():
+        return placemoe_amd.expert_layer_rows8(wl.hidden, wl.routing_weights, wl.selected, q, mapping=wl.mapping, sources=wl.sources)
+
+    want = step()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = step()
+    torch.cuda.current_stream().wait_stream(side)
+    assert_exact(got, want, "side stream")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for k in range(3):
+        wl.hidden.copy_(_randn(tuple(wl.hidden.shape), 50 + k).to(cuda))
+        graph.replay()
+        eager = step()
+        torch.cuda.synchronize()
+        assert_exact(out, eager, f"replay {k}")
+
+
+# ---------------------------------------------------------------------------
+# Checkpointed training layer
+# ---------------------------------------------------------------------------
+
+
+def _grads(wl, cuda, split, **kw):
+    leaf = lambda t: t.detach().clone().requires_grad_()  # noqa: E731
+    x, w = leaf(wl.hidden), leaf(wl.routing_weights)
+    if split:
+        weights = dict(fc1_1_weight=leaf(wl.fc1[:, :wl.I]), fc1_2_weight=leaf(wl.fc1[:, wl.I:]))
+        weights = {k: v.detach().contiguous().requires_grad_() for k, v in weights.items()}
+    else:
+        weights = dict(fc1_1_2_weight=leaf(wl.fc1))
+    down = leaf(wl.fc2)
+    out = experts.expert_layer(x, w, wl.selected, down, mapping=wl.mapping, sources=wl.sources, **weights, **kw)
+    out.backward(_randn(tuple(out.shape), 77).to(cuda))
+    fc1 = torch.cat([weights["fc1_1_weight"].grad, weights["fc1_2_weight"].grad], 1) if split else weights["fc1_1_2_weight"].grad
+    return out.detach(), {"dx": x.grad, "dw": w.grad, "d_fc1": fc1, "d_fc2": down.grad}
+
+
+@pytest.mark.parametrize("split", [False, True])
+@pytest.mark.parametrize("weighted", [False, True])
+@pytest.mark.parametrize("name,tokens", [("toy", 300), ("dsv3", 200), ("qwen3", 40)])
+def test_checkpointed_layer(cuda, name, tokens, weighted, split):
+    """The output is the uncheckpointed one bit for bit.  The gradients are the
+    formula's at the 8-bit hidden states and gate/up rows, to the bf16 bar (their products
+    run on bf16 operands, rounded between the steps); those of int8, whose
+    roundings are four times smaller, come near the uncheckpointed ones."""
+    wl = make_workload(name, device=cuda, tokens=tokens, **({"num_slots": 4} if name == "dsv3" else {}))
+    print(f"checkpointed {name} weighted={weighted} split={split}", flush=True)
+    plain, ref = _grads(wl, cuda, split, weighted_input=weighted)
+    for fmt in ("e4m3", "int8"):
+        out, got = _grads(wl, cuda, split, weighted_input=weighted, activation_checkpoint=fmt)
+        assert_exact(out, plain, f"{fmt} output")
+        want = _checkpointed_oracle(wl, fmt, cuda)
+        for k in got:
+            assert_bf16_close(got[k], want[k], name=f"{fmt} {k}")
+        for k in ("dx", "dw", "d_fc1", "d_fc2"):
+            err = ((got[k].float() - ref[k].float()).norm() / ref[k].float().norm()).item()
+            # a value is off by at most 2^-4 of itself (e4m3); three such factors meet in dx and dw
+            assert err <= (3 * 2.0**-4 if fmt == "e4m3" else 0.04), (fmt, k, err)
+
+
+def _checkpointed_oracle(wl, fmt, cuda):
+    """The gradients in 64 bits, from what 8 bits hold of the hidden states and of the layer's own gate/up rows."""
+    T, K, H, I, C = wl.T, wl.K, wl.H, wl.I, wl.C
+    r = kernels.route(wl.selected, C, mapping=wl.mapping, sources=wl.sources)
+    xp, row_src, _ = kernels.moe_scatter_src(wl.hidden, r.pos, wl.routing_weights)
+    gu, _ = kernels.gemm_fc1_swiglu(xp, wl.fc1, wl.fc1.view(-1)[I * H:], 2 * I * H, r.offsets, C, I)
+    back = lambda t: rows8.dequantize_rows(rows8.quantize_rows(t, fmt)).double()  # noqa: E731
+    gu8, x8 = back(gu), back(wl.hidden)
+    g, u = gu8[:, :I], gu8[:, I:]
+    src = row_src.long()
+    w = wl.routing_weights.double().reshape(-1)[src].unsqueeze(1)
+    dy = _randn((T, H), 77).to(cuda).double()[src // K]
+    sig = torch.sigmoid(g)
+    s = g * sig
+    off = r.offsets.tolist()
+    d_act = torch.cat([dy[off[c]:off[c + 1]] @ wl.fc2[c].double() for c in range(C)])
+    da = d_act * w
+    dg1 = torch.cat([da * u * (sig + s * (1 - sig)), da * s], 1)
+    act_w, xr = w * s * u, x8[src // K]
+    rows = [slice(off[c], off[c + 1]) for c in range(C)]
+    dw = torch.empty(T * K, dtype=torch.float64, device=cuda)
+    dw[src] = (d_act * s * u).sum(1)
+    dx = torch.zeros((T, H), dtype=torch.float64, device=cuda)
+    dx.index_add_(0, src // K, torch.cat([dg1[q] @ wl.fc1[c].double() for c, q in enumerate(rows)]))
+    return {"dx": dx, "dw": dw.view(T, K), "d_fc1": torch.stack([dg1[q].t() @ xr[q] for q in rows]),
+            "d_fc2": torch.stack([dy[q].t() @ act_w[q] for q in rows])}
+
+
+def test_checkpoint_keeps_less(cuda):
+    wl = make_workload("qwen3", device=cuda, tokens=512)
+
+    def kept(**kw):
+        x = wl.hidden.clone().requires_grad_()
+        total = []
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: (total.append(t), t)[1], lambda t: t):
+            experts.expert_layer(x, wl.routing_weights, wl.selected, wl.fc2, fc1_1_2_weight=wl.fc1, mapping=wl.mapping,
+                                 sources=wl.sources, **kw)
+        weights = {wl.fc1.data_ptr(), wl.fc2.data_ptr()}
+        seen = {t.data_ptr(): t.numel() * t.element_size() for t in total if t.data_ptr() not in weights}
+        seen.pop(wl.fc1.data_ptr() + wl.I * wl.H * 2, None)
+        return sum(seen.values())
+
+    A, H, I = wl.T * wl.K, wl.H, wl.I
+    assert kept() >= A * (4 * H + 6 * I)
+    assert kept(activation_checkpoint="e4m3") <= 1.1 * (wl.T * H + 2 * A * I) + 64 * A
+
+
+def test_checkpoint_through_the_public_op(cuda):
+    wl = make_workload("toy", device=cuda, tokens=64)
+    fc1, fc2 = wl.fc1[:8].contiguous(), wl.fc2[:8].contiguous()
+
+    def step(fmt):
+        x, a, b = wl.hidden.clone().requires_grad_(), fc1.clone().requires_grad_(), fc2.clone().requires_grad_()
+        prev = placemoe_amd.set_activation_checkpoint(fmt)
+        try:
+            out = placemoe_amd.hip_fused_moe_forward(8, wl.routing_weights, wl.selected, x, None, None, b, a)
+        finally:
+            placemoe_amd.set_activation_checkpoint(prev)
+        out.sum().backward()
+        return out.detach(), x.grad, a.grad, b.grad
+
+    plain, kept = step(None), step("int8")
+    assert_exact(kept[0], plain[0], "output")
+    for k, (a, b) in enumerate(zip(kept[1:], plain[1:])):
+        assert not torch.equal(a, b), "the checkpoint was not used"
+        assert ((a.float() - b.float()).norm() / b.float().norm()).item() <= 0.04, k
+
+
+def test_checkpointed_backward_in_a_graph(cuda):
+    wl = make_workload("qwen3", device=cuda, tokens=32)
+    dout = _randn((wl.T, wl.H), 5).to(cuda)
+    x, x_eager = (wl.hidden.clone().requires_grad_() for _ in range(2))  # the captured graph has a leaf of its own
+
+    def step(x):
+        out = experts.expert_layer(x, wl.routing_weights, wl.selected, wl.fc2, fc1_1_2_weight=wl.fc1, mapping=wl.mapping,
+                                   sources=wl.sources, activation_checkpoint="e4m3")
+        return torch.autograd.grad(out, x, dout)[0]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(x_eager)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        grad = step(x)
+    for k in range(3):
+        with torch.no_grad():
+            x.copy_(_randn(tuple(x.shape), 60 + k).to(cuda))
+            x_eager.copy_(x)
+        graph.replay()
+        eager = step(x_eager)
+        torch.cuda.synchronize()
+        assert_exact(grad, eager, f"replay {k}")

@@ -1,0 +1,130 @@
+"""Rows in 8 bits without a GPU: the oracle against the format's own float
+type, the C ABI's refusals, and the wrappers' checks (all before any launch)."""
+
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+import placemoe_amd
+from oracle import rows8_oracle as O
+from placemoe_amd import _capi, experts, rows8
+
+BF = torch.bfloat16
+
+
+@pytest.mark.parametrize("dtype", [BF, torch.float16])
+def test_oracle_rounds_like_the_e4m3_type(dtype):
+    g = torch.Generator().manual_seed(3)
+    x = (torch.randn((40, 100), generator=g) * torch.logspace(-6, 4, 40).unsqueeze(1)).to(dtype)
+    x[3] = 0
+    v, scales = O.quantize(x, "e4m3")
+    e = scales.permute(1, 0, 2).reshape(40, -1).to(torch.int64) - 127
+    unit = torch.exp2(e.double()).repeat_interleave(32, 1)[:, :100]
+    want = (x.double() / unit).float().to(torch.float8_e4m3fn).double() * unit
+    assert np.array_equal(v, want.numpy())
+    # the smallest power: half of it would not hold the block's largest value
+    most = torch.nn.functional.pad(x.double().abs(), (0, 28)).view(40, 4, 32).amax(-1)
+    u = torch.exp2(e[:, :4].double())
+    assert (most <= 448 * u).all() and ((most > 224 * u) | (most == 0)).all()
+
+
+def test_oracle_int8_is_within_half_a_step():
+    x = torch.randn((9, 70), generator=torch.Generator().manual_seed(4)).to(BF)
+    v, scales = O.quantize(x, "int8")
+    e = scales.permute(1, 0, 2).reshape(9, -1).to(torch.int64) - 127
+    unit = torch.exp2(e.double()).repeat_interleave(32, 1)[:, :70].numpy()
+    assert (np.abs(v - x.double().numpy()) <= unit / 2).all() and (np.abs(v) <= 127 * unit).all()
+
+
+P = ctypes.c_void_p(256)
+ARG, SHAPE, OK = _capi.PMX_ERR_ARG, _capi.PMX_ERR_SHAPE, _capi.PMX_OK
+
+
+@pytest.mark.parametrize("suffix", ["", "_f16"])
+def test_c_abi_refusals(suffix):
+    lib = _capi.load()
+    quantize, routed = getattr(lib, "pmx_rows8_quantize" + suffix), getattr(lib, "pmx_rows8_quantize_routed" + suffix)
+    dequantize, swiglu = getattr(lib, "pmx_rows8_dequantize" + suffix), getattr(lib, "pmx_rows8_swiglu_bwd" + suffix)
+    nt, fc1 = getattr(lib, "pmx_rows8_group_gemm_nt" + suffix), getattr(lib, "pmx_rows8_gemm_fc1_swiglu" + suffix)
+    assert quantize(P, 8, 0, 1, 4, 8, 2, P, P, None) == ARG  # no such format
+    assert quantize(P, 7, 0, 1, 4, 8, 0, P, P, None) == ARG  # rows overlap
+    assert quantize(P, 8, 0, 1, -1, 8, 0, P, P, None) == ARG
+    assert quantize(None, 8, 0, 1, 4, 8, 0, P, P, None) == ARG
+    assert quantize(None, 8, 0, 1, 0, 8, 0, None, None, None) == OK
+    assert quantize(P, 1 << 40, 0, 1 << 20, 1 << 20, 8, 0, P, P, None) == SHAPE
+    assert routed(P, P, P, 1 << 30, 4, 8, P, P, P, P, None) == SHAPE
+    assert routed(P, None, P, 4, 2, 8, P, P, P, P, None) == ARG
+    assert routed(P, P, P, 4, 0, 8, P, P, P, P, None) == ARG
+    assert dequantize(P, P, P, 4, 0, 8, 0, P, None) == ARG  # positions, but none per row
+    assert dequantize(P, P, P, 1 << 30, 4, 8, 0, P, None) == SHAPE
+    assert dequantize(P, P, None, 4, 0, 8, 5, P, None) == ARG
+    assert dequantize(None, None, None, 0, 0, 8, 0, None, None) == OK
+    assert swiglu(P, P, P, P, None, 4, 8, 4, 0, P, P, P, None) == ARG  # dw without row_src
+    assert swiglu(P, P, P, P, P, 4, 8, 4, 0, P, P, None, None) == ARG
+    assert swiglu(None, P, P, P, P, 4, 8, 4, 0, P, P, P, None) == ARG
+    assert swiglu(P, P, P, P, P, 1 << 40, 1 << 30, 4, 0, P, P, P, None) == SHAPE
+    assert nt(P, P, P, P, P, 0, 8, 8, 16, P, None) == ARG
+    assert nt(P, P, P, P, P, 4096, 8, 8, 16, P, None) == ARG
+    assert nt(P, P, P, P, P, 4, 8, 8, 24, P, None) == SHAPE  # K
+    assert nt(P, P, P, P, P, 4, 8, 12, 16, P, None) == SHAPE  # N
+    assert nt(P, P, P, P, P, 4, 8, 1 << 20, 1 << 12, P, None) == SHAPE  # 4 GiB per group
+    assert nt(P, P, P, P, P, 4, 1 << 31, 8, 16, P, None) == SHAPE
+    assert nt(ctypes.c_void_p(8), P, P, P, P, 4, 8, 8, 16, P, None) == SHAPE  # alignment
+    assert nt(None, P, P, P, P, 4, 8, 8, 16, P, None) == ARG
+    assert nt(None, None, None, None, None, 4, 0, 8, 16, None, None) == OK
+    assert fc1(P, P, 8, None, P, P, P, 4, 16, 32, 32, P, P, P, None) == ARG  # rows without a map
+    assert fc1(P, P, 8, P, P, P, P, 4, 16, 32, 24, P, P, P, None) == SHAPE  # I
+    assert fc1(P, P, 1 << 20, P, P, P, P, 4, 16, 1 << 11, 32, P, P, P, None) == SHAPE  # 2 GiB of tokens
+    assert fc1(P, P, 8, P, P, P, P, 4, 16, 32, 0, P, P, P, None) == ARG
+
+
+def _rows(shape, fmt="e4m3", dtype=BF):
+    return rows8.Rows8(torch.zeros(shape, dtype=rows8.FORMATS[fmt]),
+                       torch.full(rows8.scales_shape(shape), 127, dtype=torch.uint8), dtype)
+
+
+def test_wrappers_refuse_host_tensors():
+    i32 = torch.zeros(3, dtype=torch.int32)
+    for call in (
+        lambda: rows8.quantize_rows(torch.zeros((2, 8), dtype=BF)),
+        lambda: rows8.dequantize_rows(_rows((2, 8))),
+        lambda: rows8.swiglu_bwd_rows8(torch.zeros((2, 8), dtype=BF), _rows((2, 16))),
+        lambda: rows8.group_gemm_nt_rows8(_rows((2, 16)), _rows((2, 8, 16)), i32),
+        lambda: rows8.gemm_fc1_swiglu_rows8(_rows((2, 16)), _rows((2, 32, 16)), i32),
+    ):
+        with pytest.raises(AssertionError, match="GPU tensors"):
+            call()
+
+
+def test_operand_checks():
+    assert rows8._rows8("q", _rows((3, 4, 600)), 3) == BF
+    assert rows8.scales_shape((4, 600)) == (2, 4, 16)
+    q = _rows((4, 600))
+    for bad, match in (
+        (q.codes, "must be Rows8"),
+        (rows8.Rows8(q.codes.float(), q.scales, BF), "codes must be"),
+        (rows8.Rows8(q.codes, q.scales, torch.float32), "stand for"),
+        (rows8.Rows8(q.codes, q.scales.int(), BF), "uint8"),
+        (rows8.Rows8(q.codes, q.scales[:1], BF), "scales must be"),
+        (_rows((3, 4, 600)), "2 dimensions"),
+        (rows8.Rows8(q.codes.t().contiguous().t(), q.scales, BF), "contiguous"),
+    ):
+        with pytest.raises(AssertionError, match=match):
+            rows8._rows8("q", bad, 2)
+    with pytest.raises(AssertionError, match="e4m3 for a product"):
+        rows8._e4m3("q", _rows((4, 600), "int8"), 2)
+    with pytest.raises(ValueError, match="8-bit format"):
+        rows8._format("e5m2")
+
+
+def test_checkpoint_settings_are_checked():
+    with pytest.raises(ValueError, match="activation checkpoint"):
+        placemoe_amd.set_activation_checkpoint("fp8")
+    assert placemoe_amd.set_activation_checkpoint("int8") is None
+    assert placemoe_amd.set_activation_checkpoint(None) == "int8"
+    z = torch.zeros((2, 16), dtype=BF)
+    with pytest.raises(ValueError, match="activation checkpoint"):
+        experts.expert_layer(z, z[:, :1], torch.zeros((2, 1), dtype=torch.int64), z, fc1_1_2_weight=z,
+                             activation_checkpoint="bf16")
