@@ -1,26 +1,32 @@
 // Grouped GEMM over ragged row groups, both operands rows in 8 bits (rows8.h,
-// e4m3):
+// e4m3), sums in fp32:
 //   NT   C[rows of g] = A[rows of g] B[g]^T                          (bf16 or fp16)
 //   FC1  (gate | up) = A[rows of g] B[g]^T, act = silu(gate) * up * row_w, written
 //        as rows in 8 bits again, ready to be fc2's A
-// with fp32 accumulation on v_mfma_scale_f32_32x32x64_f8f6f4, which takes the
-// two operands' powers of two per 32 columns with the codes: no value is ever
-// scaled outside of the matrix core.  (Within one such instruction the 64
-// products are added to about 2^-12 of the largest one, as measured: 1.3e-5 of
-// a random sum, a hundredth of the bf16 result's half step.  Sums over K are
-// fp32.)  A row map lets A's rows come from anywhere: fc1 reads each token's
-// row where it lies, once per copy it is routed to, and the permuted copy of
-// the hidden states is never made.
+// A row map lets A's rows come from anywhere: fc1 reads each token's row where
+// it lies, once per copy it is routed to, and the permuted copy of the hidden
+// states is never made.
 //
-// Bound: MFMA from some hundred rows per group on (twice the rate of bf16 at
-// half the bytes), the weights' bytes below.
+// NT multiplies on v_mfma_scale_f32_32x32x64_f8f6f4, which takes the two
+// operands' powers of two per 32 columns with the codes, at twice the rate of
+// bf16.  gfx950's 8-bit matrix instructions (all of them) add products to about
+// 2^-13 of the largest one: 1.5e-5 of a random sum, a hundredth of the half
+// step to which a bf16 result is rounded.  FC1's results are rounded to 8
+// bits, and there an error of 1e-5 moves one code in some thousands across a
+// border, by a whole step: the layer's output was 0.0031 off its definition in
+// 64 bits, against 0.0024 with exact products (fc2's bf16 rows and their sum
+// account for that).  So FC1 converts the codes, with their powers of two, to
+// bf16 in registers (v_cvt_scalef32_pk_bf16_fp8, exact) and multiplies on
+// v_mfma_f32_32x32x16_bf16, whose sums are good to fp32; it reads as few bytes.
+//
+// Bound: MFMA from some hundred rows per group on, the weights' bytes below.
 //
 // Tiles of BM x BN, K in steps of 128 through a ring of NST stages filled by
-// buffer->LDS loads NST - 1 K-tiles ahead; 128-byte rows with 16-byte chunk c
-// at c ^ ((row >> 1) & 7), as in the bf16 kernels, whose K-tiles are as many
-// bytes.  The exponents of four K-tiles are 16 bytes per row (rows8.h): they
-// come with the first of the four, 64 rows per load, into a ring of their
-// own, and each wave picks a K-tile's word per row from there.
+// buffer->LDS loads; 128-byte rows with 16-byte chunk c at c ^ ((row >> 1) & 7),
+// as in the bf16 kernels, whose K-tiles are as many bytes.  The exponents of
+// four K-tiles are 16 bytes per row (rows8.h): they come with the first of the
+// four, 64 rows per load, into a ring of their own, and each wave picks a
+// K-tile's word per row from there.
 
 #include <atomic>
 
@@ -32,6 +38,9 @@ namespace {
 typedef int32_t i32x8_t __attribute__((ext_vector_type(8)));
 typedef int32_t i32x4_t __attribute__((ext_vector_type(4)));
 
+#ifndef PMX_R8_LOAD_GROUPS
+#define PMX_R8_LOAD_GROUPS 99
+#endif
 constexpr int kMaxGroups = 2048;  // groups (the m-tile prefix in LDS)
 constexpr int KT = 128;           // depth of a K-tile
 constexpr int kScaleTiles = kScaleGroup / KT;
@@ -136,6 +145,7 @@ __device__ __forceinline__ void setup(const Params8& P, const Place& at, Loads<C
   }
 }
 
+// NT: operands of a 64-deep half K-tile.
 template <class CF>
 struct Frags8 {
   i32x8_t a[CF::FM], b[CF::FN];
@@ -143,8 +153,23 @@ struct Frags8 {
   int32_t sa[(CF::FM + 1) / 2], sb[(CF::FN + 1) / 2];
 };
 
-// The I-th fragment read of a k-step, in the order its (m-major) MFMAs use
-// them: A0, B0 .. B(FN-1), A1 .. ; ids as in the reads (A first, then B).
+// FC1: codes of a 32-deep quarter (16 per lane), the K-tile's exponents of the
+// lane's rows (byte q: quarter q), and the values of half a quarter.
+template <class CF>
+struct Codes8 {
+  i32x4_t v[CF::FM + CF::FN];
+};
+template <class CF>
+struct Words8 {
+  uint32_t v[CF::FM + CF::FN];
+};
+template <class CF>
+struct Values8 {
+  bf16x8_t v[CF::FM + CF::FN];
+};
+
+// The I-th fragment in the order the (m-major) MFMAs use them: A0, B0 ..
+// B(FN-1), A1 .. ; ids count A's first, then B's.
 template <class CF>
 constexpr int order8(int i) { return i == 0 ? 0 : i <= CF::FN ? CF::FM + i - 1 : i - CF::FN; }
 
@@ -304,7 +329,7 @@ __global__ __launch_bounds__(CF::NTH, CF::NW * CF::BPC / 4) void rows8_grouped_g
     at.row_end = uni(offset(lo + 1));
   };
 
-  // Issue cursor: NST - 1 K-tiles in front of the one being multiplied.
+  // Issue cursor, running ahead of the K-tile being multiplied.
   Loads<CF> ld;
   int64_t i_tile = first;
   int32_t i_kt = 0, i_stage = 0, i_slot = 0;
@@ -358,71 +383,31 @@ __global__ __launch_bounds__(CF::NTH, CF::NW * CF::BPC / 4) void rows8_grouped_g
       for (int q = 0; q < L; ++q) ld.off[q] = kOOB;
     }
   };
+  // K-tiles in flight before the first is multiplied: FC1 refills a stage once its
+  // last quarter is in registers, NT from the next K-tile on.
+  constexpr int AHEAD = KIND == FC18 ? CF::NST : CF::NST - 1;
 #pragma unroll
-  for (int s = 0; s < CF::NST - 1; ++s) {
+  for (int s = 0; s < AHEAD; ++s) {
     issue_scales();
     static_for<0, L>(issue);
     advance_issue();
   }
+  wait_loads<(AHEAD - 1) * L>();
+  block_barrier();
 
-  // Fragments: in half ks of the K-tile lane l holds row l%32, columns 16 h ..
-  // + 15 and 32 + 16 h .. + 15 of the half's 64 (h = l/32), and the exponent
-  // of its block h.
   const int h = lane >> 5, r32 = lane & 31;
-  int32_t at[2][2];
-#pragma unroll
-  for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-    for (int e = 0; e < 2; ++e) at[ks][e] = r32 * KT + (((ks * 4 + e * 2 + h) ^ kc_swz(r32)) << 4);
-  const uint32_t pick = 0x06040200u + 0x01010101u * h;  // bytes h and 2 + h of two words
   const int32_t arow = wm * CF::FM * 32, brow = wn * CF::FN * 32;
-  auto read = [&](auto jj, auto kk, const char* stage, const char* slot, const Frags8<CF>& fm, Frags8<CF>& fr)
-      __attribute__((always_inline)) {
-    constexpr int J = decltype(jj)::value, ks = decltype(kk)::value;
-    constexpr bool is_a = J < CF::FM;
-    const int row = is_a ? arow + J * 32 : brow + (J - CF::FM) * 32;
-    const char* p = stage + (is_a ? 0 : CF::A_BYTES) + row * KT;
-    const i32x4_t lo = *reinterpret_cast<const i32x4_t*>(p + at[ks][0]);
-    const i32x4_t hi = *reinterpret_cast<const i32x4_t*>(p + at[ks][1]);
-    const i32x8_t v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-    if constexpr (is_a) fr.a[J] = v;
-    else fr.b[J - CF::FM] = v;
-    constexpr int F = is_a ? J : J - CF::FM, last = (is_a ? CF::FM : CF::FN) - 1;
-    if constexpr (F % 2 == 0) {
-      int32_t& out = is_a ? fr.sa[F / 2] : fr.sb[F / 2];
-      if constexpr (ks == 0) {
-        const char* w = slot + (is_a ? 0 : CF::SA * 1024) + (row + r32) * kScaleBytes;
-        const uint32_t w0 = *reinterpret_cast<const uint32_t*>(w);
-        const uint32_t w1 = F < last ? *reinterpret_cast<const uint32_t*>(w + 32 * kScaleBytes) : w0;
-        out = (int32_t)__builtin_amdgcn_perm(w1, w0, pick);
-      } else {
-        out = is_a ? fm.sa[F / 2] : fm.sb[F / 2];
-      }
-    }
+  // Fragment J's first row, within A's or B's rows of a stage, and its place there.
+  const auto row_of = [&](int J) __attribute__((always_inline)) { return J < CF::FM ? arow + J * 32 : brow + (J - CF::FM) * 32; };
+  const auto in_stage = [&](int J) __attribute__((always_inline)) { return (J < CF::FM ? 0 : CF::A_BYTES) + row_of(J) * KT; };
+  const auto in_slot = [&](int J) __attribute__((always_inline)) {
+    return (J < CF::FM ? 0 : CF::SA * 1024) + (row_of(J) + r32) * kScaleBytes;
   };
-
-  f32x16_t acc[CF::FM][CF::FN];
-  Frags8<CF> f0, f1;
   constexpr int NM = CF::FM * CF::FN, NR = CF::FM + CF::FN;
-  auto mfma = [&](auto xx, auto kk, auto zero, const Frags8<CF>& f) __attribute__((always_inline)) {
-    constexpr int x = decltype(xx)::value, m = x / CF::FN, n = x % CF::FN, ks = decltype(kk)::value;
-    acc[m][n] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(f.b[n], f.a[m], decltype(zero)::value ? f32x16_t{} : acc[m][n],
-                                                                0, 0, n % 2 * 2 + ks, f.sb[n / 2], m % 2 * 2 + ks, f.sa[m / 2]);
-  };
-  // The MFMAs of half `km` from `fm`, in NR groups: each reads one fragment of
-  // the other half into `fr` and (loads) issues its share of the loads of the
-  // K-tile NST - 1 ahead.
-  auto kstep = [&](auto zero, auto km, auto loads, const Frags8<CF>& fm, const char* stage, const char* slot, Frags8<CF>& fr)
-      __attribute__((always_inline)) {
-    if constexpr (decltype(loads)::value) issue_scales();
-    static_for<0, NR>([&](auto jj) __attribute__((always_inline)) {
-      constexpr int j = decltype(jj)::value;
-      if constexpr (decltype(loads)::value) static_for<j * L / NR, (j + 1) * L / NR>(issue);
-      read(Int<order8<CF>(j)>{}, Int<1 - decltype(km)::value>{}, stage, slot, fm, fr);
-      static_for<j * NM / NR, (j + 1) * NM / NR>([&](auto xx) __attribute__((always_inline)) { mfma(xx, km, zero, fm); });
-      __builtin_amdgcn_sched_barrier(0);
-    });
-  };
+  f32x16_t acc[CF::FM][CF::FN];
+  int c_stage = 0, c_slot = 0;
+  const auto next_stage = [&]() { c_stage = c_stage + 1 == CF::NST ? 0 : c_stage + 1; };
+  const auto next_slot = [&]() { c_slot = c_slot + 1 == CF::NST ? 0 : c_slot + 1; };
   // The end of a K-tile: the next one has landed (at most the loads of the
   // NST - 2 K-tiles issued after it are outstanding), and every wave has read
   // this one.
@@ -431,36 +416,174 @@ __global__ __launch_bounds__(CF::NTH, CF::NW * CF::BPC / 4) void rows8_grouped_g
     block_barrier();
   };
 
-  turn();
-  int c_stage = 0, c_slot = 0;
-  for (int64_t tile = first; tile < end; tile += step) {
-    // The tile's first K-tile: no MFMAs of this tile to read its first half behind.
-    {
-      const char* stage = lds + c_stage * CF::STAGE;
-      const char* slot = slots + c_slot * CF::SLOT;
-      static_for<0, NR>([&](auto j) __attribute__((always_inline)) {
-        read(Int<order8<CF>(decltype(j)::value)>{}, Int<0>{}, stage, slot, f0, f0);
+  if constexpr (KIND == NT8) {
+    // In half ks of the K-tile lane l holds row l%32, columns 16 h .. + 15 and
+    // 32 + 16 h .. + 15 of the half's 64 (h = l/32), and the exponent of its
+    // block h.
+    int32_t at[2][2];
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) at[ks][e] = r32 * KT + (((ks * 4 + e * 2 + h) ^ kc_swz(r32)) << 4);
+    const uint32_t pick = 0x06040200u + 0x01010101u * h;  // bytes h and 2 + h of two words
+    Frags8<CF> f0, f1;
+    auto read = [&](auto jj, auto kk, const char* stage, const char* slot, const Frags8<CF>& fm, Frags8<CF>& fr)
+        __attribute__((always_inline)) {
+      constexpr int J = decltype(jj)::value, ks = decltype(kk)::value;
+      constexpr bool is_a = J < CF::FM;
+      const char* p = stage + in_stage(J);
+      const i32x4_t lo = *reinterpret_cast<const i32x4_t*>(p + at[ks][0]);
+      const i32x4_t hi = *reinterpret_cast<const i32x4_t*>(p + at[ks][1]);
+      const i32x8_t v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+      if constexpr (is_a) fr.a[J] = v;
+      else fr.b[J - CF::FM] = v;
+      constexpr int F = is_a ? J : J - CF::FM, last = (is_a ? CF::FM : CF::FN) - 1;
+      if constexpr (F % 2 == 0) {
+        int32_t& out = is_a ? fr.sa[F / 2] : fr.sb[F / 2];
+        if constexpr (ks == 0) {
+          const char* w = slot + in_slot(J);
+          const uint32_t w0 = *reinterpret_cast<const uint32_t*>(w);
+          const uint32_t w1 = F < last ? *reinterpret_cast<const uint32_t*>(w + 32 * kScaleBytes) : w0;
+          out = (int32_t)__builtin_amdgcn_perm(w1, w0, pick);
+        } else {
+          out = is_a ? fm.sa[F / 2] : fm.sb[F / 2];
+        }
+      }
+    };
+    auto mfma = [&](auto xx, auto kk, auto zero, const Frags8<CF>& f) __attribute__((always_inline)) {
+      constexpr int x = decltype(xx)::value, m = x / CF::FN, n = x % CF::FN, ks = decltype(kk)::value;
+      acc[m][n] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
+          f.b[n], f.a[m], decltype(zero)::value ? f32x16_t{} : acc[m][n], 0, 0, n % 2 * 2 + ks, f.sb[n / 2], m % 2 * 2 + ks,
+          f.sa[m / 2]);
+    };
+    // The MFMAs of half `km` from `fm`, in NR groups: each reads one fragment of
+    // the other half into `fr` and (loads) issues its share of the loads of the
+    // K-tile NST - 1 ahead.
+    auto kstep = [&](auto zero, auto km, auto loads, const Frags8<CF>& fm, const char* stage, const char* slot, Frags8<CF>& fr)
+        __attribute__((always_inline)) {
+      if constexpr (decltype(loads)::value) issue_scales();
+      static_for<0, NR>([&](auto jj) __attribute__((always_inline)) {
+        constexpr int j = decltype(jj)::value, LG = PMX_R8_LOAD_GROUPS < NR ? PMX_R8_LOAD_GROUPS : NR;
+        if constexpr (decltype(loads)::value && j < LG) static_for<j * L / LG, (j + 1) * L / LG>(issue);
+        read(Int<order8<CF>(j)>{}, Int<1 - decltype(km)::value>{}, stage, slot, fm, fr);
+        static_for<j * NM / NR, (j + 1) * NM / NR>([&](auto xx) __attribute__((always_inline)) { mfma(xx, km, zero, fm); });
+        __builtin_amdgcn_sched_barrier(0);
       });
-      kstep(Int<1>{}, Int<0>{}, Int<1>{}, f0, stage, slot, f1);
-      advance_issue();
-      turn();
-      c_stage = c_stage + 1 == CF::NST ? 0 : c_stage + 1;
+    };
+
+    for (int64_t tile = first; tile < end; tile += step) {
+      // The tile's first K-tile: no MFMAs of this tile to read its first half behind.
+      {
+        const char* stage = lds + c_stage * CF::STAGE;
+        const char* slot = slots + c_slot * CF::SLOT;
+        static_for<0, NR>([&](auto j) __attribute__((always_inline)) {
+          read(Int<order8<CF>(decltype(j)::value)>{}, Int<0>{}, stage, slot, f0, f0);
+        });
+        kstep(Int<1>{}, Int<0>{}, Int<1>{}, f0, stage, slot, f1);
+        advance_issue();
+        turn();
+        next_stage();
+      }
+      for (int32_t kt = 1; kt < nk; ++kt) {
+        if (kt % kScaleTiles == 0) next_slot();
+        const char* stage = lds + c_stage * CF::STAGE;
+        const char* slot = slots + c_slot * CF::SLOT + kt % kScaleTiles * 4;
+        kstep(Int<0>{}, Int<1>{}, Int<1>{}, f1, stage, slot, f0);
+        kstep(Int<0>{}, Int<0>{}, Int<0>{}, f0, stage, slot, f1);
+        advance_issue();
+        turn();
+        next_stage();
+      }
+      static_for<0, NM>([&](auto x) __attribute__((always_inline)) { mfma(x, Int<1>{}, Int<0>{}, f1); });
+      next_slot();
+      Place place;
+      decode(tile, place);
+      epilogue<E, KIND, CF>(P, place, wm, wn, lane, acc);
     }
-    for (int32_t kt = 1; kt < nk; ++kt) {
-      if (kt % kScaleTiles == 0) c_slot = c_slot + 1 == CF::NST ? 0 : c_slot + 1;
+  } else {
+    // In quarter q of the K-tile lane l holds row l%32, columns 16 h .. + 15 of
+    // the quarter's 32: eight of them each for two bf16 MFMAs.
+    int32_t at[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) at[q] = r32 * KT + (((q * 2 + h) ^ kc_swz(r32)) << 4);
+    Codes8<CF> r0, r1;
+    Words8<CF> words, upcoming;
+    Values8<CF> c0, c1;
+    auto read = [&](auto jj, auto qq, const char* stage, const char* slot, Codes8<CF>& to, Words8<CF>& w)
+        __attribute__((always_inline)) {
+      constexpr int J = decltype(jj)::value, q = decltype(qq)::value;
+      to.v[J] = *reinterpret_cast<const i32x4_t*>(stage + in_stage(J) + at[q]);
+      if constexpr (q == 0) w.v[J] = *reinterpret_cast<const uint32_t*>(slot + in_slot(J));
+    };
+    // Two values, Y of the 4 * NR pairs of half s of quarter q; the conversion takes the exponent field alone.
+    auto convert = [&](auto yy, auto qq, auto ss, const Codes8<CF>& from, const Words8<CF>& w, Values8<CF>& to)
+        __attribute__((always_inline)) {
+      constexpr int J = order8<CF>(decltype(yy)::value / 4), pair = decltype(yy)::value % 4;
+      constexpr int q = decltype(qq)::value, s = decltype(ss)::value;
+      const float scale = __uint_as_float(q < 3 ? w.v[J] << (23 - 8 * q) : w.v[J] >> 1);
+      const bf16x2_t v =
+          __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((uint32_t)from.v[J][2 * s + pair / 2], scale, pair % 2 == 1);
+      to.v[J][2 * pair] = v[0];
+      to.v[J][2 * pair + 1] = v[1];
+    };
+    // The MFMAs of half s of a quarter from `now`; meanwhile the next half's
+    // values are converted, the codes after them read (s = 0) and the freed
+    // stage refilled (loads).
+    auto half = [&](auto zero, auto ss, const Values8<CF>& now, auto work) __attribute__((always_inline)) {
+      static_for<0, NM>([&](auto xx) __attribute__((always_inline)) {
+        constexpr int x = decltype(xx)::value, m = x / CF::FN, n = x % CF::FN;
+        acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(now.v[CF::FM + n], now.v[m],
+                                                            decltype(zero)::value ? f32x16_t{} : acc[m][n], 0, 0, 0);
+        work(xx);
+        __builtin_amdgcn_sched_barrier(0);
+      });
+    };
+    // Quarter q: its codes in `cur`, the first half's values in c0 when it
+    // begins.  q = 3 reads the next K-tile, the next tile's first one behind the
+    // tile's last (behind the block's last, zeros that nothing uses), and
+    // refills the stage that this one has left.
+    auto quarter = [&](auto zero, auto qq, const char* stage, const char* slot, const Codes8<CF>& cur, Codes8<CF>& next)
+        __attribute__((always_inline)) {
+      constexpr int q = decltype(qq)::value, NC = 4 * NR, qn = (q + 1) % 4;
+      Words8<CF>& w = q == 3 ? upcoming : words;
+      if constexpr (q == 3) issue_scales();
+      half(zero, Int<0>{}, c0, [&](auto xx) __attribute__((always_inline)) {
+        constexpr int x = decltype(xx)::value;
+        static_for<x * NR / NM, (x + 1) * NR / NM>(
+            [&](auto j) __attribute__((always_inline)) { read(Int<order8<CF>(decltype(j)::value)>{}, Int<qn>{}, stage, slot, next, w); });
+        if constexpr (q == 3) static_for<x * L / NM, (x + 1) * L / NM>(issue);
+        static_for<x * NC / NM, (x + 1) * NC / NM>(
+            [&](auto y) __attribute__((always_inline)) { convert(y, qq, Int<1>{}, cur, words, c1); });
+      });
+      half(Int<0>{}, Int<1>{}, c1, [&](auto xx) __attribute__((always_inline)) {
+        constexpr int x = decltype(xx)::value;
+        static_for<x * NC / NM, (x + 1) * NC / NM>(
+            [&](auto y) __attribute__((always_inline)) { convert(y, Int<qn>{}, Int<0>{}, next, w, c0); });
+      });
+      if constexpr (q == 3) words = upcoming;
+    };
+    auto ktile = [&](auto zero, int32_t kt) __attribute__((always_inline)) {
       const char* stage = lds + c_stage * CF::STAGE;
-      const char* slot = slots + c_slot * CF::SLOT + kt % kScaleTiles * 4;
-      kstep(Int<0>{}, Int<1>{}, Int<1>{}, f1, stage, slot, f0);
-      kstep(Int<0>{}, Int<0>{}, Int<0>{}, f0, stage, slot, f1);
-      advance_issue();
+      quarter(zero, Int<0>{}, stage, nullptr, r0, r1);
+      quarter(Int<0>{}, Int<1>{}, stage, nullptr, r1, r0);
+      quarter(Int<0>{}, Int<2>{}, stage, nullptr, r0, r1);
       turn();
-      c_stage = c_stage + 1 == CF::NST ? 0 : c_stage + 1;
+      next_stage();
+      const int32_t k4 = kt + 1 < nk ? (kt + 1) % kScaleTiles : 0;
+      if (k4 == 0) next_slot();
+      quarter(Int<0>{}, Int<3>{}, lds + c_stage * CF::STAGE, slots + c_slot * CF::SLOT + k4 * 4, r1, r0);
+      advance_issue();
+    };
+
+    static_for<0, NR>([&](auto j) __attribute__((always_inline)) { read(j, Int<0>{}, lds, slots, r0, words); });
+    static_for<0, 4 * NR>([&](auto y) __attribute__((always_inline)) { convert(y, Int<0>{}, Int<0>{}, r0, words, c0); });
+    for (int64_t tile = first; tile < end; tile += step) {
+      ktile(Int<1>{}, 0);
+      for (int32_t kt = 1; kt < nk; ++kt) ktile(Int<0>{}, kt);
+      Place place;
+      decode(tile, place);
+      epilogue<E, KIND, CF>(P, place, wm, wn, lane, acc);
     }
-    static_for<0, NM>([&](auto x) __attribute__((always_inline)) { mfma(x, Int<1>{}, Int<0>{}, f1); });
-    c_slot = c_slot + 1 == CF::NST ? 0 : c_slot + 1;
-    Place place;
-    decode(tile, place);
-    epilogue<E, KIND, CF>(P, place, wm, wn, lane, acc);
   }
   wait_loads<0>();
 }
