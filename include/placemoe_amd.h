@@ -513,7 +513,7 @@ int pmx_rows8_swiglu_bwd(const void* d_act, const void* codes, const void* scale
 
 /* C[rows of g] = A[rows of g] B[g]^T over 8-bit rows (e4m3), fp32 sums, C bf16
  * [M, N]; rows of g: offsets[g] .. offsets[g+1]-1 (offsets outside [0, M] are
- * clamped).  A: codes [M, K]; B: codes [G, N, K], each with its scales.  K a
+ * clamped; if they descend anywhere, nothing is written).  A: codes [M, K]; B: codes [G, N, K], each with its scales.  K a
  * multiple of 16, N of 8, pointers 16-byte aligned, N*K and the scales of all
  * rows below 2 GiB, else PMX_ERR_SHAPE. */
 int pmx_rows8_group_gemm_nt(const void* a, const void* a_scales, const void* b, const void* b_scales,
@@ -531,6 +531,21 @@ int pmx_rows8_gemm_fc1_swiglu(const void* x, const void* x_scales, int64_t T, co
                               const void* w, const void* w_scales, const int32_t* offsets, int32_t G,
                               int64_t A, int64_t H, int64_t I, const void* row_w, void* act, void* act_scales,
                               pmx_stream_t stream);
+
+/* The expert layer over 8-bit weights, forward: route, tokens to 8 bits, fc1 +
+ * SwiGLU weighted by the router, fc2, sum of each token's rows; one call, since
+ * a single token's kernels take less time than five calls.
+ * hidden bf16 [T, H]; w bf16 [T, K]; sel, M, src, src_const, S, E as in
+ * pmx_route; gate_up [C, 2I, H] and down [C, H, I] in e4m3 with their scales;
+ * out bf16 [T, H]; counts int32 [C] (NULL: not wanted); status_host as in
+ * pmx_route_reported; the workspace's first bytes hold the routing status word.
+ * H and I multiples of 16; T*H, I*H and the scales below 2 GiB each. */
+size_t pmx_rows8_layer_workspace_bytes(int64_t T, int32_t K, int64_t H, int64_t I, int32_t C);
+int pmx_rows8_layer(const void* hidden, const void* w, const int64_t* sel, const int64_t* M, const int64_t* src,
+                    int32_t src_const, int32_t S, int32_t E, const void* gate_up, const void* gate_up_scales,
+                    const void* down, const void* down_scales, int64_t T, int32_t K, int64_t H, int64_t I,
+                    int32_t C, void* out, int32_t* counts, void* workspace, size_t workspace_bytes,
+                    int32_t* status_host, pmx_stream_t stream);
 
 /* ------------------------------------------------------------------------ */
 /* fp16 tensors                                                              */
@@ -619,6 +634,11 @@ int pmx_rows8_gemm_fc1_swiglu_f16(const void* x, const void* x_scales, int64_t T
                                   const void* w, const void* w_scales, const int32_t* offsets, int32_t G,
                                   int64_t A, int64_t H, int64_t I, const void* row_w, void* act, void* act_scales,
                                   pmx_stream_t stream);
+int pmx_rows8_layer_f16(const void* hidden, const void* w, const int64_t* sel, const int64_t* M,
+                        const int64_t* src, int32_t src_const, int32_t S, int32_t E, const void* gate_up,
+                        const void* gate_up_scales, const void* down, const void* down_scales, int64_t T, int32_t K,
+                        int64_t H, int64_t I, int32_t C, void* out, int32_t* counts, void* workspace,
+                        size_t workspace_bytes, int32_t* status_host, pmx_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -166,6 +166,13 @@ SIGNATURES = {
         [c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int64, c_int64, c_int64,
          c_void_p, c_void_p, c_void_p, c_void_p],
     ),
+    "pmx_rows8_layer_workspace_bytes": (c_size_t, [c_int64, c_int32, c_int64, c_int64, c_int32]),
+    "pmx_rows8_layer": (
+        c_int,
+        [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_int32, c_void_p, c_void_p, c_void_p,
+         c_void_p, c_int64, c_int32, c_int64, c_int64, c_int32, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p,
+         c_void_p],
+    ),
     "pmx_ep_combine_workspace_bytes": (c_size_t, [c_int64]),
     "pmx_ep_combine_aggregate": (
         c_int,
@@ -187,7 +194,7 @@ F16_TWINS = (
     "pmx_swiglu_bwd_weighted", "pmx_gemm_fc1_swiglu_weighted_fwd", "pmx_swiglu_bwd_weighted_gu",
     "pmx_replica_fold", "pmx_ep_combine_aggregate", "pmx_ep_combine_aggregate_i64",
     "pmx_rows8_quantize", "pmx_rows8_quantize_routed", "pmx_rows8_dequantize", "pmx_rows8_swiglu_bwd",
-    "pmx_rows8_group_gemm_nt", "pmx_rows8_gemm_fc1_swiglu",
+    "pmx_rows8_group_gemm_nt", "pmx_rows8_gemm_fc1_swiglu", "pmx_rows8_layer",
 )
 SIGNATURES.update({name + "_f16": SIGNATURES[name] for name in F16_TWINS})
 

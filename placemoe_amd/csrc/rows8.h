@@ -21,6 +21,9 @@
 
 #include "common.h"
 
+// Between rows8_gemm.hip and rows8_layer.hip, not part of the C ABI.
+__attribute__((visibility("hidden"))) int pmx_rows8_layer_check(int64_t T, int32_t K, int64_t H, int64_t I, int32_t C);
+
 namespace {
 
 constexpr int kFmtE4M3 = 0, kFmtInt8 = 1;

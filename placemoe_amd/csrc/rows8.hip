@@ -116,8 +116,9 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const bf16_t* __rest
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t B = (N + kScaleGroup - 1) / kScaleGroup;
   // column groups fastest: a row's blocks run side by side
-  const int64_t b = blockIdx.x % B, rest = blockIdx.x / B;
-  const int64_t r0 = rest % row_tiles * kTileRows, g = rest / row_tiles;
+  // (32-bit divisions: a 64-bit one takes longer than the rows of a small call)
+  const uint32_t rest = blockIdx.x / (uint32_t)B, g = rest / (uint32_t)row_tiles;
+  const int64_t b = blockIdx.x % (uint32_t)B, r0 = (int64_t)(rest % (uint32_t)row_tiles) * kTileRows;
   const int64_t c = b * kScaleGroup + lane * 8;
   const bf16_t* xg = x + g * gsx;
   uint8_t* cg = codes + g * R * N;
@@ -146,11 +147,11 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const bf16_t* __rest
     }
   }
   if (map.pos != nullptr && b == 0) {
-    const int64_t rows = R - r0 < kTileRows ? R - r0 : kTileRows, A = R * map.K;
-    for (int64_t i = threadIdx.x; i < rows * map.K; i += 256) {
-      const int64_t a = r0 * map.K + i, p = map.pos[a];
+    const int32_t rows = (int32_t)(R - r0 < kTileRows ? R - r0 : kTileRows), A = (int32_t)R * map.K;  // T * K fits
+    for (int32_t i = threadIdx.x; i < rows * map.K; i += 256) {
+      const int32_t a = (int32_t)r0 * map.K + i, p = map.pos[a];
       if (p >= 0 && p < A) {
-        map.row_token[p] = (int32_t)(a / map.K);
+        map.row_token[p] = (int32_t)((uint32_t)a / (uint32_t)map.K);
         map.row_w[p] = map.w[a];
       }
     }
@@ -179,7 +180,7 @@ __global__ __launch_bounds__(256) void dequantize_rows_kernel(const uint8_t* __r
   constexpr int PER = 4;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t B = (N + kScaleGroup - 1) / kScaleGroup;
-  const int64_t b = blockIdx.x % B, r0 = blockIdx.x / B * (4 * PER);
+  const int64_t b = blockIdx.x % (uint32_t)B, r0 = (int64_t)(blockIdx.x / (uint32_t)B) * (4 * PER);
   const int64_t c = b * kScaleGroup + lane * 8;
   if (c >= N) return;
   uint2 v[PER];

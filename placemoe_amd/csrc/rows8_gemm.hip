@@ -32,6 +32,7 @@
 
 #include "gemm_util.h"
 #include "rows8.h"
+#include "rows8_rule.h"
 
 namespace {
 
@@ -41,8 +42,12 @@ typedef int32_t i32x4_t __attribute__((ext_vector_type(4)));
 #ifndef PMX_R8_LOAD_GROUPS
 #define PMX_R8_LOAD_GROUPS 99
 #endif
-constexpr int kMaxGroups = 2048;  // groups (the m-tile prefix in LDS)
+#ifndef PMX_R8_RG
+#define PMX_R8_RG 6
+#endif
+constexpr int kMaxGroups = 2048;  // groups (their m-tiles' prefix in LDS)
 constexpr int KT = 128;           // depth of a K-tile
+constexpr int kStreaming = 2;     // cache policy of stores that this kernel does not read back
 constexpr int kScaleTiles = kScaleGroup / KT;
 
 enum Kind8 { NT8 = 0, FC18 = 1 };
@@ -75,7 +80,7 @@ struct Cfg8 {
   static constexpr int LDS = NST * (STAGE + SLOT);
   static_assert(BM / 8 % NW == 0 && BN / 8 % NW == 0 && BN % 64 == 0, "whole loads per wave");
   static_assert(FN % 2 == 0 || WN % 2 == 0, "gate and up tiles alternate");
-  static_assert(NST >= 2 && (NST - 2) * (QA + QB) <= 63, "vmcnt is 6 bits");
+  static_assert(NST >= 2 && (NST - 1) * (QA + QB) <= 63, "vmcnt is 6 bits");
 };
 
 // Where one output tile lies.
@@ -183,35 +188,67 @@ __device__ __forceinline__ void swap_halves(uint32_t& lo, uint32_t& hi) {
 // An accumulator holds its 32 x 32 output tile transposed (B is the MFMA's
 // first operand): lane l has row l%32, columns 8*(i/4) + 4*(l/32) + i%4.
 template <class E, int KIND, class CF>
-__device__ __forceinline__ void epilogue(const Params8& P, const Place& at, int wm, int wn, int lane,
-                                         f32x16_t (&acc)[CF::FM][CF::FN]) {
+__device__ __forceinline__ void epilogue(const Params8& P, const Place& at, int wm, int wn, int wave, int lane,
+                                         [[maybe_unused]] char* stage, f32x16_t (&acc)[CF::FM][CF::FN]) {
   // Each accumulator leaves the accumulation registers where it is used: read
   // right behind their last MFMAs, they would need as many vector registers.
   const auto here = [](f32x16_t& v) __attribute__((always_inline)) { asm volatile("" : "+a"(v)); };
   asm volatile("" : "+v"(lane));
   const int h = lane >> 5;
+  // NT: the output from the tile's first row to the group's end (what lies behind fails the range check); the
+  // lane's place in a store of whole row segments.
+  const uint32_t ldc = (uint32_t)P.N * 2;
+  [[maybe_unused]] const __amdgpu_buffer_rsrc_t out =
+      make_rsrc(P.c + (int64_t)at.row0 * P.N, (uint64_t)(at.row_end - at.row0) * ldc);
+  const int32_t col = at.ntile * CF::BN + wn * CF::FN * 32 + lane % (CF::FN * 4) * 8;
+  [[maybe_unused]] const uint32_t voff =
+      col < (int32_t)P.N ? (uint32_t)(lane / (CF::FN * 4)) * ldc + (uint32_t)col * 2 : kOOB;
 #pragma unroll
   for (int m = 0; m < CF::FM; ++m) {
     const int64_t r = (int64_t)at.row0 + (wm * CF::FM + m) * 32 + (lane & 31);
     const bool in = r < at.row_end;
     if constexpr (KIND == NT8) {
+      // 32 rows of CPR 16-byte chunks pass through the wave's own 1 KB pieces
+      // of the stage just freed (those that its loads fill, so that no other
+      // wave touches them) and leave as whole row segments: straight from the
+      // registers a store would have 32 bytes of each of 32 rows, four times
+      // the requests to the L2.  Chunk c of row r at c ^ r (mod CPR), so that
+      // neither side has bank conflicts.
+      constexpr int CPR = CF::FN * 4, RPP = 64 / CPR;  // chunks of a row, rows of a piece (and of a store)
+      static_assert(32 / RPP <= CF::QA + CF::QB, "enough pieces");
+      const auto place = [&](int row, int c) {
+        const int sw = CPR == 16 ? row & 15 : kc_swz(row);
+        return stage + ((row / RPP) * CF::NW + wave) * 1024 + (row % RPP) * (CPR * 16) + ((c ^ sw) << 4);
+      };
 #pragma unroll
       for (int n = 0; n < CF::FN; ++n) {
         here(acc[m][n]);
+        const f32x16_t& v = acc[m][n];
 #pragma unroll
         for (int p = 0; p < 2; ++p) {  // 16 columns: the half-waves exchange, and each lane has 8 of them
-          const f32x16_t& v = acc[m][n];
           uint32_t w0 = E::pack2(v[8 * p], v[8 * p + 1]), w1 = E::pack2(v[8 * p + 2], v[8 * p + 3]);
           uint32_t w2 = E::pack2(v[8 * p + 4], v[8 * p + 5]), w3 = E::pack2(v[8 * p + 6], v[8 * p + 7]);
           swap_halves(w0, w2);
           swap_halves(w1, w3);
-          const int64_t col = (int64_t)at.ntile * CF::BN + (wn * CF::FN + n) * 32 + p * 16 + h * 8;
-          if (in && col < P.N) *reinterpret_cast<uint4*>(P.c + r * P.N + col) = make_uint4(w0, w1, w2, w3);
+          *reinterpret_cast<uint4*>(place(lane & 31, n * 4 + p * 2 + h)) = make_uint4(w0, w1, w2, w3);
         }
-        __builtin_amdgcn_sched_barrier(0);  // one tile's registers at a time
       }
+      wait_lds();
+#pragma unroll
+      for (int q = 0; q < 32 / RPP; ++q) {
+        const int row = q * RPP + lane / CPR;
+        const u32x4_t v = *reinterpret_cast<const u32x4_t*>(place(row, lane % CPR));
+        __builtin_amdgcn_raw_buffer_store_b128(v, out, voff + (uint32_t)((wm * CF::FM + m) * 32 + q * RPP) * ldc, 0, kStreaming);
+      }
+      __builtin_amdgcn_sched_barrier(0);  // one tile's registers at a time
     } else {
       const float w = in && P.row_w != nullptr ? E::to_f32(P.row_w[r]) : 1.0f;
+      // fc2's last K-tile takes along the blocks past I in the last 128 columns: those that no tile covers stand,
+      // as the others of zeros do, beside 2^0
+      if (in && h == 0 && wn == CF::WN - 1 && (int64_t)(at.ntile + 1) * (CF::BN / 2) >= P.I) {
+        for (int64_t j = (int64_t)(at.ntile + 1) * (CF::BN / 2); j < (P.I + KT - 1) / KT * KT; j += kScaleBlock)
+          P.qs[(j / kScaleGroup * P.M + r) * kScaleBytes + j / kScaleBlock % 16] = 127;
+      }
 #pragma unroll
       for (int n = 0; n < CF::FN; n += 2) {
         here(acc[m][n]);
@@ -237,7 +274,6 @@ __device__ __forceinline__ void epilogue(const Params8& P, const Place& at, int 
         const int64_t j = (int64_t)at.ntile * (CF::BN / 2) + (wn * CF::FN + n) * 16;
         if (in) {
           if (j + h * 16 < P.I) *reinterpret_cast<uint4*>(P.q + r * P.I + j + h * 16) = make_uint4(c[0], c[2], c[1], c[3]);
-          // also the blocks past I within the last 128 columns, which fc2's last K-tile takes along (zeros)
           if (h == 0) P.qs[(j / kScaleGroup * P.M + r) * kScaleBytes + j / kScaleBlock % 16] = (uint8_t)byte;
         }
         __builtin_amdgcn_sched_barrier(0);
@@ -250,8 +286,7 @@ template <class E, int KIND, class CF>
 __global__ __launch_bounds__(CF::NTH, CF::NW * CF::BPC / 4) void rows8_grouped_gemm_kernel(Params8 P) {
   constexpr int NW = CF::NW, L = CF::QA + CF::QB;
   __shared__ __attribute__((aligned(1024))) char lds[CF::LDS];
-  __shared__ int32_t tpre[kMaxGroups + 1];
-  __shared__ int32_t wsum[NW];
+  __shared__ int32_t tend[kMaxGroups];  // m-tiles of the groups up to and with g
   char* const slots = lds + CF::NST * CF::STAGE;
   const int t = threadIdx.x;
   const int lane = t & 63;
@@ -263,75 +298,76 @@ __global__ __launch_bounds__(CF::NTH, CF::NW * CF::BPC / 4) void rows8_grouped_g
     const int32_t o = P.offsets[g];
     return o < 0 ? 0 : o > P.M ? (int32_t)P.M : o;
   };
-  const auto m_tiles = [&](int g) {
-    const int32_t n = offset(g + 1) - offset(g);
-    return n > 0 ? (n + CF::BM - 1) / CF::BM : 0;
-  };
+  const auto m_tiles = [&](int g) { return (offset(g + 1) - offset(g) + CF::BM - 1) / CF::BM; };
 
-  // Exclusive prefix of the groups' m-tiles in tpre[0..G]: consecutive groups
-  // per thread, a wave scan of the threads' sums, then the waves' sums.
+  // Prefix of the groups' m-tiles: consecutive groups per thread, a wave scan
+  // of the threads' sums, then the waves' sums.
   {
+    int32_t* wsum = reinterpret_cast<int32_t*>(lds);
     const int per = (G + CF::NTH - 1) / CF::NTH;
     const int g0 = t * per, g1 = g0 + per < G ? g0 + per : G;
     int32_t sum = 0;
-    for (int g = g0; g < g1; ++g) sum += m_tiles(g);
+    bool descends = false;
+    for (int g = g0; g < g1; ++g) {
+      sum += m_tiles(g);
+      descends |= offset(g + 1) < offset(g);
+    }
     int32_t inc = sum;
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) {
       const int32_t v = __shfl_up(inc, off, 64);
       if (lane >= off) inc += v;
     }
-    if (lane == 63) wsum[wave] = inc;
+    const bool bad = __ballot(descends) != 0;  // not row groups: nothing to do
+    if (lane == 63) wsum[wave] = bad ? -1 : inc;
     __syncthreads();
     int32_t run = inc - sum;
-    for (int w = 0; w < wave; ++w) run += wsum[w];
-    for (int g = g0; g < g1; ++g) {
-      tpre[g] = run;
-      run += m_tiles(g);
+    for (int w = 0; w < NW; ++w) {
+      if (uni(wsum[w]) < 0) return;
+      run += w < wave ? wsum[w] : 0;
     }
-    if (t == CF::NTH - 1) tpre[G] = run;
+    for (int g = g0; g < g1; ++g) tend[g] = run += m_tiles(g);
     __syncthreads();
   }
   const int32_t ntn = (int32_t)(KIND == FC18 ? (P.I + CF::BN / 2 - 1) / (CF::BN / 2) : (P.N + CF::BN - 1) / CF::BN);
-  const int64_t total = (int64_t)uni(tpre[G]) * ntn;
+  const int32_t total = uni(tend[G - 1]) * ntn;  // the host has checked that it fits
   const int32_t nk = (int32_t)((P.K + KT - 1) / KT);
   // Blocks go round-robin over the XCDs: each XCD walks its own eighth of the
   // tile list, its blocks round-robin within it.
-  int64_t first = blockIdx.x, step = gridDim.x, end = total;
+  int32_t first = blockIdx.x, step = gridDim.x, end = total;
   if (gridDim.x % kNumXcd == 0) {
-    const int64_t x = blockIdx.x % kNumXcd;
+    const int32_t x = blockIdx.x % kNumXcd;
     step = gridDim.x / kNumXcd;
-    end = total * (x + 1) / kNumXcd;
-    first = total * x / kNumXcd + blockIdx.x / kNumXcd;
+    end = (int32_t)((int64_t)total * (x + 1) / kNumXcd);
+    first = (int32_t)((int64_t)total * x / kNumXcd) + blockIdx.x / kNumXcd;
   }
   if (first >= end) return;
 
   // Tile order: group by group, in bands of 8 m-tiles walked n-tile by n-tile:
-  // neighbouring tiles share a strip of B, and a band of A.
-  auto decode = [&](int64_t tile, Place& at) {
-    constexpr int kBand = 8;
-    const int32_t m = (int32_t)(tile / ntn);
-    int lo = 0, hi = G - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (uni(tpre[mid]) <= m) lo = mid;
-      else hi = mid - 1;
-    }
-    const int32_t m0 = uni(tpre[lo]), gm = uni(tpre[lo + 1]) - m0;
-    const int64_t local = tile - (int64_t)m0 * ntn;
-    const int32_t band = (int32_t)(local / ((int64_t)kBand * ntn)) * kBand;
-    const int32_t rest = (int32_t)(local - (int64_t)band * ntn);
-    const int32_t high = gm - band < kBand ? gm - band : kBand;
-    at.g = lo;
-    at.ntile = rest / high;
-    const int32_t row0 = uni(offset(lo)) + (band + rest % high) * CF::BM;
-    at.row0 = row0;
-    at.row_end = uni(offset(lo + 1));
+  // neighbouring tiles share a strip of B, and a band of A.  The group: 64
+  // equal parts of the prefix at once, then the entries of the one.
+  const int32_t part = (G + 63) / 64;
+  auto decode = [&](int32_t tile, Place& at) {
+    constexpr uint32_t kBand = 8;
+    const int32_t m = (int32_t)((uint32_t)tile / (uint32_t)ntn);
+    const auto first_past = [&](int32_t v) { return uni(__builtin_ctzll(__ballot(v > m))); };  // some entry is: m < tend[G-1]
+    const int32_t hi = (lane + 1) * part < G ? (lane + 1) * part : G;
+    int32_t g = first_past(tend[hi - 1]) * part;
+    if (part > 1) g += first_past(tend[g + lane < G && lane < part ? g + lane : G - 1]);
+    const int32_t m0 = g > 0 ? uni(tend[g - 1]) : 0, gm = uni(tend[g]) - m0;
+    const uint32_t local = (uint32_t)(tile - m0 * ntn);
+    const uint32_t band = local / (kBand * ntn) * kBand;
+    const uint32_t rest = local - band * ntn;
+    const uint32_t high = gm - band < kBand ? gm - band : kBand;
+    at.g = g;
+    at.ntile = (int32_t)(rest / high);
+    at.row0 = uni(offset(g)) + (int32_t)(band + rest % high) * CF::BM;
+    at.row_end = uni(offset(g + 1));
   };
 
   // Issue cursor, running ahead of the K-tile being multiplied.
   Loads<CF> ld;
-  int64_t i_tile = first;
+  int32_t i_tile = first;
   int32_t i_kt = 0, i_stage = 0, i_slot = 0;
   bool i_live = true;
   auto set_tile = [&]() {
@@ -427,28 +463,28 @@ __global__ __launch_bounds__(CF::NTH, CF::NW * CF::BPC / 4) void rows8_grouped_g
       for (int e = 0; e < 2; ++e) at[ks][e] = r32 * KT + (((ks * 4 + e * 2 + h) ^ kc_swz(r32)) << 4);
     const uint32_t pick = 0x06040200u + 0x01010101u * h;  // bytes h and 2 + h of two words
     Frags8<CF> f0, f1;
-    auto read = [&](auto jj, auto kk, const char* stage, const char* slot, const Frags8<CF>& fm, Frags8<CF>& fr)
-        __attribute__((always_inline)) {
+    auto read = [&](auto jj, auto kk, const char* stage, Frags8<CF>& fr) __attribute__((always_inline)) {
       constexpr int J = decltype(jj)::value, ks = decltype(kk)::value;
-      constexpr bool is_a = J < CF::FM;
       const char* p = stage + in_stage(J);
       const i32x4_t lo = *reinterpret_cast<const i32x4_t*>(p + at[ks][0]);
       const i32x4_t hi = *reinterpret_cast<const i32x4_t*>(p + at[ks][1]);
       const i32x8_t v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-      if constexpr (is_a) fr.a[J] = v;
+      if constexpr (J < CF::FM) fr.a[J] = v;
       else fr.b[J - CF::FM] = v;
-      constexpr int F = is_a ? J : J - CF::FM, last = (is_a ? CF::FM : CF::FN) - 1;
-      if constexpr (F % 2 == 0) {
-        int32_t& out = is_a ? fr.sa[F / 2] : fr.sb[F / 2];
-        if constexpr (ks == 0) {
-          const char* w = slot + in_slot(J);
-          const uint32_t w0 = *reinterpret_cast<const uint32_t*>(w);
-          const uint32_t w1 = F < last ? *reinterpret_cast<const uint32_t*>(w + 32 * kScaleBytes) : w0;
-          out = (int32_t)__builtin_amdgcn_perm(w1, w0, pick);
-        } else {
-          out = is_a ? fm.sa[F / 2] : fm.sb[F / 2];
-        }
-      }
+    };
+    // The exponents of a K-tile: every fragment's word, and later, when they have arrived, the lane's bytes of them.
+    Words8<CF> words;
+    auto read_words = [&](const char* slot) __attribute__((always_inline)) {
+#pragma unroll
+      for (int j = 0; j < NR; ++j) words.v[j] = *reinterpret_cast<const uint32_t*>(slot + in_slot(j));
+    };
+    auto pack_words = [&](Frags8<CF>& fr) __attribute__((always_inline)) {
+#pragma unroll
+      for (int j = 0; j < CF::FM; j += 2)
+        fr.sa[j / 2] = (int32_t)__builtin_amdgcn_perm(words.v[j + 1 < CF::FM ? j + 1 : j], words.v[j], pick);
+#pragma unroll
+      for (int j = 0; j < CF::FN; j += 2)
+        fr.sb[j / 2] = (int32_t)__builtin_amdgcn_perm(words.v[CF::FM + (j + 1 < CF::FN ? j + 1 : j)], words.v[CF::FM + j], pick);
     };
     auto mfma = [&](auto xx, auto kk, auto zero, const Frags8<CF>& f) __attribute__((always_inline)) {
       constexpr int x = decltype(xx)::value, m = x / CF::FN, n = x % CF::FN, ks = decltype(kk)::value;
@@ -456,29 +492,40 @@ __global__ __launch_bounds__(CF::NTH, CF::NW * CF::BPC / 4) void rows8_grouped_g
           f.b[n], f.a[m], decltype(zero)::value ? f32x16_t{} : acc[m][n], 0, 0, n % 2 * 2 + ks, f.sb[n / 2], m % 2 * 2 + ks,
           f.sa[m / 2]);
     };
-    // The MFMAs of half `km` from `fm`, in NR groups: each reads one fragment of
-    // the other half into `fr` and (loads) issues its share of the loads of the
-    // K-tile NST - 1 ahead.
+    // The MFMAs of half `km` from `fm`, in NR groups, beside the reads of the
+    // other half into `fr`: km = 1 reads the next K-tile's first half and its
+    // exponents, and (loads) issues the loads of the K-tile NST - 1 ahead.
     auto kstep = [&](auto zero, auto km, auto loads, const Frags8<CF>& fm, const char* stage, const char* slot, Frags8<CF>& fr)
         __attribute__((always_inline)) {
+      constexpr int kn = 1 - decltype(km)::value, RG = kn == 1 && PMX_R8_RG < NR ? PMX_R8_RG : NR;
       if constexpr (decltype(loads)::value) issue_scales();
+      if constexpr (kn == 0) read_words(slot);
       static_for<0, NR>([&](auto jj) __attribute__((always_inline)) {
         constexpr int j = decltype(jj)::value, LG = PMX_R8_LOAD_GROUPS < NR ? PMX_R8_LOAD_GROUPS : NR;
         if constexpr (decltype(loads)::value && j < LG) static_for<j * L / LG, (j + 1) * L / LG>(issue);
-        read(Int<order8<CF>(j)>{}, Int<1 - decltype(km)::value>{}, stage, slot, fm, fr);
+        if constexpr (j < RG)
+          static_for<j * NR / RG, (j + 1) * NR / RG>(
+              [&](auto i) __attribute__((always_inline)) { read(Int<order8<CF>(decltype(i)::value)>{}, Int<kn>{}, stage, fr); });
+        if constexpr (kn == 0 && j == NR / 2) pack_words(fr);
+        if constexpr (kn == 1 && j == 0) {
+#pragma unroll
+          for (int i = 0; i < (CF::FM + 1) / 2; ++i) fr.sa[i] = fm.sa[i];
+#pragma unroll
+          for (int i = 0; i < (CF::FN + 1) / 2; ++i) fr.sb[i] = fm.sb[i];
+        }
         static_for<j * NM / NR, (j + 1) * NM / NR>([&](auto xx) __attribute__((always_inline)) { mfma(xx, km, zero, fm); });
         __builtin_amdgcn_sched_barrier(0);
       });
     };
 
-    for (int64_t tile = first; tile < end; tile += step) {
+    for (int32_t tile = first; tile < end; tile += step) {
       // The tile's first K-tile: no MFMAs of this tile to read its first half behind.
       {
         const char* stage = lds + c_stage * CF::STAGE;
         const char* slot = slots + c_slot * CF::SLOT;
-        static_for<0, NR>([&](auto j) __attribute__((always_inline)) {
-          read(Int<order8<CF>(decltype(j)::value)>{}, Int<0>{}, stage, slot, f0, f0);
-        });
+        read_words(slot);
+        static_for<0, NR>([&](auto j) __attribute__((always_inline)) { read(Int<order8<CF>(decltype(j)::value)>{}, Int<0>{}, stage, f0); });
+        pack_words(f0);
         kstep(Int<1>{}, Int<0>{}, Int<1>{}, f0, stage, slot, f1);
         advance_issue();
         turn();
@@ -496,9 +543,10 @@ __global__ __launch_bounds__(CF::NTH, CF::NW * CF::BPC / 4) void rows8_grouped_g
       }
       static_for<0, NM>([&](auto x) __attribute__((always_inline)) { mfma(x, Int<1>{}, Int<0>{}, f1); });
       next_slot();
+      char* free_stage = lds + (c_stage == 0 ? CF::NST - 1 : c_stage - 1) * CF::STAGE;  // the tile's last K-tile's
       Place place;
       decode(tile, place);
-      epilogue<E, KIND, CF>(P, place, wm, wn, lane, acc);
+      epilogue<E, KIND, CF>(P, place, wm, wn, wave, lane, free_stage, acc);
     }
   } else {
     // In quarter q of the K-tile lane l holds row l%32, columns 16 h .. + 15 of
@@ -577,12 +625,12 @@ __global__ __launch_bounds__(CF::NTH, CF::NW * CF::BPC / 4) void rows8_grouped_g
 
     static_for<0, NR>([&](auto j) __attribute__((always_inline)) { read(j, Int<0>{}, lds, slots, r0, words); });
     static_for<0, 4 * NR>([&](auto y) __attribute__((always_inline)) { convert(y, Int<0>{}, Int<0>{}, r0, words, c0); });
-    for (int64_t tile = first; tile < end; tile += step) {
+    for (int32_t tile = first; tile < end; tile += step) {
       ktile(Int<1>{}, 0);
       for (int32_t kt = 1; kt < nk; ++kt) ktile(Int<0>{}, kt);
       Place place;
       decode(tile, place);
-      epilogue<E, KIND, CF>(P, place, wm, wn, lane, acc);
+      epilogue<E, KIND, CF>(P, place, wm, wn, wave, lane, nullptr, acc);
     }
   }
   wait_loads<0>();
@@ -604,12 +652,21 @@ int cu_count() {
   return cus;
 }
 
-using Rows32 = Cfg8<1, 4, 1, 2, 3, 1>;   // 32 x 256 tiles
-using Rows128 = Cfg8<2, 2, 2, 4, 2, 1>;  // 128 x 256
-using Rows256 = Cfg8<2, 2, 4, 4, 2, 1>;  // 256 x 256
+// The tilings of rows8_rule.h.
+using Rows32 = Cfg8<1, 4, 1, 2, 3, 1>;   // 32 x 256, one wave per 32 x 64
+using Rows128 = Cfg8<2, 2, 2, 2, 2, 2>;  // 128 x 128, 64 x 64
+using Rows256 = Cfg8<2, 2, 4, 4, 2, 1>;  // 256 x 256, 128 x 128
+
+// Tiles, and the cursor's step past the last one, are counted in 32 bits.
+template <int KIND, class CF>
+bool tiles_fit(const Params8& P, int cus) {
+  const int64_t ntn = KIND == FC18 ? (P.I + CF::BN / 2 - 1) / (CF::BN / 2) : (P.N + CF::BN - 1) / CF::BN;
+  return (P.M / CF::BM + P.G) * ntn <= INT32_MAX - cus * CF::BPC;
+}
 
 template <class E, int KIND, class CF>
 int launch_cfg(const Params8& P, int cus, pmx_stream_t stream) {
+  if (!tiles_fit<KIND, CF>(P, cus)) return PMX_ERR_SHAPE;
   rows8_grouped_gemm_kernel<E, KIND, CF><<<cus * CF::BPC, CF::NTH, 0, stream>>>(P);
   PMX_LAUNCH_CHECK();
   return PMX_OK;
@@ -619,9 +676,14 @@ template <class E, int KIND>
 int launch(const Params8& P, pmx_stream_t stream) {
   const int cus = cu_count();
   if (cus <= 0) return PMX_ERR_HIP;
-  if (P.M <= 32 * (int64_t)P.G) return launch_cfg<E, KIND, Rows32>(P, cus, stream);
-  if (P.M <= 160 * (int64_t)P.G) return launch_cfg<E, KIND, Rows128>(P, cus, stream);
-  return launch_cfg<E, KIND, Rows256>(P, cus, stream);
+#ifdef PMX_R8_FORCE
+  return launch_cfg<E, KIND, PMX_R8_FORCE>(P, cus, stream);
+#endif
+  switch (pmx::rows8_tiling(KIND, P.M, P.G, P.N, P.K, cus)) {
+    case Rows32::BM: return launch_cfg<E, KIND, Rows32>(P, cus, stream);
+    case Rows128::BM: return launch_cfg<E, KIND, Rows128>(P, cus, stream);
+    default: return launch_cfg<E, KIND, Rows256>(P, cus, stream);
+  }
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -636,9 +698,14 @@ int check(const Params8& P) {
   if (P.K % 16 || P.M > INT32_MAX - 256 || P.a_rows > INT32_MAX) return PMX_ERR_SHAPE;
   const int64_t kgroups = (P.K + kScaleGroup - 1) / kScaleGroup;
   if (!one_window(P.N, P.K) || !one_window(P.N, kgroups * kScaleBytes) || !one_window(P.a_rows, kgroups * kScaleBytes) ||
-      !one_window(P.row_token != nullptr ? P.a_rows : 256, P.K))
+      !one_window(P.row_token != nullptr ? P.a_rows : 256, P.K) || !one_window(256, 2 * P.N))
     return PMX_ERR_SHAPE;
   return PMX_OK;
+}
+
+template <int KIND>
+bool any_tiles_fit(const Params8& P) {
+  return tiles_fit<KIND, Rows32>(P, 1024);  // the most tiles, and more CUs than there are
 }
 
 template <class E>
@@ -676,6 +743,21 @@ int fc1_t(const void* x, const void* xs, int64_t T, const int32_t* row_token, co
 }
 
 }  // namespace
+
+// Whether a layer of T tokens, K copies each, fits both products (rows8_layer.hip asks before it launches anything).
+int pmx_rows8_layer_check(int64_t T, int32_t K, int64_t H, int64_t I, int32_t C) {
+  if (T < 0 || K <= 0 || H <= 0 || I <= 0 || C <= 0) return PMX_ERR_ARG;
+  if (H % 16 || I % 16 || I > INT32_MAX / 2 || T > INT32_MAX / K) return PMX_ERR_SHAPE;
+  static const int32_t some_map = 0;
+  Params8 P = {};
+  P.G = C, P.M = T * K;
+  P.a_rows = T, P.row_token = &some_map, P.N = 2 * I, P.K = H, P.I = I;
+  if (const int rc = check(P)) return rc;
+  if (!any_tiles_fit<FC18>(P)) return PMX_ERR_SHAPE;
+  P.a_rows = P.M, P.row_token = nullptr, P.N = H, P.K = I;
+  if (const int rc = check(P)) return rc;
+  return any_tiles_fit<NT8>(P) ? PMX_OK : PMX_ERR_SHAPE;
+}
 
 extern "C" {
 

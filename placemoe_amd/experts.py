@@ -142,21 +142,12 @@ def _poll_pending_checks() -> None:
         failed.raise_if_failed()
 
 
-def route_checked(selected, num_slots: int, mapping, sources, source: int) -> kernels.Routing:
-    """Route one batch; its status is looked at without a host sync."""
-    _poll_pending_checks()
-    # Invalid expert or source ids are clamped on the device and flagged in
-    # the routing status word, which the routing stores to pinned host
-    # memory.  It is looked at without a host sync: by the backward if it
-    # has landed by then, else by a later forward or backward (or
-    # check_pending_routes).
-    check = kernels.RouteCheck()
-    r = kernels.route(selected, num_slots, mapping=mapping, sources=sources, source=source, check=check)
+def note_routing(check: kernels.RouteCheck) -> None:
+    """A routing has been launched: look at its status now, or have a later call do it."""
     if _sync_route_checks():
         check.raise_if_failed()
     elif not check.checked:
         _PENDING_CHECKS.append(check)
-    return r
 
 
 class _ExpertLayerBase(torch.autograd.Function):
@@ -182,7 +173,15 @@ class _ExpertLayerBase(torch.autograd.Function):
             f"fc1 weight shape {tuple(w_gate.shape)} does not match fc2 {tuple(fc2_weight.shape)} "
             f"and hidden size {H} (expected {fc1_shape})"
         )
-        r = route_checked(selected, C, mapping, sources, source)
+        _poll_pending_checks()
+        # Invalid expert or source ids are clamped on the device and flagged in
+        # the routing status word, which the routing stores to pinned host
+        # memory.  It is looked at without a host sync: by the backward if it
+        # has landed by then, else by a later forward or backward (or
+        # check_pending_routes).
+        check = kernels.RouteCheck()
+        r = kernels.route(selected, C, mapping=mapping, sources=sources, source=source, check=check)
+        note_routing(check)
         if recorder is not None:
             recorder(r.counts)
         ctx.split = split

@@ -100,9 +100,12 @@ def _indices(name: str, t: torch.Tensor, numel: int | None = None) -> None:
     assert numel is None or t.numel() == numel, f"{name} must have {numel} entries, got {t.numel()}"
 
 
+_HERE = contextlib.nullcontext()
+
+
 def _on(dev: torch.device):
     """The launch device: a kernel starts on the current one, whatever its stream."""
-    return contextlib.nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+    return _HERE if dev.index == torch._C._cuda_getDevice() else torch.cuda.device(dev)
 
 
 def _launch(name: str, dtype: torch.dtype, dev: torch.device, *args) -> None:
@@ -135,14 +138,13 @@ def quantize_rows(x: torch.Tensor, fmt: str = "e4m3") -> Rows8:
     code = _format(fmt)
     assert x.dtype in HALF, f"x must be bfloat16 or float16, got {x.dtype}"
     assert x.dim() in (2, 3), f"x must be [R, N] or [G, R, N], got {tuple(x.shape)}"
-    G = x.shape[0] if x.dim() == 3 else 1
-    R, N = x.shape[-2:]
-    ld = N
-    if x.dim() == 2 and R > 1:
-        assert (N <= 1 or x.stride(1) == 1) and x.stride(0) >= N, "columns must be contiguous and rows apart"
-        ld = x.stride(0)
-    else:
-        assert x.is_contiguous(), "x must be contiguous"
+    *lead, R, N = x.shape
+    G, ld = (lead[0] if lead else 1), N
+    if not x.is_contiguous():
+        assert not lead and (N <= 1 or x.stride(1) == 1) and (R <= 1 or x.stride(0) >= N), (
+            "columns must be contiguous and the rows of a 2-D x apart"
+        )
+        ld = max(N, x.stride(0))
     q = _empty(x.shape, code, x.dtype, dev)
     _launch("pmx_rows8_quantize", x.dtype, dev, _ptr(x), ld, R * N, G, R, N, _FORMAT_CODES[code], _ptr(q.codes),
             _ptr(q.scales))
@@ -303,7 +305,7 @@ def expert_layer_rows8(hidden: torch.Tensor, routing_weights: torch.Tensor, sele
     input, as in the non-EP arithmetic); a token's rows are then summed.  H and I
     multiples of 16.
     """
-    from .experts import route_checked  # experts itself uses this module's checkpoints
+    from . import experts  # experts itself uses this module's checkpoints
 
     assert isinstance(weights, Experts8), f"weights must be Experts8, got {type(weights).__name__}"
     if torch.is_grad_enabled() and (hidden.requires_grad or routing_weights.requires_grad):
@@ -320,15 +322,45 @@ def expert_layer_rows8(hidden: torch.Tensor, routing_weights: torch.Tensor, sele
     assert hidden.shape[1] == H, f"hidden size {hidden.shape[1]} != down's hidden size {H}"
     sel = selected_experts if selected_experts.dim() == 2 else selected_experts.reshape(-1, 1)
     assert sel.shape[0] == T and routing_weights.numel() == sel.numel(), "one expert and one weight per (token, k)"
-    if H % 16 or I % 16:
-        raise ValueError(f"hidden size {H} and intermediate size {I} must be multiples of 16")
-    if sel.numel() == 0:
+    sel = sel.to(torch.int64).contiguous()
+    K = sel.shape[1]
+    if mapping is not None:
+        mapping = mapping.to(torch.int64).contiguous()
+        assert mapping.dim() == 2, "mapping must be [num_sources, num_experts]"
+        S, E = mapping.shape
+    else:
+        S, E = 1, C
+    if sources is not None:
+        assert mapping is not None, "per-token sources need a mapping table"
+        sources = sources.to(torch.int64).contiguous().reshape(-1)
+        assert sources.numel() == T, "sources must have one entry per token"
+    if T == 0 or K == 0:
         return torch.zeros_like(hidden)
-    with _on(hidden.device):
-        r = route_checked(sel, C, mapping, sources, source)
+    ws_bytes = _capi.load().pmx_rows8_layer_workspace_bytes(T, K, H, I, C)
+    if ws_bytes == 0:
+        raise ValueError(f"expert_layer_rows8: {T} tokens, {K} each, through {C} copies of {H} x {I} are not supported (sizes "
+                         "must be multiples of 16, and tokens, a copy's weights and each tensor's scales below 2 GiB)")
+    dev = hidden.device
+    with _on(dev):
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+        out = torch.empty_like(hidden)
+        counts = None if recorder is None else torch.empty(C, dtype=torch.int32, device=dev)
+        experts._poll_pending_checks()
+        check = kernels.RouteCheck()
+        status_host = check.arm(dev)
+        try:
+            _capi.call(
+                _sym("pmx_rows8_layer", dt), _ptr(hidden), _ptr(routing_weights), _ptr(sel), _ptr(mapping), _ptr(sources),
+                int(source), S, E, _ptr(weights.gate_up.codes), _ptr(weights.gate_up.scales), _ptr(weights.down.codes),
+                _ptr(weights.down.scales), T, K, H, I, C, _ptr(out), _ptr(counts), _ptr(ws), ws_bytes, status_host, _stream(dev),
+            )
+        except ValueError:  # arguments refused: nothing was launched
+            check.refused()
+            raise
+        except _capi.PmxError:  # a launch failed, others of the call may run
+            check.launch_failed()
+            raise
+        experts.note_routing(check)
         if recorder is not None:
-            recorder(r.counts)
-        x, row_token, row_w = quantize_rows_routed(hidden, r.pos, routing_weights)
-        act = gemm_fc1_swiglu_rows8(x, weights.gate_up, r.offsets, row_token, row_w)
-        y = group_gemm_nt_rows8(act, weights.down, r.offsets)
-        return kernels.moe_gather(y, r.pos)
+            recorder(counts)
+    return out

@@ -326,6 +326,45 @@ def test_products_of_activations(cuda, counts, N, K, dtype):
     _near(got, c, big * 2.0**-11, dtype, "C")
 
 
+# (rows, copies, N, K): the calls' tile heights are checked on the host by tests/test_rows8.py
+LARGE = {"one group": ([4096], 4096, 1024), "ragged large": ([1500, 0, 2400, 300, 1], 4096, 1040), "many tiles": ([700] * 12, 1000, 2064)}
+
+
+@pytest.mark.parametrize("name", LARGE)
+def test_large_products_of_integers_are_exact(cuda, name):
+    counts, N, K = LARGE[name]
+    print(f"rows8 gemm {name}", flush=True)
+    M, G = sum(counts), len(counts)
+    a, b = _ints((M, K), 1).to(cuda), _ints((G, N, K), 2).to(cuda)
+    off = _offsets(counts)
+    got = rows8.group_gemm_nt_rows8(rows8.quantize_rows(a), rows8.quantize_rows(b), off.to(cuda))
+    want = torch.cat([(a[off[g]:off[g + 1]].double() @ b[g].double().t()).float().to(BF) for g in range(G)])
+    assert_exact(got, want, name)
+
+
+@pytest.mark.parametrize("name", LARGE)
+def test_large_fc1_of_integers(cuda, name):
+    """Every gate and up value is exact in fp32, so that the activations are known to the sigmoid's 2^-17."""
+    counts, N, K = LARGE[name]
+    print(f"rows8 fc1 {name}", flush=True)
+    A, G, I, T = sum(counts), len(counts), N // 32 * 16, 777
+    x, w = (_ints((T, K), 3) * 0.03125).to(cuda), (_ints((G, 2 * I, K), 4) * 0.03125).to(cuda)
+    token = torch.randint(0, T, (A,), generator=torch.Generator().manual_seed(5)).to(torch.int32).to(cuda)
+    off = _offsets(counts)
+    act = rows8.gemm_fc1_swiglu_rows8(rows8.quantize_rows(x), rows8.quantize_rows(w), off.to(cuda), token)
+    gu = torch.cat([x[token[off[g]:off[g + 1]].long()].double() @ w[g].double().t() for g in range(G)])
+    exact = gu[:, :I] * torch.sigmoid(gu[:, :I]) * gu[:, I:]
+    got = rows8.dequantize_rows(act).double()
+    # at a block's power of two a value is off by half a step, 2^-4 of it, at least 2^-10 of the power
+    e = act.scales.permute(1, 0, 2).reshape(A, -1)[:, : -(-I // 32)].double() - 127
+    unit = torch.exp2(e).repeat_interleave(32, 1)[:, :I]
+    tol = exact.abs() * (2.0**-4 + 2.0**-16) + unit * 2.0**-10
+    assert ((got - exact).abs() <= tol).all(), ((got - exact).abs() - tol).max()
+    most = torch.nn.functional.pad(exact.abs(), (0, -I % 32)).view(A, -1, 32).amax(-1)
+    low, high = most * (1 - 2.0**-16), most * (1 + 2.0**-16)
+    assert ((low <= 448 * torch.exp2(e)) & ((high > 224 * torch.exp2(e)) | (most == 0))).all(), "exponents"
+
+
 def test_rows_of_no_group_are_left_alone(cuda):
     a, b = rows8.quantize_rows(_ints((300, 64), 1).to(cuda)), rows8.quantize_rows(_ints((2, 32, 64), 2).to(cuda))
     for offsets in ([3, 20, 290], [0, 300, 300], [5, 5, 5]):
@@ -344,13 +383,17 @@ def test_rows_of_no_group_are_left_alone(cuda):
 
 
 def test_offsets_past_the_rows_are_clamped(cuda):
-    """Offsets that leave [0, M] or descend reach no memory outside the operands."""
+    """Offsets that leave [0, M] are clamped; where they descend nothing is written."""
     a, b = rows8.quantize_rows(_ints((40, 64), 1).to(cuda)), rows8.quantize_rows(_ints((3, 32, 64), 2).to(cuda))
     want = rows8.group_gemm_nt_rows8(a, b, torch.tensor([0, 10, 10, 40], dtype=torch.int32, device=cuda))
     got = rows8.group_gemm_nt_rows8(a, b, torch.tensor([-7, 10, 10, 1 << 30], dtype=torch.int32, device=cuda))
     assert_exact(got, want, "clamped")
-    rows8.group_gemm_nt_rows8(a, b, torch.tensor([40, 30, 20, 10], dtype=torch.int32, device=cuda))
-    torch.cuda.synchronize()
+    for bad in ([40, 30, 20, 10], [0, 30, 20, 40]):
+        c = torch.full((40, 32), 7.0, dtype=BF, device=cuda)
+        off = torch.tensor(bad, dtype=torch.int32, device=cuda)
+        _capi.call("pmx_rows8_group_gemm_nt", a.codes.data_ptr(), a.scales.data_ptr(), b.codes.data_ptr(), b.scales.data_ptr(),
+                   off.data_ptr(), 3, 40, 32, 64, c.data_ptr(), torch.cuda.current_stream().cuda_stream)
+        assert (c == 7.0).all()
 
 
 def test_a_row_depends_on_itself_and_its_copy_alone(cuda):
@@ -359,7 +402,7 @@ def test_a_row_depends_on_itself_and_its_copy_alone(cuda):
     a, w = _randn((2000, K), 1).to(cuda), _randn((1, N, K), 2, std=0.05).to(cuda)
     q = rows8.quantize_rows(a)
     ref = rows8.group_gemm_nt_rows8(q, rows8.quantize_rows(w), torch.tensor([0, 2000], dtype=torch.int32, device=cuda))
-    for rows, slots in ((1, 1), (20, 3), (130, 2), (300, 5)):
+    for rows, slots in ((1, 1), (16, 1), (20, 3), (130, 2), (300, 5)):
         part = rows8.quantize_rows(a[:rows])
         counts = [0] * slots
         counts[slots // 2] = rows
@@ -367,6 +410,21 @@ def test_a_row_depends_on_itself_and_its_copy_alone(cuda):
         ww[slots // 2] = w[0]
         got = rows8.group_gemm_nt_rows8(part, rows8.quantize_rows(ww), _offsets(counts).to(cuda))
         assert_exact(got, ref[:rows], f"{rows} rows in slot {slots // 2}")
+
+
+def test_every_tiling_gives_the_same_bits(cuda):
+    """4096 rows run on 256-row tiles, 200 on 128-row ones, 10 on 32-row ones."""
+    N, K = 4096, 1024
+    x, w = _randn((4096, K), 1).to(cuda), _randn((1, N, K), 2, std=0.03).to(cuda)
+    qw = rows8.quantize_rows(w)
+    nt, fc1 = [], []
+    for rows in (4096, 200, 10):
+        q, off = rows8.quantize_rows(x[:rows]), torch.tensor([0, rows], dtype=torch.int32, device=cuda)
+        nt.append(rows8.group_gemm_nt_rows8(q, qw, off))
+        fc1.append(rows8.gemm_fc1_swiglu_rows8(q, qw, off).codes.view(torch.uint8))
+    for rows, a, b in zip((200, 10), nt[1:], fc1[1:]):
+        assert_exact(a, nt[0][:rows], f"{rows} rows")
+        assert torch.equal(b, fc1[0][:rows]), f"{rows} rows of fc1"
 
 
 @pytest.mark.parametrize("dtype", [BF, F16])

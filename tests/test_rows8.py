@@ -2,6 +2,9 @@
 type, the C ABI's refusals, and the wrappers' checks (all before any launch)."""
 
 import ctypes
+import shutil
+import subprocess
+from pathlib import Path
 
 import numpy as np
 import pytest
@@ -10,6 +13,9 @@ import torch
 import placemoe_amd
 from oracle import rows8_oracle as O
 from placemoe_amd import _capi, experts, rows8
+from tests import test_gpu_rows8
+
+ROOT = Path(__file__).resolve().parents[1]
 
 BF = torch.bfloat16
 
@@ -128,3 +134,63 @@ def test_checkpoint_settings_are_checked():
     with pytest.raises(ValueError, match="activation checkpoint"):
         experts.expert_layer(z, z[:, :1], torch.zeros((2, 1), dtype=torch.int64), z, fc1_1_2_weight=z,
                              activation_checkpoint="bf16")
+
+
+@pytest.fixture(scope="module")
+def tiling(tmp_path_factory):
+    cxx = shutil.which("g++") or shutil.which("c++")
+    if cxx is None:
+        pytest.skip("no host C++ compiler")
+    exe = tmp_path_factory.mktemp("rule") / "rows8_rule"
+    subprocess.run([cxx, "-O2", "-std=c++17", f"-I{ROOT / 'placemoe_amd' / 'csrc'}", str(ROOT / "tests" / "rows8_rule_main.cpp"),
+                    "-o", str(exe)], check=True)
+
+    def ask(calls):
+        """calls: (kind, rows, copies, N, K) -> tile heights, on 256 CUs."""
+        lines = "\n".join(f"{('nt', 'fc1').index(k)} {' '.join(map(str, c))} 256" for k, *c in calls)
+        out = subprocess.run([str(exe)], input=lines, check=True, capture_output=True, text=True).stdout
+        return [int(x) for x in out.split()]
+
+    return ask
+
+
+def test_tiling_rule_takes_the_faster_one(tiling):
+    measured = {  # us with 32 x 256, 128 x 128 and 256 x 256 tiles
+        ("nt", 640, 160, 1536, 2048): (91, 96, 121), ("nt", 10240, 160, 1536, 2048): (149, 105, 127),
+        ("nt", 96000, 160, 1536, 2048): (857, 421, 355), ("nt", 2304, 12, 1000, 1104): (20, 13, 20),
+        ("nt", 32000, 16, 4096, 7168): (2439, 1136, 848), ("nt", 64, 16, 4096, 7168): (80, 81, 105),
+        ("fc1", 640, 160, 1536, 2048): (95, 119, 196), ("fc1", 10240, 160, 1536, 2048): (171, 131, 205),
+        ("fc1", 96000, 160, 1536, 2048): (1146, 653, 606), ("fc1", 1536, 8, 1536, 2048): (36, 25, 51),
+        ("fc1", 32000, 16, 4096, 7168): (2997, 1722, 1502),
+    }
+    for call, height in zip(measured, tiling(list(measured))):
+        us = dict(zip((32, 128, 256), measured[call]))
+        assert us[height] <= 1.05 * min(us.values()), (call, height)
+
+
+def test_gpu_cases_reach_every_tiling(tiling):
+    def heights(kind, cases):
+        return {n: h for n, h in zip(cases, tiling([(kind, sum(c), len(c), N, K) for c, N, K in cases.values()]))}
+
+    small = heights("nt", test_gpu_rows8.LAYOUTS)
+    assert set(small.values()) == {32, 128}
+    assert 256 in heights("nt", test_gpu_rows8.LARGE).values()
+    assert 256 in heights("fc1", {n: (c, N // 32 * 32, K) for n, (c, N, K) in test_gpu_rows8.LARGE.items()}).values()
+    # one row of the same copy in calls of every tiling (test_a_row_depends_on_itself_and_its_copy_alone)
+    assert set(tiling([("nt", rows, 1, 264, 1104) for rows in (1, 16, 20, 130)])) == {32, 128}
+
+
+def test_layer_workspace(tiling):
+    lib = _capi.load()
+    ws = lib.pmx_rows8_layer_workspace_bytes
+    A, H, I, C = 96 * 8, 2048, 768, 160
+    assert ws(96, 8, H, I, C) >= 96 * H + A * I + 2 * A * H + lib.pmx_route_workspace_bytes(A, C)
+    assert ws(96, 8, H + 8, I, C) == 0 and ws(96, 0, H, I, C) == 0 and ws(96, 8, H, I, 5000) == 0
+    assert ws(1 << 20, 8, 1 << 12, I, C) == 0  # 4 GiB of tokens
+    layer = lib.pmx_rows8_layer
+    args = [P] * 5 + [0, 1, C] + [P] * 4 + [96, 8, H, I, C, P, None]
+    assert layer(*args, P, ws(96, 8, H, I, C) - 1, None, None) == ARG
+    assert layer(*args, None, 1 << 40, None, None) == ARG
+    assert layer(*args, ctypes.c_void_p(8), 1 << 40, None, None) == SHAPE
+    assert layer(None, *args[1:], P, 1 << 40, None, None) == ARG
+    assert layer(*args[:15], 100, *args[16:], P, 1 << 40, None, None) == SHAPE
