@@ -34,42 +34,66 @@ __device__ __forceinline__ void st8(uint8_t* p, const uint2 v) {
   *reinterpret_cast<u32x2_a1*>(p) = u32x2_a1{v.x, v.y};
 }
 
-// Columns c .. c+7 of a row of N (elements past the row: zero).
+// The row's last chunk, where fewer than 8 columns are left: the 8 columns that
+// end with the row, shifted, so that every lane makes the same load (element by
+// element the one lane held up its wave: 1531 rows of 1412 columns took 11.3 us
+// to write, of 1408 columns 7.1); its stores go out as 4, 2 and 1 elements.
+
+// Columns c .. c+7 of a row of N, c < N (elements past the row: zero).
 __device__ __forceinline__ uint4 load8(const bf16_t* row, int64_t c, int64_t N) {
-  if (c + 8 <= N) return ld16(row + c);
-  uint32_t w[4] = {0, 0, 0, 0};
-#pragma unroll
-  for (int j = 0; j < 8; ++j)
-    if (c + j < N) w[j / 2] |= (uint32_t)row[c + j] << (16 * (j & 1));
-  return make_uint4(w[0], w[1], w[2], w[3]);
-}
-__device__ __forceinline__ void store8(bf16_t* row, int64_t c, int64_t N, const uint4 v) {
-  if (c + 8 <= N) {
-    st16(row + c, v);
-  } else {
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (c + j < N) row[c + j] = (bf16_t)(w[j / 2] >> (16 * (j & 1)));
+  if (N < 8) {
+    uint64_t w[2] = {0, 0};
+    for (int j = 0; c + j < N; ++j) w[j / 4] |= (uint64_t)row[c + j] << (16 * (j & 3));
+    return make_uint4((uint32_t)w[0], (uint32_t)(w[0] >> 32), (uint32_t)w[1], (uint32_t)(w[1] >> 32));
   }
+  const int64_t at = c + 8 <= N ? c : N - 8;
+  const uint4 v = ld16(row + at);
+  const int s = 16 * (int)(c - at);
+  if (s == 0) return v;
+  uint64_t lo = (uint64_t)v.y << 32 | v.x, hi = (uint64_t)v.w << 32 | v.z;
+  lo = s < 64 ? lo >> s | hi << (64 - s) : hi >> (s - 64);
+  hi = s < 64 ? hi >> s : 0;
+  return make_uint4((uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32));
 }
 __device__ __forceinline__ uint2 load8(const uint8_t* row, int64_t c, int64_t N) {
-  if (c + 8 <= N) return ld8(row + c);
-  uint32_t w[2] = {0, 0};
-#pragma unroll
-  for (int j = 0; j < 8; ++j)
-    if (c + j < N) w[j / 4] |= (uint32_t)row[c + j] << (8 * (j & 3));
-  return make_uint2(w[0], w[1]);
+  uint64_t w = 0;
+  if (N < 8) {
+    for (int j = 0; c + j < N; ++j) w |= (uint64_t)row[c + j] << (8 * j);
+  } else {
+    const int64_t at = c + 8 <= N ? c : N - 8;
+    const uint2 v = ld8(row + at);
+    w = ((uint64_t)v.y << 32 | v.x) >> (8 * (int)(c - at));
+  }
+  return make_uint2((uint32_t)w, (uint32_t)(w >> 32));
+}
+
+typedef uint64_t u64_a1 __attribute__((aligned(1)));
+typedef uint32_t u32_a1 __attribute__((aligned(1)));
+typedef uint16_t u16_a1 __attribute__((aligned(1)));
+
+__device__ __forceinline__ void store8(bf16_t* row, int64_t c, int64_t N, const uint4 v) {
+  bf16_t* p = row + c;
+  if (c + 8 <= N) {
+    st16(p, v);
+    return;
+  }
+  const int n = (int)(N - c);
+  uint64_t w = (uint64_t)v.y << 32 | v.x;
+  if (n & 4) *reinterpret_cast<u64_a1*>(p) = w, p += 4, w = (uint64_t)v.w << 32 | v.z;
+  if (n & 2) *reinterpret_cast<u32_a1*>(p) = (uint32_t)w, p += 2, w >>= 32;
+  if (n & 1) *p = (bf16_t)w;
 }
 __device__ __forceinline__ void store8(uint8_t* row, int64_t c, int64_t N, const uint2 v) {
+  uint8_t* p = row + c;
   if (c + 8 <= N) {
-    st8(row + c, v);
-  } else {
-    const uint32_t w[2] = {v.x, v.y};
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (c + j < N) row[c + j] = (uint8_t)(w[j / 4] >> (8 * (j & 3)));
+    st8(p, v);
+    return;
   }
+  const int n = (int)(N - c);
+  uint32_t w = v.x;
+  if (n & 4) *reinterpret_cast<u32_a1*>(p) = w, p += 4, w = v.y;
+  if (n & 2) *reinterpret_cast<u16_a1*>(p) = (uint16_t)w, p += 2, w >>= 16;
+  if (n & 1) *p = (uint8_t)w;
 }
 
 // fp32 bits of the largest finite magnitude among 8 elements (16-bit
@@ -102,17 +126,16 @@ struct RowMap {
   bf16_t* row_w;       // [T * K]
 };
 
-constexpr int kTileRows = 32;
-
-// A block: 32 rows x 512 columns of one group, eight rows per wave, a lane's
+// A block: 4 * PER rows x 512 columns of one group, PER rows per wave, a lane's
 // 8 columns in one 16-byte load; all of a wave's rows are in flight
-// together.  32 rows, because their exponents are then 512 contiguous bytes
-// that one XCD's L2 collects.  A block of 32 columns is four lanes.
-template <class E, int FMT>
+// together.  PER = 8: the 32 rows' exponents are 512 contiguous bytes that
+// one XCD's L2 collects.  PER = 2, where that would be fewer blocks than CUs
+// have room for: more of them.  A block of 32 columns is four lanes.
+template <class E, int FMT, int PER>
 __global__ __launch_bounds__(256) void quantize_rows_kernel(const bf16_t* __restrict__ x, int64_t ldx, int64_t gsx,
                                                             int64_t R, int64_t N, int64_t row_tiles, RowMap map,
                                                             uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
-  constexpr int PER = kTileRows / 4;
+  constexpr int kTileRows = 4 * PER;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t B = (N + kScaleGroup - 1) / kScaleGroup;
   // column groups fastest: a row's blocks run side by side
@@ -128,6 +151,16 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const bf16_t* __rest
   for (int i = 0; i < PER; ++i) {
     const int64_t r = r0 + i * 4 + wave;
     v[i] = r < R && c < N ? load8(xg + r * ldx, c, N) : make_uint4(0, 0, 0, 0);
+  }
+  if (map.pos != nullptr && b == 0) {
+    const int32_t rows = (int32_t)(R - r0 < kTileRows ? R - r0 : kTileRows), A = (int32_t)R * map.K;  // T * K fits
+    for (int32_t i = threadIdx.x; i < rows * map.K; i += 256) {
+      const int32_t a = (int32_t)r0 * map.K + i, p = map.pos[a];
+      if (p >= 0 && p < A) {
+        map.row_token[p] = (int32_t)((uint32_t)a / (uint32_t)map.K);
+        map.row_w[p] = map.w[a];
+      }
+    }
   }
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
@@ -146,16 +179,6 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const bf16_t* __rest
       if ((lane & 3) == 0) sg[r * kScaleBytes + (lane >> 2)] = (uint8_t)byte;
     }
   }
-  if (map.pos != nullptr && b == 0) {
-    const int32_t rows = (int32_t)(R - r0 < kTileRows ? R - r0 : kTileRows), A = (int32_t)R * map.K;  // T * K fits
-    for (int32_t i = threadIdx.x; i < rows * map.K; i += 256) {
-      const int32_t a = (int32_t)r0 * map.K + i, p = map.pos[a];
-      if (p >= 0 && p < A) {
-        map.row_token[p] = (int32_t)((uint32_t)a / (uint32_t)map.K);
-        map.row_w[p] = map.w[a];
-      }
-    }
-  }
 }
 
 // ---------------------------------------------------------------------------
@@ -172,12 +195,11 @@ __device__ __forceinline__ float to_range(float v) {
 
 // A wave: 512 columns of PER rows; row r goes to out[r], or with pos [R, K] to
 // out[pos[r, k]] for every k (rows outside the output are not written).
-template <class E, int FMT>
+template <class E, int FMT, int PER>
 __global__ __launch_bounds__(256) void dequantize_rows_kernel(const uint8_t* __restrict__ codes,
                                                               const uint8_t* __restrict__ scales,
                                                               const int32_t* __restrict__ pos, int64_t R, int32_t K,
                                                               int64_t N, bf16_t* __restrict__ out) {
-  constexpr int PER = 4;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t B = (N + kScaleGroup - 1) / kScaleGroup;
   const int64_t b = blockIdx.x % (uint32_t)B, r0 = (int64_t)(blockIdx.x / (uint32_t)B) * (4 * PER);
@@ -295,6 +317,12 @@ __global__ __launch_bounds__(256) void swiglu_bwd_rows8_kernel(const bf16_t* __r
 // Launches
 // ---------------------------------------------------------------------------
 
+// Blocks of eight rows per wave that fill the chip (two per CU).
+#ifndef PMX_R8_MANY
+#define PMX_R8_MANY 512
+#endif
+constexpr int64_t kManyBlocks = PMX_R8_MANY;
+
 // a * b, or -1 where it passes 2^62 (a, b >= 0).
 int64_t product(int64_t a, int64_t b) { return a != 0 && b > (((int64_t)1 << 62) / a) ? -1 : a * b; }
 
@@ -304,15 +332,22 @@ int quantize_t(const void* x, int64_t ldx, int64_t gsx, int64_t G, int64_t R, in
   if (G < 0 || R < 0 || N < 0 || ldx < N || (format != kFmtE4M3 && format != kFmtInt8)) return PMX_ERR_ARG;
   if (G == 0 || R == 0 || N == 0) return PMX_OK;
   if (!x || !codes || !scales) return PMX_ERR_ARG;
-  const int64_t B = (N + kScaleGroup - 1) / kScaleGroup, tiles = (R + kTileRows - 1) / kTileRows;
-  const int64_t blocks = product(product(G, tiles) < 0 ? -1 : G * tiles, B);
-  if (product(G, R) < 0 || product(G * R, ldx) < 0 || blocks < 0 || blocks > INT32_MAX) return PMX_ERR_SHAPE;
+  const int64_t B = (N + kScaleGroup - 1) / kScaleGroup;
+  if (product(G, R) < 0 || product(G * R, ldx) < 0 || product(G * R, B) < 0) return PMX_ERR_SHAPE;
+  const auto blocks = [&](int64_t rows) { return G * ((R + rows - 1) / rows) * B; };
+  const int per = blocks(32) >= kManyBlocks ? 8 : 2;
+  const int64_t grid = blocks(4 * per), tiles = (R + 4 * per - 1) / (4 * per);
+  if (grid > INT32_MAX) return PMX_ERR_SHAPE;
   const auto run = [&](auto kernel) {
-    kernel<<<(unsigned)blocks, 256, 0, stream>>>((const bf16_t*)x, ldx, gsx, R, N, tiles, map, (uint8_t*)codes,
-                                                 (uint8_t*)scales);
+    kernel<<<(unsigned)grid, 256, 0, stream>>>((const bf16_t*)x, ldx, gsx, R, N, tiles, map, (uint8_t*)codes, (uint8_t*)scales);
   };
-  if (format == kFmtE4M3) run(quantize_rows_kernel<E, kFmtE4M3>);
-  else run(quantize_rows_kernel<E, kFmtInt8>);
+  if (format == kFmtE4M3) {
+    if (per == 8) run(quantize_rows_kernel<E, kFmtE4M3, 8>);
+    else run(quantize_rows_kernel<E, kFmtE4M3, 2>);
+  } else {
+    if (per == 8) run(quantize_rows_kernel<E, kFmtInt8, 8>);
+    else run(quantize_rows_kernel<E, kFmtInt8, 2>);
+  }
   PMX_LAUNCH_CHECK();
   return PMX_OK;
 }
@@ -336,13 +371,22 @@ int dequantize_t(const void* codes, const void* scales, const int32_t* pos, int6
   if (R == 0 || N == 0) return PMX_OK;
   if (!codes || !scales || !out) return PMX_ERR_ARG;
   if (pos != nullptr && R > INT32_MAX / K) return PMX_ERR_SHAPE;  // positions are int32
-  const int64_t B = (N + kScaleGroup - 1) / kScaleGroup, blocks = product((R + 15) / 16, B);
-  if (product(R, N) < 0 || blocks < 0 || blocks > INT32_MAX) return PMX_ERR_SHAPE;
+  const int64_t B = (N + kScaleGroup - 1) / kScaleGroup;
+  if (product(R, N) < 0 || product(R, B) < 0) return PMX_ERR_SHAPE;
+  const auto blocks = [&](int64_t rows) { return (R + rows - 1) / rows * B; };
+  const int per = blocks(16) >= kManyBlocks ? 4 : 1;
+  if (blocks(4 * per) > INT32_MAX) return PMX_ERR_SHAPE;
   const auto run = [&](auto kernel) {
-    kernel<<<(unsigned)blocks, 256, 0, stream>>>((const uint8_t*)codes, (const uint8_t*)scales, pos, R, K, N, (bf16_t*)out);
+    kernel<<<(unsigned)blocks(4 * per), 256, 0, stream>>>((const uint8_t*)codes, (const uint8_t*)scales, pos, R, K, N,
+                                                          (bf16_t*)out);
   };
-  if (format == kFmtE4M3) run(dequantize_rows_kernel<E, kFmtE4M3>);
-  else run(dequantize_rows_kernel<E, kFmtInt8>);
+  if (format == kFmtE4M3) {
+    if (per == 4) run(dequantize_rows_kernel<E, kFmtE4M3, 4>);
+    else run(dequantize_rows_kernel<E, kFmtE4M3, 1>);
+  } else {
+    if (per == 4) run(dequantize_rows_kernel<E, kFmtInt8, 4>);
+    else run(dequantize_rows_kernel<E, kFmtInt8, 1>);
+  }
   PMX_LAUNCH_CHECK();
   return PMX_OK;
 }

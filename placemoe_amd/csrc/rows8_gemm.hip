@@ -653,7 +653,8 @@ int cu_count() {
 }
 
 // The tilings of rows8_rule.h.
-using Rows32 = Cfg8<1, 4, 1, 2, 3, 1>;   // 32 x 256, one wave per 32 x 64
+using Narrow32 = Cfg8<1, 1, 1, 2, 3, 3>;  // 32 x 64, one wave
+using Rows32 = Cfg8<1, 4, 1, 2, 3, 1>;    // 32 x 256, one wave per 32 x 64
 using Rows128 = Cfg8<2, 2, 2, 2, 2, 2>;  // 128 x 128, 64 x 64
 using Rows256 = Cfg8<2, 2, 4, 4, 2, 1>;  // 256 x 256, 128 x 128
 
@@ -680,6 +681,7 @@ int launch(const Params8& P, pmx_stream_t stream) {
   return launch_cfg<E, KIND, PMX_R8_FORCE>(P, cus, stream);
 #endif
   switch (pmx::rows8_tiling(KIND, P.M, P.G, P.N, P.K, cus)) {
+    case 0: return launch_cfg<E, KIND, Narrow32>(P, cus, stream);
     case Rows32::BM: return launch_cfg<E, KIND, Rows32>(P, cus, stream);
     case Rows128::BM: return launch_cfg<E, KIND, Rows128>(P, cus, stream);
     default: return launch_cfg<E, KIND, Rows256>(P, cus, stream);
@@ -705,7 +707,7 @@ int check(const Params8& P) {
 
 template <int KIND>
 bool any_tiles_fit(const Params8& P) {
-  return tiles_fit<KIND, Rows32>(P, 1024);  // the most tiles, and more CUs than there are
+  return tiles_fit<KIND, Narrow32>(P, 1024);  // the most tiles, and more CUs than there are
 }
 
 template <class E>

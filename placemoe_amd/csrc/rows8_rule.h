@@ -1,6 +1,8 @@
 // Which tiles a grouped GEMM over 8-bit rows runs on.
 //
-// The host knows the rows and the copies, not the counts.  Three tilings:
+// The host knows the rows and the copies, not the counts.  Four tilings:
+//   32 x 64, a wave per block, three blocks per CU: so few tiles that wider ones
+//     would leave CUs idle (one token);
 //   32 x 256, one block per CU, three stages: copies with few rows, where the
 //     call reads every copy's weights once and the matrix cores idle;
 //   128 x 128, two blocks per CU: one block's epilogue, tile switch and loads run
@@ -16,6 +18,9 @@
 //   16     400    7168  2048  254 / 108 / 110    346 / 195 / 212
 //   16     2000   4096  7168    - /1136 / 848      - /1722 /1502
 //   12     192    1000  1104   20 /  13 /  20      -
+// 32 x 64 against 32 x 256 (weights not in a cache; NT, fc1): 8 rows over 160 copies of
+// 1536 x 2048 20 / 23, 22 / 26; 64 over 128 63 / 70, 65 / 74; 768 over 160 149 / 152,
+// 152 / 152; 2400 over 160 163 / 153, 166 / 154.
 // Past the few-rows line the rounds of tiles decide: a round costs its K-tiles
 // and a fixed part (epilogue and tile switch), both fitted to such calls.  Over
 // 170 calls (8 to 160 copies, 4 to 2000 rows, 5 layers) the choice takes 1.02
@@ -38,12 +43,12 @@ constexpr int64_t kRows8Few[2] = {16, 32};
 constexpr double kRows8Round128[2][2] = {{1.25, 2.0}, {1.9, 2.5}};
 constexpr double kRows8Round256[2][2] = {{1.7, 6.0}, {2.9, 10.0}};
 
-// The m-tile height, 32, 128 or 256, for `rows` rows over `copies` copies, N rows of a
+// The m-tile height, 32 (0: 32 x 64 tiles), 128 or 256, for `rows` rows over `copies` copies, N rows of a
 // copy's B (fc1: 2 I), K deep, on `cus` CUs.  kind: 0 NT, 1 FC1.
 inline int rows8_tiling(int kind, int64_t rows, int64_t copies, int64_t N, int64_t K, int64_t cus) {
   const auto div_up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
   const int64_t active = rows < copies ? rows : copies, nk = div_up(K, 128);
-  if (rows <= kRows8Few[kind] * active) return 32;
+  if (rows <= kRows8Few[kind] * active) return active * div_up(N, 256) <= 2 * cus ? 0 : 32;
   // a copy's last tile half full on average; an eighth of the copies past their first tile
   const auto cost = [&](int64_t tile, int64_t blocks, const double (&round)[2]) {
     const int64_t spread = active + active / 8, even = rows / tile + active / 2;

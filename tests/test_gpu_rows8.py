@@ -412,6 +412,33 @@ def test_a_row_depends_on_itself_and_its_copy_alone(cuda):
         assert_exact(got, ref[:rows], f"{rows} rows in slot {slots // 2}")
 
 
+# few rows: 32 x 64 tiles, and 32 x 256 ones
+FEW = {"few tiles": ([2] * 100, 1024, 272), "many tiles": ([3, 0, 7] * 100, 1032, 272)}
+
+
+@pytest.mark.parametrize("name", FEW)
+def test_few_rows(cuda, name):
+    counts, N, K = FEW[name]
+    M, G, I = sum(counts), len(counts), N // 32 * 16
+    a, b, off = _ints((M, K), 1).to(cuda), _ints((G, N, K), 2).to(cuda), _offsets(counts)
+    print(f"rows8 few {name}", flush=True)
+    got = rows8.group_gemm_nt_rows8(rows8.quantize_rows(a), rows8.quantize_rows(b), off.to(cuda))
+    group = torch.repeat_interleave(torch.arange(G), torch.tensor(counts)).to(cuda)
+    want = torch.cat([torch.bmm(b[group[i:i + 50]].float(), a[i:i + 50].float().unsqueeze(2))[..., 0] for i in range(0, M, 50)])
+    assert_exact(got, want.to(BF), name)
+    # fc1 against the same call with every row in a group of its own copy's weights, on 128-row tiles
+    w = rows8.quantize_rows(_randn((G, 2 * I, K), 3, std=0.06).to(cuda))
+    q = rows8.quantize_rows(_randn((M, K), 4).to(cuda))
+    act = rows8.gemm_fc1_swiglu_rows8(q, w, off.to(cuda))
+    for g in (0, 2, G - 1):
+        rows = slice(int(off[g]), int(off[g + 1]))
+        many = torch.arange(rows.start, rows.stop, dtype=torch.int32, device=cuda).repeat(100)
+        one = rows8.Rows8(w.codes[g:g + 1].contiguous(), w.scales[g:g + 1].contiguous(), BF)
+        ref = rows8.gemm_fc1_swiglu_rows8(q, one, torch.tensor([0, many.numel()], dtype=torch.int32, device=cuda), many)
+        n = rows.stop - rows.start
+        assert torch.equal(act.codes.view(torch.uint8)[rows], ref.codes.view(torch.uint8)[:n]), f"copy {g}"
+
+
 def test_every_tiling_gives_the_same_bits(cuda):
     """4096 rows run on 256-row tiles, 200 on 128-row ones, 10 on 32-row ones."""
     N, K = 4096, 1024

@@ -164,7 +164,7 @@ def test_tiling_rule_takes_the_faster_one(tiling):
         ("fc1", 32000, 16, 4096, 7168): (2997, 1722, 1502),
     }
     for call, height in zip(measured, tiling(list(measured))):
-        us = dict(zip((32, 128, 256), measured[call]))
+        us = dict(zip((32, 128, 256, 0), measured[call] + measured[call][:1]))
         assert us[height] <= 1.05 * min(us.values()), (call, height)
 
 
@@ -173,11 +173,13 @@ def test_gpu_cases_reach_every_tiling(tiling):
         return {n: h for n, h in zip(cases, tiling([(kind, sum(c), len(c), N, K) for c, N, K in cases.values()]))}
 
     small = heights("nt", test_gpu_rows8.LAYOUTS)
-    assert set(small.values()) == {32, 128}
+    assert set(small.values()) == {0, 32, 128}
     assert 256 in heights("nt", test_gpu_rows8.LARGE).values()
     assert 256 in heights("fc1", {n: (c, N // 32 * 32, K) for n, (c, N, K) in test_gpu_rows8.LARGE.items()}).values()
     # one row of the same copy in calls of every tiling (test_a_row_depends_on_itself_and_its_copy_alone)
-    assert set(tiling([("nt", rows, 1, 264, 1104) for rows in (1, 16, 20, 130)])) == {32, 128}
+    assert set(tiling([("nt", rows, 1, 264, 1104) for rows in (1, 16, 20, 130)])) == {0, 128}
+    few = [(k, sum(c), len(c), N, K) for k in ("nt", "fc1") for c, N, K in test_gpu_rows8.FEW.values()]
+    assert tiling(few) == [0, 32] * 2
 
 
 def test_layer_workspace(tiling):
