@@ -82,8 +82,9 @@ def _rows8(name: str, q: Rows8, dims: int) -> torch.dtype:
     assert q.dtype in HALF, f"{name} must stand for bfloat16 or float16 rows, got {q.dtype}"
     assert q.scales.dtype == torch.uint8, f"{name} scales must be uint8, got {q.scales.dtype}"
     assert q.codes.dim() == dims, f"{name} must have {dims} dimensions, got {q.codes.dim()}"
-    want = scales_shape(q.codes.shape)
-    assert tuple(q.scales.shape) == want, f"{name} scales must be {want}, got {tuple(q.scales.shape)}"
+    assert q.scales.shape == scales_shape(q.codes.shape), (
+        f"{name} scales must be {scales_shape(q.codes.shape)}, got {tuple(q.scales.shape)}"
+    )
     assert q.codes.is_contiguous() and q.scales.is_contiguous(), f"{name} must be contiguous"
     return q.dtype
 
@@ -100,22 +101,23 @@ def _indices(name: str, t: torch.Tensor, numel: int | None = None) -> None:
     assert numel is None or t.numel() == numel, f"{name} must have {numel} entries, got {t.numel()}"
 
 
-_HERE = contextlib.nullcontext()
-
-
 def _on(dev: torch.device):
     """The launch device: a kernel starts on the current one, whatever its stream."""
-    return _HERE if dev.index == torch._C._cuda_getDevice() else torch.cuda.device(dev)
+    return contextlib.nullcontext() if dev.index == torch._C._cuda_getDevice() else torch.cuda.device(dev)
 
 
 def _launch(name: str, dtype: torch.dtype, dev: torch.device, *args) -> None:
-    with _on(dev):
+    if dev.index == torch._C._cuda_getDevice():
+        _capi.call(_sym(name, dtype), *args, _stream(dev))
+        return
+    with torch.cuda.device(dev):
         _capi.call(_sym(name, dtype), *args, _stream(dev))
 
 
 def _empty(shape, fmt: torch.dtype, dtype: torch.dtype, dev: torch.device) -> Rows8:
+    *lead, R, N = shape
     return Rows8(torch.empty(shape, dtype=fmt, device=dev),
-                 torch.empty(scales_shape(shape), dtype=torch.uint8, device=dev), dtype)
+                 torch.empty((*lead, -(-N // GROUP), R, 16), dtype=torch.uint8, device=dev), dtype)
 
 
 # ---------------------------------------------------------------------------
