@@ -525,7 +525,7 @@ int pmx_rows8_group_gemm_nt(const void* a, const void* a_scales, const void* b, 
  * X: T rows of H (codes and scales); row_token int32 [A], NULL: row r is X's
  * row r (T = A); a token outside [0, T) reads as zeros.  w [G, 2I, H], gate
  * rows first.  row_w bf16 [A], NULL: 1.  act: codes [A, I]; of its scales the
- * bytes of the columns' multiple of 128 are written.  H and I multiples of
+ * bytes up to the columns' next multiple of 128, 256 at least, are written.  H and I multiples of
  * 16; T*H below 2 GiB with row_token. */
 int pmx_rows8_gemm_fc1_swiglu(const void* x, const void* x_scales, int64_t T, const int32_t* row_token,
                               const void* w, const void* w_scales, const int32_t* offsets, int32_t G,

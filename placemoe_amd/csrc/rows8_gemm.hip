@@ -39,12 +39,6 @@ namespace {
 typedef int32_t i32x8_t __attribute__((ext_vector_type(8)));
 typedef int32_t i32x4_t __attribute__((ext_vector_type(4)));
 
-#ifndef PMX_R8_LOAD_GROUPS
-#define PMX_R8_LOAD_GROUPS 99
-#endif
-#ifndef PMX_R8_RG
-#define PMX_R8_RG 6
-#endif
 constexpr int kMaxGroups = 2048;  // groups (their m-tiles' prefix in LDS)
 constexpr int KT = 128;           // depth of a K-tile
 constexpr int kStreaming = 2;     // cache policy of stores that this kernel does not read back
@@ -243,10 +237,11 @@ __device__ __forceinline__ void epilogue(const Params8& P, const Place& at, int 
       __builtin_amdgcn_sched_barrier(0);  // one tile's registers at a time
     } else {
       const float w = in && P.row_w != nullptr ? E::to_f32(P.row_w[r]) : 1.0f;
-      // fc2's last K-tile takes along the blocks past I in the last 128 columns: those that no tile covers stand,
+      // fc2's K-tiles take along the blocks past I in their last 128 columns: those that no tile covers stand,
       // as the others of zeros do, beside 2^0
       if (in && h == 0 && wn == CF::WN - 1 && (int64_t)(at.ntile + 1) * (CF::BN / 2) >= P.I) {
-        for (int64_t j = (int64_t)(at.ntile + 1) * (CF::BN / 2); j < (P.I + KT - 1) / KT * KT; j += kScaleBlock)
+        const int64_t end = P.I <= KT ? 2 * KT : (P.I + KT - 1) / KT * KT;  // two K-tiles at least
+        for (int64_t j = (int64_t)(at.ntile + 1) * (CF::BN / 2); j < end; j += kScaleBlock)
           P.qs[(j / kScaleGroup * P.M + r) * kScaleBytes + j / kScaleBlock % 16] = 127;
       }
 #pragma unroll
@@ -331,7 +326,9 @@ __global__ __launch_bounds__(CF::NTH, CF::NW * CF::BPC / 4) void rows8_grouped_g
   }
   const int32_t ntn = (int32_t)(KIND == FC18 ? (P.I + CF::BN / 2 - 1) / (CF::BN / 2) : (P.N + CF::BN - 1) / CF::BN);
   const int32_t total = uni(tend[G - 1]) * ntn;  // the host has checked that it fits
-  const int32_t nk = (int32_t)((P.K + KT - 1) / KT);
+  // NT by row halves: a tile's first and last K-tiles are two (the second past K, zeros, where there is but one).
+  constexpr bool kHalves = KIND == NT8 && CF::FM % 2 == 0;
+  const int32_t ktiles = (int32_t)((P.K + KT - 1) / KT), nk = kHalves && ktiles < 2 ? 2 : ktiles;
   // Blocks go round-robin over the XCDs: each XCD walks its own eighth of the
   // tile list, its blocks round-robin within it.
   int32_t first = blockIdx.x, step = gridDim.x, end = total;
@@ -393,7 +390,7 @@ __global__ __launch_bounds__(CF::NTH, CF::NW * CF::BPC / 4) void rows8_grouped_g
   auto issue = [&](auto jj) __attribute__((always_inline)) {
     constexpr int J = decltype(jj)::value;
     // kOOB's bit on top of the offset where the lane lies past K
-    const uint32_t past = i_kt == nk - 1 ? ld.past : 0u;
+    const uint32_t past = i_kt < ktiles - 1 ? 0u : i_kt == ktiles - 1 ? ld.past : ~0u;
     const uint32_t off = ld.off[J] | ((past >> J) << 31);
     char* stage = lds + i_stage * CF::STAGE;
     if constexpr (J < CF::QA) dma16(ld.a, stage + (J * NW + wave) * 1024, off, (uint32_t)i_kt * KT);
@@ -421,7 +418,7 @@ __global__ __launch_bounds__(CF::NTH, CF::NW * CF::BPC / 4) void rows8_grouped_g
   };
   // K-tiles in flight before the first is multiplied: FC1 refills a stage once its
   // last quarter is in registers, NT from the next K-tile on.
-  constexpr int AHEAD = KIND == FC18 ? CF::NST : CF::NST - 1;
+  constexpr int AHEAD = KIND == FC18 || kHalves ? CF::NST : CF::NST - 1;
 #pragma unroll
   for (int s = 0; s < AHEAD; ++s) {
     issue_scales();
@@ -452,7 +449,140 @@ __global__ __launch_bounds__(CF::NTH, CF::NW * CF::BPC / 4) void rows8_grouped_g
     block_barrier();
   };
 
-  if constexpr (KIND == NT8) {
+  if constexpr (kHalves) {
+    // In half ks of the K-tile lane l holds row l%32, columns 16 h .. + 15 and
+    // 32 + 16 h .. + 15 of the half's 64 (h = l/32), and the exponent of its
+    // block h.
+    //
+    // A K-tile is multiplied in four steps: the first half of the tile's rows in
+    // its two halves of K, then the second.  Each operand register is read
+    // again in the step behind its last use, so that one set of them does, and
+    // a stage is read within three steps: from the step before its K-tile's
+    // first to its second.  Its refill then has five steps to land; with the
+    // K halves outermost (all rows in each) it had four (65536 rows over 16
+    // groups of 4096 x 7168, operands of zeros, so that power does not limit the
+    // clock: 1533 -> 1418 us; with values 1710 and 1741, at 1.7 GHz).
+    constexpr int HM = CF::FM / 2, HN = HM * CF::FN, HL = L / 2;
+    int32_t at[2][2];
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) at[ks][e] = r32 * KT + (((ks * 4 + e * 2 + h) ^ kc_swz(r32)) << 4);
+    const uint32_t pick = 0x06040200u + 0x01010101u * h;  // bytes h and 2 + h of two words
+    i32x8_t fa[2][CF::FM], fb[2][CF::FN];
+    // the lane's exponents, two fragments to a word: byte 2 (f & 1) + ks is fragment f's in half ks of the K-tile
+    int32_t sa[HM], sb[CF::FN / 2];
+    Words8<CF> words;
+    // Fragment J (A's first, then B's) of half ks.
+    auto read = [&](auto jj, auto kk, const char* stage) __attribute__((always_inline)) {
+      constexpr int J = decltype(jj)::value, ks = decltype(kk)::value;
+      const char* p = stage + in_stage(J);
+      const i32x4_t lo = *reinterpret_cast<const i32x4_t*>(p + at[ks][0]);
+      const i32x4_t hi = *reinterpret_cast<const i32x4_t*>(p + at[ks][1]);
+      const i32x8_t v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+      if constexpr (J < CF::FM) fa[ks][J] = v;
+      else fb[ks][J - CF::FM] = v;
+    };
+    auto read_words = [&](const char* slot) __attribute__((always_inline)) {
+#pragma unroll
+      for (int j = 0; j < NR; ++j) words.v[j] = *reinterpret_cast<const uint32_t*>(slot + in_slot(j));
+    };
+    auto pack_words = [&]() __attribute__((always_inline)) {
+#pragma unroll
+      for (int j = 0; j < HM; ++j) sa[j] = (int32_t)__builtin_amdgcn_perm(words.v[2 * j + 1], words.v[2 * j], pick);
+#pragma unroll
+      for (int j = 0; j < CF::FN / 2; ++j)
+        sb[j] = (int32_t)__builtin_amdgcn_perm(words.v[CF::FM + 2 * j + 1], words.v[CF::FM + 2 * j], pick);
+    };
+    // The MFMAs of row half mh in half ks, one per group, `work(group)` behind each.
+    auto step4 = [&](auto zero, auto mm, auto kk, auto work) __attribute__((always_inline)) {
+      static_for<0, HN>([&](auto xx) __attribute__((always_inline)) {
+        constexpr int x = decltype(xx)::value, m = decltype(mm)::value * HM + x / CF::FN, n = x % CF::FN;
+        constexpr int ks = decltype(kk)::value;
+        acc[m][n] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
+            fb[ks][n], fa[ks][m], decltype(zero)::value ? f32x16_t{} : acc[m][n], 0, 0, n % 2 * 2 + ks, sb[n / 2],
+            m % 2 * 2 + ks, sa[m / 2]);
+        work(xx);
+        __builtin_amdgcn_sched_barrier(0);
+      });
+    };
+    // The MFMAs stay in front of this: left alone, the compiler sinks them past the branches of the
+    // issue cursor, behind everything that they are to hide.
+    auto hold = [&]() __attribute__((always_inline)) {
+#pragma unroll
+      for (int m = 0; m < CF::FM; ++m)
+#pragma unroll
+        for (int n = 0; n < CF::FN; ++n) {
+          f32x16_t& v = acc[m][n];
+          asm volatile("" : "+a"(v));
+        }
+    };
+    // The fragments that a step reads, C of them over its groups: id(i) is the i-th.
+    auto reads = [&](auto xx, auto cc, auto kk, const char* stage, auto id) __attribute__((always_inline)) {
+      constexpr int x = decltype(xx)::value, C = decltype(cc)::value, G2 = (HN + 1) / 2;  // in the step's first half
+      if constexpr (x < G2)
+        static_for<x * C / G2, (x + 1) * C / G2>([&](auto i) __attribute__((always_inline)) {
+          read(Int<decltype(id)::at(decltype(i)::value)>{}, kk, stage);
+        });
+    };
+    struct RowsLow { static constexpr int at(int i) { return i; } };                                    // A, first row half
+    struct RowsHigh { static constexpr int at(int i) { return HM + i; } };                              // A, second
+    struct ColsAndLow { static constexpr int at(int i) { return i < CF::FN ? CF::FM + i : i - CF::FN; } };  // B, then A's first
+    constexpr int kBoth = CF::FN + HM;
+    // `end_` (the tile's last K-tile): its stage serves the epilogue before it is refilled.  A constant: the
+    // compiler would sink the MFMAs past branches between them.
+    auto ktile = [&](auto zero, auto end_, int32_t kt) __attribute__((always_inline)) {
+      constexpr bool last = decltype(end_)::value;
+      const char* stage = lds + c_stage * CF::STAGE;
+      step4(zero, Int<0>{}, Int<0>{}, [&](auto x) __attribute__((always_inline)) { reads(x, Int<kBoth>{}, Int<1>{}, stage, ColsAndLow{}); });
+      step4(Int<0>{}, Int<0>{}, Int<1>{}, [&](auto x) __attribute__((always_inline)) {
+        reads(x, Int<HM>{}, Int<0>{}, stage, RowsHigh{});
+        reads(x, Int<HM>{}, Int<1>{}, stage, RowsHigh{});
+      });
+      wait_lds();  // every wave has read this stage
+      block_barrier();
+      next_stage();
+      const int32_t k4 = last ? 0 : (kt + 1) % kScaleTiles;
+      if (k4 == 0) next_slot();
+      step4(zero, Int<1>{}, Int<0>{}, [&](auto x) __attribute__((always_inline)) {
+        constexpr int j = decltype(x)::value;
+        if constexpr (!last) static_for<j * HL / HN, (j + 1) * HL / HN>(issue);
+      });
+      // the next K-tile has landed: what is outstanding was issued behind it
+      if constexpr (last) wait_loads<(CF::NST - 2) * L>();
+      else wait_loads<(CF::NST - 2) * L + HL>();
+      block_barrier();
+      const char* ahead = lds + c_stage * CF::STAGE;
+      read_words(slots + c_slot * CF::SLOT + k4 * 4);
+      step4(Int<0>{}, Int<1>{}, Int<1>{}, [&](auto x) __attribute__((always_inline)) {
+        constexpr int j = decltype(x)::value;
+        reads(x, Int<kBoth>{}, Int<0>{}, ahead, ColsAndLow{});
+        if constexpr (!last) static_for<HL + j * (L - HL) / HN, HL + (j + 1) * (L - HL) / HN>(issue);
+      });
+      pack_words();
+      hold();
+      if constexpr (!last) {
+        issue_scales();
+        advance_issue();
+      }
+    };
+
+    read_words(slots);
+    static_for<0, kBoth>([&](auto i) __attribute__((always_inline)) { read(Int<ColsAndLow::at(decltype(i)::value)>{}, Int<0>{}, lds); });
+    pack_words();
+    for (int32_t tile = first; tile < end; tile += step) {
+      ktile(Int<1>{}, Int<0>{}, 0);
+      for (int32_t kt = 1; kt < nk - 1; ++kt) ktile(Int<0>{}, Int<0>{}, kt);
+      ktile(Int<0>{}, Int<1>{}, nk - 1);
+      char* free_stage = lds + (c_stage == 0 ? CF::NST - 1 : c_stage - 1) * CF::STAGE;  // the tile's last K-tile's
+      Place place;
+      decode(tile, place);
+      epilogue<E, KIND, CF>(P, place, wm, wn, wave, lane, free_stage, acc);
+      issue_scales();
+      static_for<0, L>(issue);
+      advance_issue();
+    }
+  } else if constexpr (KIND == NT8) {
     // In half ks of the K-tile lane l holds row l%32, columns 16 h .. + 15 and
     // 32 + 16 h .. + 15 of the half's 64 (h = l/32), and the exponent of its
     // block h.
@@ -497,15 +627,13 @@ __global__ __launch_bounds__(CF::NTH, CF::NW * CF::BPC / 4) void rows8_grouped_g
     // exponents, and (loads) issues the loads of the K-tile NST - 1 ahead.
     auto kstep = [&](auto zero, auto km, auto loads, const Frags8<CF>& fm, const char* stage, const char* slot, Frags8<CF>& fr)
         __attribute__((always_inline)) {
-      constexpr int kn = 1 - decltype(km)::value, RG = kn == 1 && PMX_R8_RG < NR ? PMX_R8_RG : NR;
+      constexpr int kn = 1 - decltype(km)::value;
       if constexpr (decltype(loads)::value) issue_scales();
       if constexpr (kn == 0) read_words(slot);
       static_for<0, NR>([&](auto jj) __attribute__((always_inline)) {
-        constexpr int j = decltype(jj)::value, LG = PMX_R8_LOAD_GROUPS < NR ? PMX_R8_LOAD_GROUPS : NR;
-        if constexpr (decltype(loads)::value && j < LG) static_for<j * L / LG, (j + 1) * L / LG>(issue);
-        if constexpr (j < RG)
-          static_for<j * NR / RG, (j + 1) * NR / RG>(
-              [&](auto i) __attribute__((always_inline)) { read(Int<order8<CF>(decltype(i)::value)>{}, Int<kn>{}, stage, fr); });
+        constexpr int j = decltype(jj)::value;
+        if constexpr (decltype(loads)::value) static_for<j * L / NR, (j + 1) * L / NR>(issue);
+        read(Int<order8<CF>(j)>{}, Int<kn>{}, stage, fr);
         if constexpr (kn == 0 && j == NR / 2) pack_words(fr);
         if constexpr (kn == 1 && j == 0) {
 #pragma unroll

@@ -292,6 +292,10 @@ LAYOUTS = {
     "large": ([256, 257, 511, 300], 264, 272),
     "large odd": ([700, 0, 301], 520, 1040),
     "many groups": ([2, 0, 1] * 400, 16, 32),
+    "one K-tile": ([300, 100, 0, 40], 264, 112),
+    "one full K-tile": ([70, 33], 136, 128),
+    "two K-tiles": ([70, 33], 136, 144),
+    "three K-tiles": ([150, 33], 136, 384),
 }
 
 
@@ -487,7 +491,7 @@ def test_fc1_swiglu_in_8_bits(cuda, counts, I, H, T, dtype):
     tol = slack + np.maximum((np.abs(exact) + slack) * 2.0**-4, unit * 2.0**-10)
     assert (np.abs(got - exact) <= tol * 1.0001).all(), f"codes: {(np.abs(got - exact) - tol).max()}"
     # the blocks that fc2's last K-tile takes along stand beside 2^0
-    tail = act.scales.cpu().permute(1, 0, 2).reshape(A, -1)[:, nb: -(-I // 128) * 4]
+    tail = act.scales.cpu().permute(1, 0, 2).reshape(A, -1)[:, nb: max(2, -(-I // 128)) * 4]
     assert (tail == 127).all()
     plain = rows8.gemm_fc1_swiglu_rows8(rows8.Rows8(qx.codes[token.long()].contiguous(), qx.scales[:, token.long()].contiguous(), dtype),
                                         qw, off.to(cuda), None, row_w.to(cuda))
