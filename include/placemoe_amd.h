@@ -513,9 +513,10 @@ int pmx_rows8_swiglu_bwd(const void* d_act, const void* codes, const void* scale
 
 /* C[rows of g] = A[rows of g] B[g]^T over 8-bit rows (e4m3), fp32 sums, C bf16
  * [M, N]; rows of g: offsets[g] .. offsets[g+1]-1 (offsets outside [0, M] are
- * clamped; if they descend anywhere, nothing is written).  A: codes [M, K]; B: codes [G, N, K], each with its scales.  K a
- * multiple of 16, N of 8, pointers 16-byte aligned, N*K and the scales of all
- * rows below 2 GiB, else PMX_ERR_SHAPE. */
+ * clamped; if they descend anywhere, nothing is written).  A: codes [M, K]; B:
+ * codes [G, N, K], each with its scales.  K a multiple of 16, N of 8, pointers
+ * 16-byte aligned, N*K and the scales of all rows below 2 GiB, else
+ * PMX_ERR_SHAPE. */
 int pmx_rows8_group_gemm_nt(const void* a, const void* a_scales, const void* b, const void* b_scales,
                             const int32_t* offsets, int32_t G, int64_t M, int64_t N, int64_t K, void* c,
                             pmx_stream_t stream);
@@ -524,9 +525,8 @@ int pmx_rows8_group_gemm_nt(const void* a, const void* a_scales, const void* b, 
  *   (gate | up) = X[row_token[r]] w[g]^T,  act[r] = silu(gate) * up * row_w[r]
  * X: T rows of H (codes and scales); row_token int32 [A], NULL: row r is X's
  * row r (T = A); a token outside [0, T) reads as zeros.  w [G, 2I, H], gate
- * rows first.  row_w bf16 [A], NULL: 1.  act: codes [A, I]; of its scales the
- * bytes up to the columns' next multiple of 128, 256 at least, are written.  H and I multiples of
- * 16; T*H below 2 GiB with row_token. */
+ * rows first.  row_w bf16 [A], NULL: 1.  act: codes [A, I] and scales.  H and I
+ * multiples of 16; T*H below 2 GiB with row_token. */
 int pmx_rows8_gemm_fc1_swiglu(const void* x, const void* x_scales, int64_t T, const int32_t* row_token,
                               const void* w, const void* w_scales, const int32_t* offsets, int32_t G,
                               int64_t A, int64_t H, int64_t I, const void* row_w, void* act, void* act_scales,

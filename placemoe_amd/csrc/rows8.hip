@@ -318,10 +318,7 @@ __global__ __launch_bounds__(256) void swiglu_bwd_rows8_kernel(const bf16_t* __r
 // ---------------------------------------------------------------------------
 
 // Blocks of eight rows per wave that fill the chip (two per CU).
-#ifndef PMX_R8_MANY
-#define PMX_R8_MANY 512
-#endif
-constexpr int64_t kManyBlocks = PMX_R8_MANY;
+constexpr int64_t kManyBlocks = 512;
 
 // a * b, or -1 where it passes 2^62 (a, b >= 0).
 int64_t product(int64_t a, int64_t b) { return a != 0 && b > (((int64_t)1 << 62) / a) ? -1 : a * b; }

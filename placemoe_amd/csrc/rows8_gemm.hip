@@ -144,7 +144,7 @@ __device__ __forceinline__ void setup(const Params8& P, const Place& at, Loads<C
   }
 }
 
-// NT: operands of a 64-deep half K-tile.
+// NT, waves of one row tile: operands of a 64-deep half K-tile.
 template <class CF>
 struct Frags8 {
   i32x8_t a[CF::FM], b[CF::FN];
@@ -237,12 +237,14 @@ __device__ __forceinline__ void epilogue(const Params8& P, const Place& at, int 
       __builtin_amdgcn_sched_barrier(0);  // one tile's registers at a time
     } else {
       const float w = in && P.row_w != nullptr ? E::to_f32(P.row_w[r]) : 1.0f;
-      // fc2's K-tiles take along the blocks past I in their last 128 columns: those that no tile covers stand,
-      // as the others of zeros do, beside 2^0
+      // The group's blocks past I that no tile covers: 2^0, like those of zeros (fc2's last K-tiles take them along).
       if (in && h == 0 && wn == CF::WN - 1 && (int64_t)(at.ntile + 1) * (CF::BN / 2) >= P.I) {
-        const int64_t end = P.I <= KT ? 2 * KT : (P.I + KT - 1) / KT * KT;  // two K-tiles at least
-        for (int64_t j = (int64_t)(at.ntile + 1) * (CF::BN / 2); j < end; j += kScaleBlock)
-          P.qs[(j / kScaleGroup * P.M + r) * kScaleBytes + j / kScaleBlock % 16] = 127;
+        const int64_t end = (P.I + kScaleGroup - 1) / kScaleGroup * kScaleGroup;
+        for (int64_t j = (int64_t)(at.ntile + 1) * (CF::BN / 2); j < end;) {
+          uint8_t* const byte = P.qs + (j / kScaleGroup * P.M + r) * kScaleBytes + j / kScaleBlock % 16;
+          if (j % KT == 0) *reinterpret_cast<uint32_t*>(byte) = 0x7f7f7f7fu, j += KT;
+          else *byte = 127, j += kScaleBlock;
+        }
       }
 #pragma unroll
       for (int n = 0; n < CF::FN; n += 2) {
@@ -416,8 +418,8 @@ __global__ __launch_bounds__(CF::NTH, CF::NW * CF::BPC / 4) void rows8_grouped_g
       for (int q = 0; q < L; ++q) ld.off[q] = kOOB;
     }
   };
-  // K-tiles in flight before the first is multiplied: FC1 refills a stage once its
-  // last quarter is in registers, NT from the next K-tile on.
+  // K-tiles in flight before the first is multiplied: all stages, where a stage is refilled once its
+  // K-tile is in registers; NT with one row tile per wave refills it from the next K-tile on.
   constexpr int AHEAD = KIND == FC18 || kHalves ? CF::NST : CF::NST - 1;
 #pragma unroll
   for (int s = 0; s < AHEAD; ++s) {
@@ -583,9 +585,8 @@ __global__ __launch_bounds__(CF::NTH, CF::NW * CF::BPC / 4) void rows8_grouped_g
       advance_issue();
     }
   } else if constexpr (KIND == NT8) {
-    // In half ks of the K-tile lane l holds row l%32, columns 16 h .. + 15 and
-    // 32 + 16 h .. + 15 of the half's 64 (h = l/32), and the exponent of its
-    // block h.
+    // One row tile per wave: few rows, the weights' bytes bound it.  Halves of
+    // the K-tile as above, read one ahead of the MFMAs.
     int32_t at[2][2];
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks)
@@ -805,9 +806,6 @@ template <class E, int KIND>
 int launch(const Params8& P, pmx_stream_t stream) {
   const int cus = cu_count();
   if (cus <= 0) return PMX_ERR_HIP;
-#ifdef PMX_R8_FORCE
-  return launch_cfg<E, KIND, PMX_R8_FORCE>(P, cus, stream);
-#endif
   switch (pmx::rows8_tiling(KIND, P.M, P.G, P.N, P.K, cus)) {
     case 0: return launch_cfg<E, KIND, Narrow32>(P, cus, stream);
     case Rows32::BM: return launch_cfg<E, KIND, Rows32>(P, cus, stream);

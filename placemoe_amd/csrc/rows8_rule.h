@@ -10,22 +10,22 @@
 //   256 x 256, one block per CU: half the operand bytes per product.
 // Measured (us, 32 / 128 / 256; log-normal counts with sigma 0.4; N x K):
 //   copies rows   N     K     NT                 fc1 (N = 2 I)
-//   160    4      1536  2048   91 /  96 / 121     95 / 119 / 196
-//   160    32     1536  2048  107 / 100 / 124    114 / 125 / 193
-//   160    64     1536  2048  149 / 105 / 127    171 / 131 / 205
-//   160    256    1536  2048  397 / 214 / 203    501 / 299 / 330
-//   160    600    1536  2048  857 / 421 / 355   1146 / 653 / 606
-//   16     400    7168  2048  254 / 108 / 110    346 / 195 / 212
-//   16     2000   4096  7168    - /1136 / 848      - /1722 /1502
-//   12     192    1000  1104   20 /  13 /  20      -
+//   160    4      1536  2048   92 /  98 / 119     95 / 119 / 196
+//   160    32     1536  2048  107 / 103 / 120    114 / 125 / 193
+//   160    64     1536  2048  148 / 108 / 121    171 / 131 / 205
+//   160    256    1536  2048  397 / 210 / 197    501 / 299 / 330
+//   160    600    1536  2048  857 / 435 / 361   1146 / 653 / 606
+//   16     400    7168  2048  254 / 114 / 119    346 / 195 / 212
+//   16     2000   4096  7168    - /1069 / 868      - /1722 /1502
+//   12     192    1000  1104   20 /  13 /  21      -
 // 32 x 64 against 32 x 256 (weights not in a cache; NT, fc1): 8 rows over 160 copies of
 // 1536 x 2048 20 / 23, 22 / 26; 64 over 128 63 / 70, 65 / 74; 768 over 160 149 / 152,
 // 152 / 152; 2400 over 160 163 / 153, 166 / 154.
 // Past the few-rows line the rounds of tiles decide: a round costs its K-tiles
 // and a fixed part (epilogue and tile switch), both fitted to such calls.  Over
-// 170 calls (8 to 160 copies, 4 to 2000 rows, 5 layers) the choice takes 1.02
-// of the best tiling's time in geometric mean, 1.26 at worst (copies whose counts
-// straddle a tile's height).
+// 150 calls (8 to 256 copies, 0.1 to 2000 rows per copy, 10 layers) the choice takes
+// 1.02 of the best tiling's time in geometric mean, 1.33 at worst (a copy whose count
+// straddles a tile's height).
 //
 // A result's bits do not depend on the choice: every tiling adds up K in the same
 // steps.
