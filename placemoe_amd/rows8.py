@@ -179,8 +179,8 @@ def swiglu_bwd_rows8(d_act: torch.Tensor, gu: Rows8, row_w: torch.Tensor | None 
     d_act [R, I]: the gradient of the weighted activations act_w = row_w * silu(gate) * up,
     gu [R, 2I] (gate columns, then up columns), row_w [R] (None: ones).
     dG1 [R, 2I] is the gradient of (gate | up), act_w [R, I] the activations
-    themselves (for the weight gradient of fc2), and with ``row_src`` (int32 [R])
-    dw [num_assign] the weights' gradient, dw[row_src[r]] = sum_j d_act * silu(gate) * up
+    themselves (for the weight gradient of fc2), and with ``row_src`` (int32 [R], no
+    entry twice) dw [num_assign] the weights' gradient, dw[row_src[r]] = sum_j d_act * silu(gate) * up
     (entries that no row names are not written; None without ``row_src``).
     Computed in fp32, each result rounded once.
     """
@@ -312,7 +312,8 @@ def expert_layer_rows8(hidden: torch.Tensor, routing_weights: torch.Tensor, sele
     assert isinstance(weights, Experts8), f"weights must be Experts8, got {type(weights).__name__}"
     if torch.is_grad_enabled() and (hidden.requires_grad or routing_weights.requires_grad):
         raise ValueError("expert_layer_rows8 has no backward; call it under torch.no_grad()")
-    _check_dev(hidden, routing_weights, selected_experts, weights.gate_up.codes, weights.down.codes, mapping, sources)
+    _check_dev(hidden, routing_weights, selected_experts, weights.gate_up.codes, weights.gate_up.scales, weights.down.codes,
+               weights.down.scales, mapping, sources)
     dt = _half("hidden states", hidden)
     _half("routing weights", routing_weights, dt)
     assert hidden.dim() == 2, "hidden states must be [tokens, hidden size]"
@@ -337,6 +338,8 @@ def expert_layer_rows8(hidden: torch.Tensor, routing_weights: torch.Tensor, sele
         sources = sources.to(torch.int64).contiguous().reshape(-1)
         assert sources.numel() == T, "sources must have one entry per token"
     if T == 0 or K == 0:
+        if recorder is not None:
+            recorder(torch.zeros(C, dtype=torch.int32, device=hidden.device))
         return torch.zeros_like(hidden)
     ws_bytes = _capi.load().pmx_rows8_layer_workspace_bytes(T, K, H, I, C)
     if ws_bytes == 0:

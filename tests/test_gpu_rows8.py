@@ -498,6 +498,20 @@ def test_fc1_swiglu_in_8_bits(cuda, counts, I, H, T, dtype):
     assert torch.equal(plain.codes.view(torch.uint8), act.codes.view(torch.uint8)), "rows in place"
 
 
+@pytest.mark.parametrize("rows", [3, 100, 1500, 9000])
+@pytest.mark.parametrize("I", [16, 48, 144, 512, 528])
+def test_fc1_writes_every_scale(cuda, I, rows):
+    """The bytes past the last column stand for 2^0, as `quantize_rows` leaves them."""
+    G, H = 3, 64
+    x = rows8.quantize_rows(_randn((rows, H), 1).to(cuda))
+    w = rows8.quantize_rows(_randn((G, 2 * I, H), 2).to(cuda))
+    junk = torch.full((1 << 24,), 3, dtype=torch.uint8, device=cuda)  # what the outputs' memory held before
+    del junk
+    act = rows8.gemm_fc1_swiglu_rows8(x, w, _offsets([rows - 2, 1, 1]).to(cuda))
+    tail = act.scales.permute(1, 0, 2).reshape(rows, -1)[:, -(-I // 32):]
+    assert (tail == 127).all()
+
+
 def test_token_outside_reads_as_zeros(cuda):
     qx, qw = rows8.quantize_rows(_randn((4, 64), 1).to(cuda)), rows8.quantize_rows(_randn((1, 64, 64), 2).to(cuda))
     off = torch.tensor([0, 3], dtype=torch.int32, device=cuda)
@@ -524,6 +538,108 @@ def test_product_refusals(cuda):
         rows8.group_gemm_nt_rows8(a, rows8.quantize_rows(_randn((2, 12, 64), 2).to(cuda)), off)
     empty = rows8.quantize_rows(torch.empty((0, 64), dtype=BF, device=cuda))
     assert rows8.group_gemm_nt_rows8(empty, b, torch.zeros(3, dtype=torch.int32, device=cuda)).shape == (0, 32)
+
+
+# ---------------------------------------------------------------------------
+# Streams, graphs, offsets past 32 bits
+# ---------------------------------------------------------------------------
+
+
+def _every_op(x, pos, d, w, offsets, fmt="e4m3"):
+    """One call of each: x [R, N], pos [R, K], d [R, N / 2], w [G, n, N] in 8 bits."""
+    q = rows8.quantize_rows(x, fmt)
+    row_w = d[:, 0].contiguous()
+    row_src = pos[:, 0].contiguous()
+    dg, act, dw = rows8.swiglu_bwd_rows8(d, q, row_w, row_src, pos.numel())
+    c = rows8.group_gemm_nt_rows8(q, w, offsets)
+    a = rows8.gemm_fc1_swiglu_rows8(q, w, offsets)
+    return [rows8.dequantize_rows(q, pos), dg, act, dw[row_src.long()], c, a.codes.view(torch.uint8), a.scales]
+
+
+def _every_op_case(cuda, R, seed):
+    N, K, G = 1056, 3, 4
+    g = torch.Generator().manual_seed(seed)
+    w = rows8.quantize_rows(_randn((G, 96, N), seed + 1).to(cuda))
+    counts = np.random.default_rng(seed).multinomial(R, [1 / G] * G)
+    return [_randn((R, N), seed + 2).to(cuda), torch.randperm(R * K, generator=g).to(torch.int32).view(R, K).to(cuda),
+            _randn((R, N // 2), seed + 3).to(cuda), w, _offsets(counts).to(cuda)]
+
+
+def test_every_op_on_two_streams_at_once(cuda):
+    cases = [_every_op_case(cuda, R, R) for R in (37, 900)]
+    want = [_every_op(*c) for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(4):
+        for k, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[k].append(_every_op(*cases[k]))
+    torch.cuda.synchronize()
+    for k in range(2):
+        for outs in got[k]:
+            for j, (a, b) in enumerate(zip(outs, want[k])):
+                assert_exact(a, b, f"case {k}, output {j}")
+
+
+def test_every_op_in_a_graph(cuda):
+    case = _every_op_case(cuda, 130, 7)
+    _every_op(*case)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = _every_op(*case)
+    for k in range(3):
+        case[0].copy_(_randn(tuple(case[0].shape), 80 + k).to(cuda))
+        graph.replay()
+        eager = _every_op(*case)
+        torch.cuda.synchronize()
+        for j, (a, b) in enumerate(zip(outs, eager)):
+            assert_exact(a, b, f"replay {k}, output {j}")
+
+
+def test_offsets_past_32_bits(cuda):
+    """More than 2^31 elements: 500 rows over and over, each repeat the same as the first."""
+    n, times, N = 500, 1100, 4112
+    assert n * times * N > 2**31
+    rows, d = _randn((n, N), 1).to(cuda), _randn((n, N // 2), 2).to(cuda)
+    ref = rows8.quantize_rows(rows)
+    print("past 32 bits: writing", flush=True)
+    big = rows8.quantize_rows(rows.repeat(times, 1))
+    assert torch.equal(big.codes.view(torch.uint8).view(times, n, N)[[0, -2, -1]],
+                       ref.codes.view(torch.uint8).expand(3, n, N))
+    assert torch.equal(big.scales.view(-1, times, n, 16)[:, -1], ref.scales)
+    print("past 32 bits: reading back", flush=True)
+    back = rows8.dequantize_rows(big)
+    assert_exact(back[-n:], rows8.dequantize_rows(ref), "read back")
+    del back
+    print("past 32 bits: SwiGLU backward", flush=True)
+    dg, act, _ = rows8.swiglu_bwd_rows8(d.repeat(times, 1), big)
+    dg_ref, act_ref, _ = rows8.swiglu_bwd_rows8(d, ref)
+    assert_exact(dg[-n:], dg_ref, "dG1")
+    assert_exact(act[-n:], act_ref, "act_w")
+    del dg, act
+    for depth, cols in ((N, 64), (64, N)):  # long A, then a long output
+        a = big if depth == N else rows8.quantize_rows(rows[:, :64].repeat(times, 1))
+        small = ref if depth == N else rows8.quantize_rows(rows[:, :64].contiguous())
+        b = rows8.quantize_rows(_randn((2, cols, depth), 3).to(cuda))
+        half = n * times // 2
+        print(f"past 32 bits: products {depth} deep, {cols} wide", flush=True)
+        off, off_ref = _offsets([half, half]).to(cuda), _offsets([0, n]).to(cuda)
+        assert_exact(rows8.group_gemm_nt_rows8(a, b, off)[-n:], rows8.group_gemm_nt_rows8(small, b, off_ref), "product")
+        up = rows8.quantize_rows(_randn((2, 2 * cols, depth), 4).to(cuda))
+        act, act_ref = rows8.gemm_fc1_swiglu_rows8(a, up, off), rows8.gemm_fc1_swiglu_rows8(small, up, off_ref)
+        assert torch.equal(act.codes.view(torch.uint8)[-n:], act_ref.codes.view(torch.uint8))
+        assert torch.equal(act.scales[:, -n:], act_ref.scales)
+    T, K = 66000, 8
+    print("past 32 bits: spreading", flush=True)
+    pos = torch.randperm(T * K, generator=torch.Generator().manual_seed(1)).to(torch.int32).view(T, K).to(cuda)
+    few = rows8.quantize_rows(rows.repeat(T // n, 1))
+    out = rows8.dequantize_rows(few, pos)
+    plain = rows8.dequantize_rows(ref)
+    at = torch.arange(0, T, 97, device=cuda)
+    for k in range(K):
+        assert_exact(out[pos[at, k].long()], plain[at % n], f"spread {k}")
 
 
 # ---------------------------------------------------------------------------
@@ -636,6 +752,64 @@ def test_layer_refusals_and_edges(cuda):
     placemoe_amd.expert_layer_rows8(x, w, sel + 99, q)
     with pytest.raises(ValueError, match="expert id outside"):
         experts.check_pending_routes(block=True)
+
+
+def test_layer_refuses_scales_on_the_host(cuda):
+    """Each part of the weights is looked at: a host pointer never reaches a kernel."""
+    C, H, I = 4, 64, 32
+    q = rows8.Experts8.quantize(_randn((C, 2 * I, H), 1).to(cuda), _randn((C, H, I), 2).to(cuda))
+    x, w = _randn((5, H), 3).to(cuda), torch.ones((5, 1), dtype=BF, device=cuda)
+    sel = torch.zeros((5, 1), dtype=torch.int64, device=cuda)
+    host = lambda r: rows8.Rows8(r.codes, r.scales.cpu(), r.dtype)  # noqa: E731
+    for bad in (rows8.Experts8(host(q.gate_up), q.down), rows8.Experts8(q.gate_up, host(q.down))):
+        with pytest.raises(AssertionError, match="GPU tensors"):
+            placemoe_amd.expert_layer_rows8(x, w, sel, bad)
+
+
+def test_layer_without_tokens_reports_its_counts(cuda):
+    C, H, I = 4, 64, 32
+    q = rows8.Experts8.quantize(_randn((C, 2 * I, H), 1).to(cuda), _randn((C, H, I), 2).to(cuda))
+    seen = []
+    placemoe_amd.expert_layer_rows8(_randn((0, H), 3).to(cuda), torch.ones((0, 2), dtype=BF, device=cuda),
+                                    torch.zeros((0, 2), dtype=torch.int64, device=cuda), q, recorder=seen.append)
+    assert len(seen) == 1 and seen[0].dtype == torch.int32 and seen[0].tolist() == [0] * C
+
+
+def test_layer_with_one_expert_twice(cuda):
+    """A token that names a copy twice has both of its rows, each with its weight."""
+    T, C, H, I = 9, 3, 64, 48
+    hidden = _randn((T, H), 1)
+    sel = torch.arange(T).remainder(C).reshape(T, 1).repeat(1, 2)
+    w = torch.softmax(_randn((T, 2), 2).float(), -1).to(BF)
+    q = rows8.Experts8.quantize(_randn((C, 2 * I, H), 3, BF, 0.1).to(cuda), _randn((C, H, I), 4, BF, 0.1).to(cuda))
+    got = placemoe_amd.expert_layer_rows8(hidden.to(cuda), w.to(cuda), sel.to(cuda), q)
+    exact, tol = _layer_oracle(hidden, w, sel.numpy(), q, torch.finfo(BF).eps)
+    off = np.abs(got.double().cpu().numpy() - exact)
+    assert (off <= tol * 1.0001 + SUBNORMAL[BF]).all(), (off - tol).max()
+
+
+def test_two_layers_at_once(cuda):
+    """Calls on two streams share nothing: each has its workspace."""
+    C, H, I = 16, 512, 256
+    q = rows8.Experts8.quantize(_randn((C, 2 * I, H), 1, BF, 0.1).to(cuda), _randn((C, H, I), 2, BF, 0.1).to(cuda))
+    g = torch.Generator().manual_seed(5)
+    calls = []
+    for k in range(2):
+        T = (700, 33)[k]
+        sel = torch.stack([torch.randperm(C, generator=g)[:4] for _ in range(T)]).to(cuda)
+        calls.append((_randn((T, H), 10 + k).to(cuda), torch.full((T, 4), 0.25, dtype=BF, device=cuda), sel, q))
+    want = [placemoe_amd.expert_layer_rows8(*c) for c in calls]
+    streams = [torch.cuda.Stream() for _ in calls]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for k, (s, c) in enumerate(zip(streams, calls)):
+            with torch.cuda.stream(s):
+                got[k].append(placemoe_amd.expert_layer_rows8(*c))
+    torch.cuda.synchronize()
+    for k in range(2):
+        for out in got[k]:
+            assert_exact(out, want[k], f"call {k}")
 
 
 def test_layer_on_another_stream_and_in_a_graph(cuda):
@@ -801,3 +975,36 @@ def test_checkpointed_backward_in_a_graph(cuda):
         eager = step(x_eager)
         torch.cuda.synchronize()
         assert_exact(grad, eager, f"replay {k}")
+
+
+@pytest.mark.parametrize("weighted", [False, True])
+def test_checkpointed_layer_without_tokens(cuda, weighted):
+    wl = make_workload("toy", device=cuda, tokens=8)
+    x = wl.hidden[:0].clone().requires_grad_()
+    w = wl.routing_weights[:0].clone().requires_grad_()
+    fc1, fc2 = wl.fc1.clone().requires_grad_(), wl.fc2.clone().requires_grad_()
+    sources = wl.sources[:0] if wl.sources is not None else None
+    out = experts.expert_layer(x, w, wl.selected[:0], fc2, fc1_1_2_weight=fc1, mapping=wl.mapping, sources=sources,
+                               weighted_input=weighted, activation_checkpoint="e4m3")
+    out.sum().backward()
+    assert out.shape == x.shape and x.grad.shape == x.shape and w.grad.shape == w.shape
+    assert not fc1.grad.any() and not fc2.grad.any()
+
+
+@pytest.mark.parametrize("wanted", ["hidden", "weights", "fc1", "fc2"])
+def test_checkpointed_layer_with_one_gradient_wanted(cuda, wanted):
+    """Whatever is frozen, the one gradient asked for is the same."""
+    wl = make_workload("toy", device=cuda, tokens=70)
+    dout = _randn((wl.T, wl.H), 3).to(cuda)
+
+    def grads(names):
+        t = {"hidden": wl.hidden, "weights": wl.routing_weights, "fc1": wl.fc1, "fc2": wl.fc2}
+        t = {k: v.clone().requires_grad_(k in names) for k, v in t.items()}
+        out = experts.expert_layer(t["hidden"], t["weights"], wl.selected, t["fc2"], fc1_1_2_weight=t["fc1"],
+                                   mapping=wl.mapping, sources=wl.sources, activation_checkpoint="e4m3")
+        out.backward(dout)
+        return {k: v.grad for k, v in t.items()}
+
+    every, one = grads(("hidden", "weights", "fc1", "fc2")), grads((wanted,))
+    assert_exact(one[wanted], every[wanted], wanted)
+    assert all(g is None for k, g in one.items() if k != wanted)
