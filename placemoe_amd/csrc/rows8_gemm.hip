@@ -74,6 +74,7 @@ struct Cfg8 {
   static constexpr int LDS = NST * (STAGE + SLOT);
   static_assert(BM / 8 % NW == 0 && BN / 8 % NW == 0 && BN % 64 == 0, "whole loads per wave");
   static_assert(FN % 2 == 0 || WN % 2 == 0, "gate and up tiles alternate");
+  static_assert(STAGE * NST >= (kMaxGroups + 1 + NW) * 4, "the offsets, before the first load");
   static_assert(NST >= 2 && (NST - 1) * (QA + QB) <= 63, "vmcnt is 6 bits");
 };
 
@@ -111,13 +112,26 @@ __device__ __forceinline__ void setup(const Params8& P, const Place& at, Loads<C
   const int64_t kgroups = (P.K + kScaleGroup - 1) / kScaleGroup;
   const bool mapped = KIND == FC18 && P.row_token != nullptr;
   const int64_t base = mapped ? 0 : at.row0;
-  // A's row behind the tile's row, relative to `base`; -1: none
-  const auto a_row = [&](int row) -> int32_t {
-    if (row >= at.row_end - at.row0) return -1;
-    if (!mapped) return row;
-    const int32_t t = P.row_token[at.row0 + row];
-    return t < (int32_t)P.a_rows ? t : -1;
-  };
+  const int32_t rows = at.row_end - at.row0;  // some
+  const auto load_row = [&](int j) { return (j * CF::NW + wave) * 8 + lane / 8; };
+  const auto scale_row = [&](int j) { return (j * CF::NW + wave) * 64 + lane; };
+  // A's row behind each load, relative to `base`; -1: none.  The tokens' loads all at once: one behind
+  // the other they took 2 us of a call for one token.
+  int32_t a_row[CF::QA], as_row[CF::QS];
+  const auto held = [&](int row) { return row < rows ? row : rows - 1; };
+  if (mapped) {
+    const int32_t* tokens = P.row_token + at.row0;
+#pragma unroll
+    for (int j = 0; j < CF::QA; ++j) a_row[j] = tokens[held(load_row(j))];
+#pragma unroll
+    for (int j = 0; j < CF::QS; ++j) as_row[j] = tokens[held(scale_row(j))];
+  } else {
+#pragma unroll
+    for (int j = 0; j < CF::QA; ++j) a_row[j] = load_row(j);
+#pragma unroll
+    for (int j = 0; j < CF::QS; ++j) as_row[j] = scale_row(j);
+  }
+  const auto of_a = [&](int row, int32_t r) { return row < rows && r < (int32_t)P.a_rows ? r : -1; };
   const uint32_t K = (uint32_t)P.K;
   ld.a = make_rsrc(P.a + base * P.K, (uint64_t)(P.a_rows - base) * P.K);
   ld.b = make_rsrc(P.b + (int64_t)at.g * P.N * P.K, (uint64_t)P.N * P.K);
@@ -127,9 +141,9 @@ __device__ __forceinline__ void setup(const Params8& P, const Place& at, Loads<C
 #pragma unroll
   for (int j = 0; j < CF::QA + CF::QB; ++j) {
     const bool is_a = j < CF::QA;
-    const int row = ((is_a ? j : j - CF::QA) * CF::NW + wave) * 8 + lane / 8;
+    const int row = load_row(is_a ? j : j - CF::QA);
     const int c = (lane % 8) ^ kc_swz(row);
-    const int32_t r = is_a ? a_row(row) : b_row<KIND, CF>(P, at.ntile, row);
+    const int32_t r = is_a ? of_a(row, a_row[is_a ? j : 0]) : b_row<KIND, CF>(P, at.ntile, row);
     ld.off[j] = r >= 0 ? (uint32_t)r * K + (uint32_t)c * 16u : kOOB;
     ld.past |= (c * 16 < krem ? 0u : 1u) << j;
     asm volatile("" : "+v"(ld.off[j]));  // one register, worked out here
@@ -138,19 +152,11 @@ __device__ __forceinline__ void setup(const Params8& P, const Place& at, Loads<C
   for (int j = 0; j < CF::QS; ++j) {
     const int s = j * CF::NW + wave;
     const int row = (s < CF::SA ? s : s - CF::SA) * 64 + lane;
-    const int32_t r = s < CF::SA ? (row < CF::BM ? a_row(row) : -1) : b_row<KIND, CF>(P, at.ntile, row);
+    const int32_t r = s < CF::SA ? (row < CF::BM ? of_a(row, as_row[j]) : -1) : b_row<KIND, CF>(P, at.ntile, row);
     ld.soff[j] = r >= 0 ? (uint32_t)r * kScaleBytes : kOOB;
     asm volatile("" : "+v"(ld.soff[j]));
   }
 }
-
-// NT, waves of one row tile: operands of a 64-deep half K-tile.
-template <class CF>
-struct Frags8 {
-  i32x8_t a[CF::FM], b[CF::FN];
-  // the lane's exponents, two fragments to a word: byte 2 (f & 1) + ks is fragment f's in half ks of the K-tile
-  int32_t sa[(CF::FM + 1) / 2], sb[(CF::FN + 1) / 2];
-};
 
 // FC1: codes of a 32-deep quarter (16 per lane), the K-tile's exponents of the
 // lane's rows (byte q: quarter q), and the values of half a quarter.
@@ -295,19 +301,29 @@ __global__ __launch_bounds__(CF::NTH, CF::NW * CF::BPC / 4) void rows8_grouped_g
     const int32_t o = P.offsets[g];
     return o < 0 ? 0 : o > P.M ? (int32_t)P.M : o;
   };
-  const auto m_tiles = [&](int g) { return (offset(g + 1) - offset(g) + CF::BM - 1) / CF::BM; };
 
-  // Prefix of the groups' m-tiles: consecutive groups per thread, a wave scan
-  // of the threads' sums, then the waves' sums.
+  // Prefix of the groups' m-tiles: the offsets into LDS, four loads of a thread at once, then consecutive groups
+  // per thread, a wave scan of the threads' sums, and the waves' sums.
   {
-    int32_t* wsum = reinterpret_cast<int32_t*>(lds);
+    int32_t* const offs = reinterpret_cast<int32_t*>(lds);
+    int32_t* const wsum = offs + G + 1;
+    for (int g0 = t; g0 <= G; g0 += 4 * CF::NTH) {
+      int32_t v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = offset(g0 + i * CF::NTH <= G ? g0 + i * CF::NTH : G);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (g0 + i * CF::NTH <= G) offs[g0 + i * CF::NTH] = v[i];
+    }
+    __syncthreads();
     const int per = (G + CF::NTH - 1) / CF::NTH;
     const int g0 = t * per, g1 = g0 + per < G ? g0 + per : G;
+    const auto m_tiles = [&](int g) { return (offs[g + 1] - offs[g] + CF::BM - 1) / CF::BM; };
     int32_t sum = 0;
     bool descends = false;
     for (int g = g0; g < g1; ++g) {
       sum += m_tiles(g);
-      descends |= offset(g + 1) < offset(g);
+      descends |= offs[g + 1] < offs[g];
     }
     int32_t inc = sum;
 #pragma unroll
@@ -328,9 +344,11 @@ __global__ __launch_bounds__(CF::NTH, CF::NW * CF::BPC / 4) void rows8_grouped_g
   }
   const int32_t ntn = (int32_t)(KIND == FC18 ? (P.I + CF::BN / 2 - 1) / (CF::BN / 2) : (P.N + CF::BN - 1) / CF::BN);
   const int32_t total = uni(tend[G - 1]) * ntn;  // the host has checked that it fits
-  // NT by row halves: a tile's first and last K-tiles are two (the second past K, zeros, where there is but one).
-  constexpr bool kHalves = KIND == NT8 && CF::FM % 2 == 0;
-  const int32_t ktiles = (int32_t)((P.K + KT - 1) / KT), nk = kHalves && ktiles < 2 ? 2 : ktiles;
+  // The main loops.  Whole: one row tile per wave, K-tiles in pairs; halves: NT otherwise, a tile's first and
+  // last K-tiles are two.  What that adds past K is zeros.
+  constexpr bool kWhole = CF::FM == 1, kHalves = KIND == NT8 && !kWhole;
+  const int32_t ktiles = (int32_t)((P.K + KT - 1) / KT);
+  const int32_t nk = kWhole ? ktiles + ktiles % 2 : kHalves && ktiles < 2 ? 2 : ktiles;
   // Blocks go round-robin over the XCDs: each XCD walks its own eighth of the
   // tile list, its blocks round-robin within it.
   int32_t first = blockIdx.x, step = gridDim.x, end = total;
@@ -346,7 +364,7 @@ __global__ __launch_bounds__(CF::NTH, CF::NW * CF::BPC / 4) void rows8_grouped_g
   // neighbouring tiles share a strip of B, and a band of A.  The group: 64
   // equal parts of the prefix at once, then the entries of the one.
   const int32_t part = (G + 63) / 64;
-  auto decode = [&](int32_t tile, Place& at) {
+  auto decode = [&](int32_t tile, Place& at) __attribute__((always_inline)) {
     constexpr uint32_t kBand = 8;
     const int32_t m = (int32_t)((uint32_t)tile / (uint32_t)ntn);
     const auto first_past = [&](int32_t v) { return uni(__builtin_ctzll(__ballot(v > m))); };  // some entry is: m < tend[G-1]
@@ -369,15 +387,23 @@ __global__ __launch_bounds__(CF::NTH, CF::NW * CF::BPC / 4) void rows8_grouped_g
   int32_t i_tile = first;
   int32_t i_kt = 0, i_stage = 0, i_slot = 0;
   bool i_live = true;
-  auto set_tile = [&]() {
+  // kOOB's bit on top of the offsets that lie past K: in the last K-tile, and all of those behind it.  (Done once,
+  // here: a wave issues an instruction in 5 cycles, and a select per load was a sixth of those of a one-wave tile.)
+  auto past_k = [&]() __attribute__((always_inline)) {
+    const uint32_t past = i_kt == ktiles - 1 ? ld.past : ~0u;
+#pragma unroll
+    for (int q = 0; q < L; ++q) ld.off[q] |= (past >> q) << 31;
+  };
+  auto set_tile = [&]() __attribute__((always_inline)) {
     Place at;
     decode(i_tile, at);
     setup<KIND, CF>(P, at, ld, wave, lane);
+    if (ktiles == 1) past_k();
   };
   set_tile();
   // The K-tile's exponents, where it is the first of four; ahead of its other
   // loads, so that whoever waits for those has these too.
-  auto issue_scales = [&]() {
+  auto issue_scales = [&]() __attribute__((always_inline)) {
     if (i_kt % kScaleTiles != 0 || !i_live) return;
     const uint32_t kg = (uint32_t)(i_kt / kScaleTiles);
 #pragma unroll
@@ -391,19 +417,17 @@ __global__ __launch_bounds__(CF::NTH, CF::NW * CF::BPC / 4) void rows8_grouped_g
   };
   auto issue = [&](auto jj) __attribute__((always_inline)) {
     constexpr int J = decltype(jj)::value;
-    // kOOB's bit on top of the offset where the lane lies past K
-    const uint32_t past = i_kt < ktiles - 1 ? 0u : i_kt == ktiles - 1 ? ld.past : ~0u;
-    const uint32_t off = ld.off[J] | ((past >> J) << 31);
     char* stage = lds + i_stage * CF::STAGE;
-    if constexpr (J < CF::QA) dma16(ld.a, stage + (J * NW + wave) * 1024, off, (uint32_t)i_kt * KT);
-    else dma16(ld.b, stage + CF::A_BYTES + ((J - CF::QA) * NW + wave) * 1024, off, (uint32_t)i_kt * KT);
+    if constexpr (J < CF::QA) dma16(ld.a, stage + (J * NW + wave) * 1024, ld.off[J], (uint32_t)i_kt * KT);
+    else dma16(ld.b, stage + CF::A_BYTES + ((J - CF::QA) * NW + wave) * 1024, ld.off[J], (uint32_t)i_kt * KT);
   };
-  auto advance_issue = [&]() {
+  auto advance_issue = [&]() __attribute__((always_inline)) {
     i_stage = i_stage + 1 == CF::NST ? 0 : i_stage + 1;
     if (!i_live) return;
     ++i_kt;
     if (i_kt < nk) {
       if (i_kt % kScaleTiles == 0) i_slot = i_slot + 1 == CF::NST ? 0 : i_slot + 1;
+      if (i_kt >= ktiles - 1) past_k();
       return;
     }
     i_kt = 0;
@@ -418,16 +442,15 @@ __global__ __launch_bounds__(CF::NTH, CF::NW * CF::BPC / 4) void rows8_grouped_g
       for (int q = 0; q < L; ++q) ld.off[q] = kOOB;
     }
   };
-  // K-tiles in flight before the first is multiplied: all stages, where a stage is refilled once its
-  // K-tile is in registers; NT with one row tile per wave refills it from the next K-tile on.
-  constexpr int AHEAD = KIND == FC18 || kHalves ? CF::NST : CF::NST - 1;
+  // All stages are in flight before the first K-tile is multiplied: a stage is refilled once its K-tile is in
+  // registers.
 #pragma unroll
-  for (int s = 0; s < AHEAD; ++s) {
+  for (int s = 0; s < CF::NST; ++s) {
     issue_scales();
     static_for<0, L>(issue);
     advance_issue();
   }
-  wait_loads<(AHEAD - 1) * L>();
+  wait_loads<(CF::NST - 1) * L>();
   block_barrier();
 
   const int h = lane >> 5, r32 = lane & 31;
@@ -584,98 +607,104 @@ __global__ __launch_bounds__(CF::NTH, CF::NW * CF::BPC / 4) void rows8_grouped_g
       static_for<0, L>(issue);
       advance_issue();
     }
-  } else if constexpr (KIND == NT8) {
-    // One row tile per wave: few rows, the weights' bytes bound it.  Halves of
-    // the K-tile as above, read one ahead of the MFMAs.
-    int32_t at[2][2];
-#pragma unroll
-    for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) at[ks][e] = r32 * KT + (((ks * 4 + e * 2 + h) ^ kc_swz(r32)) << 4);
+  } else if constexpr (kWhole) {
+    // One row tile per wave: few rows.  The weights' bytes bound a call with many copies; with a few (one
+    // token) a wave's way through its K-tiles does, so the next K-tile is read whole while this one is
+    // multiplied, and no wave waits for LDS: 0.74 us per K-tile of fc1 (codes read a quarter ahead) -> WHOLE_FC1,
+    // 0.55 of NT (a half ahead) -> WHOLE_NT.
+    constexpr bool kNT = KIND == NT8;
     const uint32_t pick = 0x06040200u + 0x01010101u * h;  // bytes h and 2 + h of two words
-    Frags8<CF> f0, f1;
-    auto read = [&](auto jj, auto kk, const char* stage, Frags8<CF>& fr) __attribute__((always_inline)) {
-      constexpr int J = decltype(jj)::value, ks = decltype(kk)::value;
-      const char* p = stage + in_stage(J);
-      const i32x4_t lo = *reinterpret_cast<const i32x4_t*>(p + at[ks][0]);
-      const i32x4_t hi = *reinterpret_cast<const i32x4_t*>(p + at[ks][1]);
-      const i32x8_t v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-      if constexpr (J < CF::FM) fr.a[J] = v;
-      else fr.b[J - CF::FM] = v;
+    int32_t at[4];  // the lane's 16-byte chunk of each quarter: two make one of NT's operands
+#pragma unroll
+    for (int q = 0; q < 4; ++q) at[q] = r32 * KT + (((q * 2 + h) ^ kc_swz(r32)) << 4);
+    struct KTile {
+      i32x4_t v[4][NR];
+      uint32_t words[NR];
     };
-    // The exponents of a K-tile: every fragment's word, and later, when they have arrived, the lane's bytes of them.
-    Words8<CF> words;
-    auto read_words = [&](const char* slot) __attribute__((always_inline)) {
+    KTile t0, t1;
+    auto read = [&](KTile& to, const char* stage, const char* slot) __attribute__((always_inline)) {
 #pragma unroll
-      for (int j = 0; j < NR; ++j) words.v[j] = *reinterpret_cast<const uint32_t*>(slot + in_slot(j));
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < NR; ++j) to.v[i][j] = *reinterpret_cast<const i32x4_t*>(stage + in_stage(j) + at[i]);
+#pragma unroll
+      for (int j = 0; j < NR; ++j) to.words[j] = *reinterpret_cast<const uint32_t*>(slot + in_slot(j));
     };
-    auto pack_words = [&](Frags8<CF>& fr) __attribute__((always_inline)) {
+    // FC1: fragment J's values of half hh of the K-tile's eight
+    Values8<CF> c0, c1;
+    auto convert = [&](auto jj, auto hh, const KTile& from, Values8<CF>& to) __attribute__((always_inline)) {
+      constexpr int J = decltype(jj)::value, q = decltype(hh)::value / 2, s = decltype(hh)::value % 2;
+      const float scale = __uint_as_float(q < 3 ? from.words[J] << (23 - 8 * q) : from.words[J] >> 1);
 #pragma unroll
-      for (int j = 0; j < CF::FM; j += 2)
-        fr.sa[j / 2] = (int32_t)__builtin_amdgcn_perm(words.v[j + 1 < CF::FM ? j + 1 : j], words.v[j], pick);
-#pragma unroll
-      for (int j = 0; j < CF::FN; j += 2)
-        fr.sb[j / 2] = (int32_t)__builtin_amdgcn_perm(words.v[CF::FM + (j + 1 < CF::FN ? j + 1 : j)], words.v[CF::FM + j], pick);
+      for (int pair = 0; pair < 4; pair += 2) {
+        const uint32_t four = (uint32_t)from.v[q][J][2 * s + pair / 2];
+        const bf16x2_t lo = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(four, scale, false);
+        const bf16x2_t hi = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(four, scale, true);
+        to.v[J][2 * pair] = lo[0], to.v[J][2 * pair + 1] = lo[1];
+        to.v[J][2 * pair + 2] = hi[0], to.v[J][2 * pair + 3] = hi[1];
+      }
     };
-    auto mfma = [&](auto xx, auto kk, auto zero, const Frags8<CF>& f) __attribute__((always_inline)) {
-      constexpr int x = decltype(xx)::value, m = x / CF::FN, n = x % CF::FN, ks = decltype(kk)::value;
-      acc[m][n] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
-          f.b[n], f.a[m], decltype(zero)::value ? f32x16_t{} : acc[m][n], 0, 0, n % 2 * 2 + ks, f.sb[n / 2], m % 2 * 2 + ks,
-          f.sa[m / 2]);
-    };
-    // The MFMAs of half `km` from `fm`, in NR groups, beside the reads of the
-    // other half into `fr`: km = 1 reads the next K-tile's first half and its
-    // exponents, and (loads) issues the loads of the K-tile NST - 1 ahead.
-    auto kstep = [&](auto zero, auto km, auto loads, const Frags8<CF>& fm, const char* stage, const char* slot, Frags8<CF>& fr)
-        __attribute__((always_inline)) {
-      constexpr int kn = 1 - decltype(km)::value;
-      if constexpr (decltype(loads)::value) issue_scales();
-      if constexpr (kn == 0) read_words(slot);
-      static_for<0, NR>([&](auto jj) __attribute__((always_inline)) {
-        constexpr int j = decltype(jj)::value;
-        if constexpr (decltype(loads)::value) static_for<j * L / NR, (j + 1) * L / NR>(issue);
-        read(Int<order8<CF>(j)>{}, Int<kn>{}, stage, fr);
-        if constexpr (kn == 0 && j == NR / 2) pack_words(fr);
-        if constexpr (kn == 1 && j == 0) {
-#pragma unroll
-          for (int i = 0; i < (CF::FM + 1) / 2; ++i) fr.sa[i] = fm.sa[i];
-#pragma unroll
-          for (int i = 0; i < (CF::FN + 1) / 2; ++i) fr.sb[i] = fm.sb[i];
+    // K-tile kt from `cur`; `end_`: the tile's last, whose stage serves the epilogue before it is refilled.
+    auto ktile = [&](auto zero, auto end_, int32_t kt, KTile& cur, KTile& next) __attribute__((always_inline)) {
+      constexpr bool last = kNT && decltype(end_)::value;
+      turn();
+      next_stage();
+      const int32_t k4 = kt + 1 < nk ? (kt + 1) % kScaleTiles : 0;
+      if (k4 == 0) next_slot();
+      if constexpr (!last) issue_scales();
+      // the MFMAs of a step, one per column tile, and behind each what it hides
+      constexpr int STEPS = kNT ? 2 : 8, MM = STEPS * CF::FN;
+      static_for<0, MM>([&](auto xx) __attribute__((always_inline)) {
+        constexpr int x = decltype(xx)::value, step_ = x / CF::FN, n = x % CF::FN;
+        if constexpr (kNT) {
+          const auto both = [&](int j) __attribute__((always_inline)) {
+            const i32x4_t lo = cur.v[2 * step_][j], hi = cur.v[2 * step_ + 1][j];
+            return i32x8_t{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+          };
+          const int32_t sa = (int32_t)__builtin_amdgcn_perm(cur.words[0], cur.words[0], pick);
+          const int32_t sb = (int32_t)__builtin_amdgcn_perm(cur.words[1 + (n | 1)], cur.words[1 + (n & ~1)], pick);
+          acc[0][n] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
+              both(1 + n), both(0), decltype(zero)::value && step_ == 0 ? f32x16_t{} : acc[0][n], 0, 0, n % 2 * 2 + step_, sb,
+              step_, sa);
+        } else {
+          const Values8<CF>& now = step_ % 2 ? c1 : c0;
+          acc[0][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+              now.v[1 + n], now.v[0], decltype(zero)::value && step_ == 0 ? f32x16_t{} : acc[0][n], 0, 0, 0);
         }
-        static_for<j * NM / NR, (j + 1) * NM / NR>([&](auto xx) __attribute__((always_inline)) { mfma(xx, km, zero, fm); });
+        if constexpr (x == 0) read(next, lds + c_stage * CF::STAGE, slots + c_slot * CF::SLOT + k4 * 4);
+        if constexpr (!last) static_for<x * L / MM, (x + 1) * L / MM>(issue);
+        if constexpr (!kNT)
+          static_for<n * NR / CF::FN, (n + 1) * NR / CF::FN>([&](auto j) __attribute__((always_inline)) {
+            convert(j, Int<(step_ + 1) % 8>{}, step_ < 7 ? cur : next, step_ % 2 ? c0 : c1);
+          });
         __builtin_amdgcn_sched_barrier(0);
       });
+#pragma unroll
+      for (int n = 0; n < CF::FN; ++n) {
+        f32x16_t& v = acc[0][n];
+        asm volatile("" : "+a"(v));  // the MFMAs stay in front of the branches
+      }
+      if constexpr (!last) advance_issue();
     };
 
+    read(t0, lds, slots);
+    if constexpr (!kNT) static_for<0, NR>([&](auto j) __attribute__((always_inline)) { convert(j, Int<0>{}, t0, c0); });
     for (int32_t tile = first; tile < end; tile += step) {
-      // The tile's first K-tile: no MFMAs of this tile to read its first half behind.
-      {
-        const char* stage = lds + c_stage * CF::STAGE;
-        const char* slot = slots + c_slot * CF::SLOT;
-        read_words(slot);
-        static_for<0, NR>([&](auto j) __attribute__((always_inline)) { read(Int<order8<CF>(decltype(j)::value)>{}, Int<0>{}, stage, f0); });
-        pack_words(f0);
-        kstep(Int<1>{}, Int<0>{}, Int<1>{}, f0, stage, slot, f1);
-        advance_issue();
-        turn();
-        next_stage();
+      ktile(Int<1>{}, Int<0>{}, 0, t0, t1);
+      for (int32_t kt = 1; kt < nk - 1; kt += 2) {
+        ktile(Int<0>{}, Int<0>{}, kt, t1, t0);
+        ktile(Int<0>{}, Int<0>{}, kt + 1, t0, t1);
       }
-      for (int32_t kt = 1; kt < nk; ++kt) {
-        if (kt % kScaleTiles == 0) next_slot();
-        const char* stage = lds + c_stage * CF::STAGE;
-        const char* slot = slots + c_slot * CF::SLOT + kt % kScaleTiles * 4;
-        kstep(Int<0>{}, Int<1>{}, Int<1>{}, f1, stage, slot, f0);
-        kstep(Int<0>{}, Int<0>{}, Int<0>{}, f0, stage, slot, f1);
-        advance_issue();
-        turn();
-        next_stage();
-      }
-      static_for<0, NM>([&](auto x) __attribute__((always_inline)) { mfma(x, Int<1>{}, Int<0>{}, f1); });
-      next_slot();
+      ktile(Int<0>{}, Int<1>{}, nk - 1, t1, t0);
       char* free_stage = lds + (c_stage == 0 ? CF::NST - 1 : c_stage - 1) * CF::STAGE;  // the tile's last K-tile's
       Place place;
       decode(tile, place);
       epilogue<E, KIND, CF>(P, place, wm, wn, wave, lane, free_stage, acc);
+      if constexpr (kNT) {
+        issue_scales();
+        static_for<0, L>(issue);
+        advance_issue();
+      }
     }
   } else {
     // In quarter q of the K-tile lane l holds row l%32, columns 16 h .. + 15 of
