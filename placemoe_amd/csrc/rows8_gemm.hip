@@ -74,7 +74,6 @@ struct Cfg8 {
   static constexpr int LDS = NST * (STAGE + SLOT);
   static_assert(BM / 8 % NW == 0 && BN / 8 % NW == 0 && BN % 64 == 0, "whole loads per wave");
   static_assert(FN % 2 == 0 || WN % 2 == 0, "gate and up tiles alternate");
-  static_assert(STAGE * NST >= (kMaxGroups + 1 + NW) * 4, "the offsets, before the first load");
   static_assert(NST >= 2 && (NST - 1) * (QA + QB) <= 63, "vmcnt is 6 bits");
 };
 
@@ -285,6 +284,17 @@ __device__ __forceinline__ void epilogue(const Params8& P, const Place& at, int 
   }
 }
 
+// Sum over the wave's lanes up to and with this one: shifts within rows of 16 lanes, then the rows' last lanes.
+__device__ __forceinline__ int32_t wave_scan(int32_t v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr:1
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast:15 into rows 1 and 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast:31 into rows 2 and 3
+  return v;
+}
+
 template <class E, int KIND, class CF>
 __global__ __launch_bounds__(CF::NTH, CF::NW * CF::BPC / 4) void rows8_grouped_gemm_kernel(Params8 P) {
   constexpr int NW = CF::NW, L = CF::QA + CF::QB;
@@ -302,44 +312,43 @@ __global__ __launch_bounds__(CF::NTH, CF::NW * CF::BPC / 4) void rows8_grouped_g
     return o < 0 ? 0 : o > P.M ? (int32_t)P.M : o;
   };
 
-  // Prefix of the groups' m-tiles: the offsets into LDS, four loads of a thread at once, then consecutive groups
-  // per thread, a wave scan of the threads' sums, and the waves' sums.
+  // Prefix of the groups' m-tiles, a group per thread at a time: a scan within each wave, then over the waves.
+  // Four groups' loads of a thread go out together.
   {
-    int32_t* const offs = reinterpret_cast<int32_t*>(lds);
-    int32_t* const wsum = offs + G + 1;
-    for (int g0 = t; g0 <= G; g0 += 4 * CF::NTH) {
-      int32_t v[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = offset(g0 + i * CF::NTH <= G ? g0 + i * CF::NTH : G);
+    int32_t* const wsum = reinterpret_cast<int32_t*>(lds);  // two turns' worth, a wave's sum each
+    int32_t before = 0;
+    bool bad = false;  // offsets that descend are not row groups: nothing to do
+    for (int32_t base = 0; base < G; base += 4 * CF::NTH) {
+      int32_t o[4][2];
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        if (g0 + i * CF::NTH <= G) offs[g0 + i * CF::NTH] = v[i];
-    }
-    __syncthreads();
-    const int per = (G + CF::NTH - 1) / CF::NTH;
-    const int g0 = t * per, g1 = g0 + per < G ? g0 + per : G;
-    const auto m_tiles = [&](int g) { return (offs[g + 1] - offs[g] + CF::BM - 1) / CF::BM; };
-    int32_t sum = 0;
-    bool descends = false;
-    for (int g = g0; g < g1; ++g) {
-      sum += m_tiles(g);
-      descends |= offs[g + 1] < offs[g];
-    }
-    int32_t inc = sum;
 #pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const int32_t v = __shfl_up(inc, off, 64);
-      if (lane >= off) inc += v;
+        for (int e = 0; e < 2; ++e) o[i][e] = offset(base + i * CF::NTH + t + e < G ? base + i * CF::NTH + t + e : G);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int32_t g = base + i * CF::NTH + t;
+        if (base + i * CF::NTH >= G) break;
+        const int32_t inc = wave_scan((o[i][1] - o[i][0] + CF::BM - 1) / CF::BM);  // past the last group: none
+        const bool descends = __ballot(o[i][1] < o[i][0]) != 0;
+        int32_t sum = __builtin_amdgcn_readlane(inc, 63), lower = 0;
+        bad |= descends;
+        if constexpr (NW > 1) {
+          int32_t* const turn_sums = wsum + i % 2 * NW;
+          if (lane == 0) turn_sums[wave] = descends ? -1 : sum;
+          __syncthreads();
+          sum = 0;
+          for (int w = 0; w < NW; ++w) {
+            const int32_t v = uni(turn_sums[w]);
+            bad |= v < 0;
+            lower += w < wave ? v : 0;
+            sum += v;
+          }
+        }
+        if (g < G) tend[g] = before + lower + inc;
+        before += sum;
+      }
     }
-    const bool bad = __ballot(descends) != 0;  // not row groups: nothing to do
-    if (lane == 63) wsum[wave] = bad ? -1 : inc;
-    __syncthreads();
-    int32_t run = inc - sum;
-    for (int w = 0; w < NW; ++w) {
-      if (uni(wsum[w]) < 0) return;
-      run += w < wave ? wsum[w] : 0;
-    }
-    for (int g = g0; g < g1; ++g) tend[g] = run += m_tiles(g);
+    if (bad) return;
     __syncthreads();
   }
   const int32_t ntn = (int32_t)(KIND == FC18 ? (P.I + CF::BN / 2 - 1) / (CF::BN / 2) : (P.N + CF::BN - 1) / CF::BN);
