@@ -73,7 +73,7 @@ struct Cfg8 {
   static constexpr int SLOT = (SA + SB) * 1024;
   static constexpr int LDS = NST * (STAGE + SLOT);
   static_assert(BM / 8 % NW == 0 && BN / 8 % NW == 0 && BN % 64 == 0, "whole loads per wave");
-  static_assert(FN % 2 == 0 || WN % 2 == 0, "gate and up tiles alternate");
+  static_assert(FN % 2 == 0 || (FN == 1 && WN == 2), "a wave, or the two of a block, has 32 gate columns and their up columns");
   static_assert(NST >= 2 && (NST - 1) * (QA + QB) <= 63, "vmcnt is 6 bits");
 };
 
@@ -92,12 +92,13 @@ struct Loads {
 };
 
 // Row of B for the tile's virtual row: FC1 alternates 32 gate rows and the
-// matching 32 up rows.
+// matching 32 up rows; 16 and 16 where a wave has one column tile.
 template <int KIND, class CF>
 __device__ __forceinline__ int32_t b_row(const Params8& P, int32_t ntile, int row) {
   if constexpr (KIND == FC18) {
-    const int32_t I = (int32_t)P.I, j = ntile * (CF::BN / 2) + (row >> 6) * 32 + (row & 31);
-    return j < I ? (row & 32 ? I : 0) + j : -1;
+    constexpr int W = CF::FN == 1 ? 16 : 32;
+    const int32_t I = (int32_t)P.I, j = ntile * (CF::BN / 2) + row / (2 * W) * W + row % W;
+    return j < I ? (row & W ? I : 0) + j : -1;
   } else {
     const int32_t j = ntile * CF::BN + row;
     return j < (int32_t)P.N ? j : -1;
@@ -188,7 +189,8 @@ __device__ __forceinline__ void swap_halves(uint32_t& lo, uint32_t& hi) {
 // first operand): lane l has row l%32, columns 8*(i/4) + 4*(l/32) + i%4.
 template <class E, int KIND, class CF>
 __device__ __forceinline__ void epilogue(const Params8& P, const Place& at, int wm, int wn, int wave, int lane,
-                                         [[maybe_unused]] char* stage, f32x16_t (&acc)[CF::FM][CF::FN]) {
+                                         [[maybe_unused]] char* stage, [[maybe_unused]] char* shared,
+                                         f32x16_t (&acc)[CF::FM][CF::FN]) {
   // Each accumulator leaves the accumulation registers where it is used: read
   // right behind their last MFMAs, they would need as many vector registers.
   const auto here = [](f32x16_t& v) __attribute__((always_inline)) { asm volatile("" : "+a"(v)); };
@@ -216,7 +218,7 @@ __device__ __forceinline__ void epilogue(const Params8& P, const Place& at, int 
       constexpr int CPR = CF::FN * 4, RPP = 64 / CPR;  // chunks of a row, rows of a piece (and of a store)
       static_assert(32 / RPP <= CF::QA + CF::QB, "enough pieces");
       const auto place = [&](int row, int c) {
-        const int sw = CPR == 16 ? row & 15 : kc_swz(row);
+        const int sw = CPR == 16 ? row & 15 : CPR == 8 ? kc_swz(row) : row >> 2 & 3;
         return stage + ((row / RPP) * CF::NW + wave) * 1024 + (row % RPP) * (CPR * 16) + ((c ^ sw) << 4);
       };
 #pragma unroll
@@ -251,34 +253,63 @@ __device__ __forceinline__ void epilogue(const Params8& P, const Place& at, int 
           else *byte = 127, j += kScaleBlock;
         }
       }
+      // A block's exponent and codes: `f` holds the lane's N values, columns 8 (i/4) + 4 h + i%4 of the block or,
+      // one column tile per wave, of the wave's half of it.
+      const auto weigh = [&](float gate, float up) { return silu_f32(gate) * up * w; };
+      const auto most_of = [](float most, float f) {
+        const float v = __builtin_fabsf(f);
+        return v > most && v < __builtin_inff() ? v : most;
+      };
+      const auto code = [](const float* f, float inv) {
+        return codes4<kFmtE4M3>(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv);
+      };
+      const auto put_scale = [&](int64_t j, uint32_t byte) {
+        P.qs[(j / kScaleGroup * P.M + r) * kScaleBytes + j / kScaleBlock % 16] = (uint8_t)byte;
+      };
+      if constexpr (CF::FN == 1) {
+        here(acc[m][0]);
+        float f[8], most = 0.f;
 #pragma unroll
-      for (int n = 0; n < CF::FN; n += 2) {
-        here(acc[m][n]);
-        here(acc[m][n + 1]);
-        float f[16];
-        float most = 0.f;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          f[i] = silu_f32(acc[m][n][i]) * acc[m][n + 1][i] * w;
-          const float v = __builtin_fabsf(f[i]);
-          most = v > most && v < __builtin_inff() ? v : most;
-        }
+        for (int i = 0; i < 8; ++i) f[i] = weigh(acc[m][0][i], acc[m][0][i + 8]), most = most_of(most, f[i]);
         most = fmaxf(most, __shfl_xor(most, 32, 64));
-        const uint32_t byte = scale_byte<kFmtE4M3>(__float_as_uint(most));
+        float* const of_waves = reinterpret_cast<float*>(shared);  // [2][32]; a K-tile's barrier before it is used again
+        if (h == 0) of_waves[wn * 32 + lane] = most;
+        wait_lds();
+        block_barrier();
+        const uint32_t byte = scale_byte<kFmtE4M3>(__float_as_uint(fmaxf(most, of_waves[(1 - wn) * 32 + (lane & 31)])));
         const float inv = inv_scale(byte);
-        uint32_t c[4];  // columns 8 i + 4 h .. + 3
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          c[i] = codes4<kFmtE4M3>(f[4 * i] * inv, f[4 * i + 1] * inv, f[4 * i + 2] * inv, f[4 * i + 3] * inv);
-        // ... and after the exchange each lane has columns 16 h .. + 15
-        swap_halves(c[0], c[2]);
-        swap_halves(c[1], c[3]);
-        const int64_t j = (int64_t)at.ntile * (CF::BN / 2) + (wn * CF::FN + n) * 16;
+        uint32_t c0 = code(f, inv), c1 = code(f + 4, inv);
+        swap_halves(c0, c1);  // columns 8 h .. + 7 of the wave's 16
+        const int64_t j = (int64_t)at.ntile * 32 + wn * 16;
         if (in) {
-          if (j + h * 16 < P.I) *reinterpret_cast<uint4*>(P.q + r * P.I + j + h * 16) = make_uint4(c[0], c[2], c[1], c[3]);
-          if (h == 0) P.qs[(j / kScaleGroup * P.M + r) * kScaleBytes + j / kScaleBlock % 16] = (uint8_t)byte;
+          if (j < P.I) *reinterpret_cast<uint2*>(P.q + r * P.I + j + h * 8) = make_uint2(c0, c1);
+          if (h == 0 && wn == 0) put_scale(j, byte);
         }
-        __builtin_amdgcn_sched_barrier(0);
+      } else {
+#pragma unroll
+        for (int n = 0; n < CF::FN; n += 2) {
+          here(acc[m][n]);
+          here(acc[m][n + 1]);
+          float f[16], most = 0.f;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) f[i] = weigh(acc[m][n][i], acc[m][n + 1][i]), most = most_of(most, f[i]);
+          most = fmaxf(most, __shfl_xor(most, 32, 64));
+          const uint32_t byte = scale_byte<kFmtE4M3>(__float_as_uint(most));
+          const float inv = inv_scale(byte);
+          uint32_t c[4];  // columns 8 i + 4 h .. + 3
+#pragma unroll
+          for (int i = 0; i < 4; ++i) c[i] = code(f + 4 * i, inv);
+          // ... and after the exchange each lane has columns 16 h .. + 15
+          swap_halves(c[0], c[2]);
+          swap_halves(c[1], c[3]);
+          const int64_t j = (int64_t)at.ntile * (CF::BN / 2) + (wn * CF::FN + n) * 16;
+          if (in) {
+            if (j + h * 16 < P.I)
+              *reinterpret_cast<uint4*>(P.q + r * P.I + j + h * 16) = make_uint4(c[0], c[2], c[1], c[3]);
+            if (h == 0) put_scale(j, byte);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
       }
     }
   }
@@ -301,6 +332,11 @@ __global__ __launch_bounds__(CF::NTH, CF::NW * CF::BPC / 4) void rows8_grouped_g
   __shared__ __attribute__((aligned(1024))) char lds[CF::LDS];
   __shared__ int32_t tend[kMaxGroups];  // m-tiles of the groups up to and with g
   char* const slots = lds + CF::NST * CF::STAGE;
+  char* shared = nullptr;  // what FC1's two waves of one column tile each exchange
+  if constexpr (KIND == FC18 && CF::FN == 1) {
+    __shared__ char exchange[256];
+    shared = exchange;
+  }
   const int t = threadIdx.x;
   const int lane = t & 63;
   const int wave = uni(t >> 6);
@@ -611,7 +647,7 @@ __global__ __launch_bounds__(CF::NTH, CF::NW * CF::BPC / 4) void rows8_grouped_g
       char* free_stage = lds + (c_stage == 0 ? CF::NST - 1 : c_stage - 1) * CF::STAGE;  // the tile's last K-tile's
       Place place;
       decode(tile, place);
-      epilogue<E, KIND, CF>(P, place, wm, wn, wave, lane, free_stage, acc);
+      epilogue<E, KIND, CF>(P, place, wm, wn, wave, lane, free_stage, nullptr, acc);
       issue_scales();
       static_for<0, L>(issue);
       advance_issue();
@@ -671,7 +707,7 @@ __global__ __launch_bounds__(CF::NTH, CF::NW * CF::BPC / 4) void rows8_grouped_g
             return i32x8_t{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
           };
           const int32_t sa = (int32_t)__builtin_amdgcn_perm(cur.words[0], cur.words[0], pick);
-          const int32_t sb = (int32_t)__builtin_amdgcn_perm(cur.words[1 + (n | 1)], cur.words[1 + (n & ~1)], pick);
+          const int32_t sb = (int32_t)__builtin_amdgcn_perm(cur.words[(n | 1) < CF::FN ? 1 + (n | 1) : 1 + n], cur.words[1 + (n & ~1)], pick);
           acc[0][n] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
               both(1 + n), both(0), decltype(zero)::value && step_ == 0 ? f32x16_t{} : acc[0][n], 0, 0, n % 2 * 2 + step_, sb,
               step_, sa);
@@ -708,7 +744,7 @@ __global__ __launch_bounds__(CF::NTH, CF::NW * CF::BPC / 4) void rows8_grouped_g
       char* free_stage = lds + (c_stage == 0 ? CF::NST - 1 : c_stage - 1) * CF::STAGE;  // the tile's last K-tile's
       Place place;
       decode(tile, place);
-      epilogue<E, KIND, CF>(P, place, wm, wn, wave, lane, free_stage, acc);
+      epilogue<E, KIND, CF>(P, place, wm, wn, wave, lane, free_stage, shared, acc);
       if constexpr (kNT) {
         issue_scales();
         static_for<0, L>(issue);
@@ -797,7 +833,7 @@ __global__ __launch_bounds__(CF::NTH, CF::NW * CF::BPC / 4) void rows8_grouped_g
       for (int32_t kt = 1; kt < nk; ++kt) ktile(Int<0>{}, kt);
       Place place;
       decode(tile, place);
-      epilogue<E, KIND, CF>(P, place, wm, wn, wave, lane, nullptr, acc);
+      epilogue<E, KIND, CF>(P, place, wm, wn, wave, lane, nullptr, nullptr, acc);
     }
   }
   wait_loads<0>();
@@ -820,7 +856,7 @@ int cu_count() {
 }
 
 // The tilings of rows8_rule.h.
-using Narrow32 = Cfg8<1, 1, 1, 2, 3, 3>;  // 32 x 64, one wave
+using Narrow32 = Cfg8<1, 2, 1, 1, 3, 3>;  // 32 x 64, a wave per 32 x 32
 using Rows32 = Cfg8<1, 4, 1, 2, 3, 1>;    // 32 x 256, one wave per 32 x 64
 using Rows128 = Cfg8<2, 2, 2, 2, 2, 2>;  // 128 x 128, 64 x 64
 using Rows256 = Cfg8<2, 2, 4, 4, 2, 1>;  // 256 x 256, 128 x 128
