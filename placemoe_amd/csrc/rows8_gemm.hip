@@ -653,10 +653,10 @@ __global__ __launch_bounds__(CF::NTH, CF::NW * CF::BPC / 4) void rows8_grouped_g
       advance_issue();
     }
   } else if constexpr (kWhole) {
-    // One row tile per wave: few rows.  The weights' bytes bound a call with many copies; with a few (one
-    // token) a wave's way through its K-tiles does, so the next K-tile is read whole while this one is
-    // multiplied, and no wave waits for LDS: 0.74 us per K-tile of fc1 (codes read a quarter ahead) -> WHOLE_FC1,
-    // 0.55 of NT (a half ahead) -> WHOLE_NT.
+    // One row tile per wave: few rows.  The weights' bytes bound a call with many copies.  With a few (one
+    // token) a wave's way through its instructions does, one in 5 to 6 cycles: the next K-tile is read whole while
+    // this one is multiplied, so that no wave waits for LDS, and a 32 x 64 tile is two waves' (fc1, per K-tile
+    // of a token's 16: 0.74 us with one wave that reads a quarter ahead, 0.61 so, 0.50 with two waves).
     constexpr bool kNT = KIND == NT8;
     const uint32_t pick = 0x06040200u + 0x01010101u * h;  // bytes h and 2 + h of two words
     int32_t at[4];  // the lane's 16-byte chunk of each quarter: two make one of NT's operands

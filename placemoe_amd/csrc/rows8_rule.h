@@ -1,31 +1,29 @@
 // Which tiles a grouped GEMM over 8-bit rows runs on.
 //
 // The host knows the rows and the copies, not the counts.  Four tilings:
-//   32 x 64, a wave per block, three blocks per CU: so few tiles that wider ones
-//     would leave CUs idle (one token);
+//   32 x 64, two waves per block, three blocks per CU: where they are all there at
+//     once (one token);
 //   32 x 256, one block per CU, three stages: copies with few rows, where the
 //     call reads every copy's weights once and the matrix cores idle;
 //   128 x 128, two blocks per CU: one block's epilogue, tile switch and loads run
 //     behind the other's products;
 //   256 x 256, one block per CU: half the operand bytes per product.
-// Measured (us, 32 / 128 / 256; log-normal counts with sigma 0.4; N x K):
-//   copies rows   N     K     NT                 fc1 (N = 2 I)
-//   160    4      1536  2048   92 /  98 / 119     95 / 119 / 196
-//   160    32     1536  2048  107 / 103 / 120    114 / 125 / 193
-//   160    64     1536  2048  148 / 108 / 121    171 / 131 / 205
-//   160    256    1536  2048  397 / 210 / 197    501 / 299 / 330
-//   160    600    1536  2048  857 / 435 / 361   1146 / 653 / 606
-//   16     400    7168  2048  254 / 114 / 119    346 / 195 / 212
-//   16     2000   4096  7168    - /1069 / 868      - /1722 /1502
-//   12     192    1000  1104   20 /  13 /  21      -
-// 32 x 64 against 32 x 256 (weights not in a cache; NT, fc1): 8 rows over 160 copies of
-// 1536 x 2048 20 / 23, 22 / 26; 64 over 128 63 / 70, 65 / 74; 768 over 160 149 / 152,
-// 152 / 152; 2400 over 160 163 / 153, 166 / 154.
+// Measured (us, 32 x 64 / 32 x 256 / 128 / 256; log-normal counts with sigma 0.4; N x K):
+//   copies rows   N     K     NT                       fc1 (N = 2 I)
+//   16     1      7168  2048   11.5/ 13.7/ 14.7/ 27.5   14.3/ 17.4/ 21.2/ 48.5
+//   8      256    1536  2048   11.9/ 14.3/ 15.3/ 28.2   17.7/ 18.2/ 22.3/ 49.7
+//   160    640    1536  2048    90 /  90 /  98 / 112     94 /  94 / 119 / 193
+//   16     256    4096  7168    93 /  84 /  86 /  95     98 /  85 /  97 / 159
+//   160    2560   1536  2048    99 /  93 /  99 / 115    103 /  95 / 122 / 193
+//   160    5120   1536  2048   115 / 106 / 102 / 116    125 / 111 / 122 / 199
+//   160    41k    1536  2048   424 / 373 / 204 / 186    589 / 459 / 284 / 299
+//   160    96k    1536  2048     -    -  / 420 / 341      -    -  / 624 / 549
+//   16     16k    4096  7168     -    -  / 524 / 468      -    -  / 826 / 822
 // Past the few-rows line the rounds of tiles decide: a round costs its K-tiles
 // and a fixed part (epilogue and tile switch), both fitted to such calls.  Over
-// 150 calls (8 to 256 copies, 0.1 to 2000 rows per copy, 10 layers) the choice takes
-// 1.02 of the best tiling's time in geometric mean, 1.33 at worst (a copy whose count
-// straddles a tile's height).
+// 150 calls of each kind (8 to 256 copies, 0.1 to 2000 rows per copy, 10 layers)
+// the choice takes 1.015 (NT) and 1.01 (fc1) of the best tiling's time in geometric
+// mean, 1.33 at worst (a copy whose count straddles a tile's height).
 //
 // A result's bits do not depend on the choice: every tiling adds up K in the same
 // steps.
@@ -40,15 +38,16 @@ namespace pmx {
 // Rows per copy (with rows) up to which the 32-row tiles run: NT, FC1.
 constexpr int64_t kRows8Few[2] = {16, 32};
 // A round's cost in us: per K-tile of 128, and beside them.
-constexpr double kRows8Round128[2][2] = {{1.25, 2.0}, {1.9, 2.5}};
-constexpr double kRows8Round256[2][2] = {{1.7, 6.0}, {2.9, 10.0}};
+constexpr double kRows8Round128[2][2] = {{1.25, 2.0}, {1.7, 2.0}};
+constexpr double kRows8Round256[2][2] = {{1.5, 5.0}, {2.7, 8.0}};
 
 // The m-tile height, 32 (0: 32 x 64 tiles), 128 or 256, for `rows` rows over `copies` copies, N rows of a
 // copy's B (fc1: 2 I), K deep, on `cus` CUs.  kind: 0 NT, 1 FC1.
 inline int rows8_tiling(int kind, int64_t rows, int64_t copies, int64_t N, int64_t K, int64_t cus) {
   const auto div_up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
   const int64_t active = rows < copies ? rows : copies, nk = div_up(K, 128);
-  if (rows <= kRows8Few[kind] * active) return active * div_up(N, 256) <= 2 * cus ? 0 : 32;
+  if ((active > rows / 32 + active / 2 ? active : rows / 32 + active / 2) * div_up(N, 64) <= 3 * cus) return 0;
+  if (rows <= kRows8Few[kind] * active) return 32;
   // a copy's last tile half full on average; an eighth of the copies past their first tile
   const auto cost = [&](int64_t tile, int64_t blocks, const double (&round)[2]) {
     const int64_t spread = active + active / 8, even = rows / tile + active / 2;

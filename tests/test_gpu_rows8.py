@@ -298,6 +298,50 @@ LAYOUTS = {
     "three K-tiles": ([150, 33], 136, 384),
 }
 
+# the same with more tiles than the narrowest tiling has blocks: the wider ones
+WIDE = {
+    "ragged": ([5, 31, 32, 33, 64, 1, 0, 70, 129, 40] * 30, 200, 1104),
+    "ragged few": ([5, 31, 2, 33, 4, 1, 0, 7] * 60, 200, 1104),
+    "short K": ([70, 0, 33, 150] * 60, 136, 112),
+    "two K-tiles": ([70, 33, 90] * 60, 264, 144),
+    "three K-tiles": ([150, 33] * 100, 136, 384),
+    "odd N": ([130, 61, 0, 255, 128] * 30, 328, 272),
+    "deep": ([90, 40] * 60, 264, 2320),
+    "many rows": ([1300, 700] * 24, 520, 112),
+}
+
+
+@pytest.mark.parametrize("name", WIDE)
+def test_wide_products_of_integers_are_exact(cuda, name):
+    counts, N, K = WIDE[name]
+    print(f"rows8 wide {name}", flush=True)
+    M, G = sum(counts), len(counts)
+    a, b = _ints((M, K), 1).to(cuda), _ints((G, N, K), 2).to(cuda)
+    off = _offsets(counts)
+    got = rows8.group_gemm_nt_rows8(rows8.quantize_rows(a), rows8.quantize_rows(b), off.to(cuda))
+    want = torch.cat([(a[off[g]:off[g + 1]].double() @ b[g].double().t()).float().to(BF) for g in range(G)])
+    assert_exact(got, want, name)
+
+
+@pytest.mark.parametrize("name", WIDE)
+def test_wide_fc1_equals_single_copies(cuda, name):
+    """A copy's rows among those of many others, and alone on narrow tiles (tested against 64 bits): the same bits."""
+    counts, N, K = WIDE[name]
+    print(f"rows8 wide fc1 {name}", flush=True)
+    A, G, I, T = sum(counts), len(counts), N // 32 * 16, 333
+    x = rows8.quantize_rows(_randn((T, K), 3).to(cuda))
+    w = rows8.quantize_rows(_randn((G, 2 * I, K), 4, std=0.06).to(cuda))
+    token = torch.randint(0, T, (A,), generator=torch.Generator().manual_seed(5)).to(torch.int32).to(cuda)
+    row_w = torch.rand(A, generator=torch.Generator().manual_seed(6)).to(BF).to(cuda)
+    off = _offsets(counts)
+    act = rows8.gemm_fc1_swiglu_rows8(x, w, off.to(cuda), token, row_w)
+    for g in (0, 1, 3, G // 2, G - 2, G - 1):
+        rows = slice(int(off[g]), int(off[g + 1]))
+        one = rows8.Rows8(w.codes[g:g + 1].contiguous(), w.scales[g:g + 1].contiguous(), BF)
+        ref = rows8.gemm_fc1_swiglu_rows8(x, one, _offsets([rows.stop - rows.start]).to(cuda), token[rows].clone(), row_w[rows].clone())
+        assert torch.equal(act.codes.view(torch.uint8)[rows], ref.codes.view(torch.uint8)), f"copy {g}"
+        assert torch.equal(act.scales[:, rows], ref.scales), f"copy {g}"
+
 
 @pytest.mark.parametrize("dtype", [BF, F16])
 @pytest.mark.parametrize("name", LAYOUTS)
@@ -403,10 +447,12 @@ def test_offsets_past_the_rows_are_clamped(cuda):
 def test_a_row_depends_on_itself_and_its_copy_alone(cuda):
     """The same row in calls of one, a few, and many rows, in any slot: the same bits."""
     K, N = 1104, 264
-    a, w = _randn((2000, K), 1).to(cuda), _randn((1, N, K), 2, std=0.05).to(cuda)
+    a, w = _randn((2600, K), 1).to(cuda), _randn((1, N, K), 2, std=0.05).to(cuda)
     q = rows8.quantize_rows(a)
-    ref = rows8.group_gemm_nt_rows8(q, rows8.quantize_rows(w), torch.tensor([0, 2000], dtype=torch.int32, device=cuda))
-    for rows, slots in ((1, 1), (16, 1), (20, 3), (130, 2), (300, 5)):
+    ref = rows8.group_gemm_nt_rows8(rows8.quantize_rows(a.repeat(8, 1)), rows8.quantize_rows(w),
+                                    torch.tensor([0, 20800], dtype=torch.int32, device=cuda))[:2600]
+    assert_exact(rows8.group_gemm_nt_rows8(q, rows8.quantize_rows(w), _offsets([2600]).to(cuda)), ref, "2600 rows")
+    for rows, slots in ((1, 1), (16, 1), (20, 3), (130, 2), (300, 5), (400, 200), (2600, 150)):
         part = rows8.quantize_rows(a[:rows])
         counts = [0] * slots
         counts[slots // 2] = rows
@@ -417,7 +463,7 @@ def test_a_row_depends_on_itself_and_its_copy_alone(cuda):
 
 
 # few rows: 32 x 64 tiles, and 32 x 256 ones
-FEW = {"few tiles": ([2] * 100, 1024, 272), "many tiles": ([3, 0, 7] * 100, 1032, 272)}
+FEW = {"few tiles": ([2] * 100, 448, 272), "many tiles": ([3, 0, 7] * 100, 1032, 272)}
 
 
 @pytest.mark.parametrize("name", FEW)
@@ -436,7 +482,7 @@ def test_few_rows(cuda, name):
     act = rows8.gemm_fc1_swiglu_rows8(q, w, off.to(cuda))
     for g in (0, 2, G - 1):
         rows = slice(int(off[g]), int(off[g + 1]))
-        many = torch.arange(rows.start, rows.stop, dtype=torch.int32, device=cuda).repeat(100)
+        many = torch.arange(rows.start, rows.stop, dtype=torch.int32, device=cuda).repeat(3000)
         one = rows8.Rows8(w.codes[g:g + 1].contiguous(), w.scales[g:g + 1].contiguous(), BF)
         ref = rows8.gemm_fc1_swiglu_rows8(q, one, torch.tensor([0, many.numel()], dtype=torch.int32, device=cuda), many)
         n = rows.stop - rows.start
@@ -444,16 +490,16 @@ def test_few_rows(cuda, name):
 
 
 def test_every_tiling_gives_the_same_bits(cuda):
-    """4096 rows run on 256-row tiles, 200 on 128-row ones, 10 on 32-row ones."""
+    """4096 rows run on 256-row tiles, 1000 on 128-row ones, 10 on 32 x 64 ones (32 x 256 ones need many copies)."""
     N, K = 4096, 1024
     x, w = _randn((4096, K), 1).to(cuda), _randn((1, N, K), 2, std=0.03).to(cuda)
     qw = rows8.quantize_rows(w)
     nt, fc1 = [], []
-    for rows in (4096, 200, 10):
+    for rows in (4096, 1000, 10):
         q, off = rows8.quantize_rows(x[:rows]), torch.tensor([0, rows], dtype=torch.int32, device=cuda)
         nt.append(rows8.group_gemm_nt_rows8(q, qw, off))
         fc1.append(rows8.gemm_fc1_swiglu_rows8(q, qw, off).codes.view(torch.uint8))
-    for rows, a, b in zip((200, 10), nt[1:], fc1[1:]):
+    for rows, a, b in zip((1000, 10), nt[1:], fc1[1:]):
         assert_exact(a, nt[0][:rows], f"{rows} rows")
         assert torch.equal(b, fc1[0][:rows]), f"{rows} rows of fc1"
 

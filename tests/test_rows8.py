@@ -155,7 +155,7 @@ def tiling(tmp_path_factory):
 
 
 def test_tiling_rule_takes_the_faster_one(tiling):
-    measured = {  # us with 32 x 256, 128 x 128 and 256 x 256 tiles
+    measured = {  # us with 32 x 256 (or 32 x 64), 128 x 128 and 256 x 256 tiles
         ("nt", 640, 160, 1536, 2048): (91, 96, 121), ("nt", 10240, 160, 1536, 2048): (149, 105, 127),
         ("nt", 96000, 160, 1536, 2048): (857, 421, 355), ("nt", 2304, 12, 1000, 1104): (20, 13, 20),
         ("nt", 32000, 16, 4096, 7168): (2439, 1136, 848), ("nt", 64, 16, 4096, 7168): (80, 81, 105),
@@ -172,12 +172,23 @@ def test_gpu_cases_reach_every_tiling(tiling):
     def heights(kind, cases):
         return {n: h for n, h in zip(cases, tiling([(kind, sum(c), len(c), N, K) for c, N, K in cases.values()]))}
 
-    small = heights("nt", test_gpu_rows8.LAYOUTS)
-    assert set(small.values()) == {0, 32, 128}
+    def even(cases):
+        return {n: (c, N // 32 * 32, K) for n, (c, N, K) in cases.items()}
+
+    assert 0 in heights("nt", test_gpu_rows8.LAYOUTS).values()
+    assert set(heights("nt", test_gpu_rows8.WIDE).values()) == {32, 128}
+    assert set(heights("fc1", even(test_gpu_rows8.WIDE)).values()) == {32, 128}
     assert 256 in heights("nt", test_gpu_rows8.LARGE).values()
-    assert 256 in heights("fc1", {n: (c, N // 32 * 32, K) for n, (c, N, K) in test_gpu_rows8.LARGE.items()}).values()
-    # one row of the same copy in calls of every tiling (test_a_row_depends_on_itself_and_its_copy_alone)
-    assert set(tiling([("nt", rows, 1, 264, 1104) for rows in (1, 16, 20, 130)])) == {0, 128}
+    assert 256 in heights("fc1", even(test_gpu_rows8.LARGE)).values()
+    # test_wide_fc1_equals_single_copies' other side
+    alone = [("fc1", 1300, 1, 512, 112), ("fc1", 255, 1, 320, 272)]
+    assert tiling(alone) == [0, 0]
+    # one row of the same copy in calls of several tilings (test_a_row_depends_on_itself_and_its_copy_alone)
+    calls = [(20800, 1), (2600, 1), (1, 1), (400, 200), (2600, 150)]
+    assert tiling([("nt", *c, 264, 1104) for c in calls]) == [128, 0, 0, 32, 128]
+    # test_every_tiling_gives_the_same_bits
+    for kind, N in (("nt", 4096), ("fc1", 4096)):
+        assert tiling([(kind, rows, 1, N, 1024) for rows in (4096, 1000, 10)]) == [256, 128, 0]
     few = [(k, sum(c), len(c), N, K) for k in ("nt", "fc1") for c, N, K in test_gpu_rows8.FEW.values()]
     assert tiling(few) == [0, 32] * 2
 
