@@ -21,8 +21,17 @@
 
 #include "common.h"
 
-// Between rows8_gemm.hip and rows8_layer.hip, not part of the C ABI.
+// Between the sources of the layer, not part of the C ABI.
 __attribute__((visibility("hidden"))) int pmx_rows8_layer_check(int64_t T, int32_t K, int64_t H, int64_t I, int32_t C);
+// The grouped product as rows in blocks of 16-bit integers (below): y [M, N], y_scales [M, block16_row(N)].
+__attribute__((visibility("hidden"))) int pmx_rows8_group_gemm_nt_block16(const void* a, const void* a_scales, const void* b,
+                                                                          const void* b_scales, const int32_t* offsets,
+                                                                          int32_t G, int64_t M, int64_t N, int64_t K, void* y,
+                                                                          void* y_scales, pmx_stream_t stream);
+// out[t] = sum of the rows pos[t, k] of y, in k order, rounded once to bf16 or fp16.
+__attribute__((visibility("hidden"))) int pmx_rows8_sum_block16(const void* y, const void* y_scales, const int32_t* pos,
+                                                                int64_t T, int32_t K, int64_t H, bool f16, void* out,
+                                                                pmx_stream_t stream);
 
 namespace {
 
@@ -58,6 +67,25 @@ __device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d) {
     };
     return one(a) | one(b) << 8 | one(c) << 16 | one(d) << 24;
   }
+}
+
+// fc2's rows between the product and the sum over a token's experts: blocks of
+// 32 columns as 16-bit integers beside a power of two, the smallest at which
+// the largest finite magnitude is at most 32767 of it.  A value is off by at
+// most 2^-15 of its block's largest; bf16 rows were off by up to 2^-9 of
+// themselves, as much as the sum's own rounding: the layer was 1.4 times
+// further from its definition in 64 bits (0.0024, now 0.0017), for as many
+// bytes.  -32768 stands for what is not finite.
+constexpr int kBlock16 = 16;
+struct EltBlock16 {
+  static constexpr int kCode = kBlock16;
+};
+// Bytes of a row's exponents (e + 127 each): whole words of four blocks.
+__host__ __device__ constexpr int64_t block16_row(int64_t N) { return (N + 127) / 128 * 4; }
+// 32767 = 1.99994 * 2^14.
+__device__ __forceinline__ uint32_t scale16_byte(uint32_t most) {
+  const int b = (int)(most >> 23) - 14 + ((most & 0x7fffffu) > 0x7ffe00u ? 1 : 0);
+  return (uint32_t)(b < 0 ? 0 : b);
 }
 
 // Four codes -> the values that they stand for beside 2^0 (exact).

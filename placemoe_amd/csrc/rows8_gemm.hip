@@ -56,6 +56,7 @@ struct Params8 {
   int64_t M, N, K;           // M rows over all groups; N: rows of a B[g] (FC1: 2 I)
   int64_t I;
   bf16_t* c;                 // NT: [M, N]
+  uint8_t* ys;               // NT in blocks of 16-bit integers: c's exponents
   uint8_t *q, *qs;           // FC1: act's codes [M, I] and exponents
   const bf16_t* row_w;       // FC1: [M], null: 1
 };
@@ -185,6 +186,32 @@ __device__ __forceinline__ void swap_halves(uint32_t& lo, uint32_t& hi) {
   hi = v[1];
 }
 
+// The largest finite magnitude among the N values of this lane and the one 32 lanes on; `finite`: no lane of the
+// wave holds another kind.  (Maxima that pass NaN on, two values to an instruction.)
+template <int N>
+__device__ __forceinline__ float most_finite(const float* f, bool& finite) {
+  const auto halves = [](float m) __attribute__((always_inline)) {
+    const auto v = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false);
+    return __builtin_elementwise_maximum(__uint_as_float(v[0]), __uint_as_float(v[1]));
+  };
+  float most = 0.f;
+#pragma unroll
+  for (int i = 0; i < N; i += 2)
+    most = __builtin_elementwise_maximum(__builtin_elementwise_maximum(most, __builtin_fabsf(f[i])), __builtin_fabsf(f[i + 1]));
+  most = halves(most);
+  finite = __ballot(!(most < __builtin_inff())) == 0;
+  if (!finite) {
+    most = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float a = __builtin_fabsf(f[i]);
+      most = a > most && a < __builtin_inff() ? a : most;
+    }
+    most = halves(most);
+  }
+  return most;
+}
+
 // An accumulator holds its 32 x 32 output tile transposed (B is the MFMA's
 // first operand): lane l has row l%32, columns 8*(i/4) + 4*(l/32) + i%4.
 template <class E, int KIND, class CF>
@@ -221,17 +248,51 @@ __device__ __forceinline__ void epilogue(const Params8& P, const Place& at, int 
         const int sw = CPR == 16 ? row & 15 : CPR == 8 ? kc_swz(row) : row >> 2 & 3;
         return stage + ((row / RPP) * CF::NW + wave) * 1024 + (row % RPP) * (CPR * 16) + ((c ^ sw) << 4);
       };
+      [[maybe_unused]] uint32_t exps = 0;
 #pragma unroll
       for (int n = 0; n < CF::FN; ++n) {
         here(acc[m][n]);
         const f32x16_t& v = acc[m][n];
+        uint32_t w[8];  // pairs of columns 8 (i/2) + 4 h + 2 (i%2)
+        if constexpr (E::kCode == kBlock16) {
+          float f[16];
+          bool finite;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) f[i] = v[i];
+          const float most = most_finite<16>(f, finite);
+          const uint32_t byte = scale16_byte(__float_as_uint(most));
+          const float inv = inv_scale(byte);
+          exps |= byte << (8 * n);
+          // beside 1.5 * 2^23 the low 16 bits of a sum are the integer, rounded to nearest even
+          const auto code = [&](float f) { return __float_as_uint(__builtin_fmaf(f, inv, 12582912.0f)); };
+#pragma unroll
+          for (int i = 0; i < 8; ++i) w[i] = __builtin_amdgcn_perm(code(v[2 * i + 1]), code(v[2 * i]), 0x05040100u);
+          if (!finite) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              if (!(__builtin_fabsf(v[2 * i]) < __builtin_inff())) w[i] = (w[i] & 0xffff0000u) | 0x8000u;
+              if (!(__builtin_fabsf(v[2 * i + 1]) < __builtin_inff())) w[i] = (w[i] & 0xffffu) | 0x80000000u;
+            }
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) w[i] = E::pack2(v[2 * i], v[2 * i + 1]);
+        }
 #pragma unroll
         for (int p = 0; p < 2; ++p) {  // 16 columns: the half-waves exchange, and each lane has 8 of them
-          uint32_t w0 = E::pack2(v[8 * p], v[8 * p + 1]), w1 = E::pack2(v[8 * p + 2], v[8 * p + 3]);
-          uint32_t w2 = E::pack2(v[8 * p + 4], v[8 * p + 5]), w3 = E::pack2(v[8 * p + 6], v[8 * p + 7]);
-          swap_halves(w0, w2);
-          swap_halves(w1, w3);
-          *reinterpret_cast<uint4*>(place(lane & 31, n * 4 + p * 2 + h)) = make_uint4(w0, w1, w2, w3);
+          swap_halves(w[4 * p], w[4 * p + 2]);
+          swap_halves(w[4 * p + 1], w[4 * p + 3]);
+          *reinterpret_cast<uint4*>(place(lane & 31, n * 4 + p * 2 + h)) =
+              make_uint4(w[4 * p], w[4 * p + 1], w[4 * p + 2], w[4 * p + 3]);
+        }
+      }
+      if constexpr (E::kCode == kBlock16) {
+        const int64_t first = (int64_t)at.ntile * (CF::BN / 32) + wn * CF::FN;  // the wave's blocks, a multiple of FN
+        if (in && h == 0 && first * 32 < P.N) {
+          uint8_t* const e = P.ys + r * block16_row(P.N) + first;
+          if constexpr (CF::FN == 4) *reinterpret_cast<uint32_t*>(e) = exps;
+          else if constexpr (CF::FN == 2) *reinterpret_cast<uint16_t*>(e) = (uint16_t)exps;
+          else *e = (uint8_t)exps;
         }
       }
       wait_lds();
@@ -256,10 +317,6 @@ __device__ __forceinline__ void epilogue(const Params8& P, const Place& at, int 
       // A block's exponent and codes: `f` holds the lane's N values, columns 8 (i/4) + 4 h + i%4 of the block or,
       // one column tile per wave, of the wave's half of it.
       const auto weigh = [&](float gate, float up) { return silu_f32(gate) * up * w; };
-      const auto most_of = [](float most, float f) {
-        const float v = __builtin_fabsf(f);
-        return v > most && v < __builtin_inff() ? v : most;
-      };
       const auto code = [](const float* f, float inv) {
         return codes4<kFmtE4M3>(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv);
       };
@@ -268,10 +325,11 @@ __device__ __forceinline__ void epilogue(const Params8& P, const Place& at, int 
       };
       if constexpr (CF::FN == 1) {
         here(acc[m][0]);
-        float f[8], most = 0.f;
+        float f[8];
+        bool finite;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = weigh(acc[m][0][i], acc[m][0][i + 8]), most = most_of(most, f[i]);
-        most = fmaxf(most, __shfl_xor(most, 32, 64));
+        for (int i = 0; i < 8; ++i) f[i] = weigh(acc[m][0][i], acc[m][0][i + 8]);
+        const float most = most_finite<8>(f, finite);
         float* const of_waves = reinterpret_cast<float*>(shared);  // [2][32]; a K-tile's barrier before it is used again
         if (h == 0) of_waves[wn * 32 + lane] = most;
         wait_lds();
@@ -290,10 +348,11 @@ __device__ __forceinline__ void epilogue(const Params8& P, const Place& at, int 
         for (int n = 0; n < CF::FN; n += 2) {
           here(acc[m][n]);
           here(acc[m][n + 1]);
-          float f[16], most = 0.f;
+          float f[16];
+          bool finite;
 #pragma unroll
-          for (int i = 0; i < 16; ++i) f[i] = weigh(acc[m][n][i], acc[m][n + 1][i]), most = most_of(most, f[i]);
-          most = fmaxf(most, __shfl_xor(most, 32, 64));
+          for (int i = 0; i < 16; ++i) f[i] = weigh(acc[m][n][i], acc[m][n + 1][i]);
+          const float most = most_finite<16>(f, finite);
           const uint32_t byte = scale_byte<kFmtE4M3>(__float_as_uint(most));
           const float inv = inv_scale(byte);
           uint32_t c[4];  // columns 8 i + 4 h .. + 3
@@ -912,16 +971,16 @@ bool any_tiles_fit(const Params8& P) {
 
 template <class E>
 int nt_t(const void* a, const void* as, const void* b, const void* bs, const int32_t* offsets, int32_t G, int64_t M, int64_t N,
-         int64_t K, void* c, pmx_stream_t stream) {
+         int64_t K, void* c, void* ys, pmx_stream_t stream) {
   Params8 P = {};
   P.a = (const uint8_t*)a, P.as = (const uint8_t*)as, P.a_rows = M;
   P.b = (const uint8_t*)b, P.bs = (const uint8_t*)bs;
-  P.offsets = offsets, P.G = G, P.M = M, P.N = N, P.K = K, P.c = (bf16_t*)c;
+  P.offsets = offsets, P.G = G, P.M = M, P.N = N, P.K = K, P.c = (bf16_t*)c, P.ys = (uint8_t*)ys;
   if (const int rc = check(P)) return rc;
   if (N % 8) return PMX_ERR_SHAPE;
   if (M == 0) return PMX_OK;
-  if (!a || !as || !b || !bs || !offsets || !c) return PMX_ERR_ARG;
-  if (!aligned16(a) || !aligned16(as) || !aligned16(b) || !aligned16(bs) || !aligned16(c)) return PMX_ERR_SHAPE;
+  if (!a || !as || !b || !bs || !offsets || !c || (E::kCode == kBlock16 && !ys)) return PMX_ERR_ARG;
+  if (!aligned16(a) || !aligned16(as) || !aligned16(b) || !aligned16(bs) || !aligned16(c) || !aligned16(ys)) return PMX_ERR_SHAPE;
   return launch<E, NT8>(P, stream);
 }
 
@@ -961,13 +1020,19 @@ int pmx_rows8_layer_check(int64_t T, int32_t K, int64_t H, int64_t I, int32_t C)
   return any_tiles_fit<NT8>(P) ? PMX_OK : PMX_ERR_SHAPE;
 }
 
+int pmx_rows8_group_gemm_nt_block16(const void* a, const void* a_scales, const void* b, const void* b_scales,
+                                    const int32_t* offsets, int32_t G, int64_t M, int64_t N, int64_t K, void* y, void* y_scales,
+                                    pmx_stream_t stream) {
+  return nt_t<EltBlock16>(a, a_scales, b, b_scales, offsets, G, M, N, K, y, y_scales, stream);
+}
+
 extern "C" {
 
 #define PMX_ROWS8_GEMM_ENTRIES(SUFFIX, E)                                                                                   \
   int pmx_rows8_group_gemm_nt##SUFFIX(const void* a, const void* a_scales, const void* b, const void* b_scales,             \
                                       const int32_t* offsets, int32_t G, int64_t M, int64_t N, int64_t K, void* c,          \
                                       pmx_stream_t stream) {                                                                \
-    return nt_t<E>(a, a_scales, b, b_scales, offsets, G, M, N, K, c, stream);                                               \
+    return nt_t<E>(a, a_scales, b, b_scales, offsets, G, M, N, K, c, nullptr, stream);                                      \
   }                                                                                                                         \
   int pmx_rows8_gemm_fc1_swiglu##SUFFIX(const void* x, const void* x_scales, int64_t T, const int32_t* row_token,           \
                                         const void* w, const void* w_scales, const int32_t* offsets, int32_t G, int64_t A,  \

@@ -11,7 +11,7 @@ namespace {
 // Where the workspace's parts begin (bytes, multiples of 256).  The routing's
 // own workspace is first: its status word is the workspace's.
 struct Parts {
-  size_t route, phys, pos, counts, offsets, row_token, row_w, x, xs, act, acts, y, total;
+  size_t route, phys, pos, counts, offsets, row_token, row_w, x, xs, act, acts, y, ys, total;
 };
 
 // false: more than a size_t holds (or no such layer).
@@ -38,6 +38,7 @@ bool parts_of(int64_t T, int32_t K, int64_t H, int64_t I, int32_t C, Parts& p) {
   p.act = take(A * i);
   p.acts = take(gi * A * kScaleBytes);
   p.y = take(A * h * 2);
+  p.ys = take(A * block16_row(H));
   p.total = at;
   return true;
 }
@@ -54,7 +55,8 @@ int layer_t(const void* hidden, const void* w, const int64_t* sel, const int64_t
   if (T > 0 && (!hidden || !w || !out || !gate_up || !gate_up_scales || !down || !down_scales)) return PMX_ERR_ARG;
   if (!workspace || workspace_bytes < p.total) return PMX_ERR_ARG;
   const auto aligned = [](const void* q) { return (reinterpret_cast<uintptr_t>(q) & 15u) == 0; };
-  if (!aligned(workspace) || !aligned(gate_up) || !aligned(gate_up_scales) || !aligned(down) || !aligned(down_scales))
+  if (!aligned(workspace) || !aligned(gate_up) || !aligned(gate_up_scales) || !aligned(down) || !aligned(down_scales) ||
+      !aligned(out))
     return PMX_ERR_SHAPE;
   char* ws = static_cast<char*>(workspace);
   int32_t* pos = reinterpret_cast<int32_t*>(ws + p.pos);
@@ -72,10 +74,10 @@ int layer_t(const void* hidden, const void* w, const int64_t* sel, const int64_t
                                                                           gate_up_scales, offsets, C, T * K, H, I, ws + p.row_w,
                                                                           ws + p.act, ws + p.acts, stream);
   if (rc != PMX_OK) return PMX_ERR_HIP;
-  rc = (f16 ? pmx_rows8_group_gemm_nt_f16 : pmx_rows8_group_gemm_nt)(ws + p.act, ws + p.acts, down, down_scales, offsets, C,
-                                                                      T * K, H, I, ws + p.y, stream);
+  rc = pmx_rows8_group_gemm_nt_block16(ws + p.act, ws + p.acts, down, down_scales, offsets, C, T * K, H, I, ws + p.y, ws + p.ys,
+                                       stream);
   if (rc != PMX_OK) return PMX_ERR_HIP;
-  rc = (f16 ? pmx_moe_gather_f16 : pmx_moe_gather)(ws + p.y, pos, T, K, H, out, stream);
+  rc = pmx_rows8_sum_block16(ws + p.y, ws + p.ys, pos, T, K, H, f16, out, stream);
   return rc != PMX_OK ? PMX_ERR_HIP : PMX_OK;
 }
 

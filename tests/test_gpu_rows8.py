@@ -702,8 +702,10 @@ def _layer_oracle(hidden, w, phys, experts8, eps):
     between those of act - slack and act + slack at the block's power of two:
     where these agree it is exact, where a border lies between them it may be
     either, off by at most their distance (a block whose power of two itself may
-    differ: both powers are tried).  fc2 carries these distances on, adds its
-    own 2^-11, and rounds each row once; the rows' sum is rounded once more.
+    differ: both powers are tried).  fc2 carries these distances on and adds its
+    own 2^-11; its rows, 16-bit integers beside a power of two with the largest
+    of 32 columns between 16383.5 and 32767, are off by at most half of it, 2^-15 of
+    that largest.  The rows' sum is rounded once.
     """
     C = experts8.down.shape[0]
     T, K = phys.shape
@@ -742,7 +744,8 @@ def _layer_oracle(hidden, w, phys, experts8, eps):
         y, big2 = O.grouped_nt(held, down[None], one)
         off = far @ np.abs(down).T + big2 * 2.0**-11
         np.add.at(out, at[:, 0], y)
-        np.add.at(tol, at[:, 0], off + (np.abs(y) + off) * eps / 2)
+        most = np.pad(np.abs(y) + off, ((0, 0), (0, -H % 32))).reshape(len(at), -1, 32).max(-1)
+        np.add.at(tol, at[:, 0], off + np.repeat(most, 32, axis=1)[:, :H] * 2.0**-15)
     return out, tol + (np.abs(out) + tol) * eps / 2
 
 
@@ -819,6 +822,37 @@ def test_layer_without_tokens_reports_its_counts(cuda):
     placemoe_amd.expert_layer_rows8(_randn((0, H), 3).to(cuda), torch.ones((0, 2), dtype=BF, device=cuda),
                                     torch.zeros((0, 2), dtype=torch.int64, device=cuda), q, recorder=seen.append)
     assert len(seen) == 1 and seen[0].dtype == torch.int32 and seen[0].tolist() == [0] * C
+
+
+def test_layer_keeps_what_is_not_finite_to_its_token(cuda):
+    C, H, I, T = 3, 96, 64, 40
+    q = rows8.Experts8.quantize(_randn((C, 2 * I, H), 1, BF, 0.1).to(cuda), _randn((C, H, I), 2, BF, 0.1).to(cuda))
+    x, w = _randn((T, H), 3).to(cuda), torch.full((T, 2), 0.5, dtype=BF, device=cuda)
+    sel = torch.stack([torch.arange(T) % C, (torch.arange(T) + 1) % C], 1).to(cuda)
+    want = placemoe_amd.expert_layer_rows8(x, w, sel, q)
+    bad = x.clone()
+    bad[2, 7], bad[20, 50], w2 = math.nan, math.inf, w.clone()
+    w2[31, 1] = math.nan
+    got = placemoe_amd.expert_layer_rows8(bad, w2, sel, q)
+    hit = torch.tensor([2, 20, 31], device=cuda)
+    assert got[hit].isnan().all()
+    rest = torch.ones(T, dtype=torch.bool, device=cuda)
+    rest[hit] = False
+    assert_exact(got[rest], want[rest], "the other tokens")
+
+
+@pytest.mark.parametrize("K", [1, 2, 3, 4, 6, 8, 11])
+@pytest.mark.parametrize("H", [16, 48, 2064])
+def test_layer_sums_any_number_of_experts(cuda, H, K):
+    T, C, I = 5, 12, 32
+    hidden, g = _randn((T, H), H), torch.Generator().manual_seed(K)
+    sel = torch.stack([torch.randperm(C, generator=g)[:K] for _ in range(T)])
+    w = torch.softmax(torch.randn((T, K), generator=g), -1).to(BF)
+    q = rows8.Experts8.quantize(_randn((C, 2 * I, H), 1, BF, 0.1).to(cuda), _randn((C, H, I), 2, BF, 0.1).to(cuda))
+    got = placemoe_amd.expert_layer_rows8(hidden.to(cuda), w.to(cuda), sel.to(cuda), q)
+    exact, tol = _layer_oracle(hidden, w, sel.numpy(), q, torch.finfo(BF).eps)
+    off = np.abs(got.double().cpu().numpy() - exact)
+    assert (off <= tol * 1.0001 + SUBNORMAL[BF]).all(), (off - tol).max()
 
 
 def test_layer_with_one_expert_twice(cuda):
