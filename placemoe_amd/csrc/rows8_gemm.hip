@@ -13,13 +13,17 @@
 // 2^-13 of the largest one: 1.5e-5 of a random sum, a hundredth of the half
 // step to which a bf16 result is rounded.  FC1's results are rounded to 8
 // bits, and there an error of 1e-5 moves one code in some thousands across a
-// border, by a whole step: the layer's output was 0.0031 off its definition in
-// 64 bits, against 0.0024 with exact products (fc2's bf16 rows and their sum
-// account for that).  So FC1 converts the codes, with their powers of two, to
-// bf16 in registers (v_cvt_scalef32_pk_bf16_fp8, exact) and multiplies on
-// v_mfma_f32_32x32x16_bf16, whose sums are good to fp32; it reads as few bytes.
+// border, by a whole step: of the layer's output that is 0.002, more than its
+// rounding to bf16 (0.0017).  So FC1 converts the codes, with their powers of
+// two, to bf16 in registers (v_cvt_scalef32_pk_bf16_fp8, exact) and multiplies
+// on v_mfma_f32_32x32x16_bf16, whose sums are good to fp32; it reads as few bytes.
 //
 // Bound: MFMA from some hundred rows per group on, the weights' bytes below.
+// Measured: NT 65536 x 4096 x 7168 over 16 groups 1.57-1.66 ms, 2.3-2.45 PFLOP/s at
+// the power limit (torch's 8-bit product of 8192^3 in one process with it: 2.50
+// against 2.46); FC1 of 65536 rows of 160 copies of 1536 x 2048 0.42-0.46 ms, 0.9-1.0
+// PFLOP/s (bf16 products of 8192^3: 1.28); 768 rows of those copies 89 (NT) and 91 us,
+// 5.6 TB/s of weights.
 //
 // Tiles of BM x BN, K in steps of 128 through a ring of NST stages filled by
 // buffer->LDS loads; 128-byte rows with 16-byte chunk c at c ^ ((row >> 1) & 7),
