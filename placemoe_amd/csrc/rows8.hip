@@ -11,8 +11,8 @@
 // SwiGLU backward of 65536 rows of 2048 in 250 (5.4; a large copy: 4.8).
 //
 // Rows need no alignment: a lane's 8 columns are one load wherever they
-// start (gfx950 takes unaligned vector accesses), and the row's last, partial
-// 8 columns go one by one.
+// start (gfx950 takes unaligned vector accesses); a row's last, partial 8 are
+// shifted out of the 8 that end with it.
 
 #include "rows8.h"
 

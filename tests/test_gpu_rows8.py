@@ -1088,3 +1088,30 @@ def test_checkpointed_layer_with_one_gradient_wanted(cuda, wanted):
     every, one = grads(("hidden", "weights", "fc1", "fc2")), grads((wanted,))
     assert_exact(one[wanted], every[wanted], wanted)
     assert all(g is None for k, g in one.items() if k != wanted)
+
+
+def test_nothing_waits_for_the_gpu(cuda):
+    """Every op, the serving layer and a checkpointed step under torch's synchronisation errors."""
+    case = _every_op_case(cuda, 60, 3)
+    wl = make_workload("toy", device=cuda, tokens=50)
+    q = rows8.Experts8.quantize(wl.fc1, wl.fc2)
+    x = wl.hidden.clone().requires_grad_()
+
+    def step():
+        outs = _every_op(*case)[:1]
+        with torch.no_grad():
+            outs.append(placemoe_amd.expert_layer_rows8(wl.hidden, wl.routing_weights, wl.selected, q, mapping=wl.mapping,
+                                                        sources=wl.sources))
+        out = experts.expert_layer(x, wl.routing_weights, wl.selected, wl.fc2, fc1_1_2_weight=wl.fc1, mapping=wl.mapping,
+                                   sources=wl.sources, activation_checkpoint="int8")
+        return outs + [out.detach(), torch.autograd.grad(out, x, torch.ones_like(out))[0]]
+
+    want = step()
+    torch.cuda.synchronize()
+    torch.cuda.set_sync_debug_mode("error")
+    try:
+        got = step()
+    finally:
+        torch.cuda.set_sync_debug_mode("default")
+    for k, (a, b) in enumerate(zip(got, want)):
+        assert_exact(a, b, f"output {k}")
