@@ -147,7 +147,9 @@ def quantize_rows(x: torch.Tensor, fmt: str = "e4m3") -> Rows8:
             "columns must be contiguous and the rows of a 2-D x apart"
         )
         ld = max(N, x.stride(0))
-    q = _empty(x.shape, code, x.dtype, dev)
+    # (the cheapest allocations: a small call's time is the host's)
+    q = Rows8(torch.empty_like(x, dtype=code) if ld == N else x.new_empty((R, N), dtype=code),
+              x.new_empty((*lead, -(-N // GROUP), R, 16), dtype=torch.uint8), x.dtype)
     _launch("pmx_rows8_quantize", x.dtype, dev, _ptr(x), ld, R * N, G, R, N, _FORMAT_CODES[code], _ptr(q.codes),
             _ptr(q.scales))
     return q
@@ -198,11 +200,10 @@ def swiglu_bwd_rows8(d_act: torch.Tensor, gu: Rows8, row_w: torch.Tensor | None 
         assert row_w is not None, "row_src names the rows' weights: row_w is needed"
         _indices("row_src", row_src, R)
         num_assign = R if num_assign is None else int(num_assign)
-        dw = torch.empty(num_assign, dtype=dt, device=dev)
+        dw = d_act.new_empty(num_assign)
         if I == 0:
             dw.zero_()
-    dg1 = torch.empty((R, 2 * I), dtype=dt, device=dev)
-    act_w = torch.empty((R, I), dtype=dt, device=dev)
+    dg1, act_w = d_act.new_empty((R, 2 * I)), torch.empty_like(d_act)
     _launch("pmx_rows8_swiglu_bwd", dt, dev, _ptr(d_act), _ptr(gu.codes), _ptr(gu.scales), _ptr(row_w), _ptr(row_src),
             R, I, dw.numel() if dw is not None else 0, _FORMAT_CODES[gu.codes.dtype], _ptr(dg1), _ptr(act_w), _ptr(dw))
     return dg1, act_w, dw
