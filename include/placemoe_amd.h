@@ -514,9 +514,9 @@ int pmx_rows8_swiglu_bwd(const void* d_act, const void* codes, const void* scale
 /* C[rows of g] = A[rows of g] B[g]^T over 8-bit rows (e4m3), fp32 sums, C bf16
  * [M, N]; rows of g: offsets[g] .. offsets[g+1]-1 (offsets outside [0, M] are
  * clamped; if they descend anywhere, nothing is written).  A: codes [M, K]; B:
- * codes [G, N, K], each with its scales.  K a multiple of 16, N of 8, pointers
- * 16-byte aligned, N*K and the scales of all rows below 2 GiB, else
- * PMX_ERR_SHAPE. */
+ * codes [G, N, K], each with its scales.  1 <= G <= 2048; K a multiple of 16, N
+ * of 8, pointers 16-byte aligned, N*K and the scales of all rows below 2 GiB,
+ * else PMX_ERR_SHAPE. */
 int pmx_rows8_group_gemm_nt(const void* a, const void* a_scales, const void* b, const void* b_scales,
                             const int32_t* offsets, int32_t G, int64_t M, int64_t N, int64_t K, void* c,
                             pmx_stream_t stream);
@@ -542,7 +542,7 @@ int pmx_rows8_gemm_fc1_swiglu(const void* x, const void* x_scales, int64_t T, co
  * fc2's rows are kept to 16 bits beside a power of two per 32 columns (2^-15 of
  * the block's largest value), their sum is rounded once; infinities among
  * them become NaN.  Weights, scales, workspace and out are 16-byte aligned.
- * H and I multiples of 16; T*H, I*H and the scales below 2 GiB each. */
+ * C <= 2048; H and I multiples of 16; T*H, I*H and the scales below 2 GiB each. */
 size_t pmx_rows8_layer_workspace_bytes(int64_t T, int32_t K, int64_t H, int64_t I, int32_t C);
 int pmx_rows8_layer(const void* hidden, const void* w, const int64_t* sel, const int64_t* M, const int64_t* src,
                     int32_t src_const, int32_t S, int32_t E, const void* gate_up, const void* gate_up_scales,

@@ -742,7 +742,7 @@ __global__ __launch_bounds__(CF::NTH, CF::NW * CF::BPC / 4) void rows8_grouped_g
     Values8<CF> c0, c1;
     auto convert = [&](auto jj, auto hh, const KTile& from, Values8<CF>& to) __attribute__((always_inline)) {
       constexpr int J = decltype(jj)::value, q = decltype(hh)::value / 2, s = decltype(hh)::value % 2;
-      const float scale = __uint_as_float(q < 3 ? from.words[J] << (23 - 8 * q) : from.words[J] >> 1);
+      const float scale = __uint_as_float(q < 3 ? from.words[J] << (q < 3 ? 23 - 8 * q : 0) : from.words[J] >> 1);
 #pragma unroll
       for (int pair = 0; pair < 4; pair += 2) {
         const uint32_t four = (uint32_t)from.v[q][J][2 * s + pair / 2];
@@ -834,7 +834,7 @@ __global__ __launch_bounds__(CF::NTH, CF::NW * CF::BPC / 4) void rows8_grouped_g
         __attribute__((always_inline)) {
       constexpr int J = order8<CF>(decltype(yy)::value / 4), pair = decltype(yy)::value % 4;
       constexpr int q = decltype(qq)::value, s = decltype(ss)::value;
-      const float scale = __uint_as_float(q < 3 ? w.v[J] << (23 - 8 * q) : w.v[J] >> 1);
+      const float scale = __uint_as_float(q < 3 ? w.v[J] << (q < 3 ? 23 - 8 * q : 0) : w.v[J] >> 1);
       const bf16x2_t v =
           __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((uint32_t)from.v[J][2 * s + pair / 2], scale, pair % 2 == 1);
       to.v[J][2 * pair] = v[0];

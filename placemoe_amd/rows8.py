@@ -345,7 +345,8 @@ def expert_layer_rows8(hidden: torch.Tensor, routing_weights: torch.Tensor, sele
     ws_bytes = _capi.load().pmx_rows8_layer_workspace_bytes(T, K, H, I, C)
     if ws_bytes == 0:
         raise ValueError(f"expert_layer_rows8: {T} tokens, {K} each, through {C} copies of {H} x {I} are not supported (sizes "
-                         "must be multiples of 16, and tokens, a copy's weights and each tensor's scales below 2 GiB)")
+                         "must be multiples of 16, copies at most 2048, and tokens, a copy's weights and each tensor's "
+                         "scales below 2 GiB)")
     dev = hidden.device
     with _on(dev):
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)

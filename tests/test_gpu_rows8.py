@@ -1115,3 +1115,27 @@ def test_nothing_waits_for_the_gpu(cuda):
         torch.cuda.set_sync_debug_mode("default")
     for k, (a, b) in enumerate(zip(got, want)):
         assert_exact(a, b, f"output {k}")
+
+
+def test_weights_through_the_host(cuda):
+    """What a server writes down and loads again answers with the same bits."""
+    C, H, I = 6, 96, 64
+    q = rows8.Experts8.quantize(_randn((C, 2 * I, H), 1, BF, 0.1).to(cuda), _randn((C, H, I), 2, BF, 0.1).to(cuda))
+    back = rows8.Experts8(q.gate_up.to("cpu").to(cuda), q.down.to("cpu").to(cuda))
+    args = (_randn((7, H), 3).to(cuda), torch.ones((7, 1), dtype=BF, device=cuda), torch.arange(7, device=cuda).reshape(7, 1) % C)
+    assert_exact(placemoe_amd.expert_layer_rows8(*args, back), placemoe_amd.expert_layer_rows8(*args, q), "out")
+
+
+def test_checkpointed_backward_twice(cuda):
+    """A retained graph's second backward reads the same checkpoint; the hidden states may have changed since."""
+    wl = make_workload("toy", device=cuda, tokens=40)
+    x, dout = wl.hidden.clone().requires_grad_(), _randn((wl.T, wl.H), 5).to(cuda)
+    fc1 = wl.fc1.clone().requires_grad_()
+    out = experts.expert_layer(x, wl.routing_weights, wl.selected, wl.fc2, fc1_1_2_weight=fc1, mapping=wl.mapping,
+                               sources=wl.sources, activation_checkpoint="e4m3")
+    first = torch.autograd.grad(out, (x, fc1), dout, retain_graph=True)
+    with torch.no_grad():
+        x.zero_()
+    second = torch.autograd.grad(out, (x, fc1), dout)
+    for a, b in zip(first, second):
+        assert_exact(a, b, "gradient")

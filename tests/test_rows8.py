@@ -91,6 +91,13 @@ def _rows(shape, fmt="e4m3", dtype=BF):
                        torch.full(rows8.scales_shape(shape), 127, dtype=torch.uint8), dtype)
 
 
+def test_size_and_moving():
+    q = _rows((3, 5, 600))
+    assert q.shape == (3, 5, 600) and q.nbytes == 3 * 5 * (600 + 2 * 16)
+    moved = q.to("cpu")
+    assert moved.dtype == BF and torch.equal(moved.scales, q.scales) and moved.codes.shape == q.codes.shape
+
+
 def test_wrappers_refuse_host_tensors():
     i32 = torch.zeros(3, dtype=torch.int32)
     for call in (
