@@ -144,7 +144,8 @@ __device__ __forceinline__ void setup(const Params8& P, const Place& at, Loads<C
   ld.bs = make_rsrc(P.bs + (int64_t)at.g * kgroups * P.N * kScaleBytes, (uint64_t)kgroups * P.N * kScaleBytes);
   ld.past = 0;
 #pragma unroll
-  for (int j = 0; j < CF::QA + CF::QB; ++j) {
+  for (int i = 0; i < CF::QA + CF::QB; ++i) {
+    const int j = i < CF::QB ? CF::QA + i : i - CF::QB;  // B's first: A's wait for their tokens
     const bool is_a = j < CF::QA;
     const int row = load_row(is_a ? j : j - CF::QA);
     const int c = (lane % 8) ^ kc_swz(row);

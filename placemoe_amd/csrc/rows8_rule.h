@@ -2,9 +2,10 @@
 //
 // The host knows the rows and the copies, not the counts.  Four tilings:
 //   32 x 64, two waves per block, three blocks per CU: where they are all there at
-//     once (one token);
-//   32 x 256, one block per CU, three stages: copies with few rows, where the
-//     call reads every copy's weights once and the matrix cores idle;
+//     once (one token), and for copies with few rows where their rounds are shorter
+//     (8 tokens, 8 each, through 160 copies of 1536 x 2048 and back: 75 -> 70 us);
+//   32 x 256, one block per CU, three stages: copies with few rows otherwise, where
+//     the call reads every copy's weights once and the matrix cores idle;
 //   128 x 128, two blocks per CU: one block's epilogue, tile switch and loads run
 //     behind the other's products;
 //   256 x 256, one block per CU: half the operand bytes per product.
@@ -47,7 +48,9 @@ inline int rows8_tiling(int kind, int64_t rows, int64_t copies, int64_t N, int64
   const auto div_up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
   const int64_t active = rows < copies ? rows : copies, nk = div_up(K, 128);
   if ((active > rows / 32 + active / 2 ? active : rows / 32 + active / 2) * div_up(N, 64) <= 3 * cus) return 0;
-  if (rows <= kRows8Few[kind] * active) return 32;
+  // a round of either takes as long as its weights: 3 x 64 rows of B per CU, or 256
+  if (rows <= kRows8Few[kind] * active)
+    return 3 * div_up(active * div_up(N, 64), 3 * cus) < 4 * div_up(active * div_up(N, 256), cus) ? 0 : 32;
   // a copy's last tile half full on average; an eighth of the copies past their first tile
   const auto cost = [&](int64_t tile, int64_t blocks, const double (&round)[2]) {
     const int64_t spread = active + active / 8, even = rows / tile + active / 2;

@@ -191,8 +191,8 @@ def test_gpu_cases_reach_every_tiling(tiling):
     alone = [("fc1", 1300, 1, 512, 112), ("fc1", 255, 1, 320, 272)]
     assert tiling(alone) == [0, 0]
     # one row of the same copy in calls of several tilings (test_a_row_depends_on_itself_and_its_copy_alone)
-    calls = [(20800, 1), (2600, 1), (1, 1), (400, 200), (2600, 150)]
-    assert tiling([("nt", *c, 264, 1104) for c in calls]) == [128, 0, 0, 32, 128]
+    calls = [(25600, 1), (2600, 1), (1, 1), (400, 200), (6400, 10)]
+    assert tiling([("nt", *c, 248, 1104) for c in calls]) == [128, 0, 0, 32, 128]
     # test_every_tiling_gives_the_same_bits
     for kind, N in (("nt", 4096), ("fc1", 4096)):
         assert tiling([(kind, rows, 1, N, 1024) for rows in (4096, 1000, 10)]) == [256, 128, 0]
