@@ -1137,3 +1137,16 @@ def test_checkpointed_backward_twice(cuda):
     second = torch.autograd.grad(out, (x, fc1), dout)
     for a, b in zip(first, second):
         assert_exact(a, b, "gradient")
+
+
+def test_a_tokens_output_does_not_depend_on_the_call(cuda):
+    """Alone, in threes, and among 3000 others, on whatever tiles: the same bits."""
+    C, H, I, T, K = 96, 1040, 528, 3000, 4
+    g = torch.Generator().manual_seed(3)
+    q = rows8.Experts8.quantize((torch.randn((C, 2 * I, H), device=cuda) * 0.05).to(BF), (torch.randn((C, H, I), device=cuda) * 0.05).to(BF))
+    x, w = _randn((T, H), 4).to(cuda), torch.rand((T, K), generator=g).to(BF).to(cuda)
+    sel = torch.stack([torch.randperm(C, generator=g)[:K] for _ in range(T)]).to(cuda)
+    want = placemoe_amd.expert_layer_rows8(x, w, sel, q)
+    for n, upto in ((1, 150), (3, 300), (40, 400), (500, T)):
+        got = [placemoe_amd.expert_layer_rows8(x[t:t + n], w[t:t + n], sel[t:t + n], q) for t in range(0, upto, n)]
+        assert_exact(torch.cat(got), want[:upto], f"calls of {n} tokens")
