@@ -539,9 +539,8 @@ int pmx_rows8_gemm_fc1_swiglu(const void* x, const void* x_scales, int64_t T, co
  * pmx_route; gate_up [C, 2I, H] and down [C, H, I] in e4m3 with their scales;
  * out bf16 [T, H]; counts int32 [C] (NULL: not wanted); status_host as in
  * pmx_route_reported; the workspace's first bytes hold the routing status word.
- * fc2's rows are kept to 16 bits beside a power of two per 32 columns (2^-15 of
- * the block's largest value), their sum is rounded once; infinities among
- * them become NaN.  Weights, scales, workspace and out are 16-byte aligned.
+ * fc2's rows are kept as the upper 24 bits of their fp32 values (2^-16 of each),
+ * their sum is rounded once.  Weights, scales, workspace and out are 16-byte aligned.
  * C <= 2048; H and I multiples of 16; T*H, I*H and the scales below 2 GiB each. */
 size_t pmx_rows8_layer_workspace_bytes(int64_t T, int32_t K, int64_t H, int64_t I, int32_t C);
 int pmx_rows8_layer(const void* hidden, const void* w, const int64_t* sel, const int64_t* M, const int64_t* src,

@@ -23,15 +23,14 @@
 
 // Between the sources of the layer, not part of the C ABI.
 __attribute__((visibility("hidden"))) int pmx_rows8_layer_check(int64_t T, int32_t K, int64_t H, int64_t I, int32_t C);
-// The grouped product as rows in blocks of 16-bit integers (below): y [M, N], y_scales [M, block16_row(N)].
-__attribute__((visibility("hidden"))) int pmx_rows8_group_gemm_nt_block16(const void* a, const void* a_scales, const void* b,
-                                                                          const void* b_scales, const int32_t* offsets,
-                                                                          int32_t G, int64_t M, int64_t N, int64_t K, void* y,
-                                                                          void* y_scales, pmx_stream_t stream);
+// The grouped product as rows of 24-bit floats (below): y_high [M, N] 16 bits, y_low [M, N] 8; N a multiple of 16.
+__attribute__((visibility("hidden"))) int pmx_rows8_group_gemm_nt_f24(const void* a, const void* a_scales, const void* b,
+                                                                      const void* b_scales, const int32_t* offsets, int32_t G,
+                                                                      int64_t M, int64_t N, int64_t K, void* y_high, void* y_low,
+                                                                      pmx_stream_t stream);
 // out[t] = sum of the rows pos[t, k] of y, in k order, rounded once to bf16 or fp16.
-__attribute__((visibility("hidden"))) int pmx_rows8_sum_block16(const void* y, const void* y_scales, const int32_t* pos,
-                                                                int64_t T, int32_t K, int64_t H, bool f16, void* out,
-                                                                pmx_stream_t stream);
+__attribute__((visibility("hidden"))) int pmx_rows8_sum_f24(const void* y_high, const void* y_low, const int32_t* pos, int64_t T,
+                                                            int32_t K, int64_t H, bool f16, void* out, pmx_stream_t stream);
 
 namespace {
 
@@ -69,23 +68,31 @@ __device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d) {
   }
 }
 
-// fc2's rows between the product and the sum over a token's experts: blocks of
-// 32 columns as 16-bit integers beside a power of two, the smallest at which
-// the largest finite magnitude is at most 32767 of it.  A value is off by at
-// most 2^-15 of its block's largest; bf16 rows were off by up to 2^-9 of
-// themselves, as much as the sum's own rounding: the layer was 1.4 times
-// further from its definition in 64 bits (0.0024, now 0.0017), for as many
-// bytes.  -32768 stands for what is not finite.
-constexpr int kBlock16 = 16;
-struct EltBlock16 {
-  static constexpr int kCode = kBlock16;
+// fc2's rows between the product and the sum over a token's experts: the upper
+// 24 bits of an fp32, rounded to nearest, in two planes: sign, exponent and 7
+// bits (a truncated bf16), and 8 bits more.  A value is off by at most 2^-16 of
+// itself, so that the rounding of the sum is the only one that counts.  bf16
+// rows are off by up to 2^-9 of themselves, as much as that rounding (the layer
+// was 0.0024 from its definition in 64 bits, with these rows 0.0017); 16-bit
+// integers beside a power of two per 32 columns are off by a share of the
+// block's largest value (columns beside one 1000 times as loud were 0.013
+// off, beside one 8000 times as loud 0.11).
+constexpr int kF24 = 24;
+struct EltF24 {
+  static constexpr int kCode = kF24;
 };
-// Bytes of a row's exponents (e + 127 each): whole words of four blocks.
-__host__ __device__ constexpr int64_t block16_row(int64_t N) { return (N + 127) / 128 * 4; }
-// 32767 = 1.99994 * 2^14.
-__device__ __forceinline__ uint32_t scale16_byte(uint32_t most) {
-  const int b = (int)(most >> 23) - 14 + ((most & 0x7fffffu) > 0x7ffe00u ? 1 : 0);
-  return (uint32_t)(b < 0 ? 0 : b);
+// Two values' upper halves, four values' next bytes; `u` holds fp32 bits to which half a step, 0x80, has been added.
+__device__ __forceinline__ uint32_t f24_high2(const uint32_t* u) { return __builtin_amdgcn_perm(u[1], u[0], 0x07060302u); }
+__device__ __forceinline__ uint32_t f24_low4(const uint32_t* u) {
+  const uint32_t lo = __builtin_amdgcn_perm(u[1], u[0], 0x0c0c0501u), hi = __builtin_amdgcn_perm(u[3], u[2], 0x05010c0cu);
+  return lo | hi;
+}
+// Eight values from both planes.
+__device__ __forceinline__ void f24_values8(const uint4 high, const uint2 low, float* f) {
+  const uint32_t h[4] = {high.x, high.y, high.z, high.w}, l[2] = {low.x, low.y};
+  constexpr uint32_t kPick[4] = {0x0504000cu, 0x0706010cu, 0x0504020cu, 0x0706030cu};
+#pragma unroll
+  for (int j = 0; j < 8; ++j) f[j] = __uint_as_float(__builtin_amdgcn_perm(h[j / 2], l[j / 4], kPick[j % 4]));
 }
 
 // Four codes -> the values that they stand for beside 2^0 (exact).

@@ -321,37 +321,33 @@ __global__ __launch_bounds__(256) void swiglu_bwd_rows8_kernel(const bf16_t* __r
 
 // out[t] = sum_k of row pos[t, k] of y, in k order, in fp32 with one rounding.
 // A block per token, 8 columns per thread; KC > 0: K == KC, whose loads go out
-// together.  Bound by HBM: 2 K + 2 bytes per value; 8192 tokens of 2048 from 8
-// rows each 53 us, 5.8 TB/s.
+// together.  Bound by HBM: 3 K + 2 bytes per value; 8192 tokens of 2048 from 8
+// rows each 75 us, 5.8 TB/s.
 template <class E, int KC>
-__global__ __launch_bounds__(256) void sum_block16_kernel(const uint16_t* __restrict__ y, const uint8_t* __restrict__ ys,
-                                                          const int32_t* __restrict__ pos, int64_t A, int32_t K, int64_t H,
-                                                          bf16_t* __restrict__ out) {
+__global__ __launch_bounds__(256) void sum_f24_kernel(const uint16_t* __restrict__ y_high, const uint8_t* __restrict__ y_low,
+                                                      const int32_t* __restrict__ pos, int64_t A, int32_t K, int64_t H,
+                                                      bf16_t* __restrict__ out) {
   constexpr int N = KC > 0 ? KC : 1;
-  const int64_t t = blockIdx.x, row = block16_row(H);
+  const int64_t t = blockIdx.x;
   const int32_t* p = pos + t * K;
   for (int64_t c = (int64_t)threadIdx.x * 8; c < H; c += (int64_t)blockDim.x * 8) {
     float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     for (int k0 = 0; k0 < K; k0 += N) {
-      uint4 v[N];
-      uint32_t e[N];
+      uint4 high[N];
+      uint2 low[N];
 #pragma unroll
       for (int k = 0; k < N; ++k) {
         const int64_t r = p[k0 + k];
         const bool in = r >= 0 && r < A;
-        v[k] = in ? ld_stream(y + r * H + c) : make_uint4(0, 0, 0, 0);
-        e[k] = in ? ys[r * row + c / 32] : 0;
+        high[k] = in ? ld_stream(y_high + r * H + c) : make_uint4(0, 0, 0, 0);
+        low[k] = in ? ld8(y_low + r * H + c) : make_uint2(0, 0);
       }
 #pragma unroll
       for (int k = 0; k < N; ++k) {
-        const float scale = scale_of(e[k]);
-        const uint32_t w[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
+        float f[8];
+        f24_values8(high[k], low[k], f);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int code = j % 2 ? (int)w[j / 2] >> 16 : (int)(w[j / 2] << 16) >> 16;
-          const float f = code == -32768 ? __uint_as_float(0x7fc00000u) : (float)code;
-          acc[j] = __builtin_fmaf(f, scale, acc[j]);
-        }
+        for (int j = 0; j < 8; ++j) acc[j] += f[j];
       }
     }
     *reinterpret_cast<uint4*>(out + t * H + c) = pack8e<E>(acc);
@@ -359,19 +355,19 @@ __global__ __launch_bounds__(256) void sum_block16_kernel(const uint16_t* __rest
 }
 
 template <class E>
-int sum_block16_t(const void* y, const void* ys, const int32_t* pos, int64_t T, int32_t K, int64_t H, void* out,
-                  pmx_stream_t stream) {
+int sum_f24_t(const void* y_high, const void* y_low, const int32_t* pos, int64_t T, int32_t K, int64_t H, void* out,
+              pmx_stream_t stream) {
   const int64_t waves = (H / 8 + 63) / 64;
   const unsigned threads = (unsigned)(waves < 4 ? waves : 4) * 64;
   const auto run = [&](auto kernel) {
-    kernel<<<(unsigned)T, threads, 0, stream>>>((const uint16_t*)y, (const uint8_t*)ys, pos, T * K, K, H, (bf16_t*)out);
+    kernel<<<(unsigned)T, threads, 0, stream>>>((const uint16_t*)y_high, (const uint8_t*)y_low, pos, T * K, K, H, (bf16_t*)out);
   };
   switch (K) {
-    case 2: run(sum_block16_kernel<E, 2>); break;
-    case 4: run(sum_block16_kernel<E, 4>); break;
-    case 6: run(sum_block16_kernel<E, 6>); break;
-    case 8: run(sum_block16_kernel<E, 8>); break;
-    default: run(sum_block16_kernel<E, 0>);
+    case 2: run(sum_f24_kernel<E, 2>); break;
+    case 4: run(sum_f24_kernel<E, 4>); break;
+    case 6: run(sum_f24_kernel<E, 6>); break;
+    case 8: run(sum_f24_kernel<E, 8>); break;
+    default: run(sum_f24_kernel<E, 0>);
   }
   PMX_LAUNCH_CHECK();
   return PMX_OK;
@@ -480,11 +476,11 @@ int swiglu_bwd_t(const void* d, const void* codes, const void* scales, const voi
 }  // namespace
 
 // The layer has checked T, K and H (a multiple of 16), and the pointers.
-int pmx_rows8_sum_block16(const void* y, const void* y_scales, const int32_t* pos, int64_t T, int32_t K, int64_t H, bool f16,
-                          void* out, pmx_stream_t stream) {
+int pmx_rows8_sum_f24(const void* y_high, const void* y_low, const int32_t* pos, int64_t T, int32_t K, int64_t H, bool f16,
+                      void* out, pmx_stream_t stream) {
   if (T == 0) return PMX_OK;
-  return f16 ? sum_block16_t<EltF16>(y, y_scales, pos, T, K, H, out, stream)
-             : sum_block16_t<EltBF16>(y, y_scales, pos, T, K, H, out, stream);
+  return f16 ? sum_f24_t<EltF16>(y_high, y_low, pos, T, K, H, out, stream)
+             : sum_f24_t<EltBF16>(y_high, y_low, pos, T, K, H, out, stream);
 }
 
 extern "C" {

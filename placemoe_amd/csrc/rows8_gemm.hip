@@ -60,7 +60,7 @@ struct Params8 {
   int64_t M, N, K;           // M rows over all groups; N: rows of a B[g] (FC1: 2 I)
   int64_t I;
   bf16_t* c;                 // NT: [M, N]
-  uint8_t* ys;               // NT in blocks of 16-bit integers: c's exponents
+  uint8_t* c_low;            // NT in 24 bits: the low bytes [M, N] of c
   uint8_t *q, *qs;           // FC1: act's codes [M, I] and exponents
   const bf16_t* row_w;       // FC1: [M], null: 1
 };
@@ -236,6 +236,12 @@ __device__ __forceinline__ void epilogue(const Params8& P, const Place& at, int 
   const int32_t col = at.ntile * CF::BN + wn * CF::FN * 32 + lane % (CF::FN * 4) * 8;
   [[maybe_unused]] const uint32_t voff =
       col < (int32_t)P.N ? (uint32_t)(lane / (CF::FN * 4)) * ldc + (uint32_t)col * 2 : kOOB;
+  // NT in 24 bits: the same for the plane of low bytes, 16 columns per lane.
+  const int32_t col_low = at.ntile * CF::BN + wn * CF::FN * 32 + lane % (CF::FN * 2) * 16;
+  [[maybe_unused]] const __amdgpu_buffer_rsrc_t out_low =
+      make_rsrc(P.c_low + (int64_t)at.row0 * P.N, (uint64_t)(at.row_end - at.row0) * P.N);
+  [[maybe_unused]] const uint32_t voff_low =
+      col_low < (int32_t)P.N ? (uint32_t)(lane / (CF::FN * 2)) * (uint32_t)P.N + (uint32_t)col_low : kOOB;
 #pragma unroll
   for (int m = 0; m < CF::FM; ++m) {
     const int64_t r = (int64_t)at.row0 + (wm * CF::FM + m) * 32 + (lane & 31);
@@ -247,37 +253,44 @@ __device__ __forceinline__ void epilogue(const Params8& P, const Place& at, int 
       // registers a store would have 32 bytes of each of 32 rows, four times
       // the requests to the L2.  Chunk c of row r at c ^ r (mod CPR), so that
       // neither side has bank conflicts.
+      // (24 bits: the low bytes likewise through the next pieces, rows of LCPR chunks.)
       constexpr int CPR = CF::FN * 4, RPP = 64 / CPR;  // chunks of a row, rows of a piece (and of a store)
-      static_assert(32 / RPP <= CF::QA + CF::QB, "enough pieces");
+      constexpr int LCPR = CF::FN * 2, LRPP = 64 / LCPR;
+      static_assert(32 / RPP + 32 / LRPP <= CF::QA + CF::QB, "enough pieces");
       const auto place = [&](int row, int c) {
         const int sw = CPR == 16 ? row & 15 : CPR == 8 ? kc_swz(row) : row >> 2 & 3;
         return stage + ((row / RPP) * CF::NW + wave) * 1024 + (row % RPP) * (CPR * 16) + ((c ^ sw) << 4);
       };
-      [[maybe_unused]] uint32_t exps = 0;
+      [[maybe_unused]] const auto place_low = [&](int row, int c) {
+        const int sw = LCPR == 8 ? kc_swz(row) : LCPR == 4 ? row >> 2 & 3 : row >> 3 & 1;
+        return stage + ((32 / RPP + row / LRPP) * CF::NW + wave) * 1024 + (row % LRPP) * (LCPR * 16) + ((c ^ sw) << 4);
+      };
 #pragma unroll
       for (int n = 0; n < CF::FN; ++n) {
         here(acc[m][n]);
         const f32x16_t& v = acc[m][n];
         uint32_t w[8];  // pairs of columns 8 (i/2) + 4 h + 2 (i%2)
-        if constexpr (E::kCode == kBlock16) {
-          float f[16];
-          bool finite;
+        if constexpr (E::kCode == kF24) {
+          uint32_t u[16], low[4];
+          float nan = 0.f;  // NaN if one of the values is (two values to an instruction)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) f[i] = v[i];
-          const float most = most_finite<16>(f, finite);
-          const uint32_t byte = scale16_byte(__float_as_uint(most));
-          const float inv = inv_scale(byte);
-          exps |= byte << (8 * n);
-          // beside 1.5 * 2^23 the low 16 bits of a sum are the integer, rounded to nearest even
-          const auto code = [&](float f) { return __float_as_uint(__builtin_fmaf(f, inv, 12582912.0f)); };
+          for (int i = 0; i < 16; i += 2) {
+            nan = __builtin_elementwise_maximum(__builtin_elementwise_maximum(nan, v[i]), v[i + 1]);
+            u[i] = __float_as_uint(v[i]) + 0x80u;  // infinities stay: the low byte is dropped
+            u[i + 1] = __float_as_uint(v[i + 1]) + 0x80u;
+          }
+          if (__ballot(nan != nan)) {  // a NaN of ones throughout would become a zero
 #pragma unroll
-          for (int i = 0; i < 8; ++i) w[i] = __builtin_amdgcn_perm(code(v[2 * i + 1]), code(v[2 * i]), 0x05040100u);
-          if (!finite) {
+            for (int i = 0; i < 16; ++i) u[i] = v[i] != v[i] ? 0x7fc00000u : u[i];
+          }
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              if (!(__builtin_fabsf(v[2 * i]) < __builtin_inff())) w[i] = (w[i] & 0xffff0000u) | 0x8000u;
-              if (!(__builtin_fabsf(v[2 * i + 1]) < __builtin_inff())) w[i] = (w[i] & 0xffffu) | 0x80000000u;
-            }
+          for (int i = 0; i < 8; ++i) w[i] = f24_high2(u + 2 * i);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) low[i] = f24_low4(u + 4 * i);
+#pragma unroll
+          for (int p = 0; p < 2; ++p) {
+            swap_halves(low[2 * p], low[2 * p + 1]);
+            *reinterpret_cast<uint2*>(place_low(lane & 31, n * 2 + p) + h * 8) = make_uint2(low[2 * p], low[2 * p + 1]);
           }
         } else {
 #pragma unroll
@@ -291,21 +304,20 @@ __device__ __forceinline__ void epilogue(const Params8& P, const Place& at, int 
               make_uint4(w[4 * p], w[4 * p + 1], w[4 * p + 2], w[4 * p + 3]);
         }
       }
-      if constexpr (E::kCode == kBlock16) {
-        const int64_t first = (int64_t)at.ntile * (CF::BN / 32) + wn * CF::FN;  // the wave's blocks, a multiple of FN
-        if (in && h == 0 && first * 32 < P.N) {
-          uint8_t* const e = P.ys + r * block16_row(P.N) + first;
-          if constexpr (CF::FN == 4) *reinterpret_cast<uint32_t*>(e) = exps;
-          else if constexpr (CF::FN == 2) *reinterpret_cast<uint16_t*>(e) = (uint16_t)exps;
-          else *e = (uint8_t)exps;
-        }
-      }
       wait_lds();
 #pragma unroll
       for (int q = 0; q < 32 / RPP; ++q) {
         const int row = q * RPP + lane / CPR;
         const u32x4_t v = *reinterpret_cast<const u32x4_t*>(place(row, lane % CPR));
         __builtin_amdgcn_raw_buffer_store_b128(v, out, voff + (uint32_t)((wm * CF::FM + m) * 32 + q * RPP) * ldc, 0, kStreaming);
+      }
+      if constexpr (E::kCode == kF24) {
+#pragma unroll
+        for (int q = 0; q < 32 / LRPP; ++q) {
+          const u32x4_t v = *reinterpret_cast<const u32x4_t*>(place_low(q * LRPP + lane / LCPR, lane % LCPR));
+          __builtin_amdgcn_raw_buffer_store_b128(v, out_low, voff_low + (uint32_t)((wm * CF::FM + m) * 32 + q * LRPP) * (uint32_t)P.N,
+                                                 0, kStreaming);
+        }
       }
       __builtin_amdgcn_sched_barrier(0);  // one tile's registers at a time
     } else {
@@ -976,16 +988,16 @@ bool any_tiles_fit(const Params8& P) {
 
 template <class E>
 int nt_t(const void* a, const void* as, const void* b, const void* bs, const int32_t* offsets, int32_t G, int64_t M, int64_t N,
-         int64_t K, void* c, void* ys, pmx_stream_t stream) {
+         int64_t K, void* c, void* c_low, pmx_stream_t stream) {
   Params8 P = {};
   P.a = (const uint8_t*)a, P.as = (const uint8_t*)as, P.a_rows = M;
   P.b = (const uint8_t*)b, P.bs = (const uint8_t*)bs;
-  P.offsets = offsets, P.G = G, P.M = M, P.N = N, P.K = K, P.c = (bf16_t*)c, P.ys = (uint8_t*)ys;
+  P.offsets = offsets, P.G = G, P.M = M, P.N = N, P.K = K, P.c = (bf16_t*)c, P.c_low = (uint8_t*)c_low;
   if (const int rc = check(P)) return rc;
-  if (N % 8) return PMX_ERR_SHAPE;
+  if (N % (E::kCode == kF24 ? 16 : 8)) return PMX_ERR_SHAPE;
   if (M == 0) return PMX_OK;
-  if (!a || !as || !b || !bs || !offsets || !c || (E::kCode == kBlock16 && !ys)) return PMX_ERR_ARG;
-  if (!aligned16(a) || !aligned16(as) || !aligned16(b) || !aligned16(bs) || !aligned16(c) || !aligned16(ys)) return PMX_ERR_SHAPE;
+  if (!a || !as || !b || !bs || !offsets || !c || (E::kCode == kF24 && !c_low)) return PMX_ERR_ARG;
+  if (!aligned16(a) || !aligned16(as) || !aligned16(b) || !aligned16(bs) || !aligned16(c) || !aligned16(c_low)) return PMX_ERR_SHAPE;
   return launch<E, NT8>(P, stream);
 }
 
@@ -1025,10 +1037,9 @@ int pmx_rows8_layer_check(int64_t T, int32_t K, int64_t H, int64_t I, int32_t C)
   return any_tiles_fit<NT8>(P) ? PMX_OK : PMX_ERR_SHAPE;
 }
 
-int pmx_rows8_group_gemm_nt_block16(const void* a, const void* a_scales, const void* b, const void* b_scales,
-                                    const int32_t* offsets, int32_t G, int64_t M, int64_t N, int64_t K, void* y, void* y_scales,
-                                    pmx_stream_t stream) {
-  return nt_t<EltBlock16>(a, a_scales, b, b_scales, offsets, G, M, N, K, y, y_scales, stream);
+int pmx_rows8_group_gemm_nt_f24(const void* a, const void* a_scales, const void* b, const void* b_scales, const int32_t* offsets,
+                                int32_t G, int64_t M, int64_t N, int64_t K, void* y_high, void* y_low, pmx_stream_t stream) {
+  return nt_t<EltF24>(a, a_scales, b, b_scales, offsets, G, M, N, K, y_high, y_low, stream);
 }
 
 extern "C" {

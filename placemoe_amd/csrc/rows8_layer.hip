@@ -11,7 +11,7 @@ namespace {
 // Where the workspace's parts begin (bytes, multiples of 256).  The routing's
 // own workspace is first: its status word is the workspace's.
 struct Parts {
-  size_t route, phys, pos, counts, offsets, row_token, row_w, x, xs, act, acts, y, ys, total;
+  size_t route, phys, pos, counts, offsets, row_token, row_w, x, xs, act, acts, y_high, y_low, total;
 };
 
 // false: more than a size_t holds (or no such layer).
@@ -37,8 +37,8 @@ bool parts_of(int64_t T, int32_t K, int64_t H, int64_t I, int32_t C, Parts& p) {
   p.xs = take(gh * t * kScaleBytes);
   p.act = take(A * i);
   p.acts = take(gi * A * kScaleBytes);
-  p.y = take(A * h * 2);
-  p.ys = take(A * block16_row(H));
+  p.y_high = take(A * h * 2);
+  p.y_low = take(A * h);
   p.total = at;
   return true;
 }
@@ -74,10 +74,10 @@ int layer_t(const void* hidden, const void* w, const int64_t* sel, const int64_t
                                                                           gate_up_scales, offsets, C, T * K, H, I, ws + p.row_w,
                                                                           ws + p.act, ws + p.acts, stream);
   if (rc != PMX_OK) return PMX_ERR_HIP;
-  rc = pmx_rows8_group_gemm_nt_block16(ws + p.act, ws + p.acts, down, down_scales, offsets, C, T * K, H, I, ws + p.y, ws + p.ys,
-                                       stream);
+  rc = pmx_rows8_group_gemm_nt_f24(ws + p.act, ws + p.acts, down, down_scales, offsets, C, T * K, H, I, ws + p.y_high,
+                                   ws + p.y_low, stream);
   if (rc != PMX_OK) return PMX_ERR_HIP;
-  rc = pmx_rows8_sum_block16(ws + p.y, ws + p.ys, pos, T, K, H, f16, out, stream);
+  rc = pmx_rows8_sum_f24(ws + p.y_high, ws + p.y_low, pos, T, K, H, f16, out, stream);
   return rc != PMX_OK ? PMX_ERR_HIP : PMX_OK;
 }
 

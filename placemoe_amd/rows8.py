@@ -305,8 +305,8 @@ def expert_layer_rows8(hidden: torch.Tensor, routing_weights: torch.Tensor, sele
     ``Experts8.quantize``.  Tokens are quantised once, fc1 reads each where it
     lies for every copy that it is routed to, and the activations, weighted by
     the router, leave its epilogue in 8 bits for fc2 (router weights on the fc2
-    input, as in the non-EP arithmetic); a token's rows, held to 2^-15 of the largest
-    value of 32 columns, are then summed and rounded once.  H and I multiples of 16.
+    input, as in the non-EP arithmetic); a token's rows, held in 24 bits (each value to
+    2^-16 of itself), are then summed and rounded once.  H and I multiples of 16.
     """
     from . import experts  # experts itself uses this module's checkpoints
 

@@ -13,7 +13,7 @@ import torch
 import placemoe_amd
 from oracle import rows8_oracle as O
 from placemoe_amd import _capi, experts, rows8
-from tests import test_gpu_rows8
+from tests import test_gpu_rows8, test_gpu_rows8_layer
 
 ROOT = Path(__file__).resolve().parents[1]
 
@@ -198,6 +198,12 @@ def test_gpu_cases_reach_every_tiling(tiling):
         assert tiling([(kind, rows, 1, N, 1024) for rows in (4096, 1000, 10)]) == [256, 128, 0]
     few = [(k, sum(c), len(c), N, K) for k in ("nt", "fc1") for c, N, K in test_gpu_rows8.FEW.values()]
     assert tiling(few) == [0, 32] * 2
+
+
+def test_layer_cases_reach_every_tiling(tiling):
+    layers = test_gpu_rows8_layer.LAYERS.values()
+    assert tiling([("nt", T * K, C, H, I) for T, K, C, H, I in layers]) == [0, 32, 128, 256, 256, 256]
+    assert set(tiling([("fc1", T * K, C, 2 * I, H) for T, K, C, H, I in layers])) == {0, 32, 128, 256}
 
 
 def test_layer_workspace(tiling):
