@@ -175,6 +175,28 @@ def test_tiling_rule_takes_the_faster_one(tiling):
         assert us[height] <= 1.05 * min(us.values()), (call, height)
 
 
+# us on 32 x 64, 32 x 256, 128 x 128 and 256 x 256 tiles (log-normal counts with sigma 0.4)
+FOUR_TILINGS = {
+    ("nt", 1, 16, 7168, 2048): (10.8, 14.0, 14.9, 27.7), ("fc1", 1, 16, 7168, 2048): (14.4, 17.1, 20.8, 47.2),
+    ("nt", 256, 8, 1536, 2048): (11.9, 13.9, 15.2, 27.9), ("fc1", 256, 8, 1536, 2048): (17.3, 17.9, 21.6, 48.3),
+    ("nt", 640, 160, 1536, 2048): (89.2, 89.9, 97.1, 110.9), ("fc1", 640, 160, 1536, 2048): (92.4, 91.7, 116.5, 187.2),
+    ("nt", 2560, 160, 1536, 2048): (99.9, 94.3, 99.8, 112.8), ("fc1", 2560, 160, 1536, 2048): (101.8, 94.2, 119.7, 189.7),
+    ("nt", 5120, 160, 1536, 2048): (114.0, 106.4, 102.3, 114.6), ("fc1", 5120, 160, 1536, 2048): (123.9, 110.6, 124.1, 192.6),
+    ("nt", 5120, 160, 2048, 768): (56.0, 55.3, 49.5, 67.4), ("fc1", 5120, 160, 2048, 768): (74.1, 64.3, 68.1, 112.6),
+    ("nt", 10240, 160, 1536, 2048): (152.1, 146.3, 108.8, 117.2), ("fc1", 10240, 160, 1536, 2048): (178.4, 156.4, 133.9, 193.0),
+    ("nt", 64, 16, 4096, 7168): (89.2, 78.2, 81.1, 92.3), ("fc1", 64, 16, 4096, 7168): (94.2, 79.6, 94.3, 150.6),
+    ("nt", 256, 16, 4096, 7168): (91.8, 84.0, 85.6, 95.0), ("fc1", 256, 16, 4096, 7168): (96.2, 84.9, 96.2, 156.1),
+    ("nt", 160, 160, 1536, 2048): (46.6, 54.5, 59.8, 79.9), ("fc1", 80, 160, 2048, 768): (26.4, 22.6, 30.2, 48.7),
+}
+
+
+def test_tiling_rule_on_four_tilings(tiling):
+    """Each tiling at its own time: none of these calls loses more than 5% to the best one."""
+    for call, height in zip(FOUR_TILINGS, tiling(list(FOUR_TILINGS))):
+        us = dict(zip((0, 32, 128, 256), FOUR_TILINGS[call]))
+        assert us[height] <= 1.05 * min(us.values()), (call, height, us)
+
+
 def test_gpu_cases_reach_every_tiling(tiling):
     def heights(kind, cases):
         return {n: h for n, h in zip(cases, tiling([(kind, sum(c), len(c), N, K) for c, N, K in cases.values()]))}
