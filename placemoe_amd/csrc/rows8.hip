@@ -1,8 +1,9 @@
 // Rows in 8 bits (rows8.h): writing them, reading them back (in order or into
 // the rows of the expert copies), and the SwiGLU backward from 8-bit gate and
 // up rows.  An activation checkpoint of the expert layer is such a pair: its
-// hidden states and its gate/up rows, a quarter to a third of what the
-// layer keeps otherwise; the SwiGLU activations are recomputed.
+// hidden states and its gate/up rows, 2I + H / K bytes per row of the copies
+// (K experts per token) where the layer otherwise keeps 6I + 4H, or 6I + 2H with
+// the router weights on fc2's input; the SwiGLU activations are recomputed.
 //
 // All are bound by HBM: 3 bytes per value written, 1 + 2K per value read back
 // into K rows, 10 per activation of the SwiGLU backward, each with 1/32 of a

@@ -27,9 +27,10 @@ arithmetic and differ in bf16 rounding.
 ``activation_checkpoint="e4m3"`` (or ``"int8"``) leaves the output as it is, bit
 for bit, and keeps for the backward the hidden states [T, H] and the gate/up
 rows [A, 2I] in 8 bits instead of the permuted rows [A, H], the gate/up rows,
-the activations [A, I] and the expert outputs [A, H] in 16: H + 2I instead of
-4H + 6I bytes per row of a top-1 layer, less still with more experts per
-token.  Its backward takes the weights' gradient on the fc2 input side in both
+the activations [A, I] and, in EP arithmetic, the expert outputs [A, H] in 16:
+H + 2I instead of 4H + 6I bytes (non-EP: 2H + 6I) per row of a top-1 layer, less
+still with more experts per token.  (The hidden states are for fc1's weight
+gradient: where fc1 is frozen they are not kept.)  Its backward takes the weights' gradient on the fc2 input side in both
 arithmetics, where it needs no expert outputs.
 """
 
@@ -233,8 +234,11 @@ class _ExpertLayerBase(torch.autograd.Function):
             _, out = kernels.group_gemm_nt_combine_top1(act, fc2_weight, r.offsets, row_src, row_w)
         else:
             out = kernels.combine_fwd(kernels.group_gemm_nt(act, fc2_weight, r.offsets), r.pos, routing_weights)
-        x8, gu8 = rows8.quantize_rows(hidden, fmt), rows8.quantize_rows(gu, fmt)
-        ctx.save_for_backward(x8.codes, x8.scales, gu8.codes, gu8.scales, r.pos, r.offsets, routing_weights, w_gate,
+        # the hidden states are for fc1's weight gradient alone
+        x8 = rows8.quantize_rows(hidden, fmt) if ctx.fc1_needs_grad else None
+        x_codes, x_scales = (x8.codes, x8.scales) if x8 is not None else (None, None)
+        gu8 = rows8.quantize_rows(gu, fmt)
+        ctx.save_for_backward(x_codes, x_scales, gu8.codes, gu8.scales, r.pos, r.offsets, routing_weights, w_gate,
                               w_up, fc2_weight, row_src, row_w)
         return out
 
@@ -435,9 +439,9 @@ def expert_layer(
     ``recorder(counts)`` receives the int32 per-copy token counts (on the device).
     ``weighted_input``: apply the router weights to the fc2 input (the
     reference's non-EP arithmetic) instead of in the combine (EP).
-    ``activation_checkpoint``: keep for the backward only the hidden states and
-    the gate/up rows, in 8 bits (``"e4m3"`` or ``"int8"``); None keeps them, the
-    activations and the expert outputs in 16.
+    ``activation_checkpoint``: keep for the backward only the gate/up rows and,
+    unless fc1 is frozen, the hidden states, in 8 bits (``"e4m3"`` or ``"int8"``);
+    None keeps them, the activations and (EP arithmetic) the expert outputs in 16.
     """
     if activation_checkpoint is not None and activation_checkpoint not in rows8.FORMATS:
         raise ValueError(f"activation checkpoint must be None or one of {sorted(rows8.FORMATS)}, "
