@@ -221,7 +221,7 @@ __device__ __forceinline__ float most_finite(const float* f, bool& finite) {
 // first operand): lane l has row l%32, columns 8*(i/4) + 4*(l/32) + i%4.
 template <class E, int KIND, class CF>
 __device__ __forceinline__ void epilogue(const Params8& P, const Place& at, int wm, int wn, int wave, int lane,
-                                         [[maybe_unused]] char* stage, [[maybe_unused]] char* shared,
+                                         [[maybe_unused]] char* stage, [[maybe_unused]] float* shared,
                                          f32x16_t (&acc)[CF::FM][CF::FN]) {
   // Each accumulator leaves the accumulation registers where it is used: read
   // right behind their last MFMAs, they would need as many vector registers.
@@ -347,11 +347,11 @@ __device__ __forceinline__ void epilogue(const Params8& P, const Place& at, int 
 #pragma unroll
         for (int i = 0; i < 8; ++i) f[i] = weigh(acc[m][0][i], acc[m][0][i + 8]);
         const float most = most_finite<8>(f, finite);
-        float* const of_waves = reinterpret_cast<float*>(shared);  // [2][32]; a K-tile's barrier before it is used again
-        if (h == 0) of_waves[wn * 32 + lane] = most;
+        // `shared`: [2][32]; a K-tile's barrier before it is used again
+        if (h == 0) shared[wn * 32 + lane] = most;
         wait_lds();
         block_barrier();
-        const uint32_t byte = scale_byte<kFmtE4M3>(__float_as_uint(fmaxf(most, of_waves[(1 - wn) * 32 + (lane & 31)])));
+        const uint32_t byte = scale_byte<kFmtE4M3>(__float_as_uint(fmaxf(most, shared[(1 - wn) * 32 + (lane & 31)])));
         const float inv = inv_scale(byte);
         uint32_t c0 = code(f, inv), c1 = code(f + 4, inv);
         swap_halves(c0, c1);  // columns 8 h .. + 7 of the wave's 16
@@ -408,9 +408,9 @@ __global__ __launch_bounds__(CF::NTH, CF::NW * CF::BPC / 4) void rows8_grouped_g
   __shared__ __attribute__((aligned(1024))) char lds[CF::LDS];
   __shared__ int32_t tend[kMaxGroups];  // m-tiles of the groups up to and with g
   char* const slots = lds + CF::NST * CF::STAGE;
-  char* shared = nullptr;  // what FC1's two waves of one column tile each exchange
+  float* shared = nullptr;  // what FC1's two waves of one column tile each exchange
   if constexpr (KIND == FC18 && CF::FN == 1) {
-    __shared__ char exchange[256];
+    __shared__ float exchange[64];
     shared = exchange;
   }
   const int t = threadIdx.x;
