@@ -476,7 +476,9 @@ int pmx_ep_combine_aggregate_i64(const void* Y, const int64_t* pos, const void* 
  *   codes:  [.., R, N] one byte each, row-major.
  *   scales: [.., B, R, 16] bytes, B = ceil(N / 512): byte [b, r, j] = e + 127
  *           of row r's columns 512 b + 32 j .. + 31; 127 past the last column.
- * The row functions take any N and any alignment; the two products e4m3 only.
+ * The row functions take any N and any alignment, and as many rows as a grid of
+ * 2^32 threads covers (SwiGLU backward: below 2^26), else PMX_ERR_SHAPE; the two
+ * products e4m3 only.
  * No counterpart in the reference, whose expert layer is 16-bit throughout. */
 #define PMX_ROWS8_E4M3 0
 #define PMX_ROWS8_INT8 1

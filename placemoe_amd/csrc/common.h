@@ -203,6 +203,10 @@ __attribute__((visibility("hidden"))) int pmx_route_scan_launch(int32_t* table, 
                                                                 const int32_t* flags, int32_t* counts,
                                                                 int32_t* offsets, int32_t* status, hipStream_t stream);
 
+// Whether one launch holds the grid: of 2^32 threads or more, HIP runs what is
+// left modulo 2^32 and reports success (2^24 + 5 blocks of 256: five ran).
+static inline bool grid_fits(int64_t blocks, int64_t threads) { return blocks <= (int64_t)UINT32_MAX / threads; }
+
 #define PMX_LAUNCH_CHECK()                         \
   do {                                             \
     hipError_t _e = hipGetLastError();             \

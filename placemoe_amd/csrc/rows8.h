@@ -21,6 +21,12 @@
 
 #include "common.h"
 
+// Threads of a block of the sum over a token's rows; a block per token.
+inline unsigned rows8_sum_threads(int64_t H) {
+  const int64_t waves = (H / 8 + 63) / 64;
+  return (unsigned)(waves < 4 ? waves : 4) * 64;
+}
+
 // Between the sources of the layer, not part of the C ABI.
 __attribute__((visibility("hidden"))) int pmx_rows8_layer_check(int64_t T, int32_t K, int64_t H, int64_t I, int32_t C);
 // The grouped product as rows of 24-bit floats (below): y_high [M, N] 16 bits, y_low [M, N] 8; N a multiple of 16.

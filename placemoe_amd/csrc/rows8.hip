@@ -358,8 +358,7 @@ __global__ __launch_bounds__(256) void sum_f24_kernel(const uint16_t* __restrict
 template <class E>
 int sum_f24_t(const void* y_high, const void* y_low, const int32_t* pos, int64_t T, int32_t K, int64_t H, void* out,
               pmx_stream_t stream) {
-  const int64_t waves = (H / 8 + 63) / 64;
-  const unsigned threads = (unsigned)(waves < 4 ? waves : 4) * 64;
+  const unsigned threads = rows8_sum_threads(H);
   const auto run = [&](auto kernel) {
     kernel<<<(unsigned)T, threads, 0, stream>>>((const uint16_t*)y_high, (const uint8_t*)y_low, pos, T * K, K, H, (bf16_t*)out);
   };
@@ -395,7 +394,7 @@ int quantize_t(const void* x, int64_t ldx, int64_t gsx, int64_t G, int64_t R, in
   const auto blocks = [&](int64_t rows) { return G * ((R + rows - 1) / rows) * B; };
   const int per = blocks(32) >= kManyBlocks ? 8 : 2;
   const int64_t grid = blocks(4 * per), tiles = (R + 4 * per - 1) / (4 * per);
-  if (grid > INT32_MAX) return PMX_ERR_SHAPE;
+  if (!grid_fits(grid, 256)) return PMX_ERR_SHAPE;
   const auto run = [&](auto kernel) {
     kernel<<<(unsigned)grid, 256, 0, stream>>>((const bf16_t*)x, ldx, gsx, R, N, tiles, map, (uint8_t*)codes, (uint8_t*)scales);
   };
@@ -433,7 +432,7 @@ int dequantize_t(const void* codes, const void* scales, const int32_t* pos, int6
   if (product(R, N) < 0 || product(R, B) < 0) return PMX_ERR_SHAPE;
   const auto blocks = [&](int64_t rows) { return (R + rows - 1) / rows * B; };
   const int per = blocks(16) >= kManyBlocks ? 4 : 1;
-  if (blocks(4 * per) > INT32_MAX) return PMX_ERR_SHAPE;
+  if (!grid_fits(blocks(4 * per), 256)) return PMX_ERR_SHAPE;
   const auto run = [&](auto kernel) {
     kernel<<<(unsigned)blocks(4 * per), 256, 0, stream>>>((const uint8_t*)codes, (const uint8_t*)scales, pos, R, K, N,
                                                           (bf16_t*)out);
@@ -456,7 +455,7 @@ int swiglu_bwd_t(const void* d, const void* codes, const void* scales, const voi
   if ((dw == nullptr) != (row_src == nullptr)) return PMX_ERR_ARG;
   if (R == 0 || I == 0) return PMX_OK;
   if (!d || !codes || !scales || !dG1 || !act_w) return PMX_ERR_ARG;
-  if (product(R, I) < 0 || product(R, 2 * I) < 0 || (R + 3) / 4 > INT32_MAX) return PMX_ERR_SHAPE;
+  if (product(R, I) < 0 || product(R, 2 * I) < 0 || !grid_fits((R + 3) / 4, 256)) return PMX_ERR_SHAPE;
   const auto run = [&](auto kernel) {
     kernel<<<(unsigned)((R + 3) / 4), 256, 0, stream>>>((const bf16_t*)d, (const uint8_t*)codes, (const uint8_t*)scales,
                                                         (const bf16_t*)row_w, row_src, R, I, A, (bf16_t*)dG1,
@@ -476,7 +475,7 @@ int swiglu_bwd_t(const void* d, const void* codes, const void* scales, const voi
 
 }  // namespace
 
-// The layer has checked T, K and H (a multiple of 16), and the pointers.
+// The layer has checked T (with its grid), K and H (a multiple of 16), and the pointers.
 int pmx_rows8_sum_f24(const void* y_high, const void* y_low, const int32_t* pos, int64_t T, int32_t K, int64_t H, bool f16,
                       void* out, pmx_stream_t stream) {
   if (T == 0) return PMX_OK;

@@ -1022,10 +1022,10 @@ int fc1_t(const void* x, const void* xs, int64_t T, const int32_t* row_token, co
 
 }  // namespace
 
-// Whether a layer of T tokens, K copies each, fits both products (rows8_layer.hip asks before it launches anything).
+// Whether a layer of T tokens, K copies each, fits both products and the sum (rows8_layer.hip asks before it launches anything).
 int pmx_rows8_layer_check(int64_t T, int32_t K, int64_t H, int64_t I, int32_t C) {
   if (T < 0 || K <= 0 || H <= 0 || I <= 0 || C <= 0) return PMX_ERR_ARG;
-  if (H % 16 || I % 16 || I > INT32_MAX / 2 || T > INT32_MAX / K) return PMX_ERR_SHAPE;
+  if (H % 16 || I % 16 || I > INT32_MAX / 2 || T > INT32_MAX / K || !grid_fits(T, rows8_sum_threads(H))) return PMX_ERR_SHAPE;
   static const int32_t some_map = 0;
   Params8 P = {};
   P.G = C, P.M = T * K;

@@ -86,6 +86,19 @@ def test_c_abi_refusals(suffix):
     assert fc1(P, P, 8, P, P, P, P, 4, 16, 32, 0, P, P, P, None) == ARG
 
 
+def test_grids_past_one_launch_are_refused():
+    """Of 2^32 threads or more a launch runs what is left modulo 2^32, and reports success."""
+    lib = _capi.load()
+    rows = 1 << 24  # blocks of 256 threads
+    assert lib.pmx_rows8_quantize(P, 1, 0, 1, 32 * rows, 1, 0, P, P, None) == SHAPE
+    assert lib.pmx_rows8_quantize(P, 8, 0, 32 * rows // 4, 4, 8, 0, P, P, None) == SHAPE  # a block per group
+    assert lib.pmx_rows8_dequantize(P, P, None, 16 * rows, 0, 8, 0, P, None) == SHAPE
+    assert lib.pmx_rows8_dequantize(P, P, P, 16 * rows, 4, 8, 0, P, None) == SHAPE
+    assert lib.pmx_rows8_swiglu_bwd(P, P, P, P, P, 4 * rows, 8, 4, 0, P, P, P, None) == SHAPE
+    ws = lib.pmx_rows8_layer_workspace_bytes  # the sum over a token's rows: 64 threads per token
+    assert ws(4 * rows - 1, 1, 16, 16, 1) > 0 and ws(4 * rows, 1, 16, 16, 1) == 0
+
+
 def _rows(shape, fmt="e4m3", dtype=BF):
     return rows8.Rows8(torch.zeros(shape, dtype=rows8.FORMATS[fmt]),
                        torch.full(rows8.scales_shape(shape), 127, dtype=torch.uint8), dtype)
