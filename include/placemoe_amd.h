@@ -15,7 +15,8 @@
  *    see "fp16 tensors" at the end).  Index tensors are int32 unless stated.
  *  - Positions, row offsets and the row kernels' token rows are 32-bit:
  *    assignments T*K, GEMM row counts and segment-sum rows above 2^31-1
- *    return PMX_ERR_SHAPE before anything is launched.
+ *    return PMX_ERR_SHAPE before anything is launched, and so do row calls whose
+ *    grid would have 2^32 threads or more (at least 2^23 token rows).
  *  - Each declaration names the reference (pia7a/PlaceMoE) interface it
  *    replaces, as `file:line`.
  */

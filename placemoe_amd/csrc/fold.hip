@@ -83,7 +83,7 @@ int replica_fold_t(void* grads, const int32_t* copy_offsets, const int32_t* copy
                    ((reinterpret_cast<uintptr_t>(out) & 15u) == 0);
   const int64_t per_block = vec ? 256 * 8 : 256;
   const int64_t gx = (P + per_block - 1) / per_block;
-  if (gx > 0x7fffffff) return PMX_ERR_SHAPE;
+  if (!grid_fits(gx, 256)) return PMX_ERR_SHAPE;
   dim3 grid((unsigned)gx, (unsigned)E);
   if (vec) {
     replica_fold_kernel<El, true><<<grid, 256, 0, stream>>>(static_cast<bf16_t*>(grads), copy_offsets, copy_slots,

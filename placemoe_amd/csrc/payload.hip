@@ -448,7 +448,7 @@ int ep_dispatch_payload_t(const I* phys, const void* hidden, const void* weights
   if (!assign_counts || !assign_offsets || !unique_counts || !unique_offsets || !status || !workspace)
     return PMX_ERR_ARG;
   const int64_t A = T * K;
-  if (A > (int64_t)INT32_MAX) return PMX_ERR_SHAPE;
+  if (A > (int64_t)INT32_MAX || (H > 0 && !grid_fits((T + 3) / 4, 256))) return PMX_ERR_SHAPE;
   if (A > 0 && (!phys || !weights || !unique_tokens || !send_meta || !send_weights || !target_rank))
     return PMX_ERR_ARG;
   if (A > 0 && H > 0 && (!hidden || !send_hidden || !aligned16(hidden) || !aligned16(send_hidden)))
@@ -538,7 +538,7 @@ int ep_combine_aggregate_t(const void* Y, const I* pos, const void* w, const I* 
                              void* workspace, size_t workspace_bytes, pmx_stream_t stream) {
   if (N < 0 || H < 0 || R <= 0) return PMX_ERR_ARG;
   if (H % 8) return PMX_ERR_SHAPE;
-  if (N > (int64_t)INT32_MAX) return PMX_ERR_SHAPE;
+  if (N > (int64_t)INT32_MAX || (H > 0 && !grid_fits((N + 3) / 4, 256))) return PMX_ERR_SHAPE;
   if (!run_offsets || !rank_runs || !num_runs || !status || !workspace) return PMX_ERR_ARG;
   if (N > 0 && (!pos || !w || !src_rank || !src_token)) return PMX_ERR_ARG;
   if (N > 0 && H > 0 && (!Y || !out || !aligned16(Y) || !aligned16(out))) return PMX_ERR_ARG;

@@ -135,7 +135,7 @@ int launch_items(void* grads, int32_t dtype, int64_t P, int32_t C, int32_t n_ite
     return PMX_ERR_ARG;
   const int V = dtype == PMX_DTYPE_F32 ? 4 : 8;
   const int64_t gx = (P + 256 * V - 1) / (256 * V);
-  if (gx > 0x7fffffff) return PMX_ERR_SHAPE;
+  if (!grid_fits(gx, 256)) return PMX_ERR_SHAPE;
   const dim3 grid((unsigned)gx, (unsigned)n_items);
   if (dtype == PMX_DTYPE_BF16) {
     replica_items_kernel<EltBF16><<<grid, 256, 0, stream>>>(static_cast<bf16_t*>(grads), P, C, slot_offsets, slots,

@@ -976,6 +976,7 @@ int pmx_moe_scatter_src(const void* X, const int32_t* pos, const void* w, int64_
   if (T == 0 || (H == 0 && row_src == nullptr)) return PMX_OK;
   if (!X || !pos || !Xp) return PMX_ERR_ARG;
   const unsigned th = row_threads(H);
+  if (!grid_fits(T, th)) return PMX_ERR_SHAPE;
   const bf16_t* wb = static_cast<const bf16_t*>(w);
   bf16_t* rw = static_cast<bf16_t*>(row_w);
   if (H % 8 == 0 && aligned16(X) && aligned16(Xp)) {
@@ -1017,6 +1018,7 @@ int moe_gather_t(const void* Y, const int32_t* pos, int64_t T, int32_t K, int64_
   if (T == 0 || H == 0) return PMX_OK;
   if (!Y || !pos || !out) return PMX_ERR_ARG;
   const unsigned th = row_threads(H);
+  if (!grid_fits(T, th)) return PMX_ERR_SHAPE;
   if (H % 8 == 0 && aligned16(Y) && aligned16(out)) {
 #define PMX_GATHER(KC)                                                                                  \
   gather_rows_kernel<E, true, false, KC><<<(unsigned)T, th, 0, stream>>>((const bf16_t*)Y, pos, nullptr, K, H, \
@@ -1039,6 +1041,7 @@ int combine_fwd_t(const void* Y, const int32_t* pos, const void* w, int64_t T, i
   if (T == 0 || H == 0) return PMX_OK;
   if (!Y || !pos || !w || !out) return PMX_ERR_ARG;
   const unsigned th = row_threads(H);
+  if (!grid_fits(T, th)) return PMX_ERR_SHAPE;
   if (H % 8 == 0 && aligned16(Y) && aligned16(out)) {
 #define PMX_COMBINE(KC)                                                                               \
   gather_rows_kernel<E, true, true, KC><<<(unsigned)T, th, 0, stream>>>((const bf16_t*)Y, pos, (const bf16_t*)w, \
@@ -1062,7 +1065,7 @@ int combine_bwd_top1_rows_t(const void* dout, const void* Y, const int32_t* row_
   if (!dout || !Y || !row_token || !w || !dY || !dw) return PMX_ERR_ARG;
   if (H % 8 || !aligned16(dout) || !aligned16(Y) || !aligned16(dY)) return PMX_ERR_SHAPE;
   const int64_t blocks = (T + 3) / 4;  // a wave per row, 4 rows per block
-  if (blocks > 0x7fffffff) return PMX_ERR_SHAPE;
+  if (!grid_fits(blocks, 256)) return PMX_ERR_SHAPE;
   combine_bwd_top1_rows_kernel<E, 14><<<(unsigned)blocks, 256, 0, stream>>>(
       (const bf16_t*)dout, (const bf16_t*)Y, row_token, (const bf16_t*)w, T, H, (bf16_t*)dY, (bf16_t*)dw);
   PMX_LAUNCH_CHECK();
@@ -1081,12 +1084,13 @@ int combine_bwd_t(const void* dout, const void* Y, const int32_t* pos, const voi
   if (K == 1 && H % 8 == 0 && H >= 2048 && aligned16(dout) && aligned16(Y) && aligned16(dY)) {
     // top-1 rows of at least 2048 columns: a wave per token (4 tokens per block)
     const int64_t blocks = (T + 3) / 4;
-    if (blocks > 0x7fffffff) return PMX_ERR_SHAPE;
+    if (!grid_fits(blocks, 256)) return PMX_ERR_SHAPE;
     combine_bwd_top1_kernel<E, 14><<<(unsigned)blocks, 256, 0, stream>>>(
         (const bf16_t*)dout, (const bf16_t*)Y, pos, (const bf16_t*)w, T, H, (bf16_t*)dY, (bf16_t*)dw);
     PMX_LAUNCH_CHECK();
     return PMX_OK;
   }
+  if (!grid_fits(T, th)) return PMX_ERR_SHAPE;
   if (H % 8 == 0 && aligned16(dout) && aligned16(Y) && aligned16(dY)) {
 #define PMX_COMBINE_BWD(KC)                                                                            \
   combine_bwd_kernel<E, true, KC><<<(unsigned)T, th, 0, stream>>>((const bf16_t*)dout, (const bf16_t*)Y, pos, \

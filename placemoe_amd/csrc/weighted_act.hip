@@ -155,7 +155,7 @@ int swiglu_bwd_weighted_t(const void* d_act_w, const void* gu, const void* act, 
   if ((dw == nullptr) != (row_src == nullptr)) return PMX_ERR_ARG;
   if (R == 0) return PMX_OK;
   if (!row_w || (I > 0 && (!d_act_w || !gu || (ACT && !act) || !dG1))) return PMX_ERR_ARG;
-  if ((R + 3) / 4 > (int64_t)INT32_MAX || (I > 0 && R > INT64_MAX / (2 * I))) return PMX_ERR_SHAPE;
+  if (!grid_fits((R + 3) / 4, 256) || (I > 0 && R > INT64_MAX / (2 * I))) return PMX_ERR_SHAPE;
   const bool vec = I % 8 == 0 && aligned16(d_act_w) && aligned16(gu) && aligned16(act) && aligned16(dG1);
   const unsigned grid = (unsigned)((R + 3) / 4);
   if (vec)

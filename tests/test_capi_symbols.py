@@ -88,6 +88,27 @@ def test_argument_errors_are_codes_not_crashes():
         _capi.call("pmx_group_gemm_nt", None, None, None, 4, 8, 12, 8, None, None)
 
 
+@pytest.mark.parametrize("suffix", ["", "_f16"])
+def test_grids_past_one_launch_are_refused(suffix):
+    """Of 2^32 threads or more a launch runs what is left modulo 2^32 and reports success: the row
+    functions refuse such calls on the host."""
+    lib = _capi.load()
+    f = lambda name: getattr(lib, name + suffix, None) or getattr(lib, name)  # noqa: E731
+    d, H, T = ctypes.c_void_p(16), 4096, 1 << 23  # a block of 512 threads per token
+    W = 1 << 26  # a wave per token, four to a block
+    assert f("pmx_moe_scatter")(d, d, T, 2, H, d, None) == _capi.PMX_ERR_SHAPE
+    assert f("pmx_moe_scatter_src")(d, d, d, T, 1, H, d, d, d, None) == _capi.PMX_ERR_SHAPE
+    assert f("pmx_moe_gather")(d, d, T, 2, H, d, None) == _capi.PMX_ERR_SHAPE
+    assert f("pmx_combine_fwd")(d, d, d, T, 2, H, d, None) == _capi.PMX_ERR_SHAPE
+    assert f("pmx_combine_bwd")(d, d, d, d, T, 2, H, d, d, None) == _capi.PMX_ERR_SHAPE
+    assert f("pmx_combine_bwd")(d, d, d, d, W, 1, H, d, d, None) == _capi.PMX_ERR_SHAPE
+    assert f("pmx_combine_bwd_top1_rows")(d, d, d, d, W, H, d, d, None) == _capi.PMX_ERR_SHAPE
+    assert f("pmx_swiglu_bwd_weighted")(d, d, d, d, d, W, 8, 4, d, d, None) == _capi.PMX_ERR_SHAPE
+    big = 1 << 40
+    assert f("pmx_ep_combine_aggregate")(d, d, d, d, d, W, 8, 1, d, d, d, d, d, d, big, None) == _capi.PMX_ERR_SHAPE
+    assert lib.pmx_ep_dispatch_payload(d, d, d, W, 1, 8, 1, 1, d, d, d, d, d, d, d, d, d, d, d, big, None) == _capi.PMX_ERR_SHAPE
+
+
 def test_size_limits_rejected_before_any_launch():
     """Shapes beyond the 32-bit row and position indices are refused on the
     host (PMX_ERR_SHAPE) before any HIP call, so this runs without a GPU."""
