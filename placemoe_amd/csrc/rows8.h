@@ -53,7 +53,7 @@ __device__ __forceinline__ uint32_t scale_byte(uint32_t most) {
   const int b = FMT == kFmtE4M3 ? e - 8 + (m > 0x600000u ? 1 : 0) : e - 6 + (m > 0x7e0000u ? 1 : 0);
   return most == 0 ? 127u : (uint32_t)(b < 0 ? 0 : b);
 }
-// 2^(127 - b), b <= 248: a normal fp32.
+// 2^(127 - b), b <= 249 (a block of int8 at the top of bf16): a normal fp32.
 __device__ __forceinline__ float inv_scale(uint32_t b) { return __uint_as_float((254u - b) << 23); }
 // 2^(b - 127); 2^-127 is subnormal.
 __device__ __forceinline__ float scale_of(uint32_t b) { return __uint_as_float(b == 0 ? 0x400000u : b << 23); }
