@@ -10,7 +10,7 @@ import pytest
 import torch
 
 import placemoe_amd
-from placemoe_amd import rows8
+from placemoe_amd import kernels, rows8
 from tests.helpers import assert_bf16_close, assert_exact
 from tests.test_gpu_rows8 import SUBNORMAL, _layer_oracle, _randn
 
@@ -84,3 +84,19 @@ def test_layer_keeps_nan_to_its_token(cuda, name):
     rest = torch.ones(T, dtype=torch.bool, device=cuda)
     rest[hit] = False
     assert_exact(got[rest], want[rest], "the other tokens")
+
+
+def test_the_layer_in_steps(cuda):
+    """Routing, tokens to 8 bits, fc1, fc2 and the sum as calls of their own: the layer, but for fc2's rows, which
+    the public product rounds to the tensors' dtype."""
+    x, w, sel, gate_up, down = _case(cuda, "mid")
+    q, C = rows8.Experts8.quantize(gate_up, down), down.shape[0]
+    r = kernels.route(sel, C)
+    tokens, row_token, row_w = rows8.quantize_rows_routed(x, r.pos, w)
+    act = rows8.gemm_fc1_swiglu_rows8(tokens, q.gate_up, r.offsets, row_token, row_w)
+    y = rows8.group_gemm_nt_rows8(act, q.down, r.offsets)
+    got, want = kernels.moe_gather(y, r.pos).double(), placemoe_amd.expert_layer_rows8(x, w, sel, q).double()
+    # half a step of each row, and of each sum
+    rows = y.double().abs()[r.pos.long()].sum(1)
+    tol = (rows + got.abs() + want.abs()) * torch.finfo(BF).eps / 2
+    assert ((got - want).abs() <= tol).all(), ((got - want).abs() - tol).max()
