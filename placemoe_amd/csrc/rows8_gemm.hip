@@ -22,9 +22,9 @@
 // on v_mfma_f32_32x32x16_bf16, whose sums are good to fp32; it reads as few bytes.
 //
 // Bound: MFMA from some hundred rows per group on, the weights' bytes below.
-// Measured: NT 65536 x 4096 x 7168 over 16 groups 1.57-1.66 ms, 2.3-2.45 PFLOP/s at
+// Measured: NT 65536 x 4096 x 7168 over 16 groups 1.57-1.71 ms, 2.25-2.45 PFLOP/s at
 // the power limit (torch's 8-bit product of 8192^3 in one process with it: 2.50
-// against 2.46); FC1 of 65536 rows of 160 copies of 1536 x 2048 0.42-0.46 ms, 0.9-1.0
+// against 2.46); FC1 of 65536 rows of 160 copies of 1536 x 2048 0.42-0.53 ms, 0.8-1.0
 // PFLOP/s (bf16 products of 8192^3: 1.28); 768 rows of those copies 89 (NT) and 91 us,
 // 5.6 TB/s of weights.
 //
