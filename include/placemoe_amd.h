@@ -533,7 +533,8 @@ int pmx_rows8_group_gemm_nt(const void* a, const void* a_scales, const void* b, 
  * X: T rows of H (codes and scales); row_token int32 [A], NULL: row r is X's
  * row r (T = A); a token outside [0, T) reads as zeros.  w [G, 2I, H], gate
  * rows first.  row_w bf16 [A], NULL: 1.  act: codes [A, I] and scales.  fp32 sums
- * (bf16 matrix instructions).  Offsets as in pmx_rows8_group_gemm_nt.  1 <= G <=
+ * (bf16 matrix instructions: 2^128, to which 8 bits round the topmost 3% of bf16's
+ * range, counts as infinite).  Offsets as in pmx_rows8_group_gemm_nt.  1 <= G <=
  * 2048; H and I multiples of 16, pointers to codes and scales 16-byte aligned,
  * 2*I*H, the scales of X and of a w[g], and with row_token T*H below 2 GiB each,
  * else PMX_ERR_SHAPE (G: PMX_ERR_ARG). */

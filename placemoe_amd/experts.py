@@ -30,8 +30,9 @@ rows [A, 2I] in 8 bits instead of the permuted rows [A, H], the gate/up rows,
 the activations [A, I] and, in EP arithmetic, the expert outputs [A, H] in 16:
 H + 2I instead of 4H + 6I bytes (non-EP: 2H + 6I) per row of a top-1 layer, less
 still with more experts per token.  (The hidden states are for fc1's weight
-gradient: where fc1 is frozen they are not kept.)  Its backward takes the weights' gradient on the fc2 input side in both
-arithmetics, where it needs no expert outputs.
+gradient: where fc1 is frozen they are not kept.)  Its backward takes the
+weights' gradient on the fc2 input side in both arithmetics, where it needs no
+expert outputs.
 """
 
 from __future__ import annotations

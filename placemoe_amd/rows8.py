@@ -243,7 +243,8 @@ def gemm_fc1_swiglu_rows8(x: Rows8, w: Rows8, offsets: torch.Tensor, row_token: 
     """act[r] = silu(gate) * up * row_w[r], in 8 bits again, with (gate | up) =
     x[row_token[r]] @ w[g]^T: x [T, H], w [G, 2I, H] (gate rows first), both e4m3;
     row_token int32 [A] (None: row r is x[r]), row_w [A] (None: ones).  fp32
-    up to the rounding to 8 bits.  H and I multiples of 16."""
+    up to the rounding to 8 bits (2^128, to which 8 bits round the topmost 3% of
+    bfloat16's range, counts as infinite).  H and I multiples of 16."""
     dev = _check_dev(x.codes, x.scales, w.codes, w.scales, offsets, row_token, row_w)
     dt = _e4m3("x", x, 2)
     _e4m3("w", w, 3, dt)

@@ -73,3 +73,50 @@ def test_products_stay_within_what_the_instruction_cuts(cuda, counts, N, K, dtyp
         exact, tol = _bound(va[rows], O.values(qb.codes[g].cpu(), qb.scales[g].cpu()))
         tol = tol + (np.abs(exact) + tol) * torch.finfo(dtype).eps / 2 + SUBNORMAL[dtype]
         assert (np.abs(got[rows] - exact) <= tol * 1.0001).all(), (np.abs(got[rows] - exact) - tol).max()
+
+
+@pytest.mark.parametrize("x_exp,w_exp", [(-118, 110), (-126, 118), (-130, 121), (118, -110), (122, -116)])
+def test_products_at_the_ends_of_the_range(cuda, x_exp, w_exp):
+    """Blocks beside 2^-127 and near 2^118, in products of ordinary size."""
+    M, K, I = 40, 272, 64
+    x, w = _randn((M, K), 1, torch.float32), _randn((1, 2 * I, K), 2, torch.float32)
+    # (two factors: 2^-130 is no fp32 normal number)
+    half = x_exp // 2
+    x, w = (x * 2.0**half * 2.0**(x_exp - half)).to(BF), (w * 2.0**w_exp).to(BF)
+    qx, qw, off = rows8.quantize_rows(x.to(cuda)), rows8.quantize_rows(w.to(cuda)), _offsets([M]).to(cuda)
+    exact, tol = _bound(O.values(qx.codes.cpu(), qx.scales.cpu()), O.values(qw.codes[0].cpu(), qw.scales[0].cpu()))
+    got = rows8.group_gemm_nt_rows8(qx, qw, off).double().cpu().numpy()
+    limit = tol + (np.abs(exact) + tol) * torch.finfo(BF).eps / 2
+    assert (np.abs(got - exact) <= limit * 1.0001).all()
+    # fc1: fp32 sums of K products, each exact; silu(gate) to 2^-17 and 1.1 of the gate's error; half a step of e4m3
+    size = np.abs(O.values(qx.codes.cpu(), qx.scales.cpu())) @ np.abs(O.values(qw.codes[0].cpu(), qw.scales[0].cpu())).T * K * 2.0**-23
+    gate, up = exact[:, :I], exact[:, I:]
+    with np.errstate(over="ignore"):
+        act = gate / (1 + np.exp(-gate)) * up
+    slack = 1.1 * size[:, :I] * np.abs(up) + np.abs(gate) * size[:, I:] + np.abs(act) * 2.0**-16
+    q = rows8.gemm_fc1_swiglu_rows8(qx, qw, off)
+    unit = np.repeat(2.0 ** (q.scales.cpu().permute(1, 0, 2).reshape(M, -1)[:, :I // 32].numpy().astype(np.float64) - 127), 32, axis=1)
+    v = O.values(q.codes.cpu(), q.scales.cpu())
+    assert (np.abs(v - act) <= (slack + np.maximum((np.abs(act) + slack) * 2.0**-4, unit * 2.0**-10)) * 1.0001).all()
+
+
+def test_values_that_8_bits_round_past_the_range(cuda):
+    """bf16's largest values are 2^128 in 8 bits: NT multiplies them as that, fc1, in bf16, as infinities; the
+    other rows have what they have without."""
+    K, I = 64, 32
+    x, w = _randn((5, K), 1), _randn((1, 2 * I, K), 2, BF, 2.0**-100)
+    w[:, 3::5] = 0
+    loud = x.clone()
+    loud[2, 7] = torch.finfo(BF).max
+    off = _offsets([5]).to(cuda)
+    qx, ql, qw = (rows8.quantize_rows(t.to(cuda)) for t in (x, loud, w))
+    assert O.values(ql.codes.cpu(), ql.scales.cpu())[2, 7] == 2.0**128
+    others = torch.tensor([0, 1, 3, 4], device=cuda)
+    got = rows8.group_gemm_nt_rows8(ql, qw, off)
+    assert torch.equal(got[others], rows8.group_gemm_nt_rows8(qx, qw, off)[others])
+    exact, tol = _bound(O.values(ql.codes.cpu(), ql.scales.cpu()), O.values(qw.codes[0].cpu(), qw.scales[0].cpu()))
+    tol = tol + (np.abs(exact) + tol) * torch.finfo(BF).eps / 2
+    assert (np.abs(got.double().cpu().numpy() - exact) <= tol * 1.0001).all()
+    act, plain = rows8.gemm_fc1_swiglu_rows8(ql, qw, off), rows8.gemm_fc1_swiglu_rows8(qx, qw, off)
+    assert torch.equal(act.codes.view(torch.uint8)[others], plain.codes.view(torch.uint8)[others])
+    assert rows8.dequantize_rows(act)[2].isnan().any()
