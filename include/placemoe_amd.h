@@ -563,6 +563,58 @@ int pmx_rows8_layer(const void* hidden, const void* w, const int64_t* sel, const
                     int32_t* status_host, pmx_stream_t stream);
 
 /* ------------------------------------------------------------------------ */
+/* Rows in 4 bits: weights, products and the serving layer over them         */
+/* ------------------------------------------------------------------------ */
+/* As rows in 8 bits, each value held as an e2m1 float: 0, 0.5, 1, 1.5, 2, 3, 4,
+ * 6 and a sign.
+ *   e    = the smallest integer in [-127, 127] with most < 7 * 2^e, `most` the
+ *          block's largest magnitude; 0 for a block of zeros
+ *   code = x / 2^e rounded to the nearest value, ties to the even code.
+ * A block of 32 with a value that is not finite is NaN as a whole: its exponent
+ * byte is 255.  Reading back is exact, except that values beyond the output
+ * type's range become its largest finite one.
+ *   codes:  [.., R, ceil(N / 2)] bytes, column 2 j in the low half of byte j
+ *           (past an odd row's end: 0).
+ *   scales: as of rows in 8 bits.
+ * The row functions take any N and any alignment, and as many rows as a grid of
+ * 2^32 threads covers, else PMX_ERR_SHAPE.
+ * No counterpart in the reference, whose expert layer is 16-bit throughout. */
+
+/* x: G groups of R rows of N bf16, row r of group g at x + g*gsx + r*ldx
+ * elements (ldx >= N) -> codes [G, R, ceil(N / 2)], scales [G, B, R, 16]. */
+int pmx_rows4_quantize(const void* x, int64_t ldx, int64_t gsx, int64_t G, int64_t R, int64_t N, void* codes,
+                       void* scales, pmx_stream_t stream);
+/* G groups of R rows back in bf16: out [G, R, N]. */
+int pmx_rows4_dequantize(const void* codes, const void* scales, int64_t G, int64_t R, int64_t N, void* out,
+                         pmx_stream_t stream);
+
+/* C[rows of g] = bf16(A[rows of g] B[g]^T) as pmx_rows8_group_gemm_nt, B in 4
+ * bits: codes [G, N, K / 2].  a_bits: A in e4m3 (8; codes [M, K]) or in 4 bits
+ * (4; codes [M, K / 2]), anything else PMX_ERR_ARG.  K a multiple of 32, N of 8.
+ * Both in 4 bits, a sum is good to fp32 (the products of a block of 32 are whole
+ * multiples of a quarter of its powers of two); A in 8 bits, as good as
+ * pmx_rows8_group_gemm_nt's.  Sizes in bytes as there. */
+int pmx_rows4_group_gemm_nt(const void* a, const void* a_scales, int32_t a_bits, const void* b,
+                            const void* b_scales, const int32_t* offsets, int32_t G, int64_t M, int64_t N,
+                            int64_t K, void* c, pmx_stream_t stream);
+
+/* fc1 + SwiGLU as pmx_rows8_gemm_fc1_swiglu (X and act in e4m3), w [G, 2I, H] in
+ * 4 bits: codes [G, 2I, H / 2].  fp32 sums as there.  H a multiple of 32, I of 16. */
+int pmx_rows4_gemm_fc1_swiglu(const void* x, const void* x_scales, int64_t T, const int32_t* row_token,
+                              const void* w, const void* w_scales, const int32_t* offsets, int32_t G,
+                              int64_t A, int64_t H, int64_t I, const void* row_w, void* act, void* act_scales,
+                              pmx_stream_t stream);
+
+/* The expert layer as pmx_rows8_layer (tokens and activations in e4m3), gate_up
+ * [C, 2I, H] and down [C, H, I] in 4 bits.  H and I multiples of 32. */
+size_t pmx_rows4_layer_workspace_bytes(int64_t T, int32_t K, int64_t H, int64_t I, int32_t C);
+int pmx_rows4_layer(const void* hidden, const void* w, const int64_t* sel, const int64_t* M, const int64_t* src,
+                    int32_t src_const, int32_t S, int32_t E, const void* gate_up, const void* gate_up_scales,
+                    const void* down, const void* down_scales, int64_t T, int32_t K, int64_t H, int64_t I,
+                    int32_t C, void* out, int32_t* counts, void* workspace, size_t workspace_bytes,
+                    int32_t* status_host, pmx_stream_t stream);
+
+/* ------------------------------------------------------------------------ */
 /* fp16 tensors                                                              */
 /* ------------------------------------------------------------------------ */
 /* The reference's fused MoE op takes bf16 or fp16 hidden states and router
@@ -650,6 +702,23 @@ int pmx_rows8_gemm_fc1_swiglu_f16(const void* x, const void* x_scales, int64_t T
                                   int64_t A, int64_t H, int64_t I, const void* row_w, void* act, void* act_scales,
                                   pmx_stream_t stream);
 int pmx_rows8_layer_f16(const void* hidden, const void* w, const int64_t* sel, const int64_t* M,
+                        const int64_t* src, int32_t src_const, int32_t S, int32_t E, const void* gate_up,
+                        const void* gate_up_scales, const void* down, const void* down_scales, int64_t T, int32_t K,
+                        int64_t H, int64_t I, int32_t C, void* out, int32_t* counts, void* workspace,
+                        size_t workspace_bytes, int32_t* status_host, pmx_stream_t stream);
+
+int pmx_rows4_quantize_f16(const void* x, int64_t ldx, int64_t gsx, int64_t G, int64_t R, int64_t N, void* codes,
+                           void* scales, pmx_stream_t stream);
+int pmx_rows4_dequantize_f16(const void* codes, const void* scales, int64_t G, int64_t R, int64_t N, void* out,
+                             pmx_stream_t stream);
+int pmx_rows4_group_gemm_nt_f16(const void* a, const void* a_scales, int32_t a_bits, const void* b,
+                                const void* b_scales, const int32_t* offsets, int32_t G, int64_t M, int64_t N,
+                                int64_t K, void* c, pmx_stream_t stream);
+int pmx_rows4_gemm_fc1_swiglu_f16(const void* x, const void* x_scales, int64_t T, const int32_t* row_token,
+                                  const void* w, const void* w_scales, const int32_t* offsets, int32_t G,
+                                  int64_t A, int64_t H, int64_t I, const void* row_w, void* act, void* act_scales,
+                                  pmx_stream_t stream);
+int pmx_rows4_layer_f16(const void* hidden, const void* w, const int64_t* sel, const int64_t* M,
                         const int64_t* src, int32_t src_const, int32_t S, int32_t E, const void* gate_up,
                         const void* gate_up_scales, const void* down, const void* down_scales, int64_t T, int32_t K,
                         int64_t H, int64_t I, int32_t C, void* out, int32_t* counts, void* workspace,

@@ -17,6 +17,7 @@ from .fused_moe import (  # noqa: F401
 from .kernel_registry import KERNEL_REGISTRY, HardwareRequirement, KernelSpec  # noqa: F401
 from .placement import PLACEMENTS, LayerPlacement, LayerPlan, PlaceMoETopology, mirrored_r2_plan  # noqa: F401
 from .replica import OverlappedReplicaSync, fold_replica_gradients, sync_redundant_gradients  # noqa: F401
+from .rows4 import Experts4, Rows4, dequantize_rows4, expert_layer_rows4, quantize_rows4  # noqa: F401
 from .rows8 import Experts8, Rows8, dequantize_rows, expert_layer_rows8, quantize_rows  # noqa: F401
 from .statistics import ProfileStatistics, RouteStatisticsRecorder, profile_route_statistics  # noqa: F401
 

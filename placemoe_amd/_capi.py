@@ -173,6 +173,15 @@ SIGNATURES = {
          c_void_p, c_int64, c_int32, c_int64, c_int64, c_int32, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p,
          c_void_p],
     ),
+    "pmx_rows4_quantize": (
+        c_int, [c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p]
+    ),
+    "pmx_rows4_dequantize": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p]),
+    "pmx_rows4_group_gemm_nt": (
+        c_int,
+        [c_void_p, c_void_p, c_int32, c_void_p, c_void_p, c_void_p, c_int32, c_int64, c_int64, c_int64, c_void_p,
+         c_void_p],
+    ),
     "pmx_ep_combine_workspace_bytes": (c_size_t, [c_int64]),
     "pmx_ep_combine_aggregate": (
         c_int,
@@ -180,6 +189,10 @@ SIGNATURES = {
          c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p],
     ),
 }
+
+# weights in 4 bits: the arguments of the 8-bit namesakes
+for _name in ("gemm_fc1_swiglu", "layer_workspace_bytes", "layer"):
+    SIGNATURES["pmx_rows4_" + _name] = SIGNATURES["pmx_rows8_" + _name]
 
 # the EP payload entry points with int64 indices: the same arguments
 for _name in ("pmx_ep_dispatch_payload", "pmx_ep_combine_aggregate"):
@@ -195,6 +208,8 @@ F16_TWINS = (
     "pmx_replica_fold", "pmx_ep_combine_aggregate", "pmx_ep_combine_aggregate_i64",
     "pmx_rows8_quantize", "pmx_rows8_quantize_routed", "pmx_rows8_dequantize", "pmx_rows8_swiglu_bwd",
     "pmx_rows8_group_gemm_nt", "pmx_rows8_gemm_fc1_swiglu", "pmx_rows8_layer",
+    "pmx_rows4_quantize", "pmx_rows4_dequantize", "pmx_rows4_group_gemm_nt", "pmx_rows4_gemm_fc1_swiglu",
+    "pmx_rows4_layer",
 )
 SIGNATURES.update({name + "_f16": SIGNATURES[name] for name in F16_TWINS})
 

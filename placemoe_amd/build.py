@@ -58,7 +58,8 @@ HIP_FLAGS = [
 
 # Sources whose kernels must run without scratch memory (see the module
 # docstring), and the kernel-name pattern the check applies to.
-RESOURCE_CHECKED = {"grouped_gemm.hip": re.compile(r"grouped_gemm"), "rows8_gemm.hip": re.compile(r"rows8_grouped_gemm")}
+RESOURCE_CHECKED = {"grouped_gemm.hip": re.compile(r"grouped_gemm"), "rows8_gemm.hip": re.compile(r"rows8_grouped_gemm"),
+                    "rows4_gemm.hip": re.compile(r"rows8_grouped_gemm")}
 RESOURCE_FLAG = "-Rpass-analysis=kernel-resource-usage"
 
 # name -> (source, extra flags): further objects of the library, built from a

@@ -315,18 +315,26 @@ def expert_layer_rows8(hidden: torch.Tensor, routing_weights: torch.Tensor, sele
     input, as in the non-EP arithmetic); a token's rows, held in 24 bits (each value to
     2^-16 of itself), are then summed and rounded once.  H and I multiples of 16.
     """
+    assert isinstance(weights, Experts8), f"weights must be Experts8, got {type(weights).__name__}"
+    return _serving_layer("expert_layer_rows8", "pmx_rows8_layer", 16, _e4m3, hidden, routing_weights, selected_experts, weights,
+                          mapping, sources, source, recorder)
+
+
+def _serving_layer(name: str, entry: str, multiple: int, check_weights, hidden: torch.Tensor, routing_weights: torch.Tensor,
+                   selected_experts: torch.Tensor, weights, mapping: torch.Tensor | None, sources: torch.Tensor | None,
+                   source: int, recorder) -> torch.Tensor:
+    """The layer ``name`` over weights in 8 or 4 bits; ``check_weights`` looks one matrix over, ``entry`` is the C-ABI's call."""
     from . import experts  # experts itself uses this module's checkpoints
 
-    assert isinstance(weights, Experts8), f"weights must be Experts8, got {type(weights).__name__}"
     if torch.is_grad_enabled() and (hidden.requires_grad or routing_weights.requires_grad):
-        raise ValueError("expert_layer_rows8 has no backward; call it under torch.no_grad()")
+        raise ValueError(f"{name} has no backward; call it under torch.no_grad()")
     _check_dev(hidden, routing_weights, selected_experts, weights.gate_up.codes, weights.gate_up.scales, weights.down.codes,
                weights.down.scales, mapping, sources)
     dt = _half("hidden states", hidden)
     _half("routing weights", routing_weights, dt)
     assert hidden.dim() == 2, "hidden states must be [tokens, hidden size]"
-    _e4m3("gate_up", weights.gate_up, 3, dt)
-    _e4m3("down", weights.down, 3, dt)
+    check_weights("gate_up", weights.gate_up, 3, dt)
+    check_weights("down", weights.down, 3, dt)
     C, H, I = weights.down.shape
     assert tuple(weights.gate_up.shape) == (C, 2 * I, H), "gate_up and down describe different layers"
     T = hidden.shape[0]
@@ -349,10 +357,10 @@ def expert_layer_rows8(hidden: torch.Tensor, routing_weights: torch.Tensor, sele
         if recorder is not None:
             recorder(torch.zeros(C, dtype=torch.int32, device=hidden.device))
         return torch.zeros_like(hidden)
-    ws_bytes = _capi.load().pmx_rows8_layer_workspace_bytes(T, K, H, I, C)
+    ws_bytes = getattr(_capi.load(), entry + "_workspace_bytes")(T, K, H, I, C)
     if ws_bytes == 0:
-        raise ValueError(f"expert_layer_rows8: {T} tokens, {K} each, through {C} copies of {H} x {I} are not supported (sizes "
-                         "must be multiples of 16, copies at most 2048, and tokens, a copy's weights and each tensor's "
+        raise ValueError(f"{name}: {T} tokens, {K} each, through {C} copies of {H} x {I} are not supported (sizes "
+                         f"must be multiples of {multiple}, copies at most 2048, and tokens, a copy's weights and each tensor's "
                          "scales below 2 GiB)")
     dev = hidden.device
     with _on(dev):
@@ -364,7 +372,7 @@ def expert_layer_rows8(hidden: torch.Tensor, routing_weights: torch.Tensor, sele
         status_host = check.arm(dev)
         try:
             _capi.call(
-                _sym("pmx_rows8_layer", dt), _ptr(hidden), _ptr(routing_weights), _ptr(sel), _ptr(mapping), _ptr(sources),
+                _sym(entry, dt), _ptr(hidden), _ptr(routing_weights), _ptr(sel), _ptr(mapping), _ptr(sources),
                 int(source), S, E, _ptr(weights.gate_up.codes), _ptr(weights.gate_up.scales), _ptr(weights.down.codes),
                 _ptr(weights.down.scales), T, K, H, I, C, _ptr(out), _ptr(counts), _ptr(ws), ws_bytes, status_host, _stream(dev),
             )
