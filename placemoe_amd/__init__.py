@@ -14,6 +14,7 @@ from .fused_moe import (  # noqa: F401
     set_activation_checkpoint,
     set_router_weight_point,
 )
+from .gated import gated_ffn  # noqa: F401
 from .kernel_registry import KERNEL_REGISTRY, HardwareRequirement, KernelSpec  # noqa: F401
 from .placement import PLACEMENTS, LayerPlacement, LayerPlan, PlaceMoETopology, mirrored_r2_plan  # noqa: F401
 from .replica import OverlappedReplicaSync, fold_replica_gradients, sync_redundant_gradients  # noqa: F401

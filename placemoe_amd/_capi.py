@@ -182,6 +182,13 @@ SIGNATURES = {
         [c_void_p, c_void_p, c_int32, c_void_p, c_void_p, c_void_p, c_int32, c_int64, c_int64, c_int64, c_void_p,
          c_void_p],
     ),
+    "pmx_gated_ffn_workspace_bytes": (c_size_t, [c_int64] * 4),
+    "pmx_gated_ffn_fwd": (
+        c_int, [c_void_p] * 3 + [c_int64] * 4 + [c_int32] + [c_void_p] * 4
+    ),
+    "pmx_gated_ffn_bwd": (
+        c_int, [c_void_p] * 6 + [c_int64] * 4 + [c_int32] + [c_void_p] * 4 + [c_size_t, c_void_p]
+    ),
     "pmx_ep_combine_workspace_bytes": (c_size_t, [c_int64]),
     "pmx_ep_combine_aggregate": (
         c_int,
@@ -209,7 +216,7 @@ F16_TWINS = (
     "pmx_rows8_quantize", "pmx_rows8_quantize_routed", "pmx_rows8_dequantize", "pmx_rows8_swiglu_bwd",
     "pmx_rows8_group_gemm_nt", "pmx_rows8_gemm_fc1_swiglu", "pmx_rows8_layer",
     "pmx_rows4_quantize", "pmx_rows4_dequantize", "pmx_rows4_group_gemm_nt", "pmx_rows4_gemm_fc1_swiglu",
-    "pmx_rows4_layer",
+    "pmx_rows4_layer", "pmx_gated_ffn_fwd", "pmx_gated_ffn_bwd",
 )
 SIGNATURES.update({name + "_f16": SIGNATURES[name] for name in F16_TWINS})
 

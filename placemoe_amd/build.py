@@ -14,8 +14,9 @@ per-kernel resource report and fails if any of their kernels uses scratch
 memory or spills vector registers
 (``resource_usage.json`` beside the library keeps the report).
 
-The grouped GEMM source is compiled twice into the library: once for bf16
-and once with ``-DPMX_ELT_F16`` for the fp16 entry points (``EXTRA_OBJECTS``).
+The grouped GEMM source is compiled four times into the library: for bf16 and
+with ``-DPMX_ELT_F16`` for the fp16 entry points, and each again with
+``-DPMX_GATED`` for the dense gated block (``EXTRA_OBJECTS``).
 
 Test variants: ``_lib/variants/libplacemoe_amd_<name>.so`` is the same library
 with extra defines for one source (``VARIANTS``), e.g. a two-entry LDS tile
@@ -64,8 +65,11 @@ RESOURCE_FLAG = "-Rpass-analysis=kernel-resource-usage"
 
 # name -> (source, extra flags): further objects of the library, built from a
 # source a second time with other defines.
-#   grouped_gemm.f16: the grouped GEMM for fp16 tensors (entry points *_f16).
-EXTRA_OBJECTS = {"grouped_gemm.f16": ("grouped_gemm.hip", ["-DPMX_ELT_F16"])}
+#   grouped_gemm.f16: the grouped GEMM for fp16 tensors (entry points *_f16);
+#   grouped_gemm.gated, .gated_f16: its kernels for the dense gated block.
+EXTRA_OBJECTS = {"grouped_gemm.f16": ("grouped_gemm.hip", ["-DPMX_ELT_F16"]),
+                 "grouped_gemm.gated": ("grouped_gemm.hip", ["-DPMX_GATED"]),
+                 "grouped_gemm.gated_f16": ("grouped_gemm.hip", ["-DPMX_GATED", "-DPMX_ELT_F16"])}
 
 # name -> (source, extra flags): library variants for tests and comparisons.
 #   tiletab2: a two-entry LDS tile table (the on-the-spot tile decode runs at small shapes);

@@ -173,16 +173,15 @@ __device__ __forceinline__ void epilogue(const GemmParams& P, const TileInfo& ti
         const int64_t j = (int64_t)ti.ntile * (CF::BN / 2) + (wn * CF::FN + nt) * 8 + c4;
         if (j >= I) continue;
         const f32x4_t g4 = acc[mt][nt], u4 = acc[mt][nt + 1];
-        st4(P.gu + r * 2 * I + j, pack4(g4[0], g4[1], g4[2], g4[3]));
-        st4(P.gu + r * 2 * I + I + j, pack4(u4[0], u4[1], u4[2], u4[3]));
+        if (!kGated || P.gu != nullptr) {
+          st4(P.gu + r * 2 * I + j, pack4(g4[0], g4[1], g4[2], g4[3]));
+          st4(P.gu + r * 2 * I + I + j, pack4(u4[0], u4[1], u4[2], u4[3]));
+        }
         float g[4], u[4];
 #pragma unroll
         for (int e = 0; e < 4; e += 2) {
           g[e] = g4[e], g[e + 1] = g4[e + 1], u[e] = u4[e], u[e + 1] = u4[e + 1];
-          Elt::round2(g[e], g[e + 1]);
-          Elt::round2(u[e], u[e + 1]);
-          g[e] = silu_f32(g[e]), g[e + 1] = silu_f32(g[e + 1]);
-          Elt::round2(g[e], g[e + 1]);
+          activate2(P, g + e, u + e);
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e) g[e] *= u[e];
@@ -210,7 +209,7 @@ __device__ __forceinline__ void epilogue(const GemmParams& P, const TileInfo& ti
         unpack8e<Elt>(make_uint4(da.x, da.y, db.x, db.y), d);
         unpack8e<Elt>(make_uint4(ga.x, ga.y, gb.x, gb.y), g);
         unpack8e<Elt>(make_uint4(ua.x, ua.y, ub.x, ub.y), u);
-        swiglu_bwd8<Elt>(d, g, u, dg, du);
+        activate_bwd8(P, d, g, u, dg, du);
         const uint4 pg = pack8e<Elt>(dg), pu = pack8e<Elt>(du);
         bf16_t* o = P.c0 + r * 2 * I;
         if (ina) st4(o + ja, make_uint2(pg.x, pg.y)), st4(o + I + ja, make_uint2(pu.x, pu.y));
@@ -264,7 +263,7 @@ __global__ __launch_bounds__(CF::NT, CF::NW * CF::BPC / 4) void few_rows_grouped
     const int per = (G + CF::NT - 1) / CF::NT;
     const int g0 = t * per, g1 = g0 + per < G ? g0 + per : G;
     int32_t sum = 0;
-    for (int g = g0; g < g1; ++g) sum += (P.offsets[g + 1] - P.offsets[g] + CF::BM - 1) / CF::BM;
+    for (int g = g0; g < g1; ++g) sum += (group_row(P, g + 1) - group_row(P, g) + CF::BM - 1) / CF::BM;
     int32_t inc = sum;
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) {
@@ -277,7 +276,7 @@ __global__ __launch_bounds__(CF::NT, CF::NW * CF::BPC / 4) void few_rows_grouped
     for (int w = 0; w < wave; ++w) run += wsum[w];
     for (int g = g0; g < g1; ++g) {
       tpre[g] = run;
-      run += (P.offsets[g + 1] - P.offsets[g] + CF::BM - 1) / CF::BM;
+      run += (group_row(P, g + 1) - group_row(P, g) + CF::BM - 1) / CF::BM;
     }
     if (t == CF::NT - 1) tpre[G] = run;
     __syncthreads();
@@ -312,8 +311,8 @@ __global__ __launch_bounds__(CF::NT, CF::NW * CF::BPC / 4) void few_rows_grouped
     ti.g = lo;
     ti.ntile = local / gm;
     ti.mtile = local - ti.ntile * gm;
-    ti.row0 = uni(P.offsets[lo]) + ti.mtile * CF::BM;
-    ti.row_end = uni(P.offsets[lo + 1]);
+    ti.row0 = uni(group_row(P, lo)) + ti.mtile * CF::BM;
+    ti.row_end = uni(group_row(P, lo + 1));
     ti.nk = nk;
   };
 
@@ -487,7 +486,7 @@ __global__ __launch_bounds__(kWgNT, 4) void few_rows_wgrad_grouped_gemm_kernel(G
   const int64_t tile = (blockIdx.x + g) % kNumXcd * per_x + j % per_x;
   if (tile >= per_g) return;
   const int64_t m0 = tile / ntn * kWgT, n0 = tile % ntn * kWgT;
-  const int64_t row0 = P.offsets[g], row_end = P.offsets[g + 1];
+  const int64_t row0 = group_row(P, g), row_end = group_row(P, g + 1);
 
   f32x4_t acc[4][4];
 #pragma unroll

@@ -1,0 +1,274 @@
+// The dense gated block: out = (gate(x Wg^T) * (x Wu^T)) Wd^T, forward and
+// backward, with Wg and Wu the two halves of one matrix.
+//
+// Many tokens: the grouped GEMM's kernels, built for one group that is the whole
+// call (gated_gemm.h):
+//   forward   gu, act = fc1 (both projections, gate and product in its epilogue);  out = act Wd^T
+//   backward  dgu = the gate's gradients of (dout Wd), in its epilogue;  dWd = dout^T act;
+//             dW = dgu^T x;  dx = dgu W
+// gu, act and dgu are held in 16 bits, as are the sums dout Wd on their way
+// through the epilogue: each is an operand of a 16-bit product or, dout Wd, a
+// tile that passes through LDS as such.  (Each such rounding is the outputs' own,
+// 2^-9 of a value; the outputs are 1.0 to 1.7 times as far from the definition in
+// 64 bits as results rounded once are.)  A weight gradient's tiles are few where
+// the weights are small: its rows are cut into chunks whose fp32 sums are then
+// added in order (sum_parts_kernel).
+//
+// Few tokens: a call reads every weight once, and what counts is how many bytes
+// are on their way.  256 x 256 tiles would put 16 of them on the whole chip.
+// Here a block has 16 rows of the weights (fc1: 8 gate rows and their 8 up rows)
+// for all tokens, its waves a share of the columns each, straight from memory to
+// the matrix instruction (16 weight rows x 16 tokens, 32 columns); their sums
+// meet in LDS.  Bound: HBM.
+
+#include "gated.h"
+#include "gated_rule.h"
+
+namespace {
+
+constexpr int kFewWaves = 8;
+constexpr int kFewSteps = 8;  // steps of 32 columns that a wave has on their way
+
+template <class E>
+__device__ __forceinline__ f32x4_t mfma16(const uint4& w, const uint4& x, const f32x4_t& c) {
+  if constexpr (E::kCode == EltF16::kCode) {
+    typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, w), __builtin_bit_cast(f16x8_t, x), c, 0, 0, 0);
+  } else {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, w), __builtin_bit_cast(bf16x8_t, x), c, 0, 0, 0);
+  }
+}
+
+// The sums of 16 weight rows (wrow: the lane's, that of row lane % 16) with
+// tokens 0 .. 15 of x [T, K]: red[wave][weight row][token], after a barrier.
+// K a multiple of 8.  Lanes past K, and past T, multiply zeros.
+template <class E>
+__device__ __forceinline__ void few_products(const bf16_t* wrow, const bf16_t* x, int64_t T, int64_t K, int lane, int wave,
+                                             float (*red)[16][16]) {
+  const int t = lane & 15, quarter = lane >> 4;
+  const bool token = t < T;
+  const bf16_t* xrow = x + (token ? t : 0) * K;
+  const int64_t chunks = K / 8;
+  f32x4_t acc = {};
+  for (int64_t c0 = (int64_t)wave * 4; c0 < chunks; c0 += 4 * kFewWaves * kFewSteps) {
+    uint4 w[kFewSteps], v[kFewSteps];
+#pragma unroll
+    for (int s = 0; s < kFewSteps; ++s) {
+      const int64_t c = c0 + s * (4 * kFewWaves) + quarter;
+      const bool in = c < chunks;
+      w[s] = in ? ld_stream(wrow + c * 8) : make_uint4(0, 0, 0, 0);
+      v[s] = in && token ? *reinterpret_cast<const uint4*>(xrow + c * 8) : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int s = 0; s < kFewSteps; ++s) acc = mfma16<E>(w[s], v[s], acc);
+  }
+  // lane: token lane % 16, weight rows 4 (lane / 16) .. + 3
+#pragma unroll
+  for (int e = 0; e < 4; ++e) red[wave][quarter * 4 + e][t] = acc[e];
+  __syncthreads();
+}
+
+// fc1: eight columns of act (gu) per block.
+template <class E>
+__global__ __launch_bounds__(64 * kFewWaves) void gated_few_fc1_kernel(const bf16_t* __restrict__ x, const bf16_t* __restrict__ w,
+                                                                       int64_t T, int64_t H, int64_t I, Gate gate,
+                                                                       bf16_t* __restrict__ gu, bf16_t* __restrict__ act) {
+  __shared__ float red[kFewWaves][16][16];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t j0 = (int64_t)blockIdx.x * 8;
+  const int r = lane & 15;
+  few_products<E>(w + ((r < 8 ? 0 : I) + j0 + r % 8) * H, x, T, H, lane, wave, red);
+  const int64_t t = threadIdx.x >> 3;
+  const int j = threadIdx.x & 7;
+  if (t >= T || t >= 16) return;
+  float g = 0.f, u = 0.f;
+#pragma unroll
+  for (int i = 0; i < kFewWaves; ++i) g += red[i][j][t], u += red[i][8 + j][t];
+  if (gu != nullptr) {
+    gu[t * 2 * I + j0 + j] = (bf16_t)E::from_f32(g);
+    gu[t * 2 * I + I + j0 + j] = (bf16_t)E::from_f32(u);
+  }
+  act[t * I + j0 + j] = (bf16_t)E::from_f32(gate.value(g) * u);
+}
+
+// fc2: 16 columns of out per block.
+template <class E>
+__global__ __launch_bounds__(64 * kFewWaves) void gated_few_fc2_kernel(const bf16_t* __restrict__ act, const bf16_t* __restrict__ w,
+                                                                       int64_t T, int64_t N, int64_t I, bf16_t* __restrict__ out) {
+  __shared__ float red[kFewWaves][16][16];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t n0 = (int64_t)blockIdx.x * 16;
+  const int64_t n = n0 + (lane & 15);
+  few_products<E>(w + (n < N ? n : N - 1) * I, act, T, I, lane, wave, red);
+  const int64_t t = threadIdx.x >> 4;
+  const int j = threadIdx.x & 15;
+  if (t >= T || t >= 16 || n0 + j >= N) return;
+  float sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < kFewWaves; ++i) sum += red[i][j][t];
+  out[t * N + n0 + j] = (bf16_t)E::from_f32(sum);
+}
+
+// The chunks' sums, in order: a thread per four neighbouring elements.
+template <class E>
+__global__ __launch_bounds__(256) void sum_parts_kernel(const float* __restrict__ parts, int32_t splits, int64_t size,
+                                                        bf16_t* __restrict__ out) {
+  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i >= size) return;  // a multiple of 8
+  f32x4_t sum = *reinterpret_cast<const f32x4_t*>(parts + i);
+  for (int32_t s = 1; s < splits; ++s) sum += *reinterpret_cast<const f32x4_t*>(parts + s * size + i);
+  *reinterpret_cast<uint2*>(out + i) = make_uint2(E::pack2(sum[0], sum[1]), E::pack2(sum[2], sum[3]));
+}
+
+bool gate_of(int32_t gate, Gate& g) {
+  constexpr float kGelu = 1.5957691216057308f;  // 2 sqrt(2 / pi)
+  switch (gate) {
+    case PMX_GATE_SILU: g = {1.0f, 0.0f}; return true;
+    case PMX_GATE_GELU_TANH: g = {kGelu, kGelu * 0.044715f}; return true;
+    case PMX_GATE_QUICK_GELU: g = {1.702f, 0.0f}; return true;
+    default: return false;
+  }
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+// One descriptor holds offsets below 2^31 bytes.
+bool one_window(int64_t rows, int64_t cols) { return rows < (int64_t)0x7fffffff / 2 / cols; }
+
+// Sizes that every product of the block takes; PMX_OK to go on.
+int check(int64_t T, int64_t H, int64_t I, int64_t N) {
+  if (T < 0 || H <= 0 || I <= 0 || N <= 0) return PMX_ERR_ARG;
+  if (H % 8 || I % 8 || N % 8 || T > INT32_MAX - 256 || I > INT32_MAX / 2) return PMX_ERR_SHAPE;
+  const int64_t I2 = 2 * I;
+  // whole weights through one descriptor, 256 rows of every operand, and as many gu rows
+  if (!one_window(I2, H) || !one_window(N, I) || !one_window(256, I2) || !one_window(256, H) || !one_window(256, N)) return PMX_ERR_SHAPE;
+  return PMX_OK;
+}
+
+int cu_count() {
+  int dev = 0, cus = 0;
+  if (hipGetDevice(&dev) != hipSuccess) return -1;
+  if (hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || cus <= 0) return -1;
+  return cus;
+}
+
+// The chunks of a weight gradient [M, N] over K rows; one where the operands pass what one descriptor holds.
+void chunks_of(int64_t K, int64_t M, int64_t N, int64_t cus, int64_t& chunk, int32_t& splits) {
+  splits = one_window(K, M) && one_window(K, N) && one_window(2 * M, N) ? pmx::gated_splits(K, M, N, cus) : 1;
+  chunk = pmx::gated_chunk(K, splits);
+  splits = (int32_t)((K + chunk - 1) / chunk);
+}
+
+// The backward's workspace: dgu, then the fp32 sums of one weight gradient's chunks.
+constexpr int64_t kCus = 256;  // of the workspace's estimate and of the call alike
+size_t dgu_bytes(int64_t T, int64_t I) { return ((size_t)T * 2 * I * 2 + 255) / 256 * 256; }
+size_t parts_bytes(int64_t K, int64_t M, int64_t N) {
+  int64_t chunk;
+  int32_t splits;
+  chunks_of(K, M, N, kCus, chunk, splits);
+  return splits > 1 ? (size_t)splits * M * N * 4 : 0;
+}
+
+template <class E>
+struct Gemms;
+template <>
+struct Gemms<EltBF16> {
+  static constexpr auto fc1 = pmx_gated_fc1;
+  static constexpr auto nt = pmx_gated_nt, nn = pmx_gated_nn;
+  static constexpr auto dgate = pmx_gated_dgate;
+  static constexpr auto tn = pmx_gated_tn;
+};
+template <>
+struct Gemms<EltF16> {
+  static constexpr auto fc1 = pmx_gated_fc1_f16;
+  static constexpr auto nt = pmx_gated_nt_f16, nn = pmx_gated_nn_f16;
+  static constexpr auto dgate = pmx_gated_dgate_f16;
+  static constexpr auto tn = pmx_gated_tn_f16;
+};
+
+template <class E>
+int forward_t(const void* x, const void* gate_up, const void* down, int64_t T, int64_t H, int64_t I, int64_t N, int32_t kind,
+              void* gu, void* act, void* out, pmx_stream_t stream) {
+  Gate gate;
+  if (!gate_of(kind, gate)) return PMX_ERR_ARG;
+  if (const int rc = check(T, H, I, N)) return rc;
+  if (T == 0) return PMX_OK;
+  if (!x || !gate_up || !down || !act || !out) return PMX_ERR_ARG;
+  if (!aligned16(x) || !aligned16(gate_up) || !aligned16(down) || !aligned16(gu) || !aligned16(act) || !aligned16(out)) return PMX_ERR_SHAPE;
+  if (T <= pmx::kGatedFewTokens) {
+    gated_few_fc1_kernel<E><<<(unsigned)(I / 8), 64 * kFewWaves, 0, stream>>>((const bf16_t*)x, (const bf16_t*)gate_up, T, H, I, gate,
+                                                                              (bf16_t*)gu, (bf16_t*)act);
+    PMX_LAUNCH_CHECK();
+    gated_few_fc2_kernel<E><<<(unsigned)((N + 15) / 16), 64 * kFewWaves, 0, stream>>>((const bf16_t*)act, (const bf16_t*)down, T, N, I,
+                                                                                      (bf16_t*)out);
+    PMX_LAUNCH_CHECK();
+    return PMX_OK;
+  }
+  // The sizes have been checked: what fails from here on is a launch.
+  if (Gemms<E>::fc1(x, gate_up, T, H, I, gate.a, gate.b, gu, act, stream) != PMX_OK) return PMX_ERR_HIP;
+  return Gemms<E>::nt(act, down, T, N, I, out, stream) != PMX_OK ? PMX_ERR_HIP : PMX_OK;
+}
+
+template <class E>
+int weight_gradient(const void* a, const void* b, int64_t K, int64_t M, int64_t N, void* c, float* parts, pmx_stream_t stream) {
+  int64_t chunk;
+  int32_t splits;
+  chunks_of(K, M, N, kCus, chunk, splits);
+  if (Gemms<E>::tn(a, b, K, M, N, chunk, splits, c, parts, stream) != PMX_OK) return PMX_ERR_HIP;
+  if (splits > 1) {
+    sum_parts_kernel<E><<<(unsigned)((M * N / 4 + 255) / 256), 256, 0, stream>>>(parts, splits, M * N, (bf16_t*)c);
+    PMX_LAUNCH_CHECK();
+  }
+  return PMX_OK;
+}
+
+template <class E>
+int backward_t(const void* dout, const void* x, const void* gate_up, const void* down, const void* gu, const void* act, int64_t T,
+               int64_t H, int64_t I, int64_t N, int32_t kind, void* dx, void* dgate_up, void* ddown, void* workspace,
+               size_t workspace_bytes, pmx_stream_t stream) {
+  Gate gate;
+  if (!gate_of(kind, gate)) return PMX_ERR_ARG;
+  if (const int rc = check(T, H, I, N)) return rc;
+  if (T == 0) return PMX_OK;
+  if (!dout || (!dx && !dgate_up && !ddown)) return PMX_ERR_ARG;
+  if (((dx || dgate_up) && (!down || !gu)) || (dgate_up && !x) || (dx && !gate_up) || (ddown && !act)) return PMX_ERR_ARG;
+  const void* all[] = {dout, x, gate_up, down, gu, act, dx, dgate_up, ddown, workspace};
+  for (const void* p : all)
+    if (!aligned16(p)) return PMX_ERR_SHAPE;
+  if (!workspace || workspace_bytes < pmx_gated_ffn_workspace_bytes(T, H, I, N)) return PMX_ERR_ARG;
+  void* dgu = workspace;
+  float* parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + dgu_bytes(T, I));
+  int rc = PMX_OK;
+  if (dx || dgate_up) rc = Gemms<E>::dgate(dout, down, gu, T, N, I, gate.a, gate.b, dgu, stream);
+  if (rc == PMX_OK && ddown) rc = weight_gradient<E>(dout, act, T, N, I, ddown, parts, stream);
+  if (rc == PMX_OK && dgate_up) rc = weight_gradient<E>(dgu, x, T, 2 * I, H, dgate_up, parts, stream);
+  if (rc == PMX_OK && dx) rc = Gemms<E>::nn(dgu, gate_up, T, H, 2 * I, dx, stream);
+  return rc != PMX_OK ? PMX_ERR_HIP : PMX_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t pmx_gated_ffn_workspace_bytes(int64_t T, int64_t H, int64_t I, int64_t N) {
+  if (check(T, H, I, N) != PMX_OK || T == 0) return 0;
+  const size_t a = parts_bytes(T, N, I), b = parts_bytes(T, 2 * I, H);
+  return dgu_bytes(T, I) + (a > b ? a : b);
+}
+
+#define PMX_GATED_FFN(SUFFIX, E)                                                                                            \
+  int pmx_gated_ffn_fwd##SUFFIX(const void* x, const void* gate_up, const void* down, int64_t T, int64_t H, int64_t I,      \
+                                int64_t N, int32_t gate, void* gu, void* act, void* out, pmx_stream_t stream) {             \
+    return forward_t<E>(x, gate_up, down, T, H, I, N, gate, gu, act, out, stream);                                          \
+  }                                                                                                                         \
+  int pmx_gated_ffn_bwd##SUFFIX(const void* dout, const void* x, const void* gate_up, const void* down, const void* gu,     \
+                                const void* act, int64_t T, int64_t H, int64_t I, int64_t N, int32_t gate, void* dx,        \
+                                void* dgate_up, void* ddown, void* workspace, size_t workspace_bytes, pmx_stream_t stream) { \
+    return backward_t<E>(dout, x, gate_up, down, gu, act, T, H, I, N, gate, dx, dgate_up, ddown, workspace, workspace_bytes, \
+                         stream);                                                                                           \
+  }
+
+PMX_GATED_FFN(, EltBF16)
+PMX_GATED_FFN(_f16, EltF16)
+
+}  // extern "C"

@@ -1,0 +1,117 @@
+// The dense gated block's products: host side of the build of grouped_gemm.hip
+// with -DPMX_GATED.
+#include "gated.h"
+#include "gated_rule.h"
+
+namespace {
+
+#ifndef PMX_GATED_FORCE
+#define PMX_GATED_FORCE 0
+#endif
+
+template <int KIND>
+int launch_rows(const GemmParams& P, hipStream_t stream) {
+  const int64_t ntn = KIND == KIND_FC1 ? (P.I + 127) / 128 : (P.N + BN - 1) / BN;
+  if (ntn >= (int64_t)1 << 19) return PMX_ERR_SHAPE;  // the LDS tile table keeps an n-tile index in 19 bits
+  const int grid = grid_size();
+  if (grid <= 0) return PMX_ERR_HIP;
+  const int tiling = PMX_GATED_FORCE ? PMX_GATED_FORCE : pmx::gated_tiling(KIND, P.M, P.N, P.K, grid);
+  if (tiling == Few64::BM) return launch_few<KIND, Few64>(P, grid, stream);
+  if (tiling == Few128::BM) return launch_few<KIND, Few128>(P, grid, stream);
+  const bool fast = P.K % BK == 0;
+  if constexpr (use_w4<KIND>()) {
+    if (fast) w4::grouped_gemm_w4_kernel<KIND><<<grid, w4::NT, 0, stream>>>(P);
+    else grouped_gemm_kernel<KIND, kBM><<<grid, NTHREADS, 0, stream>>>(P);
+  } else {
+    if (!fast) grouped_gemm_kernel<KIND, kBM><<<grid, NTHREADS, 0, stream>>>(P);
+    else if (KIND == KIND_NT || P.M < kRsMaxRowsPerCopy) grouped_gemm_kernel<KIND, kBM, false, true, true><<<grid, NTHREADS, 0, stream>>>(P);
+    else grouped_gemm_kernel<KIND, kBM, false, true><<<grid, NTHREADS, 0, stream>>>(P);
+  }
+  PMX_LAUNCH_CHECK();
+  return PMX_OK;
+}
+
+GemmParams dense(const void* a, const void* b, int64_t M, int64_t N, int64_t K, int64_t ldb) {
+  GemmParams P = {};
+  P.a = one(a, 0, K);
+  P.b = one(b, 0, ldb);
+  P.G = 1, P.chunk = P.rows = (uint32_t)M;
+  P.M = M, P.N = N, P.K = K;
+  P.ldc = N;
+  return P;
+}
+
+}  // namespace
+
+int PMX_GEMM_FN(pmx_gated_fc1)(const void* x, const void* w, int64_t T, int64_t H, int64_t I, float a, float b, void* gu,
+                               void* act, pmx_stream_t stream) {
+  if (!fits_rsrc(I, H) || !fits_rsrc(kBM, H)) return PMX_ERR_SHAPE;
+  GemmParams P = dense(x, w, T, 2 * I, H, H);
+  P.b.p1 = P.b.p0 + I * H;
+  P.b.split = I;
+  P.I = I;
+  P.gu = static_cast<bf16_t*>(gu);
+  P.act = static_cast<bf16_t*>(act);
+  P.gate = {a, b};
+  return launch_rows<KIND_FC1>(P, stream);
+}
+
+int PMX_GEMM_FN(pmx_gated_nt)(const void* a, const void* b, int64_t M, int64_t N, int64_t K, void* c, pmx_stream_t stream) {
+  if (!fits_rsrc(N, K) || !fits_rsrc(kBM, K)) return PMX_ERR_SHAPE;
+  GemmParams P = dense(a, b, M, N, K, K);
+  P.c0 = static_cast<bf16_t*>(c);
+  return launch_rows<KIND_NT>(P, stream);
+}
+
+int PMX_GEMM_FN(pmx_gated_nn)(const void* a, const void* b, int64_t M, int64_t N, int64_t K, void* c, pmx_stream_t stream) {
+  if (!fits_rsrc(K, N) || !fits_rsrc(kBM, K)) return PMX_ERR_SHAPE;
+  GemmParams P = dense(a, b, M, N, K, N);
+  P.c0 = static_cast<bf16_t*>(c);
+  return launch_rows<KIND_NN>(P, stream);
+}
+
+int PMX_GEMM_FN(pmx_gated_dgate)(const void* dout, const void* w, const void* gu, int64_t T, int64_t N, int64_t I, float a,
+                                 float b, void* dgu, pmx_stream_t stream) {
+  if (!fits_rsrc(N, I) || !fits_rsrc(kBM, N)) return PMX_ERR_SHAPE;
+  GemmParams P = dense(dout, w, T, I, N, I);
+  P.I = I;
+  P.c0 = static_cast<bf16_t*>(dgu);
+  P.ldc = 2 * I;
+  P.gin = static_cast<const bf16_t*>(gu);
+  P.gate = {a, b};
+  return launch_rows<KIND_NNS>(P, stream);
+}
+
+int PMX_GEMM_FN(pmx_gated_tn)(const void* a, const void* b, int64_t K, int64_t M, int64_t N, int64_t chunk, int32_t splits,
+                              void* c, float* parts, pmx_stream_t stream) {
+  if (!fits_rsrc(BK, M) || !fits_rsrc(BK, N)) return PMX_ERR_SHAPE;
+  const int grid = grid_size();
+  if (grid <= 0) return PMX_ERR_HIP;
+  GemmParams P = {};
+  P.a = one(a, 0, M);
+  P.b = one(b, 0, N);
+  P.G = splits, P.chunk = (uint32_t)chunk, P.rows = (uint32_t)K;
+  P.K = K, P.M = M, P.N = N;
+  P.c0 = P.c1 = static_cast<bf16_t*>(c);
+  P.parts = splits > 1 ? parts : nullptr;
+  P.cgs = splits > 1 ? M * N : 0;
+  P.ldc = N;
+  P.csplit = INT64_MAX;
+  const int64_t tiles = ((M + fr::kWgT - 1) / fr::kWgT) * ((N + fr::kWgT - 1) / fr::kWgT);
+  const int64_t blocks = (tiles + kNumXcd - 1) / kNumXcd * kNumXcd;
+  if (K <= kFewRowsWgrad && splits == 1 && blocks < (int64_t)1 << 30) {  // 128 x 128 tiles, four blocks per CU
+    fr::few_rows_wgrad_grouped_gemm_kernel<<<(unsigned)blocks, fr::kWgNT, 0, stream>>>(P);
+    PMX_LAUNCH_CHECK();
+    return PMX_OK;
+  }
+  // the four-wave kernel: every row of the operands, and the gradient, within 31-bit offsets
+  if (fits_rsrc(K, M) && fits_rsrc(K, N) && fits_rsrc(2 * M, N)) {
+    w4::grouped_gemm_w4_kernel<KIND_TN><<<grid, w4::NT, 0, stream>>>(P);
+  } else if (splits > 1) {
+    return PMX_ERR_SHAPE;
+  } else {
+    grouped_gemm_kernel<KIND_TN, kBM><<<grid, NTHREADS, 0, stream>>>(P);
+  }
+  PMX_LAUNCH_CHECK();
+  return PMX_OK;
+}

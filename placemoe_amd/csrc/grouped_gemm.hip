@@ -50,6 +50,17 @@
 #define PMX_GEMM_FN(name) name
 #endif
 
+// With -DPMX_GATED a build of its own for the dense gated block
+// (gated_gemm.h, its entry points): every row is the one block's, or the rows
+// are cut into equal chunks (weight gradients), so that there are no offsets to
+// read; the activation is one of a family, and its results are rounded once.
+#ifdef PMX_GATED
+#include "gate.h"
+constexpr bool kGated = true;
+#else
+constexpr bool kGated = false;
+#endif
+
 namespace {
 
 #ifdef PMX_ELT_F16
@@ -141,7 +152,23 @@ struct GemmParams {
   const int32_t* row_tok;
   const bf16_t* row_w;
   bf16_t* cout;
+#ifdef PMX_GATED
+  Gate gate;      // KIND_FC1 (gu null: not wanted) and KIND_NNS
+  uint32_t chunk;  // rows of a group (the last one: what is left)
+  uint32_t rows;   // in all, below 2^31
+  float* parts;   // KIND_TN: each group's fp32 sums, cgs elements apart, in the place of c0
+#endif
 };
+
+// First row of group g; of g = G: the rows' end.
+__device__ __forceinline__ int32_t group_row(const GemmParams& P, int64_t g) {
+#ifdef PMX_GATED
+  const uint32_t r = (uint32_t)g * P.chunk;  // below rows + chunk (32 bits: uniform values stay scalar)
+  return (int32_t)(r < P.rows ? r : P.rows);
+#else
+  return P.offsets[g];
+#endif
+}
 
 template <int KIND>
 constexpr bool a_is_mn() { return KIND == KIND_TN; }
@@ -518,6 +545,31 @@ __device__ __forceinline__ uint4 win_load(const OutWin& w, uint32_t voff, uint32
   return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(w.r, voff + row * w.rowb, 0, kCpolNT));
 }
 
+// Two gate values -> their activations, with the rounding points of the
+// reference's expert layer (the sums g and u, then silu(g)); the gated block
+// rounds the product alone.
+__device__ __forceinline__ void activate2([[maybe_unused]] const GemmParams& P, float* g, float* u) {
+#ifdef PMX_GATED
+  g[0] = P.gate.value(g[0]), g[1] = P.gate.value(g[1]);
+#else
+  Elt::round2(g[0], g[1]);
+  Elt::round2(u[0], u[1]);
+  g[0] = silu_f32(g[0]), g[1] = silu_f32(g[1]);
+  Elt::round2(g[0], g[1]);
+#endif
+}
+
+// Gradients of eight gate and up values from the activations' (rounded to 16 bits, as the staged tile holds them).
+__device__ __forceinline__ void activate_bwd8([[maybe_unused]] const GemmParams& P, const float* d, const float* g, const float* u,
+                                              float* dg, float* du) {
+#ifdef PMX_GATED
+#pragma unroll
+  for (int q = 0; q < 8; ++q) P.gate.gradients(d[q], g[q], u[q], dg[q], du[q]);
+#else
+  swiglu_bwd8<Elt>(d, g, u, dg, du);
+#endif
+}
+
 // Eight values of a row times the row's weight, rounded: the fc2 input of the
 // non-EP arithmetic from the staged (already rounded) activations.
 __device__ __forceinline__ uint4 weighted8(const uint4& v, float w) {
@@ -580,9 +632,9 @@ __device__ __forceinline__ void epilogue(const GemmParams& P, const TileInfo& ti
       const int64_t j0 = (int64_t)ti.ntile * 128 + wn * 32;
       float rw[4];  // the act stores' rows, loaded before the first store
       if (P.row_w != nullptr) row_weights(P, ti.row0 + rb, ti.row_end, lane >> 2, 16, rw);
-      stage_half<2>(stage, wave, lane, half, [&](int mt, int nt, int i) { return acc4(acc[mt][nt], i); });
       const int cc = lane & 7;
-      {
+      if (!kGated || P.gu != nullptr) {
+        stage_half<2>(stage, wave, lane, half, [&](int mt, int nt, int i) { return acc4(acc[mt][nt], i); });
         const OutWin w = out_window(P.gu, ti.row0 + rb, ti.row_end, 2 * I);
         const int64_t j = j0 + (cc & 3) * 8;
         const uint32_t voff = j < I ? (uint32_t)(lane >> 3) * w.rowb + (uint32_t)((cc < 4 ? 0 : I) + j) * 2u : kOOB;
@@ -595,10 +647,7 @@ __device__ __forceinline__ void epilogue(const GemmParams& P, const TileInfo& ti
         for (int k = 0; k < 4; k += 2) {
           g[k] = acc[mt][0][i + k], g[k + 1] = acc[mt][0][i + k + 1];
           u[k] = acc[mt][1][i + k], u[k + 1] = acc[mt][1][i + k + 1];
-          Elt::round2(g[k], g[k + 1]);
-          Elt::round2(u[k], u[k + 1]);
-          g[k] = silu_f32(g[k]), g[k + 1] = silu_f32(g[k + 1]);
-          Elt::round2(g[k], g[k + 1]);
+          activate2(P, g + k, u + k);
         }
         return pack4(g[0] * u[0], g[1] * u[1], g[2] * u[2], g[3] * u[3]);
       });
@@ -641,7 +690,7 @@ __device__ __forceinline__ void epilogue(const GemmParams& P, const TileInfo& ti
         unpack8e<Elt>(v, d);
         unpack8e<Elt>(gv[q], g);
         unpack8e<Elt>(uv[q], u);
-        swiglu_bwd8<Elt>(d, g, u, dg, du);
+        activate_bwd8(P, d, g, u, dg, du);
         win_store(wo, vg, q * 8, pack8e<Elt>(dg));
         win_store(wo, vu, q * 8, pack8e<Elt>(du));
       }
@@ -896,8 +945,8 @@ __device__ __forceinline__ TileInfo decode_tile(const GemmParams& P, int64_t til
     band_order<band_height<KIND>()>(local, tiles_per_group / ntn, ntn, m, n);
     ti.g = (int32_t)g;
     ti.mtile = (int32_t)m;
-    ti.row0 = P.offsets[g];
-    ti.row_end = P.offsets[g + 1];
+    ti.row0 = group_row(P, g);
+    ti.row_end = group_row(P, g + 1);
     ti.nk = (int32_t)(((int64_t)ti.row_end - ti.row0 + BK - 1) / BK);
   } else {
     band_order<band_height<KIND>()>(tile, tpre[G], ntn, m, n);
@@ -910,8 +959,8 @@ __device__ __forceinline__ TileInfo decode_tile(const GemmParams& P, int64_t til
     }
     ti.g = lo;
     ti.mtile = (int32_t)m - rd(tpre[lo]);
-    ti.row0 = P.offsets[lo] + ti.mtile * BM;
-    ti.row_end = P.offsets[lo + 1];
+    ti.row0 = group_row(P, lo) + ti.mtile * BM;
+    ti.row_end = group_row(P, lo + 1);
     ti.nk = (int32_t)((P.K + BK - 1) / BK);
   }
   ti.ntile = (int32_t)n;
@@ -956,7 +1005,7 @@ __device__ __noinline__ int32_t build_wgrad_order(const GemmParams& P, int32_t* 
                                                   int64_t total, int64_t tiles_per_group, int32_t xcd,
                                                   int32_t* costs, int32_t cost_slots) {
   const int G = P.G;
-  if (t < G) nk[t] = (int32_t)(((int64_t)P.offsets[t + 1] - P.offsets[t] + BK - 1) / BK);
+  if (t < G) nk[t] = (int32_t)(((int64_t)group_row(P, t + 1) - group_row(P, t) + BK - 1) / BK);
   __syncthreads();
   if (t < G) {
     const int32_t mine = nk[t];
@@ -1013,7 +1062,7 @@ __device__ __forceinline__ void group_prefix(const GemmParams& P, int32_t* tpre,
   for (int i = 0; i < GPT; ++i) {
     const int g = t * GPT + i;
     int32_t v = 0;
-    if (g < G) v = (P.offsets[g + 1] - P.offsets[g] + BM - 1) / BM;
+    if (g < G) v = (group_row(P, g + 1) - group_row(P, g) + BM - 1) / BM;
     loc[i] = sum;
     sum += v;
   }
@@ -1725,9 +1774,9 @@ __device__ __forceinline__ void epilogue(const GemmParams& P, const TileInfo& ti
       // [gate 64 | up 64] (gu), then act = bf16(bf16(silu(gate)) * up).
       const int64_t I = P.I;
       const int64_t jb = (int64_t)ti.ntile * 128 + wn * 64;
-      stage_round<FN>(stage, wave, lane, round, [&](int mt, int nt) { return bf16x4(acc[mt][nt]); },
-                      [](int nt) { return ((nt & 2) ? 4 : 0) + (nt >> 2) * 2 + (nt & 1); });
-      {
+      if (!kGated || P.gu != nullptr) {
+        stage_round<FN>(stage, wave, lane, round, [&](int mt, int nt) { return bf16x4(acc[mt][nt]); },
+                        [](int nt) { return ((nt & 2) ? 4 : 0) + (nt >> 2) * 2 + (nt & 1); });
         const OutWin w = out_window(P.gu, ti.row0 + rb, ti.row_end, 2 * I);
         const int64_t j = jb + (cc & 7) * 8;
         const uint32_t voff = j < I ? (uint32_t)rq * w.rowb + (uint32_t)((cc < 8 ? 0 : I) + j) * 2u : kOOB;
@@ -1744,10 +1793,7 @@ __device__ __forceinline__ void epilogue(const GemmParams& P, const TileInfo& ti
         for (int e = 0; e < 4; e += 2) {
           g[e] = acc[mt][ng][e], g[e + 1] = acc[mt][ng][e + 1];
           u[e] = acc[mt][ng + 2][e], u[e + 1] = acc[mt][ng + 2][e + 1];
-          Elt::round2(g[e], g[e + 1]);
-          Elt::round2(u[e], u[e + 1]);
-          g[e] = silu_f32(g[e]), g[e + 1] = silu_f32(g[e + 1]);
-          Elt::round2(g[e], g[e + 1]);
+          activate2(P, g + e, u + e);
         }
         return pack4(g[0] * u[0], g[1] * u[1], g[2] * u[2], g[3] * u[3]);
       }, [](int k) { return k; });
@@ -1802,13 +1848,31 @@ __device__ __forceinline__ void epilogue(const GemmParams& P, const TileInfo& ti
           unpack8e<Elt>(v, d);
           unpack8e<Elt>(nns_g[qq & 1][q], g);
           unpack8e<Elt>(nns_u[qq & 1][q], u);
-          swiglu_bwd8<Elt>(d, g, u, dg, du);
+          activate_bwd8(P, d, g, u, dg, du);
           win_store(wo, vg, r, pack8e<Elt>(dg));
           win_store(wo, vu, r, pack8e<Elt>(du));
         }
         __builtin_amdgcn_sched_barrier(0);
       }
     } else if constexpr (KIND == KIND_TN) {
+#ifdef PMX_GATED
+      if (P.parts != nullptr) {
+        // a chunk's fp32 sums, straight from the registers: lane l has row l%16, columns 4 (l/16) .. + 3 of a 16 x 16 tile
+        const __amdgpu_buffer_rsrc_t out = make_rsrc(P.parts + ti.g * P.cgs, (uint64_t)P.M * P.N * 4);
+#pragma unroll
+        for (int mt = round * (FM / 2); mt < (round + 1) * (FM / 2); ++mt) {
+#pragma unroll
+          for (int nt = 0; nt < FN; ++nt) {
+            const int64_t m = (int64_t)ti.mtile * BM + wm * 128 + mt * 16 + (lane & 15);
+            const int64_t col = (int64_t)ti.ntile * BN + wn * 128 + nt * 16 + (lane >> 4) * 4;
+            const uint32_t at = m < P.M && col < P.N ? (uint32_t)(m * P.N + col) * 4u : kOOB;
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, acc[mt][nt]), out, at, 0, 0);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        continue;
+      }
+#endif
       // Rows m of copy g's gradient: those below csplit in c0, the rest in
       // c1 (split fc1), each tensor through a descriptor over the copy's rows
       // in it (the host sends a copy of more than 2 GiB to the 8-wave kernel).
@@ -2287,6 +2351,14 @@ RowSrc one(const void* p, int64_t gs, int64_t ld) {
   return s;
 }
 
+#ifdef PMX_GATED
+
+}  // namespace
+
+#include "gated_gemm.h"
+
+#else
+
 // fc1 + SwiGLU; row_w (or null): each row's act times its router weight.
 int fc1_swiglu(const void* X, const void* w_gate, const void* w_up, int64_t w_copy_stride, const int32_t* offsets,
                int32_t G, int64_t A, int64_t H, int64_t I, const void* row_w, void* gu, void* act,
@@ -2459,3 +2531,5 @@ int PMX_GEMM_FN(pmx_group_gemm_tn)(const void* A, const void* B, const int32_t* 
 }
 
 }  // extern "C"
+
+#endif  // PMX_GATED

@@ -1,0 +1,97 @@
+"""The dense gated block: what every token passes beside the routed experts
+(a model's shared experts) or in their place (its dense layers).
+
+``gated_ffn`` is differentiable in the tokens and both weights; a handful of
+tokens (serving) run on kernels of their own.  Kernels are enqueued on the
+current stream of the tensors' device and waited for by nobody.  Wrong devices,
+dtypes and shapes raise ``AssertionError``, limits of the kernels
+``ValueError``, both before anything is launched; there is no CPU fallback.
+"""
+
+from __future__ import annotations
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _capi
+from .kernels import _check_dev, _half, _ptr
+from .rows8 import _launch
+
+GATES = {"silu": 0, "gelu_tanh": 1, "quick_gelu": 2}
+
+
+def _forward(x: torch.Tensor, gate_up: torch.Tensor, down: torch.Tensor, gate: int, keep: bool):
+    """(out, gu or None, act)."""
+    T, H = x.shape
+    N, I = down.shape
+    act, out = x.new_empty((T, I)), x.new_empty((T, N))
+    gu = x.new_empty((T, 2 * I)) if keep else None
+    _launch("pmx_gated_ffn_fwd", x.dtype, x.device, _ptr(x), _ptr(gate_up), _ptr(down), T, H, I, N, gate, _ptr(gu), _ptr(act),
+            _ptr(out))
+    return out, gu, act
+
+
+class _GatedFFN(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, gate_up, down, gate):
+        need_x, need_up, need_down = ctx.needs_input_grad[:3]
+        out, gu, act = _forward(x, gate_up, down, gate, need_x or need_up)
+        ctx.gate = gate
+        # what the wanted gradients read
+        ctx.save_for_backward(x if need_up else None, gate_up if need_x else None, down if need_x or need_up else None, gu,
+                              act if need_down else None)
+        ctx.sizes = (*x.shape, down.shape[1])
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_out):
+        x, gate_up, down, gu, act = ctx.saved_tensors
+        T, H, I = ctx.sizes
+        N = grad_out.shape[1]
+        grad_out = grad_out.contiguous()
+        dx, dup, ddown = (grad_out.new_empty(shape) if need else None
+                          for shape, need in zip(((T, H), (2 * I, H), (N, I)), ctx.needs_input_grad))
+        if T == 0:
+            for d in (dup, ddown):
+                if d is not None:
+                    d.zero_()
+            return dx, dup, ddown, None
+        ws_bytes = _capi.load().pmx_gated_ffn_workspace_bytes(T, H, I, N)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=grad_out.device)
+        _launch("pmx_gated_ffn_bwd", grad_out.dtype, grad_out.device, _ptr(grad_out), _ptr(x), _ptr(gate_up), _ptr(down), _ptr(gu),
+                _ptr(act), T, H, I, N, ctx.gate, _ptr(dx), _ptr(dup), _ptr(ddown), _ptr(ws), ws_bytes)
+        return dx, dup, ddown, None
+
+
+def gated_ffn(x: torch.Tensor, gate_up: torch.Tensor, down: torch.Tensor, activation: str = "silu") -> torch.Tensor:
+    """out = (gate(x @ Wg^T) * (x @ Wu^T)) @ down^T, [..., H] -> [..., N].
+
+    x [..., H], gate_up [2I, H] (the rows of Wg, then those of Wu) and down
+    [N, I], all bfloat16 or all float16, contiguous; H, I and N multiples of 8.
+    ``activation``: "silu", "gelu_tanh" (GELU's tanh form) or "quick_gelu"
+    (g sigmoid(1.702 g)).
+
+    Sums are held in fp32.  The block's inner values (gate, up, their product
+    and its gradients) are rounded to the tensors' dtype where a product reads
+    them or the backward keeps them.  For the backward x, gate and up rows
+    [tokens, 2I] and their products [tokens, I] are kept, as far as the
+    gradients that are wanted read them.
+    """
+    if activation not in GATES:
+        raise ValueError(f"activation must be one of {sorted(GATES)}, got {activation!r}")
+    _check_dev(x, gate_up, down)
+    dt = _half("x", x)
+    _half("gate_up", gate_up, dt)
+    _half("down", down, dt)
+    assert gate_up.dim() == 2 and down.dim() == 2, "gate_up and down must be matrices"
+    N, I = down.shape
+    H = gate_up.shape[1]
+    assert gate_up.shape[0] == 2 * I, f"gate_up must have {2 * I} rows, twice the columns of down, got {gate_up.shape[0]}"
+    assert x.dim() >= 1 and x.shape[-1] == H, f"x must be [..., {H}], got {tuple(x.shape)}"
+    rows = x.reshape(-1, H) if x.dim() != 2 else x
+    if torch.is_grad_enabled() and (x.requires_grad or gate_up.requires_grad or down.requires_grad):
+        out = _GatedFFN.apply(rows, gate_up, down, GATES[activation])
+    else:
+        out = _forward(rows, gate_up, down, GATES[activation], False)[0]
+    return out if x.dim() == 2 else out.view(*x.shape[:-1], N)
