@@ -624,24 +624,24 @@ int pmx_rows4_layer(const void* hidden, const void* w, const int64_t* sel, const
  *   gate(g) = g sigmoid(g)                       PMX_GATE_SILU
  *             g (1 + tanh(sqrt(2/pi) (g + 0.044715 g^3))) / 2   PMX_GATE_GELU_TANH
  *             g sigmoid(1.702 g)                 PMX_GATE_QUICK_GELU
- * fp32 sums; g, u and act are rounded to bf16 where they are kept, act once as
- * fc2's operand, whatever gu is.  Any other gate: PMX_ERR_ARG.  H, I and N
+ * fp32 sums; act is rounded to bf16, fc2's operand.  Any other gate: PMX_ERR_ARG.  H, I and N
  * multiples of 8, tensors contiguous and 16-byte aligned, each weight matrix and 256 rows of each
  * operand below 2 GiB, else PMX_ERR_SHAPE.  T = 0: nothing is written. */
 #define PMX_GATE_SILU 0
 #define PMX_GATE_GELU_TANH 1
 #define PMX_GATE_QUICK_GELU 2
 
-/* gu [T, 2I] (NULL: not kept) and act [T, I] are what the backward reads. */
+/* gates (NULL: not kept) and act [T, I] bf16 are what the backward reads: gates
+ * fp32 [T, I / 4, 2, 4], g of four neighbouring columns, then their u. */
 int pmx_gated_ffn_fwd(const void* x, const void* gate_up, const void* down, int64_t T, int64_t H, int64_t I,
-                      int64_t N, int32_t gate, void* gu, void* act, void* out, pmx_stream_t stream);
+                      int64_t N, int32_t gate, float* gates, void* act, void* out, pmx_stream_t stream);
 
 /* Gradients of x, W and Wd from dout [T, N], each NULL where it is not wanted
  * (and what only it reads may then be NULL: dx gate_up; dgate_up x; ddown act;
- * the first two down and gu).  dout Wd and the gradients of g and u are rounded to
- * bf16 on their way.  workspace: 16-byte aligned, one call's at a time. */
+ * the first two down and gates).  The gradients of g and u are rounded to bf16 on
+ * their way.  workspace: 16-byte aligned, one call's at a time. */
 size_t pmx_gated_ffn_workspace_bytes(int64_t T, int64_t H, int64_t I, int64_t N);
-int pmx_gated_ffn_bwd(const void* dout, const void* x, const void* gate_up, const void* down, const void* gu,
+int pmx_gated_ffn_bwd(const void* dout, const void* x, const void* gate_up, const void* down, const float* gates,
                       const void* act, int64_t T, int64_t H, int64_t I, int64_t N, int32_t gate, void* dx,
                       void* dgate_up, void* ddown, void* workspace, size_t workspace_bytes, pmx_stream_t stream);
 
@@ -756,8 +756,8 @@ int pmx_rows4_layer_f16(const void* hidden, const void* w, const int64_t* sel, c
                         size_t workspace_bytes, int32_t* status_host, pmx_stream_t stream);
 
 int pmx_gated_ffn_fwd_f16(const void* x, const void* gate_up, const void* down, int64_t T, int64_t H, int64_t I,
-                          int64_t N, int32_t gate, void* gu, void* act, void* out, pmx_stream_t stream);
-int pmx_gated_ffn_bwd_f16(const void* dout, const void* x, const void* gate_up, const void* down, const void* gu,
+                          int64_t N, int32_t gate, float* gates, void* act, void* out, pmx_stream_t stream);
+int pmx_gated_ffn_bwd_f16(const void* dout, const void* x, const void* gate_up, const void* down, const float* gates,
                           const void* act, int64_t T, int64_t H, int64_t I, int64_t N, int32_t gate, void* dx,
                           void* dgate_up, void* ddown, void* workspace, size_t workspace_bytes,
                           pmx_stream_t stream);

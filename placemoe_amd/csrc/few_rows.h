@@ -173,10 +173,15 @@ __device__ __forceinline__ void epilogue(const GemmParams& P, const TileInfo& ti
         const int64_t j = (int64_t)ti.ntile * (CF::BN / 2) + (wn * CF::FN + nt) * 8 + c4;
         if (j >= I) continue;
         const f32x4_t g4 = acc[mt][nt], u4 = acc[mt][nt + 1];
-        if (!kGated || P.gu != nullptr) {
-          st4(P.gu + r * 2 * I + j, pack4(g4[0], g4[1], g4[2], g4[3]));
-          st4(P.gu + r * 2 * I + I + j, pack4(u4[0], u4[1], u4[2], u4[3]));
+#ifdef PMX_GATED
+        if (P.gates != nullptr) {
+          f32x4_t* const to = reinterpret_cast<f32x4_t*>(P.gates + (r * I + j) * 2);
+          to[0] = g4, to[1] = u4;
         }
+#else
+        st4(P.gu + r * 2 * I + j, pack4(g4[0], g4[1], g4[2], g4[3]));
+        st4(P.gu + r * 2 * I + I + j, pack4(u4[0], u4[1], u4[2], u4[3]));
+#endif
         float g[4], u[4];
 #pragma unroll
         for (int e = 0; e < 4; e += 2) {
@@ -201,6 +206,19 @@ __device__ __forceinline__ void epilogue(const GemmParams& P, const TileInfo& ti
         const int64_t ja = (int64_t)ti.ntile * CF::BN + (wn * CF::FN + nt) * 16 + c4, jb = ja + 16;
         // columns past I: read column ja's place again, write nothing
         const bool ina = ja < I, inb = jb < I;
+#ifdef PMX_GATED
+        const f32x4_t* const from = reinterpret_cast<const f32x4_t*>(P.gates + r * 2 * I);
+        const int64_t at = ina ? ja / 2 : 0, bt = inb ? jb / 2 : 0;  // four floats each
+        const f32x4_t g[2] = {from[at], from[bt]}, u[2] = {from[at + 1], from[bt + 1]};
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          float dg[4], du[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) P.gate.gradients(acc[mt][nt + k][e], g[k][e], u[k][e], dg[e], du[e]);
+          bf16_t* const o = P.c0 + r * 2 * I + (k ? jb : ja);
+          if (k ? inb : ina) st4(o, pack4(dg[0], dg[1], dg[2], dg[3])), st4(o + I, pack4(du[0], du[1], du[2], du[3]));
+        }
+#else
         const bf16_t* gr = P.gin + r * 2 * I;
         const int64_t la = ina ? ja : 0, lb = inb ? jb : 0;
         const uint2 ga = ld4(gr + la), gb = ld4(gr + lb), ua = ld4(gr + I + la), ub = ld4(gr + I + lb);
@@ -209,11 +227,12 @@ __device__ __forceinline__ void epilogue(const GemmParams& P, const TileInfo& ti
         unpack8e<Elt>(make_uint4(da.x, da.y, db.x, db.y), d);
         unpack8e<Elt>(make_uint4(ga.x, ga.y, gb.x, gb.y), g);
         unpack8e<Elt>(make_uint4(ua.x, ua.y, ub.x, ub.y), u);
-        activate_bwd8(P, d, g, u, dg, du);
+        swiglu_bwd8<Elt>(d, g, u, dg, du);
         const uint4 pg = pack8e<Elt>(dg), pu = pack8e<Elt>(du);
         bf16_t* o = P.c0 + r * 2 * I;
         if (ina) st4(o + ja, make_uint2(pg.x, pg.y)), st4(o + I + ja, make_uint2(pu.x, pu.y));
         if (inb) st4(o + jb, make_uint2(pg.z, pg.w)), st4(o + I + jb, make_uint2(pu.z, pu.w));
+#endif
       }
     } else {
       const bool mapped = P.row_tok != nullptr;

@@ -6,9 +6,9 @@
 // The block's products on the grouped GEMM's kernels (a build of
 // grouped_gemm.hip of their own; _f16: fp16 tensors).  Checked by the caller.
 #define PMX_GATED_GEMMS(SUFFIX)                                                                                              \
-  /* act [T, I] (and, unless null, gu [T, 2I]) of x [T, H], w [2I, H] */                                                     \
+  /* act [T, I] (and, unless null, gates [T, I / 4, 2, 4] in fp32) of x [T, H], w [2I, H] */                                 \
   __attribute__((visibility("hidden"))) int pmx_gated_fc1##SUFFIX(const void* x, const void* w, int64_t T, int64_t H,        \
-                                                                  int64_t I, float a, float b, void* gu, void* act,          \
+                                                                  int64_t I, float a, float b, float* gates, void* act,      \
                                                                   pmx_stream_t stream);                                      \
   /* c [M, N] = a [M, K] b [N, K]^T */                                                                                       \
   __attribute__((visibility("hidden"))) int pmx_gated_nt##SUFFIX(const void* a, const void* b, int64_t M, int64_t N,         \
@@ -16,8 +16,8 @@
   /* c [M, N] = a [M, K] b [K, N] */                                                                                         \
   __attribute__((visibility("hidden"))) int pmx_gated_nn##SUFFIX(const void* a, const void* b, int64_t M, int64_t N,         \
                                                                  int64_t K, void* c, pmx_stream_t stream);                   \
-  /* dgu [T, 2I] from dout [T, N], w [N, I] and gu */                                                                        \
-  __attribute__((visibility("hidden"))) int pmx_gated_dgate##SUFFIX(const void* dout, const void* w, const void* gu,         \
+  /* dgu [T, 2I] from dout [T, N], w [N, I] and gates */                                                                     \
+  __attribute__((visibility("hidden"))) int pmx_gated_dgate##SUFFIX(const void* dout, const void* w, const float* gates,     \
                                                                     int64_t T, int64_t N, int64_t I, float a, float b,       \
                                                                     void* dgu, pmx_stream_t stream);                         \
   /* c [M, N] = a [K, M]^T b [K, N]; with splits > 1 the K rows in chunks of `chunk`, each one's fp32 sums in parts */       \

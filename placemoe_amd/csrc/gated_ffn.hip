@@ -3,14 +3,17 @@
 //
 // Many tokens: the grouped GEMM's kernels, built for one group that is the whole
 // call (gated_gemm.h):
-//   forward   gu, act = fc1 (both projections, gate and product in its epilogue);  out = act Wd^T
+//   forward   act = fc1 (both projections, gate and product in its epilogue);  out = act Wd^T
 //   backward  dgu = the gate's gradients of (dout Wd), in its epilogue;  dWd = dout^T act;
 //             dW = dgu^T x;  dx = dgu W
-// gu, act and dgu are held in 16 bits, as are the sums dout Wd on their way
-// through the epilogue: each is an operand of a 16-bit product or, dout Wd, a
-// tile that passes through LDS as such.  (Each such rounding is the outputs' own,
-// 2^-9 of a value; the outputs are 1.0 to 1.7 times as far from the definition in
-// 64 bits as results rounded once are.)  A weight gradient's tiles are few where
+// act and dgu are rounded to 16 bits, being operands of 16-bit products: each
+// such rounding is as large as the outputs' own, so that every output is 1.4 times as
+// far from the definition in 64 bits as one rounded once is.  The gate and up
+// sums between the forward and the backward are kept in fp32: in 16 bits, as dout Wd
+// staged in 16, they made dx and dW twice as far (0.0034, rounded once 0.0017, now 0.0023, in bf16).  As the
+// accumulators hold them they go to memory and back without a turn through LDS: 8192
+// tokens of 7168 x 2048, forward and backward, 1883 -> 1777 us.
+// A weight gradient's tiles are few where
 // the weights are small: its rows are cut into chunks whose fp32 sums are then
 // added in order (sum_parts_kernel).
 //
@@ -68,11 +71,11 @@ __device__ __forceinline__ void few_products(const bf16_t* wrow, const bf16_t* x
   __syncthreads();
 }
 
-// fc1: eight columns of act (gu) per block.
+// fc1: eight columns of act (and gates) per block.
 template <class E>
 __global__ __launch_bounds__(64 * kFewWaves) void gated_few_fc1_kernel(const bf16_t* __restrict__ x, const bf16_t* __restrict__ w,
                                                                        int64_t T, int64_t H, int64_t I, Gate gate,
-                                                                       bf16_t* __restrict__ gu, bf16_t* __restrict__ act) {
+                                                                       float* __restrict__ gates, bf16_t* __restrict__ act) {
   __shared__ float red[kFewWaves][16][16];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t j0 = (int64_t)blockIdx.x * 8;
@@ -84,9 +87,9 @@ __global__ __launch_bounds__(64 * kFewWaves) void gated_few_fc1_kernel(const bf1
   float g = 0.f, u = 0.f;
 #pragma unroll
   for (int i = 0; i < kFewWaves; ++i) g += red[i][j][t], u += red[i][8 + j][t];
-  if (gu != nullptr) {
-    gu[t * 2 * I + j0 + j] = (bf16_t)E::from_f32(g);
-    gu[t * 2 * I + I + j0 + j] = (bf16_t)E::from_f32(u);
+  if (gates != nullptr) {  // four columns' gates, then their ups
+    float* const to = gates + (t * I + j0 + (j & 4)) * 2 + (j & 3);
+    to[0] = g, to[4] = u;
   }
   act[t * I + j0 + j] = (bf16_t)E::from_f32(gate.value(g) * u);
 }
@@ -140,7 +143,7 @@ int check(int64_t T, int64_t H, int64_t I, int64_t N) {
   if (T < 0 || H <= 0 || I <= 0 || N <= 0) return PMX_ERR_ARG;
   if (H % 8 || I % 8 || N % 8 || T > INT32_MAX - 256 || I > INT32_MAX / 2) return PMX_ERR_SHAPE;
   const int64_t I2 = 2 * I;
-  // whole weights through one descriptor, 256 rows of every operand, and as many gu rows
+  // whole weights through one descriptor, 256 rows of every operand
   if (!one_window(I2, H) || !one_window(N, I) || !one_window(256, I2) || !one_window(256, H) || !one_window(256, N)) return PMX_ERR_SHAPE;
   return PMX_OK;
 }
@@ -188,16 +191,16 @@ struct Gemms<EltF16> {
 
 template <class E>
 int forward_t(const void* x, const void* gate_up, const void* down, int64_t T, int64_t H, int64_t I, int64_t N, int32_t kind,
-              void* gu, void* act, void* out, pmx_stream_t stream) {
+              float* gates, void* act, void* out, pmx_stream_t stream) {
   Gate gate;
   if (!gate_of(kind, gate)) return PMX_ERR_ARG;
   if (const int rc = check(T, H, I, N)) return rc;
   if (T == 0) return PMX_OK;
   if (!x || !gate_up || !down || !act || !out) return PMX_ERR_ARG;
-  if (!aligned16(x) || !aligned16(gate_up) || !aligned16(down) || !aligned16(gu) || !aligned16(act) || !aligned16(out)) return PMX_ERR_SHAPE;
+  if (!aligned16(x) || !aligned16(gate_up) || !aligned16(down) || !aligned16(gates) || !aligned16(act) || !aligned16(out)) return PMX_ERR_SHAPE;
   if (T <= pmx::kGatedFewTokens) {
     gated_few_fc1_kernel<E><<<(unsigned)(I / 8), 64 * kFewWaves, 0, stream>>>((const bf16_t*)x, (const bf16_t*)gate_up, T, H, I, gate,
-                                                                              (bf16_t*)gu, (bf16_t*)act);
+                                                                              gates, (bf16_t*)act);
     PMX_LAUNCH_CHECK();
     gated_few_fc2_kernel<E><<<(unsigned)((N + 15) / 16), 64 * kFewWaves, 0, stream>>>((const bf16_t*)act, (const bf16_t*)down, T, N, I,
                                                                                       (bf16_t*)out);
@@ -205,7 +208,7 @@ int forward_t(const void* x, const void* gate_up, const void* down, int64_t T, i
     return PMX_OK;
   }
   // The sizes have been checked: what fails from here on is a launch.
-  if (Gemms<E>::fc1(x, gate_up, T, H, I, gate.a, gate.b, gu, act, stream) != PMX_OK) return PMX_ERR_HIP;
+  if (Gemms<E>::fc1(x, gate_up, T, H, I, gate.a, gate.b, gates, act, stream) != PMX_OK) return PMX_ERR_HIP;
   return Gemms<E>::nt(act, down, T, N, I, out, stream) != PMX_OK ? PMX_ERR_HIP : PMX_OK;
 }
 
@@ -223,7 +226,7 @@ int weight_gradient(const void* a, const void* b, int64_t K, int64_t M, int64_t 
 }
 
 template <class E>
-int backward_t(const void* dout, const void* x, const void* gate_up, const void* down, const void* gu, const void* act, int64_t T,
+int backward_t(const void* dout, const void* x, const void* gate_up, const void* down, const float* gates, const void* act, int64_t T,
                int64_t H, int64_t I, int64_t N, int32_t kind, void* dx, void* dgate_up, void* ddown, void* workspace,
                size_t workspace_bytes, pmx_stream_t stream) {
   Gate gate;
@@ -231,15 +234,15 @@ int backward_t(const void* dout, const void* x, const void* gate_up, const void*
   if (const int rc = check(T, H, I, N)) return rc;
   if (T == 0) return PMX_OK;
   if (!dout || (!dx && !dgate_up && !ddown)) return PMX_ERR_ARG;
-  if (((dx || dgate_up) && (!down || !gu)) || (dgate_up && !x) || (dx && !gate_up) || (ddown && !act)) return PMX_ERR_ARG;
-  const void* all[] = {dout, x, gate_up, down, gu, act, dx, dgate_up, ddown, workspace};
+  if (((dx || dgate_up) && (!down || !gates)) || (dgate_up && !x) || (dx && !gate_up) || (ddown && !act)) return PMX_ERR_ARG;
+  const void* all[] = {dout, x, gate_up, down, gates, act, dx, dgate_up, ddown, workspace};
   for (const void* p : all)
     if (!aligned16(p)) return PMX_ERR_SHAPE;
   if (!workspace || workspace_bytes < pmx_gated_ffn_workspace_bytes(T, H, I, N)) return PMX_ERR_ARG;
   void* dgu = workspace;
   float* parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + dgu_bytes(T, I));
   int rc = PMX_OK;
-  if (dx || dgate_up) rc = Gemms<E>::dgate(dout, down, gu, T, N, I, gate.a, gate.b, dgu, stream);
+  if (dx || dgate_up) rc = Gemms<E>::dgate(dout, down, gates, T, N, I, gate.a, gate.b, dgu, stream);
   if (rc == PMX_OK && ddown) rc = weight_gradient<E>(dout, act, T, N, I, ddown, parts, stream);
   if (rc == PMX_OK && dgate_up) rc = weight_gradient<E>(dgu, x, T, 2 * I, H, dgate_up, parts, stream);
   if (rc == PMX_OK && dx) rc = Gemms<E>::nn(dgu, gate_up, T, H, 2 * I, dx, stream);
@@ -258,14 +261,14 @@ size_t pmx_gated_ffn_workspace_bytes(int64_t T, int64_t H, int64_t I, int64_t N)
 
 #define PMX_GATED_FFN(SUFFIX, E)                                                                                            \
   int pmx_gated_ffn_fwd##SUFFIX(const void* x, const void* gate_up, const void* down, int64_t T, int64_t H, int64_t I,      \
-                                int64_t N, int32_t gate, void* gu, void* act, void* out, pmx_stream_t stream) {             \
-    return forward_t<E>(x, gate_up, down, T, H, I, N, gate, gu, act, out, stream);                                          \
+                                int64_t N, int32_t gate, float* gates, void* act, void* out, pmx_stream_t stream) {         \
+    return forward_t<E>(x, gate_up, down, T, H, I, N, gate, gates, act, out, stream);                                       \
   }                                                                                                                         \
-  int pmx_gated_ffn_bwd##SUFFIX(const void* dout, const void* x, const void* gate_up, const void* down, const void* gu,     \
+  int pmx_gated_ffn_bwd##SUFFIX(const void* dout, const void* x, const void* gate_up, const void* down, const float* gates, \
                                 const void* act, int64_t T, int64_t H, int64_t I, int64_t N, int32_t gate, void* dx,        \
                                 void* dgate_up, void* ddown, void* workspace, size_t workspace_bytes, pmx_stream_t stream) { \
-    return backward_t<E>(dout, x, gate_up, down, gu, act, T, H, I, N, gate, dx, dgate_up, ddown, workspace, workspace_bytes, \
-                         stream);                                                                                           \
+    return backward_t<E>(dout, x, gate_up, down, gates, act, T, H, I, N, gate, dx, dgate_up, ddown, workspace,              \
+                         workspace_bytes, stream);                                                                                           \
   }
 
 PMX_GATED_FFN(, EltBF16)

@@ -43,14 +43,14 @@ GemmParams dense(const void* a, const void* b, int64_t M, int64_t N, int64_t K, 
 
 }  // namespace
 
-int PMX_GEMM_FN(pmx_gated_fc1)(const void* x, const void* w, int64_t T, int64_t H, int64_t I, float a, float b, void* gu,
+int PMX_GEMM_FN(pmx_gated_fc1)(const void* x, const void* w, int64_t T, int64_t H, int64_t I, float a, float b, float* gates,
                                void* act, pmx_stream_t stream) {
   if (!fits_rsrc(I, H) || !fits_rsrc(kBM, H)) return PMX_ERR_SHAPE;
   GemmParams P = dense(x, w, T, 2 * I, H, H);
   P.b.p1 = P.b.p0 + I * H;
   P.b.split = I;
   P.I = I;
-  P.gu = static_cast<bf16_t*>(gu);
+  P.gates = gates;
   P.act = static_cast<bf16_t*>(act);
   P.gate = {a, b};
   return launch_rows<KIND_FC1>(P, stream);
@@ -70,14 +70,14 @@ int PMX_GEMM_FN(pmx_gated_nn)(const void* a, const void* b, int64_t M, int64_t N
   return launch_rows<KIND_NN>(P, stream);
 }
 
-int PMX_GEMM_FN(pmx_gated_dgate)(const void* dout, const void* w, const void* gu, int64_t T, int64_t N, int64_t I, float a,
+int PMX_GEMM_FN(pmx_gated_dgate)(const void* dout, const void* w, const float* gates, int64_t T, int64_t N, int64_t I, float a,
                                  float b, void* dgu, pmx_stream_t stream) {
   if (!fits_rsrc(N, I) || !fits_rsrc(kBM, N)) return PMX_ERR_SHAPE;
   GemmParams P = dense(dout, w, T, I, N, I);
   P.I = I;
   P.c0 = static_cast<bf16_t*>(dgu);
   P.ldc = 2 * I;
-  P.gin = static_cast<const bf16_t*>(gu);
+  P.gates = const_cast<float*>(gates);
   P.gate = {a, b};
   return launch_rows<KIND_NNS>(P, stream);
 }

@@ -56,9 +56,6 @@
 // read; the activation is one of a family, and its results are rounded once.
 #ifdef PMX_GATED
 #include "gate.h"
-constexpr bool kGated = true;
-#else
-constexpr bool kGated = false;
 #endif
 
 namespace {
@@ -153,7 +150,10 @@ struct GemmParams {
   const bf16_t* row_w;
   bf16_t* cout;
 #ifdef PMX_GATED
-  Gate gate;      // KIND_FC1 (gu null: not wanted) and KIND_NNS
+  Gate gate;      // KIND_FC1 and KIND_NNS
+  // The gate and up sums that KIND_FC1 leaves (null: not wanted) for KIND_NNS, in fp32 [rows, I / 4, 2, 4]: four
+  // neighbouring columns' gates, then their ups, as a lane holds them.
+  float* gates;
   uint32_t chunk;  // rows of a group (the last one: what is left)
   uint32_t rows;   // in all, below 2^31
   float* parts;   // KIND_TN: each group's fp32 sums, cgs elements apart, in the place of c0
@@ -547,7 +547,7 @@ __device__ __forceinline__ uint4 win_load(const OutWin& w, uint32_t voff, uint32
 
 // Two gate values -> their activations, with the rounding points of the
 // reference's expert layer (the sums g and u, then silu(g)); the gated block
-// rounds the product alone.
+// rounds the product with u alone.
 __device__ __forceinline__ void activate2([[maybe_unused]] const GemmParams& P, float* g, float* u) {
 #ifdef PMX_GATED
   g[0] = P.gate.value(g[0]), g[1] = P.gate.value(g[1]);
@@ -559,16 +559,40 @@ __device__ __forceinline__ void activate2([[maybe_unused]] const GemmParams& P, 
 #endif
 }
 
-// Gradients of eight gate and up values from the activations' (rounded to 16 bits, as the staged tile holds them).
-__device__ __forceinline__ void activate_bwd8([[maybe_unused]] const GemmParams& P, const float* d, const float* g, const float* u,
-                                              float* dg, float* du) {
 #ifdef PMX_GATED
-#pragma unroll
-  for (int q = 0; q < 8; ++q) P.gate.gradients(d[q], g[q], u[q], dg[q], du[q]);
-#else
-  swiglu_bwd8<Elt>(d, g, u, dg, du);
-#endif
+// Gate and up sums of rows row0 .. row0+63 (as out_window; not wanted: no rows.  A branch around the stores cost
+// the four-wave kernel 18 spilled registers, this way it has 99 to spare).
+struct GatesWin {
+  __amdgpu_buffer_rsrc_t r;
+  uint32_t rowb;
+  // The lane's four columns from j on, of row `row`; `rows` further on (uniform).
+  __device__ __forceinline__ uint32_t at(int row, int64_t j, int64_t I) const { return j < I ? (uint32_t)row * rowb + (uint32_t)j * 8u : kOOB; }
+  __device__ __forceinline__ void store(uint32_t o, int rows, const f32x4_t& g, const f32x4_t& u) const {
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, g), r, o, (uint32_t)rows * rowb, 0);
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, u), r, o + 16u, (uint32_t)rows * rowb, 0);
+  }
+  __device__ __forceinline__ void load(uint32_t o, int rows, f32x4_t& g, f32x4_t& u) const {
+    g = __builtin_bit_cast(f32x4_t, __builtin_amdgcn_raw_buffer_load_b128(r, o, (uint32_t)rows * rowb, 0));
+    u = __builtin_bit_cast(f32x4_t, __builtin_amdgcn_raw_buffer_load_b128(r, o + 16u, (uint32_t)rows * rowb, 0));
+  }
+};
+__device__ __forceinline__ GatesWin gates_window(const GemmParams& P, int64_t row0, int64_t row_end) {
+  const int64_t rows = row_end - row0 < 0 || P.gates == nullptr ? 0 : (row_end - row0 > 64 ? 64 : row_end - row0);
+  return {make_rsrc(P.gates + row0 * 2 * P.I, (uint64_t)(rows * P.I * 8)), (uint32_t)(P.I * 8)};
 }
+// The gradients of four columns' gate and up values, written to both halves of their row in `w`.
+__device__ __forceinline__ void gradients4(const GemmParams& P, const OutWin& w, int row, int64_t j, int64_t I, const f32x4_t& d,
+                                           const f32x4_t& g, const f32x4_t& u) {
+  float dg[4], du[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) P.gate.gradients(d[e], g[e], u[e], dg[e], du[e]);
+  const uint2 pg = pack4(dg[0], dg[1], dg[2], dg[3]), pu = pack4(du[0], du[1], du[2], du[3]);
+  const uint32_t o = j < I ? (uint32_t)row * w.rowb + (uint32_t)j * 2u : kOOB;
+  typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+  __builtin_amdgcn_raw_buffer_store_b64(u32x2_t{pg.x, pg.y}, w.r, o, 0, 0);
+  __builtin_amdgcn_raw_buffer_store_b64(u32x2_t{pu.x, pu.y}, w.r, o + (uint32_t)I * 2u, 0, 0);
+}
+#endif
 
 // Eight values of a row times the row's weight, rounded: the fc2 input of the
 // non-EP arithmetic from the staged (already rounded) activations.
@@ -632,15 +656,29 @@ __device__ __forceinline__ void epilogue(const GemmParams& P, const TileInfo& ti
       const int64_t j0 = (int64_t)ti.ntile * 128 + wn * 32;
       float rw[4];  // the act stores' rows, loaded before the first store
       if (P.row_w != nullptr) row_weights(P, ti.row0 + rb, ti.row_end, lane >> 2, 16, rw);
+#ifdef PMX_GATED
+      {
+        const GatesWin w = gates_window(P, ti.row0 + rb, ti.row_end);
+#pragma unroll
+        for (int mtl = 0; mtl < 2; ++mtl)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const f32x16_t &g = acc[2 * half + mtl][0], &u = acc[2 * half + mtl][1];
+            w.store(w.at(lane & 31, j0 + 8 * q + 4 * (lane >> 5), I), mtl * 32, f32x4_t{g[4 * q], g[4 * q + 1], g[4 * q + 2], g[4 * q + 3]},
+                    f32x4_t{u[4 * q], u[4 * q + 1], u[4 * q + 2], u[4 * q + 3]});
+          }
+      }
+#else
+      stage_half<2>(stage, wave, lane, half, [&](int mt, int nt, int i) { return acc4(acc[mt][nt], i); });
       const int cc = lane & 7;
-      if (!kGated || P.gu != nullptr) {
-        stage_half<2>(stage, wave, lane, half, [&](int mt, int nt, int i) { return acc4(acc[mt][nt], i); });
+      {
         const OutWin w = out_window(P.gu, ti.row0 + rb, ti.row_end, 2 * I);
         const int64_t j = j0 + (cc & 3) * 8;
         const uint32_t voff = j < I ? (uint32_t)(lane >> 3) * w.rowb + (uint32_t)((cc < 4 ? 0 : I) + j) * 2u : kOOB;
 #pragma unroll
         for (int q = 0; q < 8; ++q) win_store(w, voff, q * 8, staged_chunk(stage, wave, q * 8 + (lane >> 3), cc));
       }
+#endif
       stage_half<1>(stage, wave, lane, half, [&](int mt, int, int i) {
         float g[4], u[4];
 #pragma unroll
@@ -670,6 +708,26 @@ __device__ __forceinline__ void epilogue(const GemmParams& P, const TileInfo& ti
       // that their latency overlaps the staging.
       // gate/up (gin) and [d_gate | d_up] (c0) share one row layout.
       const int64_t I = P.I;
+#ifdef PMX_GATED
+      const GatesWin wi = gates_window(P, ti.row0 + rb, ti.row_end);
+      const OutWin wo = out_window(P.c0, ti.row0 + rb, ti.row_end, 2 * I);
+#pragma unroll
+      for (int mtl = 0; mtl < 2; ++mtl)
+#pragma unroll
+        for (int nt = 0; nt < NTT; ++nt) {
+          const int row = mtl * 32 + (lane & 31);
+          const int64_t j = (int64_t)ti.ntile * BN + wn * WCOLS + nt * 32 + 4 * (lane >> 5);
+          f32x4_t g[4], u[4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) wi.load(wi.at(lane & 31, j + 8 * q, I), mtl * 32, g[q], u[q]);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const f32x16_t& d = acc[2 * half + mtl][nt];
+            gradients4(P, wo, row, j + 8 * q, I, f32x4_t{d[4 * q], d[4 * q + 1], d[4 * q + 2], d[4 * q + 3]}, g[q], u[q]);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+#else
       const int cc = lane & 7;
       const int64_t j = (int64_t)ti.ntile * BN + wn * WCOLS + cc * 8;
       const OutWin wi = out_window(P.gin, ti.row0 + rb, ti.row_end, 2 * I);
@@ -690,10 +748,11 @@ __device__ __forceinline__ void epilogue(const GemmParams& P, const TileInfo& ti
         unpack8e<Elt>(v, d);
         unpack8e<Elt>(gv[q], g);
         unpack8e<Elt>(uv[q], u);
-        activate_bwd8(P, d, g, u, dg, du);
+        swiglu_bwd8<Elt>(d, g, u, dg, du);
         win_store(wo, vg, q * 8, pack8e<Elt>(dg));
         win_store(wo, vu, q * 8, pack8e<Elt>(du));
       }
+#endif
     } else if constexpr (KIND == KIND_TN) {
       stage_half<NTT>(stage, wave, lane, half, [&](int mt, int nt, int i) { return acc4(acc[mt][nt], i); });
       const int cc = lane & 7;  // 16-byte chunk (8 columns) of the wave's 64
@@ -1744,7 +1803,7 @@ __device__ __forceinline__ void epilogue(const GemmParams& P, const TileInfo& ti
   // those of rows l and 64 + l, and a store's lanes fetch theirs with a
   // cross-lane read.  Targets outside [0, M) are not written.
   const bool mapped = (KIND == KIND_NT || KIND == KIND_NN) && P.row_tok != nullptr;
-  uint4 nns_g[KIND == KIND_NNS ? 2 : 1][4], nns_u[KIND == KIND_NNS ? 2 : 1][4];  // KIND_NNS: two quarters of gate/up
+  [[maybe_unused]] uint4 nns_g[KIND == KIND_NNS ? 2 : 1][4], nns_u[KIND == KIND_NNS ? 2 : 1][4];  // KIND_NNS: two quarters of gate/up
   int32_t tok2[2] = {-1, -1};
   uint32_t wt2[2] = {0, 0};
   if constexpr (KIND == KIND_NT || KIND == KIND_NN) {
@@ -1774,9 +1833,24 @@ __device__ __forceinline__ void epilogue(const GemmParams& P, const TileInfo& ti
       // [gate 64 | up 64] (gu), then act = bf16(bf16(silu(gate)) * up).
       const int64_t I = P.I;
       const int64_t jb = (int64_t)ti.ntile * 128 + wn * 64;
-      if (!kGated || P.gu != nullptr) {
-        stage_round<FN>(stage, wave, lane, round, [&](int mt, int nt) { return bf16x4(acc[mt][nt]); },
-                        [](int nt) { return ((nt & 2) ? 4 : 0) + (nt >> 2) * 2 + (nt & 1); });
+#ifdef PMX_GATED
+      {
+        const GatesWin w = gates_window(P, ti.row0 + rb, ti.row_end);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int nt = (k >> 1) * 4 + (k & 1);
+          const uint32_t o = w.at(cc, jb + k * 16 + rq * 4, I);
+#pragma unroll
+          for (int mtl = 0; mtl < 4; ++mtl) {
+            w.store(o, mtl * 16, acc[4 * round + mtl][nt], acc[4 * round + mtl][nt + 2]);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+        }
+      }
+#else
+      stage_round<FN>(stage, wave, lane, round, [&](int mt, int nt) { return bf16x4(acc[mt][nt]); },
+                      [](int nt) { return ((nt & 2) ? 4 : 0) + (nt >> 2) * 2 + (nt & 1); });
+      {
         const OutWin w = out_window(P.gu, ti.row0 + rb, ti.row_end, 2 * I);
         const int64_t j = jb + (cc & 7) * 8;
         const uint32_t voff = j < I ? (uint32_t)rq * w.rowb + (uint32_t)((cc < 8 ? 0 : I) + j) * 2u : kOOB;
@@ -1786,6 +1860,7 @@ __device__ __forceinline__ void epilogue(const GemmParams& P, const TileInfo& ti
           if (q % 8 == 7) __builtin_amdgcn_sched_barrier(0);  // at most 8 staged reads in flight
         }
       }
+#endif
       stage_round<4>(stage, wave, lane, round, [&](int mt, int k) {
         const int ng = (k >> 1) * 4 + (k & 1);
         float g[4], u[4];
@@ -1816,6 +1891,29 @@ __device__ __forceinline__ void epilogue(const GemmParams& P, const TileInfo& ti
       // issue order).  The next round's first loads go out during this
       // round's last quarter.
       const int64_t I = P.I;
+#ifdef PMX_GATED
+      // Straight from and to the registers' layout, four tiles of 16 x 16 at a time, the next four's gate and up
+      // values on their way meanwhile.
+      const GatesWin wi = gates_window(P, ti.row0 + rb, ti.row_end);
+      const OutWin wo = out_window(P.c0, ti.row0 + rb, ti.row_end, 2 * I);
+      const int64_t j0 = (int64_t)ti.ntile * BN + wn * 128 + rq * 4;
+      f32x4_t g[2][4], u[2][4];
+      const auto load_4 = [&](int b) __attribute__((always_inline)) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) wi.load(wi.at(cc, j0 + (b % 2 * 4 + k) * 16, I), b / 2 * 16, g[b & 1][k], u[b & 1][k]);
+      };
+      load_4(0);
+#pragma unroll
+      for (int b = 0; b < 8; ++b) {
+        if (b < 7) load_4(b + 1);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int nt = b % 2 * 4 + k;
+          gradients4(P, wo, b / 2 * 16 + cc, j0 + nt * 16, I, acc[4 * round + b / 2][nt], g[b & 1][k], u[b & 1][k]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+#else
       const int64_t j = (int64_t)ti.ntile * BN + wn * 128 + cc * 8;
       const uint32_t vg = j < I ? (uint32_t)rq * (uint32_t)(4 * I) + (uint32_t)j * 2u : kOOB;  // row rq of a quarter
       const uint32_t vu = vg + (uint32_t)I * 2u;
@@ -1848,12 +1946,13 @@ __device__ __forceinline__ void epilogue(const GemmParams& P, const TileInfo& ti
           unpack8e<Elt>(v, d);
           unpack8e<Elt>(nns_g[qq & 1][q], g);
           unpack8e<Elt>(nns_u[qq & 1][q], u);
-          activate_bwd8(P, d, g, u, dg, du);
+          swiglu_bwd8<Elt>(d, g, u, dg, du);
           win_store(wo, vg, r, pack8e<Elt>(dg));
           win_store(wo, vu, r, pack8e<Elt>(du));
         }
         __builtin_amdgcn_sched_barrier(0);
       }
+#endif
     } else if constexpr (KIND == KIND_TN) {
 #ifdef PMX_GATED
       if (P.parts != nullptr) {

@@ -21,24 +21,24 @@ GATES = {"silu": 0, "gelu_tanh": 1, "quick_gelu": 2}
 
 
 def _forward(x: torch.Tensor, gate_up: torch.Tensor, down: torch.Tensor, gate: int, keep: bool):
-    """(out, gu or None, act)."""
+    """(out, gate and up sums or None, act)."""
     T, H = x.shape
     N, I = down.shape
     act, out = x.new_empty((T, I)), x.new_empty((T, N))
-    gu = x.new_empty((T, 2 * I)) if keep else None
-    _launch("pmx_gated_ffn_fwd", x.dtype, x.device, _ptr(x), _ptr(gate_up), _ptr(down), T, H, I, N, gate, _ptr(gu), _ptr(act),
+    gates = x.new_empty((T, 2 * I), dtype=torch.float32) if keep else None
+    _launch("pmx_gated_ffn_fwd", x.dtype, x.device, _ptr(x), _ptr(gate_up), _ptr(down), T, H, I, N, gate, _ptr(gates), _ptr(act),
             _ptr(out))
-    return out, gu, act
+    return out, gates, act
 
 
 class _GatedFFN(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, gate_up, down, gate):
         need_x, need_up, need_down = ctx.needs_input_grad[:3]
-        out, gu, act = _forward(x, gate_up, down, gate, need_x or need_up)
+        out, gates, act = _forward(x, gate_up, down, gate, need_x or need_up)
         ctx.gate = gate
         # what the wanted gradients read
-        ctx.save_for_backward(x if need_up else None, gate_up if need_x else None, down if need_x or need_up else None, gu,
+        ctx.save_for_backward(x if need_up else None, gate_up if need_x else None, down if need_x or need_up else None, gates,
                               act if need_down else None)
         ctx.sizes = (*x.shape, down.shape[1])
         return out
@@ -46,7 +46,7 @@ class _GatedFFN(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_out):
-        x, gate_up, down, gu, act = ctx.saved_tensors
+        x, gate_up, down, gates, act = ctx.saved_tensors
         T, H, I = ctx.sizes
         N = grad_out.shape[1]
         grad_out = grad_out.contiguous()
@@ -59,7 +59,7 @@ class _GatedFFN(torch.autograd.Function):
             return dx, dup, ddown, None
         ws_bytes = _capi.load().pmx_gated_ffn_workspace_bytes(T, H, I, N)
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=grad_out.device)
-        _launch("pmx_gated_ffn_bwd", grad_out.dtype, grad_out.device, _ptr(grad_out), _ptr(x), _ptr(gate_up), _ptr(down), _ptr(gu),
+        _launch("pmx_gated_ffn_bwd", grad_out.dtype, grad_out.device, _ptr(grad_out), _ptr(x), _ptr(gate_up), _ptr(down), _ptr(gates),
                 _ptr(act), T, H, I, N, ctx.gate, _ptr(dx), _ptr(dup), _ptr(ddown), _ptr(ws), ws_bytes)
         return dx, dup, ddown, None
 
@@ -72,11 +72,11 @@ def gated_ffn(x: torch.Tensor, gate_up: torch.Tensor, down: torch.Tensor, activa
     ``activation``: "silu", "gelu_tanh" (GELU's tanh form) or "quick_gelu"
     (g sigmoid(1.702 g)).
 
-    Sums are held in fp32.  The block's inner values (gate, up, their product
-    and its gradients) are rounded to the tensors' dtype where a product reads
-    them or the backward keeps them.  For the backward x, gate and up rows
-    [tokens, 2I] and their products [tokens, I] are kept, as far as the
-    gradients that are wanted read them.
+    Sums are held in fp32; the gated products, and in the backward the gradients
+    of gate and up, are rounded to the tensors' dtype, being operands of
+    products.  For the backward x, the gate and up sums [tokens, 2I] in fp32 and
+    their products [tokens, I] are kept, as far as the gradients that are
+    wanted read them.
     """
     if activation not in GATES:
         raise ValueError(f"activation must be one of {sorted(GATES)}, got {activation!r}")
