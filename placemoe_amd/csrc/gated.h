@@ -20,9 +20,9 @@
   __attribute__((visibility("hidden"))) int pmx_gated_dgate##SUFFIX(const void* dout, const void* w, const float* gates,     \
                                                                     int64_t T, int64_t N, int64_t I, float a, float b,       \
                                                                     void* dgu, pmx_stream_t stream);                         \
-  /* c [M, N] = a [K, M]^T b [K, N]; with splits > 1 the K rows in chunks of `chunk`, each one's fp32 sums in parts */       \
+  /* c [M, N] = a [K, M]^T b [K, N], small: on 128 x 128 tiles; splits > 1: the K rows in chunks, their fp32 sums in parts */\
   __attribute__((visibility("hidden"))) int pmx_gated_tn##SUFFIX(const void* a, const void* b, int64_t K, int64_t M,         \
-                                                                 int64_t N, int64_t chunk, int32_t splits, void* c,          \
-                                                                 float* parts, pmx_stream_t stream);
+                                                                 int64_t N, bool small, int64_t chunk, int32_t splits,       \
+                                                                 void* c, float* parts, pmx_stream_t stream);
 PMX_GATED_GEMMS()
 PMX_GATED_GEMMS(_f16)

@@ -148,28 +148,26 @@ int check(int64_t T, int64_t H, int64_t I, int64_t N) {
   return PMX_OK;
 }
 
-int cu_count() {
-  int dev = 0, cus = 0;
-  if (hipGetDevice(&dev) != hipSuccess) return -1;
-  if (hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || cus <= 0) return -1;
-  return cus;
-}
-
-// The chunks of a weight gradient [M, N] over K rows; one where the operands pass what one descriptor holds.
-void chunks_of(int64_t K, int64_t M, int64_t N, int64_t cus, int64_t& chunk, int32_t& splits) {
-  splits = one_window(K, M) && one_window(K, N) && one_window(2 * M, N) ? pmx::gated_splits(K, M, N, cus) : 1;
-  chunk = pmx::gated_chunk(K, splits);
-  splits = (int32_t)((K + chunk - 1) / chunk);
+// How a weight gradient [M, N] over K rows runs; on small tiles where the operands pass what one descriptor holds (a
+// chunk's kernel has one for each).
+struct Wgrad {
+  bool small;
+  int64_t chunk;
+  int32_t splits;
+};
+Wgrad wgrad_of(int64_t K, int64_t M, int64_t N) {
+  constexpr int64_t kCus = 256;  // the same for the workspace and the call
+  const pmx::GatedWgrad w = pmx::gated_wgrad(K, M, N, kCus);
+  if (!one_window(K, M) || !one_window(K, N) || !one_window(2 * M, N)) return {w.small, pmx::gated_chunk(K, 1), 1};
+  const int64_t chunk = pmx::gated_chunk(K, w.splits);
+  return {w.small, chunk, (int32_t)((K + chunk - 1) / chunk)};
 }
 
 // The backward's workspace: dgu, then the fp32 sums of one weight gradient's chunks.
-constexpr int64_t kCus = 256;  // of the workspace's estimate and of the call alike
 size_t dgu_bytes(int64_t T, int64_t I) { return ((size_t)T * 2 * I * 2 + 255) / 256 * 256; }
 size_t parts_bytes(int64_t K, int64_t M, int64_t N) {
-  int64_t chunk;
-  int32_t splits;
-  chunks_of(K, M, N, kCus, chunk, splits);
-  return splits > 1 ? (size_t)splits * M * N * 4 : 0;
+  const Wgrad w = wgrad_of(K, M, N);
+  return w.splits > 1 ? (size_t)w.splits * M * N * 4 : 0;
 }
 
 template <class E>
@@ -214,12 +212,10 @@ int forward_t(const void* x, const void* gate_up, const void* down, int64_t T, i
 
 template <class E>
 int weight_gradient(const void* a, const void* b, int64_t K, int64_t M, int64_t N, void* c, float* parts, pmx_stream_t stream) {
-  int64_t chunk;
-  int32_t splits;
-  chunks_of(K, M, N, kCus, chunk, splits);
-  if (Gemms<E>::tn(a, b, K, M, N, chunk, splits, c, parts, stream) != PMX_OK) return PMX_ERR_HIP;
-  if (splits > 1) {
-    sum_parts_kernel<E><<<(unsigned)((M * N / 4 + 255) / 256), 256, 0, stream>>>(parts, splits, M * N, (bf16_t*)c);
+  const Wgrad w = wgrad_of(K, M, N);
+  if (Gemms<E>::tn(a, b, K, M, N, w.small, w.chunk, w.splits, c, parts, stream) != PMX_OK) return PMX_ERR_HIP;
+  if (w.splits > 1) {
+    sum_parts_kernel<E><<<(unsigned)((M * N / 4 + 255) / 256), 256, 0, stream>>>(parts, w.splits, M * N, (bf16_t*)c);
     PMX_LAUNCH_CHECK();
   }
   return PMX_OK;

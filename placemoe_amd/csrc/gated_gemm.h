@@ -5,27 +5,25 @@
 
 namespace {
 
-#ifndef PMX_GATED_FORCE
-#define PMX_GATED_FORCE 0
-#endif
-
 template <int KIND>
 int launch_rows(const GemmParams& P, hipStream_t stream) {
   const int64_t ntn = KIND == KIND_FC1 ? (P.I + 127) / 128 : (P.N + BN - 1) / BN;
   if (ntn >= (int64_t)1 << 19) return PMX_ERR_SHAPE;  // the LDS tile table keeps an n-tile index in 19 bits
   const int grid = grid_size();
   if (grid <= 0) return PMX_ERR_HIP;
-  const int tiling = PMX_GATED_FORCE ? PMX_GATED_FORCE : pmx::gated_tiling(KIND, P.M, P.N, P.K, grid);
+  const int tiling = pmx::gated_tiling(KIND, P.M, P.N, P.K, grid);
   if (tiling == Few64::BM) return launch_few<KIND, Few64>(P, grid, stream);
   if (tiling == Few128::BM) return launch_few<KIND, Few128>(P, grid, stream);
   const bool fast = P.K % BK == 0;
   if constexpr (use_w4<KIND>()) {
     if (fast) w4::grouped_gemm_w4_kernel<KIND><<<grid, w4::NT, 0, stream>>>(P);
     else grouped_gemm_kernel<KIND, kBM><<<grid, NTHREADS, 0, stream>>>(P);
+  } else if (!fast) {
+    grouped_gemm_kernel<KIND, kBM><<<grid, NTHREADS, 0, stream>>>(P);
+  } else if constexpr (KIND == KIND_NT) {  // the kernels of few copies with many rows, as in grouped_gemm.hip
+    grouped_gemm_kernel<KIND, kBM, false, true, true><<<grid, NTHREADS, 0, stream>>>(P);
   } else {
-    if (!fast) grouped_gemm_kernel<KIND, kBM><<<grid, NTHREADS, 0, stream>>>(P);
-    else if (KIND == KIND_NT || P.M < kRsMaxRowsPerCopy) grouped_gemm_kernel<KIND, kBM, false, true, true><<<grid, NTHREADS, 0, stream>>>(P);
-    else grouped_gemm_kernel<KIND, kBM, false, true><<<grid, NTHREADS, 0, stream>>>(P);
+    grouped_gemm_kernel<KIND, kBM, false, true><<<grid, NTHREADS, 0, stream>>>(P);
   }
   PMX_LAUNCH_CHECK();
   return PMX_OK;
@@ -82,8 +80,8 @@ int PMX_GEMM_FN(pmx_gated_dgate)(const void* dout, const void* w, const float* g
   return launch_rows<KIND_NNS>(P, stream);
 }
 
-int PMX_GEMM_FN(pmx_gated_tn)(const void* a, const void* b, int64_t K, int64_t M, int64_t N, int64_t chunk, int32_t splits,
-                              void* c, float* parts, pmx_stream_t stream) {
+int PMX_GEMM_FN(pmx_gated_tn)(const void* a, const void* b, int64_t K, int64_t M, int64_t N, bool small, int64_t chunk,
+                              int32_t splits, void* c, float* parts, pmx_stream_t stream) {
   if (!fits_rsrc(BK, M) || !fits_rsrc(BK, N)) return PMX_ERR_SHAPE;
   const int grid = grid_size();
   if (grid <= 0) return PMX_ERR_HIP;
@@ -97,9 +95,10 @@ int PMX_GEMM_FN(pmx_gated_tn)(const void* a, const void* b, int64_t K, int64_t M
   P.cgs = splits > 1 ? M * N : 0;
   P.ldc = N;
   P.csplit = INT64_MAX;
-  const int64_t tiles = ((M + fr::kWgT - 1) / fr::kWgT) * ((N + fr::kWgT - 1) / fr::kWgT);
-  const int64_t blocks = (tiles + kNumXcd - 1) / kNumXcd * kNumXcd;
-  if (K <= kFewRowsWgrad && splits == 1 && blocks < (int64_t)1 << 30) {  // 128 x 128 tiles, four blocks per CU
+  if (small) {  // 128 x 128 tiles, four blocks per CU
+    const int64_t tiles = ((M + fr::kWgT - 1) / fr::kWgT) * ((N + fr::kWgT - 1) / fr::kWgT);
+    const int64_t blocks = (tiles + kNumXcd - 1) / kNumXcd * kNumXcd;
+    if (splits != 1 || blocks >= (int64_t)1 << 30) return PMX_ERR_SHAPE;
     fr::few_rows_wgrad_grouped_gemm_kernel<<<(unsigned)blocks, fr::kWgNT, 0, stream>>>(P);
     PMX_LAUNCH_CHECK();
     return PMX_OK;

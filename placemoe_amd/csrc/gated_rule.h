@@ -11,27 +11,74 @@ namespace pmx {
 // share of the weights' columns (gated_ffn.hip).
 constexpr int64_t kGatedFewTokens = 16;
 
-// The m-tile height, 64 (64 x 128 tiles), 128 (128 x 256) or 256 (256 x 256), of a product of `rows` rows, N
-// columns (fc1: 2 I) and depth K on `cus` CUs.  kind: 0 fc1, 1 fc2, 2 fc1 dgrad, 3 fc2 dgrad.
+// The products of rows run on 64 x 128 tiles (two blocks per CU), 128 x 256 ones
+// or 256 x 256 ones.  A call takes as long as its rounds of tiles, each its K-tiles
+// of 64 and a fixed part (epilogue, tile switch), in us; a CU with one 64 x 128
+// tile is faster through it than one with two.  Fitted to 105 calls of each kind
+// (7 layers from 512 x 264 to 7168 x 2048, 17 to 8192 rows), of which the tiling
+// that this rule takes is within 0.3% of the best one's time in geometric mean, 1.20
+// at worst (64 / 128 / 256):
+//   rows   H     I      fc1                fc2                fc1 dgrad          fc2 dgrad
+//   256    2048  768     17 /  30 /  52      9 /  15 /  20     14 /  24 /  34     19 /  37 /  72
+//   2048   2048  768     27 /  35 /  58     15 /  18 /  29     23 /  27 /  45     22 /  41 /  74
+//   8192   2048  768     87 /  70 /  63     49 /  37 /  30     79 /  57 /  48     51 /  46 /  80
+//   1024   7168  2048    76 /  91 / 164     50 /  35 /  57     86 /  60 / 105     56 /  92 / 172
+//   8192   7168  2048   622 / 410 / 363    308 / 216 / 210    589 / 404 / 392    330 / 243 / 220
+struct GatedRound {
+  double ktile, fixed;
+};
+constexpr double kGated64[4][4] = {  // K-tile with two blocks on a CU, with one, fixed, of the call
+    {0.63, 0.342, 5.04, 0.2}, {0.645, 0.328, 3.78, 1.6}, {0.624, 0.344, 4.45, 1.0}, {0.662, 0.349, 7.44, 0.0}};
+constexpr GatedRound kGated128[4] = {{0.711, 7.44}, {0.636, 7.49}, {0.656, 7.85}, {0.725, 12.4}};
+constexpr GatedRound kGated256[4] = {{1.196, 13.8}, {1.056, 9.6}, {1.109, 9.5}, {1.371, 20.9}};
+// 256 x 256 tiles whose depth is not a multiple of 64: the kernel whose loads are masked.
+constexpr double kGatedMasked = 1.45;
+
+// The m-tile height of a product of `rows` rows, N columns (fc1: 2 I) and depth K on `cus` CUs.
+// kind: 0 fc1, 1 fc2, 2 fc1 dgrad, 3 fc2 dgrad.
 inline int gated_tiling(int kind, int64_t rows, int64_t N, int64_t K, int64_t cus) {
-  (void)kind, (void)K, (void)cus, (void)N;
-  return rows <= 64 ? 64 : 256;
+  const auto div_up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
+  const double nk = (double)div_up(K, 64);
+  const int64_t per_cu = div_up(div_up(rows, 64) * div_up(N, 128), cus);
+  const double* c = kGated64[kind];
+  const double t64 = ((double)(per_cu / 2) * c[0] + (double)(per_cu % 2) * c[1]) * nk + (double)div_up(per_cu, 2) * c[2] + c[3];
+  const auto rounds = [&](int64_t height, const GatedRound& r) {
+    return (double)div_up(div_up(rows, height) * div_up(N, 256), cus) * (nk * r.ktile + r.fixed);
+  };
+  const double t128 = rounds(128, kGated128[kind]), t256 = rounds(256, kGated256[kind]) * (K % 64 ? kGatedMasked : 1.0);
+  return t64 <= t128 && t64 <= t256 ? 64 : t128 <= t256 ? 128 : 256;
 }
 
-// Chunks of the K rows of a weight gradient [M, N] on `cus` CUs: their 256 x 256 tiles fill the chip where one
-// gradient's own do not.
-inline int32_t gated_splits(int64_t K, int64_t M, int64_t N, int64_t cus) {
+// A weight gradient [M, N] over K rows on `cus` CUs: 128 x 128 tiles that load a
+// K-tile at a time, or 256 x 256 ones over `splits` chunks of the rows, so that they fill the
+// chip where one gradient's own do not; the chunks' fp32 sums are then added by a
+// kernel more.  Costs in us fitted to 110 calls of each (512 x 264 to 7168 x 2048, 17 to
+// 16384 rows), of which the choice is within 2% of the best in geometric mean, 1.31
+// at worst (128 x 128 / 256 x 256 whole / in chunks, their sum included):
+//   rows    M     N      128     256      chunks
+//   1024    2816  4096    29      32       -
+//   1531    2000  1416    33      41       22 + 13 (5)
+//   16384   1536  2048   294     308       89 + 14 (5)
+//   16384   2048  768    274     302       53 + 14 (10)
+//   8192    4096  7168   604     361       -
+struct GatedWgrad {
+  bool small;  // 128 x 128 tiles
+  int32_t splits;
+};
+inline GatedWgrad gated_wgrad(int64_t K, int64_t M, int64_t N, int64_t cus) {
   const auto div_up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
   const int64_t tiles = div_up(M, 256) * div_up(N, 256), nk = div_up(K, 64);
-  double best = 0;
-  int32_t splits = 1;
-  for (int32_t s = 1; s <= 64 && s <= nk; ++s) {
-    // us: a K-tile, a tile's epilogue and switch; the chunks' sums are written and read again
-    const double cost = (double)div_up(tiles * s, cus) * ((double)div_up(nk, s) * 1.7 + 5.0) +
-                        (s > 1 ? 4.0 + (double)s * (double)M * (double)N * 8.0 / 4.0e6 : 0.0);
-    if (s == 1 || cost < best) best = cost, splits = s;
+  const double per_cu = (double)div_up(div_up(M, 128) * div_up(N, 128), cus);
+  const double ktile = 0.46 * per_cu > 1.03 ? 0.46 * per_cu : 1.03;
+  GatedWgrad best = {true, 1};
+  double least = (double)nk * ktile + 3.0 + 1.07 * per_cu;
+  for (int64_t s = 1; s <= 32 && s <= nk; ++s) {
+    const double sums = s > 1 ? (double)s * (double)M * (double)N * 4e-6 : 0.0;  // MB
+    const double rounds = (double)div_up(tiles * s, cus);
+    const double cost = rounds * ((double)div_up(nk, s) * 1.30 + 1.6) + 7.7 + sums * 0.15 + (s > 1 ? 4.5 + sums / 7.0 : 0.0);
+    if (cost < least) least = cost, best = {false, (int32_t)s};
   }
-  return splits;
+  return best;
 }
 
 // Rows of a chunk, whole K-tiles; the number of chunks is what they make.
