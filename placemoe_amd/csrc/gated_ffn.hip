@@ -22,15 +22,17 @@
 // Here a block has 16 rows of the weights (fc1: 8 gate rows and their 8 up rows)
 // for all tokens, its waves a share of the columns each, straight from memory to
 // the matrix instruction (16 weight rows x 16 tokens, 32 columns); their sums
-// meet in LDS.  Bound: HBM.
+// meet in LDS.  Bound: HBM; from some tens of tokens on, their being read again by
+// every block.  One token through 7168 x 2048: 23.7 us, 3.7 TB/s of weights (a large
+// copy: 4.8), on 64 x 128 tiles 72; 64 tokens 66 and 80.  (32 weight rows per block:
+// as fast for few, 30% slower where that leaves less than a block per CU.)
 
 #include "gated.h"
 #include "gated_rule.h"
 
 namespace {
 
-constexpr int kFewWaves = 8;
-constexpr int kFewSteps = 8;  // steps of 32 columns that a wave has on their way
+constexpr int kFewWaves = 8;  // (4 or 16, and 4 to 16 steps on their way: within 5%)
 
 template <class E>
 __device__ __forceinline__ f32x4_t mfma16(const uint4& w, const uint4& x, const f32x4_t& c) {
@@ -43,73 +45,99 @@ __device__ __forceinline__ f32x4_t mfma16(const uint4& w, const uint4& x, const 
 }
 
 // The sums of 16 weight rows (wrow: the lane's, that of row lane % 16) with
-// tokens 0 .. 15 of x [T, K]: red[wave][weight row][token], after a barrier.
-// K a multiple of 8.  Lanes past K, and past T, multiply zeros.
-template <class E>
+// tokens 0 .. 16 FT - 1 of x [T, K]: red[wave][weight row][token], after a barrier.
+// K a multiple of 8.  Lanes past K, and past T, multiply zeros.  A wave has
+// kSteps steps of 32 columns on their way; a token's sum is the same however many there are.
+template <class E, int FT>
 __device__ __forceinline__ void few_products(const bf16_t* wrow, const bf16_t* x, int64_t T, int64_t K, int lane, int wave,
-                                             float (*red)[16][16]) {
+                                             float (*red)[16][16 * FT]) {
+  constexpr int kSteps = FT == 1 ? 8 : FT == 2 ? 6 : 4;
   const int t = lane & 15, quarter = lane >> 4;
-  const bool token = t < T;
-  const bf16_t* xrow = x + (token ? t : 0) * K;
-  const int64_t chunks = K / 8;
-  f32x4_t acc = {};
-  for (int64_t c0 = (int64_t)wave * 4; c0 < chunks; c0 += 4 * kFewWaves * kFewSteps) {
-    uint4 w[kFewSteps], v[kFewSteps];
+  bool token[FT];
+  const bf16_t* xrow[FT];
 #pragma unroll
-    for (int s = 0; s < kFewSteps; ++s) {
+  for (int f = 0; f < FT; ++f) {
+    token[f] = f * 16 + t < T;
+    xrow[f] = x + (token[f] ? f * 16 + t : 0) * K;
+  }
+  const int64_t chunks = K / 8;
+  f32x4_t acc[FT] = {};
+  for (int64_t c0 = (int64_t)wave * 4; c0 < chunks; c0 += 4 * kFewWaves * kSteps) {
+    uint4 w[kSteps], v[kSteps][FT];
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
       const int64_t c = c0 + s * (4 * kFewWaves) + quarter;
       const bool in = c < chunks;
       w[s] = in ? ld_stream(wrow + c * 8) : make_uint4(0, 0, 0, 0);
-      v[s] = in && token ? *reinterpret_cast<const uint4*>(xrow + c * 8) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int f = 0; f < FT; ++f) v[s][f] = in && token[f] ? *reinterpret_cast<const uint4*>(xrow[f] + c * 8) : make_uint4(0, 0, 0, 0);
     }
 #pragma unroll
-    for (int s = 0; s < kFewSteps; ++s) acc = mfma16<E>(w[s], v[s], acc);
+    for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+      for (int f = 0; f < FT; ++f) acc[f] = mfma16<E>(w[s], v[s][f], acc[f]);
   }
   // lane: token lane % 16, weight rows 4 (lane / 16) .. + 3
 #pragma unroll
-  for (int e = 0; e < 4; ++e) red[wave][quarter * 4 + e][t] = acc[e];
+  for (int f = 0; f < FT; ++f)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) red[wave][quarter * 4 + e][f * 16 + t] = acc[f][e];
   __syncthreads();
 }
 
 // fc1: eight columns of act (and gates) per block.
-template <class E>
+template <class E, int FT>
 __global__ __launch_bounds__(64 * kFewWaves) void gated_few_fc1_kernel(const bf16_t* __restrict__ x, const bf16_t* __restrict__ w,
                                                                        int64_t T, int64_t H, int64_t I, Gate gate,
                                                                        float* __restrict__ gates, bf16_t* __restrict__ act) {
-  __shared__ float red[kFewWaves][16][16];
+  __shared__ float red[kFewWaves][16][16 * FT];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t j0 = (int64_t)blockIdx.x * 8;
   const int r = lane & 15;
-  few_products<E>(w + ((r < 8 ? 0 : I) + j0 + r % 8) * H, x, T, H, lane, wave, red);
-  const int64_t t = threadIdx.x >> 3;
+  few_products<E, FT>(w + ((r < 8 ? 0 : I) + j0 + r % 8) * H, x, T, H, lane, wave, red);
   const int j = threadIdx.x & 7;
-  if (t >= T || t >= 16) return;
-  float g = 0.f, u = 0.f;
+  for (int64_t t = threadIdx.x >> 3; t < T && t < 16 * FT; t += 8 * kFewWaves) {
+    float g = 0.f, u = 0.f;
 #pragma unroll
-  for (int i = 0; i < kFewWaves; ++i) g += red[i][j][t], u += red[i][8 + j][t];
-  if (gates != nullptr) {  // four columns' gates, then their ups
-    float* const to = gates + (t * I + j0 + (j & 4)) * 2 + (j & 3);
-    to[0] = g, to[4] = u;
+    for (int i = 0; i < kFewWaves; ++i) g += red[i][j][t], u += red[i][8 + j][t];
+    if (gates != nullptr) {  // four columns' gates, then their ups
+      float* const to = gates + (t * I + j0 + (j & 4)) * 2 + (j & 3);
+      to[0] = g, to[4] = u;
+    }
+    act[t * I + j0 + j] = (bf16_t)E::from_f32(gate.value(g) * u);
   }
-  act[t * I + j0 + j] = (bf16_t)E::from_f32(gate.value(g) * u);
 }
 
 // fc2: 16 columns of out per block.
-template <class E>
+template <class E, int FT>
 __global__ __launch_bounds__(64 * kFewWaves) void gated_few_fc2_kernel(const bf16_t* __restrict__ act, const bf16_t* __restrict__ w,
                                                                        int64_t T, int64_t N, int64_t I, bf16_t* __restrict__ out) {
-  __shared__ float red[kFewWaves][16][16];
+  __shared__ float red[kFewWaves][16][16 * FT];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t n0 = (int64_t)blockIdx.x * 16;
   const int64_t n = n0 + (lane & 15);
-  few_products<E>(w + (n < N ? n : N - 1) * I, act, T, I, lane, wave, red);
-  const int64_t t = threadIdx.x >> 4;
+  few_products<E, FT>(w + (n < N ? n : N - 1) * I, act, T, I, lane, wave, red);
   const int j = threadIdx.x & 15;
-  if (t >= T || t >= 16 || n0 + j >= N) return;
-  float sum = 0.f;
+  if (n0 + j >= N) return;
+  for (int64_t t = threadIdx.x >> 4; t < T && t < 16 * FT; t += 4 * kFewWaves) {
+    float sum = 0.f;
 #pragma unroll
-  for (int i = 0; i < kFewWaves; ++i) sum += red[i][j][t];
-  out[t * N + n0 + j] = (bf16_t)E::from_f32(sum);
+    for (int i = 0; i < kFewWaves; ++i) sum += red[i][j][t];
+    out[t * N + n0 + j] = (bf16_t)E::from_f32(sum);
+  }
+}
+
+template <class E, int FT>
+int few_forward(const void* x, const void* gate_up, const void* down, int64_t T, int64_t H, int64_t I, int64_t N, const Gate& gate,
+                float* gates, void* act, void* out, pmx_stream_t stream) {
+  
+  gated_few_fc1_kernel<E, FT><<<(unsigned)(I / 8), 64 * kFewWaves, 0, stream>>>((const bf16_t*)x, (const bf16_t*)gate_up, T, H, I, gate,
+                                                                                gates, (bf16_t*)act);
+  PMX_LAUNCH_CHECK();
+  gated_few_fc2_kernel<E, FT><<<(unsigned)((N + 15) / 16), 64 * kFewWaves, 0, stream>>>((const bf16_t*)act, (const bf16_t*)down, T, N, I,
+                                                                                        (bf16_t*)out);
+  PMX_LAUNCH_CHECK();
+  return PMX_OK;
 }
 
 // The chunks' sums, in order: a thread per four neighbouring elements.
@@ -148,6 +176,8 @@ int check(int64_t T, int64_t H, int64_t I, int64_t N) {
   return PMX_OK;
 }
 
+constexpr int64_t kCus = 256;  // of the rules here: the same for the workspace and the call
+
 // How a weight gradient [M, N] over K rows runs; on small tiles where the operands pass what one descriptor holds (a
 // chunk's kernel has one for each).
 struct Wgrad {
@@ -156,7 +186,6 @@ struct Wgrad {
   int32_t splits;
 };
 Wgrad wgrad_of(int64_t K, int64_t M, int64_t N) {
-  constexpr int64_t kCus = 256;  // the same for the workspace and the call
   const pmx::GatedWgrad w = pmx::gated_wgrad(K, M, N, kCus);
   if (!one_window(K, M) || !one_window(K, N) || !one_window(2 * M, N)) return {w.small, pmx::gated_chunk(K, 1), 1};
   const int64_t chunk = pmx::gated_chunk(K, w.splits);
@@ -196,14 +225,10 @@ int forward_t(const void* x, const void* gate_up, const void* down, int64_t T, i
   if (T == 0) return PMX_OK;
   if (!x || !gate_up || !down || !act || !out) return PMX_ERR_ARG;
   if (!aligned16(x) || !aligned16(gate_up) || !aligned16(down) || !aligned16(gates) || !aligned16(act) || !aligned16(out)) return PMX_ERR_SHAPE;
-  if (T <= pmx::kGatedFewTokens) {
-    gated_few_fc1_kernel<E><<<(unsigned)(I / 8), 64 * kFewWaves, 0, stream>>>((const bf16_t*)x, (const bf16_t*)gate_up, T, H, I, gate,
-                                                                              gates, (bf16_t*)act);
-    PMX_LAUNCH_CHECK();
-    gated_few_fc2_kernel<E><<<(unsigned)((N + 15) / 16), 64 * kFewWaves, 0, stream>>>((const bf16_t*)act, (const bf16_t*)down, T, N, I,
-                                                                                      (bf16_t*)out);
-    PMX_LAUNCH_CHECK();
-    return PMX_OK;
+  if (pmx::gated_few(T, H, I, N, kCus)) {
+    if (T <= 16) return few_forward<E, 1>(x, gate_up, down, T, H, I, N, gate, gates, act, out, stream);
+    if (T <= 32) return few_forward<E, 2>(x, gate_up, down, T, H, I, N, gate, gates, act, out, stream);
+    return few_forward<E, 4>(x, gate_up, down, T, H, I, N, gate, gates, act, out, stream);
   }
   // The sizes have been checked: what fails from here on is a launch.
   if (Gemms<E>::fc1(x, gate_up, T, H, I, gate.a, gate.b, gates, act, stream) != PMX_OK) return PMX_ERR_HIP;

@@ -7,10 +7,6 @@
 
 namespace pmx {
 
-// Tokens up to which the forward runs on the kernels that give every wave a
-// share of the weights' columns (gated_ffn.hip).
-constexpr int64_t kGatedFewTokens = 16;
-
 // The products of rows run on 64 x 128 tiles (two blocks per CU), 128 x 256 ones
 // or 256 x 256 ones.  A call takes as long as its rounds of tiles, each its K-tiles
 // of 64 and a fixed part (epilogue, tile switch), in us; a CU with one 64 x 128
@@ -36,7 +32,11 @@ constexpr double kGatedMasked = 1.45;
 
 // The m-tile height of a product of `rows` rows, N columns (fc1: 2 I) and depth K on `cus` CUs.
 // kind: 0 fc1, 1 fc2, 2 fc1 dgrad, 3 fc2 dgrad.
-inline int gated_tiling(int kind, int64_t rows, int64_t N, int64_t K, int64_t cus) {
+struct GatedTiling {
+  int height;
+  double us;
+};
+inline GatedTiling gated_fastest(int kind, int64_t rows, int64_t N, int64_t K, int64_t cus) {
   const auto div_up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
   const double nk = (double)div_up(K, 64);
   const int64_t per_cu = div_up(div_up(rows, 64) * div_up(N, 128), cus);
@@ -46,7 +46,22 @@ inline int gated_tiling(int kind, int64_t rows, int64_t N, int64_t K, int64_t cu
     return (double)div_up(div_up(rows, height) * div_up(N, 256), cus) * (nk * r.ktile + r.fixed);
   };
   const double t128 = rounds(128, kGated128[kind]), t256 = rounds(256, kGated256[kind]) * (K % 64 ? kGatedMasked : 1.0);
-  return t64 <= t128 && t64 <= t256 ? 64 : t128 <= t256 ? 128 : 256;
+  if (t64 <= t128 && t64 <= t256) return {64, t64};
+  return t128 <= t256 ? GatedTiling{128, t128} : GatedTiling{256, t256};
+}
+inline int gated_tiling(int kind, int64_t rows, int64_t N, int64_t K, int64_t cus) { return gated_fastest(kind, rows, N, K, cus).height; }
+
+// Whether the forward of T tokens runs on the kernels that give every wave a share of the
+// weights' columns (gated_ffn.hip): up to 64 tokens, where reading the weights once, at 4.3 TB/s, and the tokens for each
+// 8 columns of act and 16 of out, at 8.4 TB/s from the L2s, takes less than the tiles of rows and the weights' way from
+// memory (the times above are of weights at hand; 5 layers, 1 to 64 tokens, weights from memory: 7168 x 2048, 64 tokens
+// 66 us for 80; 4096 x 11008, 32 tokens 123 for 129, 48 159 for 135).
+inline bool gated_few(int64_t T, int64_t H, int64_t I, int64_t N, int64_t cus) {
+  if (T > 64) return false;
+  const double weights = 2.0 * ((double)(2 * I) * (double)H + (double)N * (double)I);
+  const double tokens = (double)T * ((double)(I / 8) * (double)H + (double)(N / 16) * (double)I) * 2.0;
+  return 5.0 + weights / 4.3e6 + tokens / 8.4e6 <=
+         gated_fastest(0, T, 2 * I, H, cus).us + gated_fastest(1, T, N, I, cus).us + weights / 5.5e6;
 }
 
 // A weight gradient [M, N] over K rows on `cus` CUs: 128 x 128 tiles that load a

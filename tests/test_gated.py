@@ -77,3 +77,52 @@ def test_wrapper_refuses():
         placemoe_amd.gated_ffn(x, up, down)
     with pytest.raises(ValueError, match="activation"):
         placemoe_amd.gated_ffn(x, up, down, activation="relu")
+
+
+@pytest.fixture(scope="module")
+def rule(tmp_path_factory):
+    import shutil
+    import subprocess
+    from pathlib import Path
+
+    if shutil.which("g++") is None:
+        pytest.skip("g++ not available")
+    exe = tmp_path_factory.mktemp("rule") / "gated_rule"
+    subprocess.run(["g++", "-O1", "-std=c++17", "-Wall", "-Werror", str(Path(__file__).with_name("gated_rule_main.cpp")), "-o", str(exe)],
+                   check=True)
+
+    def ask(*lines):
+        out = subprocess.run([str(exe)], input="\n".join(lines), capture_output=True, text=True, check=True).stdout.split("\n")
+        return [[int(v) for v in line.split()] for line in out if line]
+
+    return ask
+
+
+def test_tilings_are_the_measured_best(rule):
+    """Of calls whose times lie well apart (gated_rule.h): kind, rows, N, K -> height of the fastest tiles."""
+    best = {(0, 256, 1536, 2048): 64, (0, 8192, 1536, 2048): 256, (1, 1024, 7168, 2048): 128, (2, 1024, 7168, 4096): 128,
+            (3, 1024, 2048, 7168): 64, (3, 8192, 768, 2048): 128, (0, 8192, 4096, 7168): 256, (1, 2048, 4096, 11008): 128,
+            (2, 1536, 4096, 22016): 128, (3, 17, 264, 512): 64}
+    got = rule(*(f"tiling {k} {r} {n} {d}" for k, r, n, d in best))
+    assert [g[0] for g in got] == list(best.values())
+
+
+def test_few_tokens(rule):
+    asked = {(1, 7168, 2048, 7168): 1, (64, 7168, 2048, 7168): 1, (65, 7168, 2048, 7168): 0, (64, 2048, 768, 2048): 1,
+             (16, 4096, 11008, 4096): 1, (64, 4096, 11008, 4096): 0, (1, 8, 8, 8): 1}
+    assert [g[0] for g in rule(*(f"few {t} {h} {i} {n}" for t, h, i, n in asked))] == list(asked.values())
+
+
+def test_weight_gradients(rule):
+    import random
+
+    rng = random.Random(5)
+    cases = [(16384, 1536, 2048), (16384, 2048, 768), (8192, 4096, 7168), (17, 2000, 1416), (1, 8, 8), (1 << 31, 8, 8)]
+    cases += [(rng.randint(1, 20000), 8 * rng.randint(1, 1000), 8 * rng.randint(1, 1000)) for _ in range(300)]
+    for (K, M, N), (small, splits, chunk) in zip(cases, rule(*(f"wgrad {k} {m} {n} 0" for k, m, n in cases))):
+        # chunks of whole K-tiles that cover the rows, the last of them with some; small tiles take them whole
+        count = -(-K // chunk)
+        assert chunk % 64 == 0 and count <= splits <= 32 and (count - 1) * chunk < K, (K, M, N)
+        assert not (small and splits > 1)
+    assert rule("wgrad 8192 4096 7168 0")[0][:2] == [0, 1] and rule("wgrad 17 2000 1416 0")[0][:2] == [1, 1]
+    assert rule("wgrad 16384 1536 2048 0")[0][:2] == [0, 5] and rule("wgrad 16384 2048 768 0")[0][:2] == [0, 10]
