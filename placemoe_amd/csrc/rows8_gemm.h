@@ -1077,11 +1077,12 @@ int launch_cfg(const Params8& P, int cus, pmx_stream_t stream) {
   return PMX_OK;
 }
 
-template <class E, int KIND, class F>
+template <class E, int KIND, class F>  // 4-bit rows: NT alone
 int launch(const Params8& P, pmx_stream_t stream) {
   const int cus = cu_count();
   if (cus <= 0) return PMX_ERR_HIP;
-  switch (pmx::rows8_tiling(KIND, P.M, P.G, P.N, P.K * F::A / 8, cus)) {
+  const pmx::Rows8Lines& line = F::B == 8 ? pmx::kRows8Lines[KIND] : F::A == 8 ? pmx::kRows8x4Lines[KIND] : pmx::kRows4x4Lines[NT8];
+  switch (pmx::rows8_tiling(line, P.M, P.G, P.N, P.K / (8 / F::A), cus)) {
     case 0: return launch_cfg<E, KIND, Narrow32<F>>(P, cus, stream);
     case 32: return launch_cfg<E, KIND, Rows32<F>>(P, cus, stream);
     case 128: return launch_cfg<E, KIND, Rows128<F>>(P, cus, stream);

@@ -28,6 +28,22 @@
 // the choice takes 1.015 (NT) and 1.011 (fc1) of the best tiling's time in geometric
 // mean, 1.33 at worst (a row each for 96 copies of 1040 x 528: 14.9 us for 11.2).
 //
+// With weights in 4 bits the lines lie elsewhere: half the weights' bytes, more stages of them on
+// their way, and rows in 4 bits at twice the depth per K-tile (K there: A's bytes per row).  Over 183 calls of each
+// kind (10 layers, 0.05 to 2000 rows per copy) the choice takes 1.009 (8-bit rows), 1.012 (4-bit rows) and
+// 1.007 (fc1) of the best tiling's time, 1.27 at worst (768 rows of 16 copies of 4096 x 7168: 70 us for 55; with
+// the lines of 8-bit weights 1.027, 1.015 and 1.010, 1.42 at worst).  us, as above:
+//   copies rows   N     K     NT, rows in 8 bits       NT, rows in 4            fc1
+//   160    64     1536  2048    20/  23/  26/  50        18/  20/  21/  34        30/  32/  39/  88
+//   160    640    1536  2048    45/  44/  58/  95        40/  42/  45/  64        67/  59/ 103/ 170
+//   160    1600   1536  2048    46/  46/  60/  95        41/  42/  46/  64        68/  59/ 103/ 171
+//   160    5120   1536  2048    67/  62/  64/  97        46/  50/  47/  66        97/  84/ 105/ 172
+//   160    20480  1536  2048   192/ 162/ 101/ 115       112/ 104/  64/  81       284/ 228/ 162/ 194
+//   160    81920  1536  2048   684/ 559/ 296/ 280       392/ 354/ 192/ 188      1035/ 811/ 516/ 505
+//   16     1      4096  7168    20/  26/  30/  70        12/  18/  20/  42        31/  42/  52/ 132
+//   16     256    4096  7168    44/  38/  46/  74        39/  38/  39/  46        61/  46/  88/ 139
+//   16     16000  4096  7168   996/ 830/ 436/ 409       550/ 490/ 275/ 253      1603/1276/ 820/ 763
+//
 // A result's bits do not depend on the choice: every tiling adds up K in the same
 // steps.
 //
@@ -38,23 +54,28 @@
 
 namespace pmx {
 
-// Rows per copy (with rows) up to which the 32-row tiles run: NT, FC1.
-constexpr int64_t kRows8Few[2] = {16, 32};
-// A round's cost in us: per K-tile of 128, and beside them.
-constexpr double kRows8Round128[2][2] = {{1.25, 2.0}, {1.7, 2.0}};
-constexpr double kRows8Round256[2][2] = {{1.5, 5.0}, {2.7, 8.0}};
+struct Rows8Lines {
+  int64_t few;         // rows per copy (with rows) up to which the 32-row tiles run
+  double narrow;       // a 32 x 64 round beside a 32 x 256 one that reads as much
+  double round128[2];  // a round's cost in us: per K-tile of 128, and beside them
+  double round256[2];
+};
+// NT, FC1
+constexpr Rows8Lines kRows8Lines[2] = {{16, 1.0, {1.25, 2.0}, {1.5, 5.0}}, {32, 1.0, {1.7, 2.0}, {2.7, 8.0}}};
+constexpr Rows8Lines kRows8x4Lines[2] = {{24, 1.05, {0.9, 3.0}, {1.5, 5.0}}, {48, 1.05, {0.9, 3.0}, {1.5, 5.0}}};
+constexpr Rows8Lines kRows4x4Lines[1] = {{12, 1.0, {1.0, 3.0}, {1.5, 6.0}}};
 
 // The m-tile height, 32 (0: 32 x 64 tiles), 128 or 256, for `rows` rows over `copies` copies, N rows of a
-// copy's B (fc1: 2 I), K deep, on `cus` CUs.  kind: 0 NT, 1 FC1.
-inline int rows8_tiling(int kind, int64_t rows, int64_t copies, int64_t N, int64_t K, int64_t cus) {
+// copy's B (fc1: 2 I), K deep, on `cus` CUs.
+inline int rows8_tiling(const Rows8Lines& line, int64_t rows, int64_t copies, int64_t N, int64_t K, int64_t cus) {
   const auto div_up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
   const int64_t active = rows < copies ? rows : copies, nk = div_up(K, 128);
   const int64_t mtiles = active > rows / 32 + active / 2 ? active : rows / 32 + active / 2;
   if (mtiles * div_up(N, 64) <= 3 * cus) return 0;
   // a round reads, per CU, 3 x 64 rows of B or 256, and with each tile a copy's rows of A, rows / active
-  if (rows <= kRows8Few[kind] * active)
-    return div_up(mtiles * div_up(N, 64), 3 * cus) * 3 * (64 * active + rows) <
-                   div_up(mtiles * div_up(N, 256), cus) * (256 * active + rows)
+  if (rows <= line.few * active)
+    return line.narrow * (double)(div_up(mtiles * div_up(N, 64), 3 * cus) * 3 * (64 * active + rows)) <
+                   (double)(div_up(mtiles * div_up(N, 256), cus) * (256 * active + rows))
                ? 0 : 32;
   // a copy's last tile half full on average; an eighth of the copies past their first tile
   const auto cost = [&](int64_t tile, int64_t blocks, const double (&round)[2]) {
@@ -62,7 +83,11 @@ inline int rows8_tiling(int kind, int64_t rows, int64_t copies, int64_t N, int64
     const int64_t rounds = div_up((spread > even ? spread : even) * div_up(N, tile), blocks);
     return (double)rounds * (round[0] * (double)nk + round[1]);
   };
-  return cost(256, cus, kRows8Round256[kind]) < cost(128, 2 * cus, kRows8Round128[kind]) ? 256 : 128;
+  return cost(256, cus, line.round256) < cost(128, 2 * cus, line.round128) ? 256 : 128;
+}
+// With weights in 8 bits; kind: 0 NT, 1 FC1.
+inline int rows8_tiling(int kind, int64_t rows, int64_t copies, int64_t N, int64_t K, int64_t cus) {
+  return rows8_tiling(kRows8Lines[kind], rows, copies, N, K, cus);
 }
 
 }  // namespace pmx
