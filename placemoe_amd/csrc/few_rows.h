@@ -484,11 +484,13 @@ __global__ __launch_bounds__(CF::NT, CF::NW * CF::BPC / 4) void few_rows_grouped
 // through the same LDS and leaves as whole 128-byte row pieces.
 constexpr int kWgT = 128, kWgNT = 256;
 
-__global__ __launch_bounds__(kWgNT, 4) void few_rows_wgrad_grouped_gemm_kernel(GemmParams P) {
+constexpr int kWgStage = 2 * kWgT * BK * 2;
+
+// Block `block`'s tile of the gradients, through NST stages of `lds` (1, or 2: a
+// K-tile is on its way while the one before it is multiplied).
+template <int NST>
+__device__ __forceinline__ void wgrad_tile(const GemmParams& P, uint32_t block, char* lds) {
   constexpr int QL = 4;  // 1 KB loads per wave and operand
-  __shared__ __attribute__((aligned(1024))) char lds[2 * kWgT * BK * 2];
-  char* As = lds;
-  char* Bs = lds + kWgT * BK * 2;
   const int lane = threadIdx.x & 63;
   const int wave = uni(threadIdx.x >> 6);
   const int wm = wave >> 1, wn = wave & 1;
@@ -501,8 +503,8 @@ __global__ __launch_bounds__(kWgNT, 4) void few_rows_wgrad_grouped_gemm_kernel(G
   // kernel.)
   const int64_t ntn = (P.N + kWgT - 1) / kWgT, per_g = (P.M + kWgT - 1) / kWgT * ntn;
   const int64_t per_x = (per_g + kNumXcd - 1) / kNumXcd;
-  const int64_t j = blockIdx.x / kNumXcd, g = j / per_x;
-  const int64_t tile = (blockIdx.x + g) % kNumXcd * per_x + j % per_x;
+  const int64_t j = block / kNumXcd, g = j / per_x;
+  const int64_t tile = (block + g) % kNumXcd * per_x + j % per_x;
   if (tile >= per_g) return;
   const int64_t m0 = tile / ntn * kWgT, n0 = tile % ntn * kWgT;
   const int64_t row0 = group_row(P, g), row_end = group_row(P, g + 1);
@@ -532,17 +534,33 @@ __global__ __launch_bounds__(kWgNT, 4) void few_rows_wgrad_grouped_gemm_kernel(G
     const bf16x4_t v1 = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(LDS_TR_PTR(p + 4 * (2 * kWgT)));
     return bf16x8_t{v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
   };
-  for (int64_t r = row0; r < row_end; r += BK) {
+  const auto issue = [&](int64_t r, char* stage) __attribute__((always_inline)) {
     const int64_t rows = uni64(row_end - r < BK ? row_end - r : BK);
     const __amdgpu_buffer_rsrc_t ra = make_rsrc(P.a.p0 + uni64(r) * P.a.ld, (uint64_t)rows * P.a.ld * 2);
     const __amdgpu_buffer_rsrc_t rb = make_rsrc(P.b.p0 + uni64(r) * P.b.ld, (uint64_t)rows * P.b.ld * 2);
 #pragma unroll
     for (int q = 0; q < QL; ++q) {
-      dma16(ra, As + (q * 4 + wave) * 1024, oa[q], 0);
-      dma16(rb, Bs + (q * 4 + wave) * 1024, ob[q], 0);
+      dma16(ra, stage + (q * 4 + wave) * 1024, oa[q], 0);
+      dma16(rb, stage + kWgT * BK * 2 + (q * 4 + wave) * 1024, ob[q], 0);
     }
-    wait_loads<0>();
+  };
+  char* As = lds;
+  if constexpr (NST > 1) {
+    if (row0 < row_end) issue(row0, lds);
+  }
+  for (int64_t r = row0; r < row_end; r += BK) {
+    const int64_t rows = uni64(row_end - r < BK ? row_end - r : BK);
+    if constexpr (NST == 1) {
+      issue(r, lds);
+      wait_loads<0>();
+    } else if (r + BK < row_end) {
+      issue(r + BK, As == lds ? lds + kWgStage : lds);
+      wait_loads<2 * QL>();  // this K-tile has landed, the next one is on its way
+    } else {
+      wait_loads<0>();
+    }
     block_barrier();
+    char* const Bs = As + kWgT * BK * 2;
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
       if (ks * 32 >= rows) break;
@@ -558,6 +576,7 @@ __global__ __launch_bounds__(kWgNT, 4) void few_rows_wgrad_grouped_gemm_kernel(G
     }
     wait_lds();
     block_barrier();  // every wave has read the stage
+    if constexpr (NST > 1) As = As == lds ? lds + kWgStage : lds;
   }
 
   // The wave's 64 x 64 tile through its own 8 KB: row r at 128 bytes, 16-byte
@@ -590,5 +609,23 @@ __global__ __launch_bounds__(kWgNT, 4) void few_rows_wgrad_grouped_gemm_kernel(G
     }
   }
 }
+
+#ifdef PMX_GATED
+// Two gradients in one launch, the first's blocks first: each alone leaves CUs idle.
+struct Two {
+  GemmParams p[2];
+};
+template <int NST>
+__global__ __launch_bounds__(kWgNT, NST == 1 ? 4 : 2) void wgrad_grouped_gemm_kernel(Two two, uint32_t first) {
+  __shared__ __attribute__((aligned(1024))) char lds[NST * kWgStage];
+  const bool second = blockIdx.x >= first;
+  wgrad_tile<NST>(two.p[second], second ? blockIdx.x - first : blockIdx.x, lds);
+}
+#else
+__global__ __launch_bounds__(kWgNT, 4) void few_rows_wgrad_grouped_gemm_kernel(GemmParams P) {
+  __shared__ __attribute__((aligned(1024))) char lds[kWgStage];
+  wgrad_tile<1>(P, blockIdx.x, lds);
+}
+#endif
 
 }  // namespace fr

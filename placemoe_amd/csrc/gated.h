@@ -3,6 +3,15 @@
 
 #include "gate.h"
 
+// A weight gradient c [M, N] = a [K, M]^T b [K, N]; splits > 1: the K rows in chunks, their fp32 sums in parts.
+struct GatedWgradCall {
+  const void *a, *b;
+  int64_t M, N, chunk;
+  int32_t splits;
+  void* c;
+  float* parts;
+};
+
 // The block's products on the grouped GEMM's kernels (a build of
 // grouped_gemm.hip of their own; _f16: fp16 tensors).  Checked by the caller.
 #define PMX_GATED_GEMMS(SUFFIX)                                                                                              \
@@ -20,9 +29,10 @@
   __attribute__((visibility("hidden"))) int pmx_gated_dgate##SUFFIX(const void* dout, const void* w, const float* gates,     \
                                                                     int64_t T, int64_t N, int64_t I, float a, float b,       \
                                                                     void* dgu, pmx_stream_t stream);                         \
-  /* c [M, N] = a [K, M]^T b [K, N], small: on 128 x 128 tiles; splits > 1: the K rows in chunks, their fp32 sums in parts */\
-  __attribute__((visibility("hidden"))) int pmx_gated_tn##SUFFIX(const void* a, const void* b, int64_t K, int64_t M,         \
-                                                                 int64_t N, bool small, int64_t chunk, int32_t splits,       \
-                                                                 void* c, float* parts, pmx_stream_t stream);
+  /* a gradient on 256 x 256 tiles */                                                                                        \
+  __attribute__((visibility("hidden"))) int pmx_gated_tn##SUFFIX(const GatedWgradCall& w, int64_t K, pmx_stream_t stream);   \
+  /* one or two on 128 x 128 tiles, whole */                                                                                 \
+  __attribute__((visibility("hidden"))) int pmx_gated_tn_small##SUFFIX(const GatedWgradCall* w, int32_t n, int64_t K,        \
+                                                                       pmx_stream_t stream);
 PMX_GATED_GEMMS()
 PMX_GATED_GEMMS(_f16)

@@ -207,6 +207,7 @@ struct Gemms<EltBF16> {
   static constexpr auto nt = pmx_gated_nt, nn = pmx_gated_nn;
   static constexpr auto dgate = pmx_gated_dgate;
   static constexpr auto tn = pmx_gated_tn;
+  static constexpr auto tn_small = pmx_gated_tn_small;
 };
 template <>
 struct Gemms<EltF16> {
@@ -214,6 +215,7 @@ struct Gemms<EltF16> {
   static constexpr auto nt = pmx_gated_nt_f16, nn = pmx_gated_nn_f16;
   static constexpr auto dgate = pmx_gated_dgate_f16;
   static constexpr auto tn = pmx_gated_tn_f16;
+  static constexpr auto tn_small = pmx_gated_tn_small_f16;
 };
 
 template <class E>
@@ -235,15 +237,26 @@ int forward_t(const void* x, const void* gate_up, const void* down, int64_t T, i
   return Gemms<E>::nt(act, down, T, N, I, out, stream) != PMX_OK ? PMX_ERR_HIP : PMX_OK;
 }
 
+// The gradients `w`, one or two, over K rows: those on small tiles in one launch.
 template <class E>
-int weight_gradient(const void* a, const void* b, int64_t K, int64_t M, int64_t N, void* c, float* parts, pmx_stream_t stream) {
-  const Wgrad w = wgrad_of(K, M, N);
-  if (Gemms<E>::tn(a, b, K, M, N, w.small, w.chunk, w.splits, c, parts, stream) != PMX_OK) return PMX_ERR_HIP;
-  if (w.splits > 1) {
-    sum_parts_kernel<E><<<(unsigned)((M * N / 4 + 255) / 256), 256, 0, stream>>>(parts, w.splits, M * N, (bf16_t*)c);
-    PMX_LAUNCH_CHECK();
+int weight_gradients(GatedWgradCall* w, int n, int64_t K, float* parts, pmx_stream_t stream) {
+  GatedWgradCall small[2];
+  int few = 0;
+  for (int i = 0; i < n; ++i) {
+    const Wgrad how = wgrad_of(K, w[i].M, w[i].N);
+    w[i].chunk = how.chunk, w[i].splits = how.splits, w[i].parts = parts;
+    if (how.small) {
+      small[few++] = w[i];
+      continue;
+    }
+    if (Gemms<E>::tn(w[i], K, stream) != PMX_OK) return PMX_ERR_HIP;
+    if (how.splits > 1) {
+      const int64_t size = w[i].M * w[i].N;
+      sum_parts_kernel<E><<<(unsigned)((size / 4 + 255) / 256), 256, 0, stream>>>(parts, how.splits, size, (bf16_t*)w[i].c);
+      PMX_LAUNCH_CHECK();
+    }
   }
-  return PMX_OK;
+  return few > 0 ? Gemms<E>::tn_small(small, few, K, stream) : PMX_OK;
 }
 
 template <class E>
@@ -264,8 +277,11 @@ int backward_t(const void* dout, const void* x, const void* gate_up, const void*
   float* parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + dgu_bytes(T, I));
   int rc = PMX_OK;
   if (dx || dgate_up) rc = Gemms<E>::dgate(dout, down, gates, T, N, I, gate.a, gate.b, dgu, stream);
-  if (rc == PMX_OK && ddown) rc = weight_gradient<E>(dout, act, T, N, I, ddown, parts, stream);
-  if (rc == PMX_OK && dgate_up) rc = weight_gradient<E>(dgu, x, T, 2 * I, H, dgate_up, parts, stream);
+  GatedWgradCall w[2];
+  int n = 0;
+  if (ddown) w[n++] = {dout, act, N, I, 0, 0, ddown, nullptr};
+  if (dgate_up) w[n++] = {dgu, x, 2 * I, H, 0, 0, dgate_up, nullptr};
+  if (rc == PMX_OK) rc = weight_gradients<E>(w, n, T, parts, stream);
   if (rc == PMX_OK && dx) rc = Gemms<E>::nn(dgu, gate_up, T, H, 2 * I, dx, stream);
   return rc != PMX_OK ? PMX_ERR_HIP : PMX_OK;
 }

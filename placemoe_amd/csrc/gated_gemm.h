@@ -80,37 +80,54 @@ int PMX_GEMM_FN(pmx_gated_dgate)(const void* dout, const void* w, const float* g
   return launch_rows<KIND_NNS>(P, stream);
 }
 
-int PMX_GEMM_FN(pmx_gated_tn)(const void* a, const void* b, int64_t K, int64_t M, int64_t N, bool small, int64_t chunk,
-                              int32_t splits, void* c, float* parts, pmx_stream_t stream) {
-  if (!fits_rsrc(BK, M) || !fits_rsrc(BK, N)) return PMX_ERR_SHAPE;
+namespace {
+GemmParams wgrad(const GatedWgradCall& w, int64_t K) {
+  GemmParams P = {};
+  P.a = one(w.a, 0, w.M);
+  P.b = one(w.b, 0, w.N);
+  P.G = w.splits, P.chunk = (uint32_t)w.chunk, P.rows = (uint32_t)K;
+  P.K = K, P.M = w.M, P.N = w.N;
+  P.c0 = P.c1 = static_cast<bf16_t*>(w.c);
+  P.parts = w.splits > 1 ? w.parts : nullptr;
+  P.cgs = w.splits > 1 ? w.M * w.N : 0;
+  P.ldc = w.N;
+  P.csplit = INT64_MAX;
+  return P;
+}
+}  // namespace
+
+int PMX_GEMM_FN(pmx_gated_tn)(const GatedWgradCall& w, int64_t K, pmx_stream_t stream) {
+  if (!fits_rsrc(BK, w.M) || !fits_rsrc(BK, w.N)) return PMX_ERR_SHAPE;
   const int grid = grid_size();
   if (grid <= 0) return PMX_ERR_HIP;
-  GemmParams P = {};
-  P.a = one(a, 0, M);
-  P.b = one(b, 0, N);
-  P.G = splits, P.chunk = (uint32_t)chunk, P.rows = (uint32_t)K;
-  P.K = K, P.M = M, P.N = N;
-  P.c0 = P.c1 = static_cast<bf16_t*>(c);
-  P.parts = splits > 1 ? parts : nullptr;
-  P.cgs = splits > 1 ? M * N : 0;
-  P.ldc = N;
-  P.csplit = INT64_MAX;
-  if (small) {  // 128 x 128 tiles, four blocks per CU
-    const int64_t tiles = ((M + fr::kWgT - 1) / fr::kWgT) * ((N + fr::kWgT - 1) / fr::kWgT);
-    const int64_t blocks = (tiles + kNumXcd - 1) / kNumXcd * kNumXcd;
-    if (splits != 1 || blocks >= (int64_t)1 << 30) return PMX_ERR_SHAPE;
-    fr::few_rows_wgrad_grouped_gemm_kernel<<<(unsigned)blocks, fr::kWgNT, 0, stream>>>(P);
-    PMX_LAUNCH_CHECK();
-    return PMX_OK;
-  }
+  const GemmParams P = wgrad(w, K);
   // the four-wave kernel: every row of the operands, and the gradient, within 31-bit offsets
-  if (fits_rsrc(K, M) && fits_rsrc(K, N) && fits_rsrc(2 * M, N)) {
+  if (fits_rsrc(K, w.M) && fits_rsrc(K, w.N) && fits_rsrc(2 * w.M, w.N)) {
     w4::grouped_gemm_w4_kernel<KIND_TN><<<grid, w4::NT, 0, stream>>>(P);
-  } else if (splits > 1) {
+  } else if (w.splits > 1) {
     return PMX_ERR_SHAPE;
   } else {
     grouped_gemm_kernel<KIND_TN, kBM><<<grid, NTHREADS, 0, stream>>>(P);
   }
+  PMX_LAUNCH_CHECK();
+  return PMX_OK;
+}
+
+int PMX_GEMM_FN(pmx_gated_tn_small)(const GatedWgradCall* w, int32_t n, int64_t K, pmx_stream_t stream) {
+  fr::Two two = {};
+  int64_t first = 0, blocks = 0;
+  for (int32_t i = 0; i < n; ++i) {
+    if (!fits_rsrc(BK, w[i].M) || !fits_rsrc(BK, w[i].N)) return PMX_ERR_SHAPE;
+    two.p[i] = wgrad(w[i], K);
+    const int64_t tiles = ((w[i].M + fr::kWgT - 1) / fr::kWgT) * ((w[i].N + fr::kWgT - 1) / fr::kWgT);
+    blocks += (tiles + kNumXcd - 1) / kNumXcd * kNumXcd;
+    if (i == 0) first = blocks;
+  }
+  if (blocks >= (int64_t)1 << 24) return PMX_ERR_SHAPE;
+  const int grid = grid_size();
+  if (grid <= 0) return PMX_ERR_HIP;
+  if (pmx::gated_wgrad_two(blocks, K, grid)) fr::wgrad_grouped_gemm_kernel<2><<<(unsigned)blocks, fr::kWgNT, 0, stream>>>(two, (uint32_t)first);
+  else fr::wgrad_grouped_gemm_kernel<1><<<(unsigned)blocks, fr::kWgNT, 0, stream>>>(two, (uint32_t)first);
   PMX_LAUNCH_CHECK();
   return PMX_OK;
 }

@@ -64,18 +64,21 @@ inline bool gated_few(int64_t T, int64_t H, int64_t I, int64_t N, int64_t cus) {
          gated_fastest(0, T, 2 * I, H, cus).us + gated_fastest(1, T, N, I, cus).us + weights / 5.5e6;
 }
 
-// A weight gradient [M, N] over K rows on `cus` CUs: 128 x 128 tiles that load a
-// K-tile at a time, or 256 x 256 ones over `splits` chunks of the rows, so that they fill the
-// chip where one gradient's own do not; the chunks' fp32 sums are then added by a
-// kernel more.  Costs in us fitted to 110 calls of each (512 x 264 to 7168 x 2048, 17 to
-// 16384 rows), of which the choice is within 2% of the best in geometric mean, 1.31
-// at worst (128 x 128 / 256 x 256 whole / in chunks, their sum included):
-//   rows    M     N      128     256      chunks
-//   1024    2816  4096    29      32       -
-//   1531    2000  1416    33      41       22 + 13 (5)
-//   16384   1536  2048   294     308       89 + 14 (5)
-//   16384   2048  768    274     302       53 + 14 (10)
-//   8192    4096  7168   604     361       -
+// A weight gradient [M, N] over K rows on `cus` CUs: 128 x 128 tiles, or 256 x 256 ones
+// over `splits` chunks of the rows, so that they fill the chip where one
+// gradient's own do not; the chunks' fp32 sums are then added by a kernel more.
+// The small tiles come in two kernels: four blocks per CU that load a K-tile and
+// multiply it in turn, or two that load the next one meanwhile, where there are no
+// more.  Costs in us fitted to 110 calls of each (512 x 264 to 7168 x 2048, 17 to 16384 rows;
+// four blocks / two / 256 x 256 / in chunks and their sum):
+//   rows    M     N
+//   64      2000  1416     6 /   7 /  12 /   -
+//   1531    2000  1416    33 /  24 /  41 /  22 + 13 (5)
+//   1024    2816  4096    29 /  36 /  32 /   -
+//   16384   1536  2048   294 / 182 / 308 /  89 + 14 (5)
+//   16384   2048  768    274 / 183 / 302 /  53 + 14 (10)
+//   8192    4096  7168   604 / 599 / 361 /   -
+inline bool gated_wgrad_two(int64_t blocks, int64_t K, int64_t cus) { return blocks <= 2 * cus && K > 256; }
 struct GatedWgrad {
   bool small;  // 128 x 128 tiles
   int32_t splits;
@@ -83,10 +86,11 @@ struct GatedWgrad {
 inline GatedWgrad gated_wgrad(int64_t K, int64_t M, int64_t N, int64_t cus) {
   const auto div_up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
   const int64_t tiles = div_up(M, 256) * div_up(N, 256), nk = div_up(K, 64);
-  const double per_cu = (double)div_up(div_up(M, 128) * div_up(N, 128), cus);
+  const int64_t blocks = div_up(M, 128) * div_up(N, 128);
+  const double per_cu = (double)div_up(blocks, cus);
   const double ktile = 0.46 * per_cu > 1.03 ? 0.46 * per_cu : 1.03;
   GatedWgrad best = {true, 1};
-  double least = (double)nk * ktile + 3.0 + 1.07 * per_cu;
+  double least = gated_wgrad_two(blocks, K, cus) ? (double)nk * 0.72 + 5.0 : (double)nk * ktile + 3.0 + 1.07 * per_cu;
   for (int64_t s = 1; s <= 32 && s <= nk; ++s) {
     const double sums = s > 1 ? (double)s * (double)M * (double)N * 4e-6 : 0.0;  // MB
     const double rounds = (double)div_up(tiles * s, cus);

@@ -2340,6 +2340,7 @@ int launch_few(const GemmParams& P, int cus, hipStream_t stream) {
   return PMX_OK;
 }
 
+#ifndef PMX_GATED
 template <int KIND>
 int launch(const GemmParams& P, hipStream_t stream) {
   // The LDS tile table keeps an n-tile index in 19 bits.
@@ -2438,6 +2439,7 @@ int launch(const GemmParams& P, hipStream_t stream) {
   PMX_LAUNCH_CHECK();
   return PMX_OK;
 }
+#endif
 
 inline bool a16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 

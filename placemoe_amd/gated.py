@@ -11,7 +11,6 @@ dtypes and shapes raise ``AssertionError``, limits of the kernels
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _capi
 from .kernels import _check_dev, _half, _ptr
@@ -44,7 +43,6 @@ class _GatedFFN(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad_out):
         x, gate_up, down, gates, act = ctx.saved_tensors
         T, H, I = ctx.sizes
