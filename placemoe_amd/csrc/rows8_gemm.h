@@ -707,26 +707,31 @@ __global__ __launch_bounds__(CF::NTH, CF::NW * CF::BPC / 4) void rows8_grouped_g
     };
     // The MFMAs of row half mh in half ks, one per group, `work(group)` behind each.
     auto step4 = [&](auto zero, auto mm, auto kk, auto work) __attribute__((always_inline)) {
-      static_for<0, HN>([&](auto xx) __attribute__((always_inline)) {
-        constexpr int x = decltype(xx)::value, m = decltype(mm)::value * HM + x / CF::FN, n = x % CF::FN;
-        constexpr int ks = decltype(kk)::value;
-        if constexpr (F::A == 8) {
+      if constexpr (F::A == 8) {
+        static_for<0, HN>([&](auto xx) __attribute__((always_inline)) {
+          constexpr int x = decltype(xx)::value, m = decltype(mm)::value * HM + x / CF::FN, n = x % CF::FN;
+          constexpr int ks = decltype(kk)::value;
           acc[m][n] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
               fb[ks][n], fa[ks][m], decltype(zero)::value ? f32x16_t{} : acc[m][n], F::kTypeB, F::kTypeA, n % 2 * 2 + ks,
               sb[0][n / 2], m % 2 * 2 + ks, sa[0][m / 2]);
-        } else {
+          work(xx);
+          __builtin_amdgcn_sched_barrier(0);
+        });
+      } else {
+        // the first 16 bytes of every fragment, then the second: an accumulator's two products lie apart
+        static_for<0, 2 * HN>([&](auto yy) __attribute__((always_inline)) {
+          constexpr int y = decltype(yy)::value, e = y / HN, x = y % HN;
+          constexpr int m = decltype(mm)::value * HM + x / CF::FN, n = x % CF::FN, ks = decltype(kk)::value;
           const i32x8_t &a = fa[ks][m], &b = fb[ks][n];
           acc[m][n] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
-              i32x8_t{b[0], b[1], b[2], b[3], 0, 0, 0, 0}, i32x8_t{a[0], a[1], a[2], a[3], 0, 0, 0, 0},
-              decltype(zero)::value ? f32x16_t{} : acc[m][n], F::kTypeB, F::kTypeA, n % 2 * 2, sb[ks][n / 2], m % 2 * 2,
-              sa[ks][m / 2]);
-          acc[m][n] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
-              i32x8_t{b[4], b[5], b[6], b[7], 0, 0, 0, 0}, i32x8_t{a[4], a[5], a[6], a[7], 0, 0, 0, 0}, acc[m][n], F::kTypeB,
-              F::kTypeA, n % 2 * 2 + 1, sb[ks][n / 2], m % 2 * 2 + 1, sa[ks][m / 2]);
-        }
-        work(xx);
-        __builtin_amdgcn_sched_barrier(0);
-      });
+              i32x8_t{b[4 * e], b[4 * e + 1], b[4 * e + 2], b[4 * e + 3], 0, 0, 0, 0},
+              i32x8_t{a[4 * e], a[4 * e + 1], a[4 * e + 2], a[4 * e + 3], 0, 0, 0, 0},
+              decltype(zero)::value && e == 0 ? f32x16_t{} : acc[m][n], F::kTypeB, F::kTypeA, n % 2 * 2 + e, sb[ks][n / 2],
+              m % 2 * 2 + e, sa[ks][m / 2]);
+          if constexpr (y % 2 == 1) work(Int<y / 2>{});
+          __builtin_amdgcn_sched_barrier(0);
+        });
+      }
     };
     // The MFMAs stay in front of this: left alone, the compiler sinks them past the branches of the
     // issue cursor, behind everything that they are to hide.
