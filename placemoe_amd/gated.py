@@ -48,15 +48,18 @@ class _GatedFFN(torch.autograd.Function):
         T, H, I = ctx.sizes
         N = grad_out.shape[1]
         grad_out = grad_out.contiguous()
-        dx, dup, ddown = (grad_out.new_empty(shape) if need else None
-                          for shape, need in zip(((T, H), (2 * I, H), (N, I)), ctx.needs_input_grad))
+        need_x, need_up, need_down = ctx.needs_input_grad[:3]
+        new = grad_out.new_empty
+        dx = new((T, H)) if need_x else None
+        dup = new((2 * I, H)) if need_up else None
+        ddown = new((N, I)) if need_down else None
         if T == 0:
             for d in (dup, ddown):
                 if d is not None:
                     d.zero_()
             return dx, dup, ddown, None
         ws_bytes = _capi.load().pmx_gated_ffn_workspace_bytes(T, H, I, N)
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=grad_out.device)
+        ws = new(ws_bytes, dtype=torch.uint8)
         _launch("pmx_gated_ffn_bwd", grad_out.dtype, grad_out.device, _ptr(grad_out), _ptr(x), _ptr(gate_up), _ptr(down), _ptr(gates),
                 _ptr(act), T, H, I, N, ctx.gate, _ptr(dx), _ptr(dup), _ptr(ddown), _ptr(ws), ws_bytes)
         return dx, dup, ddown, None

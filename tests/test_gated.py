@@ -38,6 +38,8 @@ def test_c_abi_refusals(suffix):
         assert call(H=1 << 20, I=1 << 10) == SHAPE  # weights of 4 GiB
         assert call(N=1 << 20, I=1 << 10) == SHAPE
         assert call(T=1 << 31) == SHAPE
+        for name in "HIN":  # 256 rows of an operand pass one descriptor
+            assert call(**{**dict(H=8, I=8, N=8), name: 1 << 22}) == SHAPE
         assert call(T=0, at=(None,) * 9 if call is backward else (None,) * 6) == OK
     for k in range(6):  # x, gate_up, down, gu, act, out
         at = [P] * 6
