@@ -30,6 +30,18 @@ def _forward(x: torch.Tensor, gate_up: torch.Tensor, down: torch.Tensor, gate: i
     return out, gates, act
 
 
+class _NoSecond(torch.autograd.Function):
+    """A gradient as it is, differentiable by nobody."""
+
+    @staticmethod
+    def forward(ctx, grad, _):
+        return grad.view_as(grad)
+
+    @staticmethod
+    def backward(ctx, _):
+        raise RuntimeError("gated_ffn has no second derivative")
+
+
 class _GatedFFN(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, gate_up, down, gate):
@@ -48,6 +60,8 @@ class _GatedFFN(torch.autograd.Function):
         T, H, I = ctx.sizes
         N = grad_out.shape[1]
         grad_out = grad_out.contiguous()
+        if grad_out.data_ptr() % 16:  # a part of a larger gradient
+            grad_out = grad_out.clone()
         need_x, need_up, need_down = ctx.needs_input_grad[:3]
         new = grad_out.new_empty
         dx = new((T, H)) if need_x else None
@@ -62,6 +76,9 @@ class _GatedFFN(torch.autograd.Function):
         ws = new(ws_bytes, dtype=torch.uint8)
         _launch("pmx_gated_ffn_bwd", grad_out.dtype, grad_out.device, _ptr(grad_out), _ptr(x), _ptr(gate_up), _ptr(down), _ptr(gates),
                 _ptr(act), T, H, I, N, ctx.gate, _ptr(dx), _ptr(dup), _ptr(ddown), _ptr(ws), ws_bytes)
+        if torch.is_grad_enabled():  # create_graph: a loss over these gradients must not miss its terms silently
+            mark = torch.empty(0, requires_grad=True)
+            dx, dup, ddown = (None if d is None else _NoSecond.apply(d, mark) for d in (dx, dup, ddown))
         return dx, dup, ddown, None
 
 

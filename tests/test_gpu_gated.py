@@ -259,6 +259,28 @@ def test_a_leaf_used_twice_and_two_backwards(cuda):
         d.sum().backward()
 
 
+def test_a_gradient_at_an_odd_address(cuda):
+    """Out's gradient as a part of a larger one, two bytes past a boundary."""
+    x, up, down, dout = _case(cuda, 20, 64, 48, 56, BF)
+    want = _run(x, up, down, dout, "silu")
+    leaves = [t.clone().requires_grad_(True) for t in (x, up, down)]
+    both = torch.cat([leaves[0].detach().flatten()[:1], placemoe_amd.gated_ffn(*leaves).flatten()])
+    both.backward(torch.cat([dout.flatten()[:1], dout.flatten()]))
+    for leaf, w in zip(leaves, want[1:]):
+        assert_exact(leaf.grad, w)
+
+
+def test_a_loss_over_gradients_is_refused(cuda):
+    x, up, down, dout = _case(cuda, 20, 64, 48, 56, BF)
+    a = x.clone().requires_grad_(True)
+    for weights in ((up, down), tuple(t.clone().requires_grad_(True) for t in (up, down))):
+        out = placemoe_amd.gated_ffn(a, *weights)
+        (d,) = torch.autograd.grad(out, a, dout, create_graph=True)
+        assert_exact(d, _run(x, up, down, dout, "silu")[1])
+        with pytest.raises(RuntimeError, match="second"):
+            (out.sum() + d.square().sum()).backward()
+
+
 def test_no_tokens(cuda):
     x, up, down, dout = _case(cuda, 4, 64, 48, 56, BF)
     got = _run(x[:0], up, down, dout[:0], "silu")

@@ -2,6 +2,9 @@
 refusals, and the wrappers' checks (all before any launch)."""
 
 import ctypes
+import shutil
+import subprocess
+from pathlib import Path
 
 import numpy as np
 import pytest
@@ -11,6 +14,7 @@ import placemoe_amd
 from oracle import rows4_oracle as O
 from placemoe_amd import _capi, rows4, rows8
 
+ROOT = Path(__file__).resolve().parent.parent
 BF = torch.bfloat16
 P = ctypes.c_void_p(256)
 ARG, SHAPE, OK = _capi.PMX_ERR_ARG, _capi.PMX_ERR_SHAPE, _capi.PMX_OK
@@ -122,3 +126,37 @@ def test_wrappers_refuse_host_tensors():
     ):
         with pytest.raises(AssertionError, match="GPU tensors"):
             call()
+
+
+# us on 32 x 64, 32 x 256, 128 x 128 and 256 x 256 tiles (log-normal counts with sigma 0.4):
+# NT of 8-bit rows, NT of 4-bit rows, fc1
+MEASURED = {
+    (64, 160, 1536, 2048): ((20, 23, 26, 50), (18, 20, 21, 34), (30, 32, 39, 88)),
+    (640, 160, 1536, 2048): ((45, 44, 58, 95), (40, 42, 45, 64), (67, 59, 103, 170)),
+    (1600, 160, 1536, 2048): ((46, 46, 60, 95), (41, 42, 46, 64), (68, 59, 103, 171)),
+    (5120, 160, 1536, 2048): ((67, 62, 64, 97), (46, 50, 47, 66), (97, 84, 105, 172)),
+    (20480, 160, 1536, 2048): ((192, 162, 101, 115), (112, 104, 64, 81), (284, 228, 162, 194)),
+    (81920, 160, 1536, 2048): ((684, 559, 296, 280), (392, 354, 192, 188), (1035, 811, 516, 505)),
+    (1, 16, 4096, 7168): ((20, 26, 30, 70), (12, 18, 20, 42), (31, 42, 52, 132)),
+    (256, 16, 4096, 7168): ((44, 38, 46, 74), (39, 38, 39, 46), (61, 46, 88, 139)),
+    (16000, 16, 4096, 7168): ((996, 830, 436, 409), (550, 490, 275, 253), (1603, 1276, 820, 763)),
+}
+
+
+def test_tiling_rule_takes_a_fast_one(tmp_path):
+    """None of these calls loses more than a twelfth to its best tiling."""
+    cxx = shutil.which("g++") or shutil.which("c++")
+    if cxx is None:
+        pytest.skip("no host C++ compiler")
+    exe = tmp_path / "rows4_rule"
+    subprocess.run([cxx, "-O2", "-std=c++17", f"-I{ROOT / 'placemoe_amd' / 'csrc'}", str(ROOT / "tests" / "rows4_rule_main.cpp"),
+                    "-o", str(exe)], check=True)
+    calls = [(line, call, us) for call, lines in MEASURED.items() for line, us in zip((0, 2, 1), lines)]
+    asked = "\n".join(f"{line} {' '.join(map(str, call))} 256" for line, call, _ in calls)
+    heights = subprocess.run([str(exe)], input=asked, check=True, capture_output=True, text=True).stdout.split()
+    taken = set()
+    for (line, call, us), height in zip(calls, map(int, heights)):
+        t = dict(zip((0, 32, 128, 256), us))
+        assert t[height] <= 13 / 12 * min(us), (line, call, height, t)
+        taken.add(height)
+    assert taken == {0, 32, 128, 256}
