@@ -23,7 +23,7 @@
 // for all tokens, its waves a share of the columns each, straight from memory to
 // the matrix instruction (16 weight rows x 16 tokens, 32 columns); their sums
 // meet in LDS.  Bound: HBM; from some tens of tokens on, their being read again by
-// every block.  One token through 7168 x 2048: 23.7 us, 3.7 TB/s of weights (a large
+// every block.  One token through 7168 x 2048: 22.4 us, 3.9 TB/s of weights (a large
 // copy: 4.8), on 64 x 128 tiles 72; 64 tokens 66 and 80.  (32 weight rows per block:
 // as fast for few, 30% slower where that leaves less than a block per CU.)
 
@@ -130,7 +130,6 @@ __global__ __launch_bounds__(64 * kFewWaves) void gated_few_fc2_kernel(const bf1
 template <class E, int FT>
 int few_forward(const void* x, const void* gate_up, const void* down, int64_t T, int64_t H, int64_t I, int64_t N, const Gate& gate,
                 float* gates, void* act, void* out, pmx_stream_t stream) {
-  
   gated_few_fc1_kernel<E, FT><<<(unsigned)(I / 8), 64 * kFewWaves, 0, stream>>>((const bf16_t*)x, (const bf16_t*)gate_up, T, H, I, gate,
                                                                                 gates, (bf16_t*)act);
   PMX_LAUNCH_CHECK();
@@ -305,7 +304,7 @@ size_t pmx_gated_ffn_workspace_bytes(int64_t T, int64_t H, int64_t I, int64_t N)
                                 const void* act, int64_t T, int64_t H, int64_t I, int64_t N, int32_t gate, void* dx,        \
                                 void* dgate_up, void* ddown, void* workspace, size_t workspace_bytes, pmx_stream_t stream) { \
     return backward_t<E>(dout, x, gate_up, down, gates, act, T, H, I, N, gate, dx, dgate_up, ddown, workspace,              \
-                         workspace_bytes, stream);                                                                                           \
+                         workspace_bytes, stream);                                                                          \
   }
 
 PMX_GATED_FFN(, EltBF16)
