@@ -19,15 +19,22 @@ from .rows8 import _launch
 GATES = {"silu": 0, "gelu_tanh": 1, "quick_gelu": 2}
 
 
-def _forward(x: torch.Tensor, gate_up: torch.Tensor, down: torch.Tensor, gate: int, keep: bool):
-    """(out, gate and up sums or None, act)."""
+def _forward(x: torch.Tensor, gate_up: torch.Tensor, down: torch.Tensor, gate: int, keep_gates: bool, keep_act: bool):
+    """(out, what is kept): the gate and up sums in fp32, behind them act where both are wanted (one tensor: each
+    takes some microseconds of a small call), or act alone."""
     T, H = x.shape
     N, I = down.shape
-    act, out = x.new_empty((T, I)), x.new_empty((T, N))
-    gates = x.new_empty((T, 2 * I), dtype=torch.float32) if keep else None
-    _launch("pmx_gated_ffn_fwd", x.dtype, x.device, _ptr(x), _ptr(gate_up), _ptr(down), T, H, I, N, gate, _ptr(gates), _ptr(act),
-            _ptr(out))
-    return out, gates, act
+    out = x.new_empty((T, N))
+    if keep_gates:
+        kept = x.new_empty((T * I * 5 + 1) // 2 if keep_act else T * I * 2, dtype=torch.float32)
+        gates = kept.data_ptr()
+        own_act = None if keep_act else x.new_empty((T, I))
+        act = gates + T * I * 8 if keep_act else own_act.data_ptr()
+    else:
+        kept = x.new_empty((T, I))
+        gates, act = None, kept.data_ptr()
+    _launch("pmx_gated_ffn_fwd", x.dtype, x.device, _ptr(x), _ptr(gate_up), _ptr(down), T, H, I, N, gate, gates, act, _ptr(out))
+    return out, kept
 
 
 class _NoSecond(torch.autograd.Function):
@@ -46,17 +53,17 @@ class _GatedFFN(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, gate_up, down, gate):
         need_x, need_up, need_down = ctx.needs_input_grad[:3]
-        out, gates, act = _forward(x, gate_up, down, gate, need_x or need_up)
+        out, kept = _forward(x, gate_up, down, gate, need_x or need_up, need_down)
         ctx.gate = gate
         # what the wanted gradients read
-        ctx.save_for_backward(x if need_up else None, gate_up if need_x else None, down if need_x or need_up else None, gates,
-                              act if need_down else None)
+        ctx.save_for_backward(x if need_up else None, gate_up if need_x else None, down if need_x or need_up else None, kept)
+        ctx.has_gates = need_x or need_up  # (in the backward these flags say what the one call wants)
         ctx.sizes = (*x.shape, down.shape[1])
         return out
 
     @staticmethod
     def backward(ctx, grad_out):
-        x, gate_up, down, gates, act = ctx.saved_tensors
+        x, gate_up, down, kept = ctx.saved_tensors
         T, H, I = ctx.sizes
         N = grad_out.shape[1]
         grad_out = grad_out.contiguous()
@@ -72,10 +79,12 @@ class _GatedFFN(torch.autograd.Function):
                 if d is not None:
                     d.zero_()
             return dx, dup, ddown, None
+        gates = kept.data_ptr()
+        act = gates + (T * I * 8 if ctx.has_gates else 0)
         ws_bytes = _capi.load().pmx_gated_ffn_workspace_bytes(T, H, I, N)
         ws = new(ws_bytes, dtype=torch.uint8)
-        _launch("pmx_gated_ffn_bwd", grad_out.dtype, grad_out.device, _ptr(grad_out), _ptr(x), _ptr(gate_up), _ptr(down), _ptr(gates),
-                _ptr(act), T, H, I, N, ctx.gate, _ptr(dx), _ptr(dup), _ptr(ddown), _ptr(ws), ws_bytes)
+        _launch("pmx_gated_ffn_bwd", grad_out.dtype, grad_out.device, _ptr(grad_out), _ptr(x), _ptr(gate_up), _ptr(down),
+                gates if ctx.has_gates else None, act if need_down else None, T, H, I, N, ctx.gate, _ptr(dx), _ptr(dup), _ptr(ddown), _ptr(ws), ws_bytes)
         if torch.is_grad_enabled():  # create_graph: a loss over these gradients must not miss its terms silently
             mark = torch.empty(0, requires_grad=True)
             dx, dup, ddown = (None if d is None else _NoSecond.apply(d, mark) for d in (dx, dup, ddown))
@@ -111,5 +120,5 @@ def gated_ffn(x: torch.Tensor, gate_up: torch.Tensor, down: torch.Tensor, activa
     if torch.is_grad_enabled() and (x.requires_grad or gate_up.requires_grad or down.requires_grad):
         out = _GatedFFN.apply(rows, gate_up, down, GATES[activation])
     else:
-        out = _forward(rows, gate_up, down, GATES[activation], False)[0]
+        out = _forward(rows, gate_up, down, GATES[activation], False, False)[0]
     return out if x.dim() == 2 else out.view(*x.shape[:-1], N)

@@ -236,6 +236,18 @@ def test_only_the_wanted_gradients(cuda, T):
                 assert leaf.grad is None
 
 
+@pytest.mark.parametrize("T", [3, 120])
+def test_some_gradients_of_a_graph_that_has_all(cuda, T):
+    case = _case(cuda, T, 264, 136, 200, BF)
+    full = _run(*case, "silu")
+    leaves = [t.clone().requires_grad_(True) for t in case[:3]]
+    out = placemoe_amd.gated_ffn(*leaves)
+    for mask in (1, 2, 4, 3, 5, 6, 7):
+        wanted = [k for k in range(3) if mask >> k & 1]
+        for k, d in zip(wanted, torch.autograd.grad(out, [leaves[k] for k in wanted], case[3], retain_graph=True)):
+            assert_exact(d, full[1 + k], f"mask {mask}, leaf {k}")
+
+
 def test_a_leaf_used_twice_and_two_backwards(cuda):
     """Tied tokens and weights accumulate; a retained graph gives its gradients again."""
     x, up, down, dout = _case(cuda, 50, 64, 48, 64, BF)
