@@ -20,19 +20,17 @@ GATES = {"silu": 0, "gelu_tanh": 1, "quick_gelu": 2}
 
 
 def _forward(x: torch.Tensor, gate_up: torch.Tensor, down: torch.Tensor, gate: int, keep_gates: bool, keep_act: bool):
-    """(out, what is kept): the gate and up sums in fp32, behind them act where both are wanted (one tensor: each
-    takes some microseconds of a small call), or act alone."""
+    """(out, what is kept): the bytes of the gate and up sums in fp32 and, behind them, of act; of either alone where
+    the other is not wanted (one tensor: each takes some microseconds of a small call)."""
     T, H = x.shape
     N, I = down.shape
     out = x.new_empty((T, N))
-    if keep_gates:
-        kept = x.new_empty((T * I * 5 + 1) // 2 if keep_act else T * I * 2, dtype=torch.float32)
-        gates = kept.data_ptr()
-        own_act = None if keep_act else x.new_empty((T, I))
-        act = gates + T * I * 8 if keep_act else own_act.data_ptr()
-    else:
-        kept = x.new_empty((T, I))
-        gates, act = None, kept.data_ptr()
+    behind = 8 * T * I if keep_gates else 0
+    alone = keep_gates and not keep_act
+    kept = x.new_empty(behind if alone else behind + 2 * T * I, dtype=torch.uint8)
+    passing = x.new_empty((T, I)) if alone else None  # act, on its way to fc2 only
+    gates = kept.data_ptr() if keep_gates else None
+    act = passing.data_ptr() if alone else kept.data_ptr() + behind
     _launch("pmx_gated_ffn_fwd", x.dtype, x.device, _ptr(x), _ptr(gate_up), _ptr(down), T, H, I, N, gate, gates, act, _ptr(out))
     return out, kept
 

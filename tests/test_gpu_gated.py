@@ -248,6 +248,24 @@ def test_some_gradients_of_a_graph_that_has_all(cuda, T):
             assert_exact(d, full[1 + k], f"mask {mask}, leaf {k}")
 
 
+def test_under_checkpoints_and_saved_elsewhere(cuda):
+    """Recomputed in the backward, and with what is kept moved to the host meanwhile."""
+    from torch.utils.checkpoint import checkpoint
+
+    x, up, down, dout = _case(cuda, 90, 264, 136, 200, BF)
+    want = _run(x, up, down, dout, "silu")
+    for way in ("reentrant", "not", "host"):
+        leaves = [t.clone().requires_grad_(True) for t in (x, up, down)]
+        if way == "host":
+            with torch.autograd.graph.save_on_cpu():
+                out = placemoe_amd.gated_ffn(*leaves)
+        else:
+            out = checkpoint(placemoe_amd.gated_ffn, *leaves, use_reentrant=way == "reentrant")
+        out.backward(dout)
+        for a, w in zip([out.detach(), *(t.grad for t in leaves)], want):
+            assert_exact(a, w, way)
+
+
 def test_a_leaf_used_twice_and_two_backwards(cuda):
     """Tied tokens and weights accumulate; a retained graph gives its gradients again."""
     x, up, down, dout = _case(cuda, 50, 64, 48, 64, BF)
