@@ -31,6 +31,9 @@
 // against 2.46); FC1 of 65536 rows of 160 copies of 1536 x 2048 0.42-0.53 ms, 0.8-1.0
 // PFLOP/s (bf16 products of 8192^3: 1.28); 768 rows of those copies 89 (NT) and 91 us,
 // 5.6 TB/s of weights.
+// 4-bit weights: both operands in 4 bits, NT of the same size 0.91-0.97 ms, 4.0-4.2 PFLOP/s at
+// the power limit (operands of zeros 0.715); FC1 of 65536 rows of 160 copies of 1536 x 2048
+// 0.48-0.50 ms; 768 rows of them, NT, 45 us, 5.9 TB/s of weights.
 //
 // Tiles of BM x BN, K in steps of 128 bytes of A (128 columns, or 256) through a ring of NST stages filled by
 // buffer->LDS loads; 128-byte rows with 16-byte chunk c at c ^ ((row >> 1) & 7),
