@@ -33,7 +33,7 @@
 // 5.6 TB/s of weights.
 // 4-bit weights: both operands in 4 bits, NT of the same size 0.91-0.97 ms, 4.0-4.2 PFLOP/s at
 // the power limit (operands of zeros 0.715); FC1 of 65536 rows of 160 copies of 1536 x 2048
-// 0.48-0.50 ms; 768 rows of them, NT, 45 us, 5.9 TB/s of weights.
+// 0.41-0.46 ms; 768 rows of them, NT, 45 us, 5.9 TB/s of weights.
 //
 // Tiles of BM x BN, K in steps of 128 bytes of A (128 columns, or 256) through a ring of NST stages filled by
 // buffer->LDS loads; 128-byte rows with 16-byte chunk c at c ^ ((row >> 1) & 7),
@@ -90,6 +90,9 @@ struct Params8 {
   uint8_t* c_low;            // NT in 24 bits: the low bytes [M, N] of c
   uint8_t *q, *qs;           // FC1: act's codes [M, I] and exponents
   const bf16_t* row_w;       // FC1: [M], null: 1
+  // Of 8-bit rows with 4-bit B, on 256-row tiles: without each group's rows past its whole 256s where they are 128 or
+  // fewer; on 128-row tiles: those alone (rows8_rests_apart).
+  bool rests_apart;
 };
 
 // WM x WN waves, each FM x FN tiles of 32 x 32; NST stages; BPC blocks per CU.
@@ -475,6 +478,15 @@ __global__ __launch_bounds__(CF::NTH, CF::NW * CF::BPC / 4) void rows8_grouped_g
     return o < 0 ? 0 : o > P.M ? (int32_t)P.M : o;
   };
 
+  constexpr bool kMayPart = CF::F::kMixed && CF::BM >= 128;
+  const auto tiles_of = [&](int32_t rows) __attribute__((always_inline)) {
+    if constexpr (kMayPart) {
+      const int32_t rest = rows & 255;
+      if (P.rests_apart) return CF::BM == 256 ? (rows >> 8) + (rest > 128) : (int32_t)(rest > 0 && rest <= 128);
+    }
+    return (rows + CF::BM - 1) / CF::BM;
+  };
+
   // Prefix of the groups' m-tiles, a group per thread at a time: a scan within each wave, then over the waves.
   // Four groups' loads of a thread go out together.
   {
@@ -491,7 +503,7 @@ __global__ __launch_bounds__(CF::NTH, CF::NW * CF::BPC / 4) void rows8_grouped_g
       for (int i = 0; i < 4; ++i) {
         const int32_t g = base + i * CF::NTH + t;
         if (base + i * CF::NTH >= G) break;
-        const int32_t inc = wave_scan((o[i][1] - o[i][0] + CF::BM - 1) / CF::BM);  // past the last group: none
+        const int32_t inc = wave_scan(tiles_of(o[i][1] - o[i][0]));  // past the last group: none
         const bool descends = __ballot(o[i][1] < o[i][0]) != 0;
         int32_t sum = __builtin_amdgcn_readlane(inc, 63), lower = 0;
         bad |= descends;
@@ -553,6 +565,9 @@ __global__ __launch_bounds__(CF::NTH, CF::NW * CF::BPC / 4) void rows8_grouped_g
     at.ntile = (int32_t)(rest / high);
     at.row0 = uni(offset(g)) + (int32_t)(band + rest % high) * CF::BM;
     at.row_end = uni(offset(g + 1));
+    if constexpr (kMayPart && CF::BM == 128) {
+      if (P.rests_apart) at.row0 += (at.row_end - at.row0) & ~255;  // the group's one tile
+    }
   };
 
   // Issue cursor, running ahead of the K-tile being multiplied.
@@ -1090,7 +1105,17 @@ int launch(const Params8& P, pmx_stream_t stream) {
   const int cus = cu_count();
   if (cus <= 0) return PMX_ERR_HIP;
   const pmx::Rows8Lines& line = F::B == 8 ? pmx::kRows8Lines[KIND] : F::A == 8 ? pmx::kRows8x4Lines[KIND] : pmx::kRows4x4Lines[NT8];
-  switch (pmx::rows8_tiling(line, P.M, P.G, P.N, P.K / (8 / F::A), cus)) {
+  const int64_t ka = P.K / (8 / F::A);
+  if constexpr (F::kMixed) {
+    if (pmx::rows8_rests_apart(line, P.M, P.G, P.N, ka, cus)) {
+      Params8 Q = P;
+      Q.rests_apart = true;
+      if (!tiles_fit<KIND, Rows128<F>>(P, cus)) return PMX_ERR_SHAPE;  // nothing is launched but both
+      if (const int rc = launch_cfg<E, KIND, Rows256<F>>(Q, cus, stream)) return rc;
+      return launch_cfg<E, KIND, Rows128<F>>(Q, cus, stream);
+    }
+  }
+  switch (pmx::rows8_tiling(line, P.M, P.G, P.N, ka, cus)) {
     case 0: return launch_cfg<E, KIND, Narrow32<F>>(P, cus, stream);
     case 32: return launch_cfg<E, KIND, Rows32<F>>(P, cus, stream);
     case 128: return launch_cfg<E, KIND, Rows128<F>>(P, cus, stream);

@@ -65,6 +65,13 @@ constexpr Rows8Lines kRows8Lines[2] = {{16, 1.0, {1.25, 2.0}, {1.5, 5.0}}, {32, 
 constexpr Rows8Lines kRows8x4Lines[2] = {{24, 1.05, {0.9, 3.0}, {1.5, 5.0}}, {48, 1.05, {0.9, 3.0}, {1.5, 5.0}}};
 constexpr Rows8Lines kRows4x4Lines[1] = {{12, 1.0, {1.0, 3.0}, {1.5, 6.0}}};
 
+// A call in tiles of one height: a copy's last tile half full on average; an eighth of the copies past their first tile.
+inline double rows8_cost(int64_t tile, int64_t blocks, const double (&round)[2], int64_t rows, int64_t active, int64_t N, int64_t nk) {
+  const int64_t spread = active + active / 8, even = rows / tile + active / 2;
+  const int64_t tiles = (spread > even ? spread : even) * ((N + tile - 1) / tile);
+  return (double)((tiles + blocks - 1) / blocks) * (round[0] * (double)nk + round[1]);
+}
+
 // The m-tile height, 32 (0: 32 x 64 tiles), 128 or 256, for `rows` rows over `copies` copies, N rows of a
 // copy's B (fc1: 2 I), K deep, on `cus` CUs.
 inline int rows8_tiling(const Rows8Lines& line, int64_t rows, int64_t copies, int64_t N, int64_t K, int64_t cus) {
@@ -77,13 +84,27 @@ inline int rows8_tiling(const Rows8Lines& line, int64_t rows, int64_t copies, in
     return line.narrow * (double)(div_up(mtiles * div_up(N, 64), 3 * cus) * 3 * (64 * active + rows)) <
                    (double)(div_up(mtiles * div_up(N, 256), cus) * (256 * active + rows))
                ? 0 : 32;
-  // a copy's last tile half full on average; an eighth of the copies past their first tile
-  const auto cost = [&](int64_t tile, int64_t blocks, const double (&round)[2]) {
-    const int64_t spread = active + active / 8, even = rows / tile + active / 2;
-    const int64_t rounds = div_up((spread > even ? spread : even) * div_up(N, tile), blocks);
-    return (double)rounds * (round[0] * (double)nk + round[1]);
-  };
-  return cost(256, cus, line.round256) < cost(128, 2 * cus, line.round128) ? 256 : 128;
+  return rows8_cost(256, cus, line.round256, rows, active, N, nk) < rows8_cost(128, 2 * cus, line.round128, rows, active, N, nk) ? 256 : 128;
+}
+
+// Rows in 8 bits with weights in 4, past the few-rows line: whether a copy's rows past its whole 256s, where they are
+// 128 or fewer (half of the copies), run on 128-row tiles in a launch of their own, and the other rows on 256-row
+// tiles.  That saves half a 256-row tile per copy and costs half a 128-row one, a quarter of a round more for each
+// launch's last, and the launch.  Over 110 (NT) and 97 (fc1) calls of 10 layers, 100 to 4000 rows per copy, it takes 30 of
+// each, to 0.962 and 0.942 of the better tiling's time, 1.08 at worst; at 160 copies (us, 128 / 256 / so):
+//   rows   N     K     NT                 fc1
+//   41k    1536  2048  164 / 175 / 152    307 / 294 / 261
+//   82k    1536  2048  313 / 284 / 270    536 / 486 / 466
+//   82k    2048  768   167 / 172 / 154    313 / 285 / 261
+// (Rows in 4 bits gain nothing: 0.87 to 1.07 of the better one's in such calls, 0.99 on average.)
+inline bool rows8_rests_apart(const Rows8Lines& line, int64_t rows, int64_t copies, int64_t N, int64_t K, int64_t cus) {
+  if (rows < 256 * copies || rows <= line.few * copies) return false;
+  const int64_t nk = (K + 127) / 128;
+  const auto rounds = [&](double mtiles, int64_t tile, int64_t blocks) { return mtiles * (double)((N + tile - 1) / tile) / (double)blocks + 0.25; };
+  const double apart = rounds((double)(rows / 256), 256, cus) * (line.round256[0] * (double)nk + line.round256[1]) +
+                       rounds((double)(copies + 1) / 2, 128, 2 * cus) * (line.round128[0] * (double)nk + line.round128[1]) + 12.0;
+  return apart < rows8_cost(256, cus, line.round256, rows, copies, N, nk) &&
+         apart < rows8_cost(128, 2 * cus, line.round128, rows, copies, N, nk);
 }
 // With weights in 8 bits; kind: 0 NT, 1 FC1.
 inline int rows8_tiling(int kind, int64_t rows, int64_t copies, int64_t N, int64_t K, int64_t cus) {

@@ -368,6 +368,43 @@ def test_wide_fc1_equals_single_copies(cuda, name):
         assert torch.equal(act.scales[:, rows], ref.scales), f"copy {g}"
 
 
+# Sixteen kinds of rests past whole 256s, ten of each: calls whose short rests are launched apart
+RESTS = ([0, 1, 127, 128, 129, 255, 256, 257, 383, 384, 385, 511, 512, 513, 641, 1100] * 10, 512, 2048)
+
+
+@pytest.mark.parametrize("dtype", [BF, F16])
+def test_rests_apart_equal_single_copies(cuda, dtype):
+    """Each copy alone runs on other tiles: the same bits; rows before the first group and behind the last stay."""
+    counts, N, K = RESTS
+    before, behind = 3, 5
+    G, M, I = len(counts), before + sum(counts) + behind, N // 2
+    off = (_offsets(counts) + before).to(torch.int32)
+    x = rows8.quantize_rows(_randn((M, K), 11).to(cuda).to(dtype))
+    w = rows4.quantize_rows4(_randn((G, N, K), 12, std=0.06).to(cuda).to(dtype))
+    suffix = "_f16" if dtype == F16 else ""
+    s, on = torch.cuda.current_stream().cuda_stream, off.to(cuda)
+    lib = _capi.load()
+    c = torch.full((M, N), -7.0, dtype=dtype, device=cuda)
+    assert getattr(lib, "pmx_rows4_group_gemm_nt" + suffix)(
+        x.codes.data_ptr(), x.scales.data_ptr(), 8, w.codes.data_ptr(), w.scales.data_ptr(), on.data_ptr(), G, M, N, K, c.data_ptr(),
+        s) == _capi.PMX_OK
+    act = torch.full((M, I), 0x55, dtype=torch.uint8, device=cuda)
+    scales = torch.full((1, M, 16), 0x55, dtype=torch.uint8, device=cuda)
+    assert getattr(lib, "pmx_rows4_gemm_fc1_swiglu" + suffix)(
+        x.codes.data_ptr(), x.scales.data_ptr(), M, None, w.codes.data_ptr(), w.scales.data_ptr(), on.data_ptr(), G, M, K, I, None,
+        act.data_ptr(), scales.data_ptr(), s) == _capi.PMX_OK
+    for rows in (slice(0, before), slice(M - behind, M)):
+        assert (c[rows] == -7).all() and (act[rows] == 0x55).all() and (scales[:, rows] == 0x55).all()
+    for g, n in enumerate(counts):
+        rows = slice(int(off[g]), int(off[g]) + n)
+        one = rows4.Rows4(w.codes[g:g + 1].contiguous(), w.scales[g:g + 1].contiguous(), K, dtype)
+        xg = rows8.Rows8(x.codes[rows].contiguous(), x.scales[:, rows].contiguous(), dtype)
+        alone = _offsets([n]).to(cuda)
+        assert_exact(c[rows], rows4.group_gemm_nt_rows4(xg, one, alone), f"copy {g}")
+        ref = rows4.gemm_fc1_swiglu_rows4(xg, one, alone)
+        assert torch.equal(act[rows], ref.codes.view(torch.uint8)) and torch.equal(scales[:, rows], ref.scales), f"copy {g}"
+
+
 @pytest.mark.parametrize("rows", [3, 100, 1500, 9000])
 @pytest.mark.parametrize("I", [16, 48, 144, 512, 528])
 def test_fc1_writes_every_scale(cuda, I, rows):

@@ -13,6 +13,7 @@ import torch
 import placemoe_amd
 from oracle import rows4_oracle as O
 from placemoe_amd import _capi, rows4, rows8
+from tests import test_gpu_rows4
 
 ROOT = Path(__file__).resolve().parent.parent
 BF = torch.bfloat16
@@ -143,20 +144,60 @@ MEASURED = {
 }
 
 
-def test_tiling_rule_takes_a_fast_one(tmp_path):
-    """None of these calls loses more than a twelfth to its best tiling."""
+# ... and on 256 x 256 ones with the short rests on 128 x 128 ones, in the same order
+APART = {
+    (16000, 160, 1536, 2048): ((94.8, 109.2, 92.5), (173.9, 200.8, 150.8)),
+    (40960, 160, 1536, 2048): ((163.8, 175.4, 152.0), (306.7, 293.9, 260.6)),
+    (81920, 160, 1536, 2048): ((312.6, 283.8, 269.9), (535.7, 486.0, 465.8)),
+    (65600, 160, 2048, 768): ((135.4, 149.1, 135.8), (259.4, 242.1, 219.8)),
+    (81920, 160, 2048, 768): ((166.7, 172.2, 153.7), (313.3, 284.8, 261.0)),
+    (5760, 16, 4096, 7168): ((181.5, 177.7, 208.2), (336.4, 317.8, 381.8)),
+    (16000, 16, 4096, 7168): ((453.8, 409.7, 385.9), (823.1, 769.9, 710.0)),
+    (2048, 8, 2048, 1024): ((12.2, 17.9, 26.1), (19.1, 29.3, 40.8)),
+    (179200, 256, 512, 512): ((80.2, 82.6, 85.1), (139.8, 136.4, 133.7)),
+    (32000, 32, 2816, 4096): ((362.0, 338.8, 329.2), (669.2, 647.4, 619.8)),
+}
+
+
+@pytest.fixture(scope="module")
+def tiling(tmp_path_factory):
     cxx = shutil.which("g++") or shutil.which("c++")
     if cxx is None:
         pytest.skip("no host C++ compiler")
-    exe = tmp_path / "rows4_rule"
+    exe = tmp_path_factory.mktemp("rule") / "rows4_rule"
     subprocess.run([cxx, "-O2", "-std=c++17", f"-I{ROOT / 'placemoe_amd' / 'csrc'}", str(ROOT / "tests" / "rows4_rule_main.cpp"),
                     "-o", str(exe)], check=True)
+
+    def ask(calls):
+        """calls: (line, rows, copies, N, K) -> tile heights, on 256 CUs."""
+        asked = "\n".join(f"{' '.join(map(str, c))} 256" for c in calls)
+        return [int(x) for x in subprocess.run([str(exe)], input=asked, check=True, capture_output=True, text=True).stdout.split()]
+
+    return ask
+
+
+def test_tiling_rule_takes_a_fast_one(tiling):
+    """None of these calls loses more than a twelfth to its best tiling."""
     calls = [(line, call, us) for call, lines in MEASURED.items() for line, us in zip((0, 2, 1), lines)]
-    asked = "\n".join(f"{line} {' '.join(map(str, call))} 256" for line, call, _ in calls)
-    heights = subprocess.run([str(exe)], input=asked, check=True, capture_output=True, text=True).stdout.split()
     taken = set()
-    for (line, call, us), height in zip(calls, map(int, heights)):
+    for (line, call, us), height in zip(calls, tiling([(line, *call) for line, call, _ in calls])):
+        taken.add(height)
+        if height == 384:  # timed in APART
+            assert min(us) in us[2:]
+            continue
         t = dict(zip((0, 32, 128, 256), us))
         assert t[height] <= 13 / 12 * min(us), (line, call, height, t)
-        taken.add(height)
-    assert taken == {0, 32, 128, 256}
+    assert taken == {0, 32, 128, 256, 384}
+
+
+def test_rests_are_apart_where_that_is_fast(tiling):
+    calls = [(line, call, us) for call, lines in APART.items() for line, us in enumerate(lines)]
+    apart = 0
+    for (line, call, us), height in zip(calls, tiling([(line, *call) for line, call, _ in calls])):
+        t = dict(zip((128, 256, 384), us))
+        # where copies have fewer than 256 rows, rests are not looked at
+        assert t[height] <= (13 / 12 if call[0] >= 256 * call[1] else 1.25) * min(us), (line, call, height, t)
+        apart += height == 384
+    assert apart >= 8
+    counts, N, K = test_gpu_rows4.RESTS
+    assert tiling([(line, 8 + sum(counts), len(counts), N, K) for line in (0, 1)]) == [384, 384]
