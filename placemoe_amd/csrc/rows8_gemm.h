@@ -23,7 +23,7 @@
 // on v_mfma_f32_32x32x16_bf16, whose sums are good to fp32; it reads as few bytes.
 // (Over 4-bit weights the layer is 0.0017 from its definition in 64 bits so; with the 8-bit
 // instruction in FC1 0.0017-0.0026, and 8192 tokens through 8 of 160 copies of 2048 x
-// 768 took 530 us for 694.)
+// 768 took 530 us for 694, rests not apart.)
 //
 // Bound: MFMA from some hundred rows per group on, the weights' bytes below.
 // Measured, 8-bit weights: NT 65536 x 4096 x 7168 over 16 groups 1.57-1.71 ms, 2.25-2.45 PFLOP/s at
