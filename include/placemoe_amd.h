@@ -624,14 +624,15 @@ int pmx_rows4_layer(const void* hidden, const void* w, const int64_t* sel, const
  *   gate(g) = g sigmoid(g)                       PMX_GATE_SILU
  *             g (1 + tanh(sqrt(2/pi) (g + 0.044715 g^3))) / 2   PMX_GATE_GELU_TANH
  *             g sigmoid(1.702 g)                 PMX_GATE_QUICK_GELU
- * fp32 sums; act is rounded to bf16, fc2's operand.  Any other gate: PMX_ERR_ARG.  H, I and N
+ * fp32 sums; act is rounded to bf16, fc2's operand (up to 16 tokens: to two of them).  Any other gate: PMX_ERR_ARG.  H, I and N
  * multiples of 8, tensors contiguous and 16-byte aligned, each weight matrix and 256 rows of each
  * operand below 2 GiB, else PMX_ERR_SHAPE.  T = 0: nothing is written. */
 #define PMX_GATE_SILU 0
 #define PMX_GATE_GELU_TANH 1
 #define PMX_GATE_QUICK_GELU 2
 
-/* gates (NULL: not kept) and act [T, I] bf16 are what the backward reads: gates
+/* act: bf16 [T, I], for up to 16 tokens [2, T, I], the values and what their rounding left
+ * (which is scratch memory).  gates (NULL: not kept) and act [T, I] are what the backward reads: gates
  * fp32 [T, I / 4, 2, 4], g of four neighbouring columns, then their u. */
 int pmx_gated_ffn_fwd(const void* x, const void* gate_up, const void* down, int64_t T, int64_t H, int64_t I,
                       int64_t N, int32_t gate, float* gates, void* act, void* out, pmx_stream_t stream);

@@ -23,7 +23,7 @@
 // for all tokens, its waves a share of the columns each, straight from memory to
 // the matrix instruction (16 weight rows x 16 tokens, 32 columns); their sums
 // meet in LDS.  Bound: HBM; from some tens of tokens on, their being read again by
-// every block.  One token through 7168 x 2048: 22.4 us, 3.9 TB/s of weights (a large
+// every block.  One token through 7168 x 2048: 22.9 us, 3.8 TB/s of weights (a large
 // copy: 4.8), on 64 x 128 tiles 72; 64 tokens 66 and 80.  (32 weight rows per block:
 // as fast for few, 30% slower where that leaves less than a block per CU.)
 
@@ -48,7 +48,8 @@ __device__ __forceinline__ f32x4_t mfma16(const uint4& w, const uint4& x, const 
 // tokens 0 .. 16 FT - 1 of x [T, K]: red[wave][weight row][token], after a barrier.
 // K a multiple of 8.  Lanes past K, and past T, multiply zeros.  A wave has
 // kSteps steps of 32 columns on their way; a token's sum is the same however many there are.
-template <class E, int FT>
+// PLANES 2: x [2, T, K], whose two planes add up to the tokens.
+template <class E, int FT, int PLANES>
 __device__ __forceinline__ void few_products(const bf16_t* wrow, const bf16_t* x, int64_t T, int64_t K, int lane, int wave,
                                              float (*red)[16][16 * FT]) {
   constexpr int kSteps = FT == 1 ? 8 : FT == 2 ? 6 : 4;
@@ -63,19 +64,24 @@ __device__ __forceinline__ void few_products(const bf16_t* wrow, const bf16_t* x
   const int64_t chunks = K / 8;
   f32x4_t acc[FT] = {};
   for (int64_t c0 = (int64_t)wave * 4; c0 < chunks; c0 += 4 * kFewWaves * kSteps) {
-    uint4 w[kSteps], v[kSteps][FT];
+    uint4 w[kSteps], v[kSteps][PLANES][FT];
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
       const int64_t c = c0 + s * (4 * kFewWaves) + quarter;
       const bool in = c < chunks;
       w[s] = in ? ld_stream(wrow + c * 8) : make_uint4(0, 0, 0, 0);
 #pragma unroll
-      for (int f = 0; f < FT; ++f) v[s][f] = in && token[f] ? *reinterpret_cast<const uint4*>(xrow[f] + c * 8) : make_uint4(0, 0, 0, 0);
+      for (int p = 0; p < PLANES; ++p)
+#pragma unroll
+        for (int f = 0; f < FT; ++f)
+          v[s][p][f] = in && token[f] ? *reinterpret_cast<const uint4*>(xrow[f] + p * T * K + c * 8) : make_uint4(0, 0, 0, 0);
     }
 #pragma unroll
     for (int s = 0; s < kSteps; ++s)
 #pragma unroll
-      for (int f = 0; f < FT; ++f) acc[f] = mfma16<E>(w[s], v[s][f], acc[f]);
+      for (int p = 0; p < PLANES; ++p)
+#pragma unroll
+        for (int f = 0; f < FT; ++f) acc[f] = mfma16<E>(w[s], v[s][p][f], acc[f]);
   }
   // lane: token lane % 16, weight rows 4 (lane / 16) .. + 3
 #pragma unroll
@@ -84,6 +90,12 @@ __device__ __forceinline__ void few_products(const bf16_t* wrow, const bf16_t* x
     for (int e = 0; e < 4; ++e) red[wave][quarter * 4 + e][f * 16 + t] = acc[f][e];
   __syncthreads();
 }
+
+// act among up to 16 tokens: rounded, and what that leaves kept behind it for fc2.  There one rounded value may be most
+// of an output (two fp16 tokens of 280 x 64: out 0.00037 from 64 bits; so 0.00021, as rounded once).  One token
+// through 7168 x 2048 takes 0.6 us more, 16 tokens 33.4 for 29.7; 64 would take 81 for 64.
+template <int FT>
+constexpr int act_planes() { return FT == 1 ? 2 : 1; }
 
 // fc1: eight columns of act (and gates) per block.
 template <class E, int FT>
@@ -94,7 +106,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void gated_few_fc1_kernel(const bf1
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t j0 = (int64_t)blockIdx.x * 8;
   const int r = lane & 15;
-  few_products<E, FT>(w + ((r < 8 ? 0 : I) + j0 + r % 8) * H, x, T, H, lane, wave, red);
+  few_products<E, FT, 1>(w + ((r < 8 ? 0 : I) + j0 + r % 8) * H, x, T, H, lane, wave, red);
   const int j = threadIdx.x & 7;
   for (int64_t t = threadIdx.x >> 3; t < T && t < 16 * FT; t += 8 * kFewWaves) {
     float g = 0.f, u = 0.f;
@@ -104,7 +116,11 @@ __global__ __launch_bounds__(64 * kFewWaves) void gated_few_fc1_kernel(const bf1
       float* const to = gates + (t * I + j0 + (j & 4)) * 2 + (j & 3);
       to[0] = g, to[4] = u;
     }
-    act[t * I + j0 + j] = (bf16_t)E::from_f32(gate.value(g) * u);
+    const float v = gate.value(g) * u;
+    const bf16_t high = (bf16_t)E::from_f32(v);
+    [[maybe_unused]] const float left = v - E::to_f32(high);
+    act[t * I + j0 + j] = high;
+    if constexpr (act_planes<FT>() == 2) act[(T + t) * I + j0 + j] = __builtin_isfinite(left) ? (bf16_t)E::from_f32(left) : (bf16_t)0;
   }
 }
 
@@ -116,7 +132,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void gated_few_fc2_kernel(const bf1
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t n0 = (int64_t)blockIdx.x * 16;
   const int64_t n = n0 + (lane & 15);
-  few_products<E, FT>(w + (n < N ? n : N - 1) * I, act, T, I, lane, wave, red);
+  few_products<E, FT, act_planes<FT>()>(w + (n < N ? n : N - 1) * I, act, T, I, lane, wave, red);
   const int j = threadIdx.x & 15;
   if (n0 + j >= N) return;
   for (int64_t t = threadIdx.x >> 4; t < T && t < 16 * FT; t += 4 * kFewWaves) {

@@ -27,8 +27,9 @@ def _forward(x: torch.Tensor, gate_up: torch.Tensor, down: torch.Tensor, gate: i
     out = x.new_empty((T, N))
     behind = 8 * T * I if keep_gates else 0
     alone = keep_gates and not keep_act
-    kept = x.new_empty(behind if alone else behind + 2 * T * I, dtype=torch.uint8)
-    passing = x.new_empty((T, I)) if alone else None  # act, on its way to fc2 only
+    size = (2 if T <= 16 else 1) * T * I  # act's
+    kept = x.new_empty(behind if alone else behind + 2 * size, dtype=torch.uint8)
+    passing = x.new_empty(size) if alone else None  # act, on its way to fc2 only
     gates = kept.data_ptr() if keep_gates else None
     act = passing.data_ptr() if alone else kept.data_ptr() + behind
     _launch("pmx_gated_ffn_fwd", x.dtype, x.device, _ptr(x), _ptr(gate_up), _ptr(down), T, H, I, N, gate, gates, act, _ptr(out))
@@ -99,7 +100,8 @@ def gated_ffn(x: torch.Tensor, gate_up: torch.Tensor, down: torch.Tensor, activa
 
     Sums are held in fp32; the gated products, and in the backward the gradients
     of gate and up, are rounded to the tensors' dtype, being operands of
-    products.  For the backward x, the gate and up sums [tokens, 2I] in fp32 and
+    products (of up to 16 tokens the kernels for few hold the gated products in
+    two such values each).  For the backward x, the gate and up sums [tokens, 2I] in fp32 and
     their products [tokens, I] are kept, as far as the gradients that are
     wanted read them.
     """

@@ -45,8 +45,8 @@ def _gate(g, kind):
     return g * s, s + k * g * s * torch.sigmoid(-k * g)
 
 
-def _reference(x, up, down, dout, kind):
-    """[(value, tolerance)] of out, dx, dgate_up, ddown."""
+def _reference(x, up, down, dout, kind, two=False):
+    """[(value, tolerance)] of out, dx, dgate_up, ddown; two: fc2 of the forward reads act in two values."""
     half = torch.finfo(x.dtype).eps / 2
     tiny = 2.0**-133 if x.dtype == BF else 2.0**-24
     x, up, down, dout = (t.detach().double() for t in (x, up, down, dout))
@@ -57,9 +57,10 @@ def _reference(x, up, down, dout, kind):
     a, slope = _gate(g, kind)
     h = a * u
     d_h = 1.2 * d_g * u.abs() + a.abs() * d_u + 1.2 * d_g * d_u + h.abs() * 2.0**-17
+    d_h2 = d_h + (h.abs() + d_h) * half * half + tiny
     d_h = d_h + (h.abs() + d_h) * half + tiny
     out = h @ down.t()
-    d_out = d_h @ down.abs().t() + h.abs() @ down.abs().t() * (2 * I * ROUND)
+    d_out = (d_h2 if two else d_h) @ down.abs().t() + h.abs() @ down.abs().t() * (3 * I * ROUND)
     # backward: gate and up sums as the forward left them, dh from the accumulators
     dh = dout @ down
     d_dh = dout.abs() @ down.abs() * (N * ROUND)
@@ -234,6 +235,22 @@ def test_only_the_wanted_gradients(cuda, T):
                 assert_exact(leaf.grad, full[1 + k], f"mask {mask}, leaf {k}")
             else:
                 assert leaf.grad is None
+
+
+@pytest.mark.parametrize("kind", GATES)
+@pytest.mark.parametrize("dtype", [BF, F16])
+@pytest.mark.parametrize("T,H,I,N", [(1, 520, 264, 520), (2, 280, 64, 280), (7, 1416, 1000, 1416), (16, 128, 1000, 72), (16, 2048, 768, 2048)])
+def test_few_tokens_are_rounded_once(cuda, T, H, I, N, dtype, kind):
+    """Of up to 16 tokens out alone is rounded: to half a step and what its sums are off."""
+    case = _case(cuda, T, H, I, N, dtype, seed=T)
+    with torch.no_grad():
+        out = placemoe_amd.gated_ffn(*case[:3], activation=kind)
+    (v, tol), *_ = _reference(*case, kind, two=True)
+    assert ((out.double() - v).abs() <= tol * 1.0001).all()
+    eps = torch.finfo(dtype).eps
+    # one rounding, of root mean square at most eps / sqrt(12) of its values, and what the sums are off
+    assert (out.double() - v).norm() <= eps / math.sqrt(12) * v.norm() + (tol - v.abs() * eps / 2).clamp(min=0).norm()
+    assert_exact(_run(*case, kind)[0], out, "with gradients")
 
 
 @pytest.mark.parametrize("T", [3, 120])
