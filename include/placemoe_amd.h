@@ -632,7 +632,7 @@ int pmx_rows4_layer(const void* hidden, const void* w, const int64_t* sel, const
 #define PMX_GATE_QUICK_GELU 2
 
 /* act: bf16 [T, I], for up to 16 tokens [2, T, I], the values and what their rounding left
- * (which is scratch memory).  gates (NULL: not kept) and act [T, I] are what the backward reads: gates
+ * of them.  gates (NULL: not kept) and act are what the backward reads: gates
  * fp32 [T, I / 4, 2, 4], g of four neighbouring columns, then their u. */
 int pmx_gated_ffn_fwd(const void* x, const void* gate_up, const void* down, int64_t T, int64_t H, int64_t I,
                       int64_t N, int32_t gate, float* gates, void* act, void* out, pmx_stream_t stream);
@@ -640,7 +640,7 @@ int pmx_gated_ffn_fwd(const void* x, const void* gate_up, const void* down, int6
 /* Gradients of x, W and Wd from dout [T, N], each NULL where it is not wanted
  * (and what only it reads may then be NULL: dx gate_up; dgate_up x; ddown act;
  * the first two down and gates).  The gradients of g and u are rounded to bf16 on
- * their way.  workspace: 16-byte aligned, one call's at a time. */
+ * their way (up to 16 tokens to two of them for dgate_up).  workspace: 16-byte aligned, one call's at a time. */
 size_t pmx_gated_ffn_workspace_bytes(int64_t T, int64_t H, int64_t I, int64_t N);
 int pmx_gated_ffn_bwd(const void* dout, const void* x, const void* gate_up, const void* down, const float* gates,
                       const void* act, int64_t T, int64_t H, int64_t I, int64_t N, int32_t gate, void* dx,

@@ -216,7 +216,14 @@ __device__ __forceinline__ void epilogue(const GemmParams& P, const TileInfo& ti
 #pragma unroll
           for (int e = 0; e < 4; ++e) P.gate.gradients(acc[mt][nt + k][e], g[k][e], u[k][e], dg[e], du[e]);
           bf16_t* const o = P.c0 + r * 2 * I + (k ? jb : ja);
-          if (k ? inb : ina) st4(o, pack4(dg[0], dg[1], dg[2], dg[3])), st4(o + I, pack4(du[0], du[1], du[2], du[3]));
+          if (k ? inb : ina) {
+            const uint2 pg = pack4(dg[0], dg[1], dg[2], dg[3]), pu = pack4(du[0], du[1], du[2], du[3]);
+            st4(o, pg), st4(o + I, pu);
+            if (P.left != nullptr) {
+              bf16_t* const l = P.left + (o - P.c0);
+              st4(l, left4(dg, pg)), st4(l + I, left4(du, pu));
+            }
+          }
         }
 #else
         const bf16_t* gr = P.gin + r * 2 * I;

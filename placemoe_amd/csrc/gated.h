@@ -25,10 +25,10 @@ struct GatedWgradCall {
   /* c [M, N] = a [M, K] b [K, N] */                                                                                         \
   __attribute__((visibility("hidden"))) int pmx_gated_nn##SUFFIX(const void* a, const void* b, int64_t M, int64_t N,         \
                                                                  int64_t K, void* c, pmx_stream_t stream);                   \
-  /* dgu [T, 2I] from dout [T, N], w [N, I] and gates */                                                                     \
+  /* dgu [T, 2I] from dout [T, N], w [N, I] and gates; left: null, or up to 64 rows, what dgu's rounding leaves */           \
   __attribute__((visibility("hidden"))) int pmx_gated_dgate##SUFFIX(const void* dout, const void* w, const float* gates,     \
                                                                     int64_t T, int64_t N, int64_t I, float a, float b,       \
-                                                                    void* dgu, pmx_stream_t stream);                         \
+                                                                    void* dgu, void* left, pmx_stream_t stream);             \
   /* a gradient on 256 x 256 tiles */                                                                                        \
   __attribute__((visibility("hidden"))) int pmx_gated_tn##SUFFIX(const GatedWgradCall& w, int64_t K, pmx_stream_t stream);   \
   /* one or two on 128 x 128 tiles, whole */                                                                                 \

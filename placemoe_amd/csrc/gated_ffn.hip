@@ -94,8 +94,11 @@ __device__ __forceinline__ void few_products(const bf16_t* wrow, const bf16_t* x
 // act among up to 16 tokens: rounded, and what that leaves kept behind it for fc2.  There one rounded value may be most
 // of an output (two fp16 tokens of 280 x 64: out 0.00037 from 64 bits; so 0.00021, as rounded once).  One token
 // through 7168 x 2048 takes 0.6 us more, 16 tokens 33.4 for 29.7; 64 would take 81 for 64.
+// The weights' gradients of so few tokens are sums of as few products: they read act and dgu so too, each as twice
+// the rows, beside two copies of the tokens' other rows.
+constexpr int64_t kTwoValues = 16;
 template <int FT>
-constexpr int act_planes() { return FT == 1 ? 2 : 1; }
+constexpr int act_planes() { return FT * 16 <= kTwoValues ? 2 : 1; }
 
 // fc1: eight columns of act (and gates) per block.
 template <class E, int FT>
@@ -166,6 +169,17 @@ __global__ __launch_bounds__(256) void sum_parts_kernel(const float* __restrict_
   *reinterpret_cast<uint2*>(out + i) = make_uint2(E::pack2(sum[0], sum[1]), E::pack2(sum[2], sum[3]));
 }
 
+// Two copies, one behind the other, of a (na chunks of 16 bytes) and of b.
+__global__ __launch_bounds__(256) void two_copies_kernel(const uint4* __restrict__ a, int64_t na, uint4* __restrict__ a2,
+                                                         const uint4* __restrict__ b, int64_t nb, uint4* __restrict__ b2) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i < na) {
+    a2[i] = a2[na + i] = a[i];
+  } else if (i - na < nb) {
+    b2[i - na] = b2[nb + i - na] = b[i - na];
+  }
+}
+
 bool gate_of(int32_t gate, Gate& g) {
   constexpr float kGelu = 1.5957691216057308f;  // 2 sqrt(2 / pi)
   switch (gate) {
@@ -207,8 +221,11 @@ Wgrad wgrad_of(int64_t K, int64_t M, int64_t N) {
   return {w.small, chunk, (int32_t)((K + chunk - 1) / chunk)};
 }
 
-// The backward's workspace: dgu, then the fp32 sums of one weight gradient's chunks.
-size_t dgu_bytes(int64_t T, int64_t I) { return ((size_t)T * 2 * I * 2 + 255) / 256 * 256; }
+// The backward's workspace: dgu (up to kTwoValues tokens: and what its rounding left), two copies of dout and of x
+// there, then the fp32 sums of one weight gradient's chunks.
+int64_t wgrad_rows(int64_t T) { return T <= kTwoValues ? 2 * T : T; }
+size_t dgu_bytes(int64_t T, int64_t I) { return ((size_t)wgrad_rows(T) * 2 * I * 2 + 255) / 256 * 256; }
+size_t copies_bytes(int64_t T, int64_t cols) { return T <= kTwoValues ? ((size_t)2 * T * cols * 2 + 255) / 256 * 256 : 0; }
 size_t parts_bytes(int64_t K, int64_t M, int64_t N) {
   const Wgrad w = wgrad_of(K, M, N);
   return w.splits > 1 ? (size_t)w.splits * M * N * 4 : 0;
@@ -289,14 +306,25 @@ int backward_t(const void* dout, const void* x, const void* gate_up, const void*
     if (!aligned16(p)) return PMX_ERR_SHAPE;
   if (!workspace || workspace_bytes < pmx_gated_ffn_workspace_bytes(T, H, I, N)) return PMX_ERR_ARG;
   void* dgu = workspace;
-  float* parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + dgu_bytes(T, I));
+  char* at = static_cast<char*>(workspace) + dgu_bytes(T, I);
+  char* const dout2 = at;
+  char* const x2 = at += copies_bytes(T, N);
+  float* parts = reinterpret_cast<float*>(at += copies_bytes(T, H));
+  const bool two = T <= kTwoValues;
+  if (two && (ddown || dgate_up)) {
+    const int64_t na = ddown ? T * N / 8 : 0, nb = dgate_up ? T * H / 8 : 0;
+    two_copies_kernel<<<(unsigned)((na + nb + 255) / 256), 256, 0, stream>>>((const uint4*)dout, na, (uint4*)dout2, (const uint4*)x, nb,
+                                                                            (uint4*)x2);
+    PMX_LAUNCH_CHECK();
+  }
   int rc = PMX_OK;
-  if (dx || dgate_up) rc = Gemms<E>::dgate(dout, down, gates, T, N, I, gate.a, gate.b, dgu, stream);
+  if (dx || dgate_up)
+    rc = Gemms<E>::dgate(dout, down, gates, T, N, I, gate.a, gate.b, dgu, two ? (bf16_t*)dgu + T * 2 * I : nullptr, stream);
   GatedWgradCall w[2];
   int n = 0;
-  if (ddown) w[n++] = {dout, act, N, I, 0, 0, ddown, nullptr};
-  if (dgate_up) w[n++] = {dgu, x, 2 * I, H, 0, 0, dgate_up, nullptr};
-  if (rc == PMX_OK) rc = weight_gradients<E>(w, n, T, parts, stream);
+  if (ddown) w[n++] = {two ? dout2 : dout, act, N, I, 0, 0, ddown, nullptr};
+  if (dgate_up) w[n++] = {dgu, two ? x2 : x, 2 * I, H, 0, 0, dgate_up, nullptr};
+  if (rc == PMX_OK) rc = weight_gradients<E>(w, n, wgrad_rows(T), parts, stream);
   if (rc == PMX_OK && dx) rc = Gemms<E>::nn(dgu, gate_up, T, H, 2 * I, dx, stream);
   return rc != PMX_OK ? PMX_ERR_HIP : PMX_OK;
 }
@@ -307,8 +335,8 @@ extern "C" {
 
 size_t pmx_gated_ffn_workspace_bytes(int64_t T, int64_t H, int64_t I, int64_t N) {
   if (check(T, H, I, N) != PMX_OK || T == 0) return 0;
-  const size_t a = parts_bytes(T, N, I), b = parts_bytes(T, 2 * I, H);
-  return dgu_bytes(T, I) + (a > b ? a : b);
+  const size_t a = parts_bytes(wgrad_rows(T), N, I), b = parts_bytes(wgrad_rows(T), 2 * I, H);
+  return dgu_bytes(T, I) + copies_bytes(T, N) + copies_bytes(T, H) + (a > b ? a : b);
 }
 
 #define PMX_GATED_FFN(SUFFIX, E)                                                                                            \

@@ -11,7 +11,7 @@ int launch_rows(const GemmParams& P, hipStream_t stream) {
   if (ntn >= (int64_t)1 << 19) return PMX_ERR_SHAPE;  // the LDS tile table keeps an n-tile index in 19 bits
   const int grid = grid_size();
   if (grid <= 0) return PMX_ERR_HIP;
-  const int tiling = pmx::gated_tiling(KIND, P.M, P.N, P.K, grid);
+  const int tiling = P.left != nullptr ? Few64::BM : pmx::gated_tiling(KIND, P.M, P.N, P.K, grid);
   if (tiling == Few64::BM) return launch_few<KIND, Few64>(P, grid, stream);
   if (tiling == Few128::BM) return launch_few<KIND, Few128>(P, grid, stream);
   const bool fast = P.K % BK == 0;
@@ -69,11 +69,12 @@ int PMX_GEMM_FN(pmx_gated_nn)(const void* a, const void* b, int64_t M, int64_t N
 }
 
 int PMX_GEMM_FN(pmx_gated_dgate)(const void* dout, const void* w, const float* gates, int64_t T, int64_t N, int64_t I, float a,
-                                 float b, void* dgu, pmx_stream_t stream) {
+                                 float b, void* dgu, void* left, pmx_stream_t stream) {
   if (!fits_rsrc(N, I) || !fits_rsrc(kBM, N)) return PMX_ERR_SHAPE;
   GemmParams P = dense(dout, w, T, I, N, I);
   P.I = I;
   P.c0 = static_cast<bf16_t*>(dgu);
+  P.left = static_cast<bf16_t*>(left);
   P.ldc = 2 * I;
   P.gates = const_cast<float*>(gates);
   P.gate = {a, b};

@@ -156,6 +156,7 @@ struct GemmParams {
   float* gates;
   uint32_t chunk;  // rows of a group (the last one: what is left)
   uint32_t rows;   // in all, below 2^31
+  bf16_t* left;    // KIND_NNS, 64-row tiles: what the rounding of c0 left, laid out like it (null: not wanted)
   float* parts;   // KIND_TN: each group's fp32 sums, cgs elements apart, in the place of c0
 #endif
 };
@@ -579,6 +580,15 @@ struct GatesWin {
 __device__ __forceinline__ GatesWin gates_window(const GemmParams& P, int64_t row0, int64_t row_end) {
   const int64_t rows = row_end - row0 < 0 || P.gates == nullptr ? 0 : (row_end - row0 > 64 ? 64 : row_end - row0);
   return {make_rsrc(P.gates + row0 * 2 * P.I, (uint64_t)(rows * P.I * 8)), (uint32_t)(P.I * 8)};
+}
+// What rounding four values to p left (nothing, where that is not finite).
+__device__ __forceinline__ uint2 left4(const float* v, uint2 p) {
+  float f[4];
+  Elt::unpack2(p.x, f[0], f[1]);
+  Elt::unpack2(p.y, f[2], f[3]);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) f[e] = __builtin_isfinite(v[e] - f[e]) ? v[e] - f[e] : 0.f;
+  return pack4(f[0], f[1], f[2], f[3]);
 }
 // The gradients of four columns' gate and up values, written to both halves of their row in `w`.
 __device__ __forceinline__ void gradients4(const GemmParams& P, const OutWin& w, int row, int64_t j, int64_t I, const f32x4_t& d,

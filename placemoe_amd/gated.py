@@ -100,8 +100,8 @@ def gated_ffn(x: torch.Tensor, gate_up: torch.Tensor, down: torch.Tensor, activa
 
     Sums are held in fp32; the gated products, and in the backward the gradients
     of gate and up, are rounded to the tensors' dtype, being operands of
-    products (of up to 16 tokens the kernels for few hold the gated products in
-    two such values each).  For the backward x, the gate and up sums [tokens, 2I] in fp32 and
+    products (up to 16 tokens, for fc2 and the weights' gradients, to two such
+    values each).  For the backward x, the gate and up sums [tokens, 2I] in fp32 and
     their products [tokens, I] are kept, as far as the gradients that are
     wanted read them.
     """

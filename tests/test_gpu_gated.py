@@ -46,7 +46,8 @@ def _gate(g, kind):
 
 
 def _reference(x, up, down, dout, kind, two=False):
-    """[(value, tolerance)] of out, dx, dgate_up, ddown; two: fc2 of the forward reads act in two values."""
+    """[(value, tolerance)] of out, dx, dgate_up, ddown; two: fc2 of the forward and the weights' gradients
+    read act and the gradients of gate and up in two values."""
     half = torch.finfo(x.dtype).eps / 2
     tiny = 2.0**-133 if x.dtype == BF else 2.0**-24
     x, up, down, dout = (t.detach().double() for t in (x, up, down, dout))
@@ -67,14 +68,15 @@ def _reference(x, up, down, dout, kind, two=False):
     dg, du = dh * u * slope, dh * a
     most = dh.abs() + d_dh
     d_dg = d_dh * u.abs() * slope.abs() + most * (d_u * 1.2 + (u.abs() + d_u) * (d_g + 2.0**-15))
-    d_dg = d_dg + (dg.abs() + d_dg) * half + tiny
+    d_dg2, d_dg = (d_dg + (dg.abs() + d_dg) * r + tiny for r in (half * half, half))
     d_du = d_dh * a.abs() + most * (1.2 * d_g + a.abs() * 2.0**-16)
-    d_du = d_du + (du.abs() + d_du) * half + tiny
+    d_du2, d_du = (d_du + (du.abs() + d_du) * r + tiny for r in (half * half, half))
     dgu, d_dgu = torch.cat((dg, du), 1), torch.cat((d_dg, d_du), 1)
     dx, d_dx = dgu @ up, d_dgu @ up.abs() + dgu.abs() @ up.abs() * (4 * I * ROUND)
-    dup, d_dup = dgu.t() @ x, d_dgu.t() @ x.abs() + dgu.abs().t() @ x.abs() * (2 * T * ROUND)
+    d_dgu2 = torch.cat((d_dg2, d_du2), 1)
+    dup, d_dup = dgu.t() @ x, (d_dgu2 if two else d_dgu).t() @ x.abs() + dgu.abs().t() @ x.abs() * (2 * T * ROUND)
     ddown = dout.t() @ h
-    d_ddown = dout.abs().t() @ d_h + dout.abs().t() @ h.abs() * (2 * T * ROUND)
+    d_ddown = dout.abs().t() @ (d_h2 if two else d_h) + dout.abs().t() @ h.abs() * (2 * T * ROUND)
     return [(v, t + (v.abs() + t) * half + tiny) for v, t in ((out, d_out), (dx, d_dx), (dup, d_dup), (ddown, d_ddown))]
 
 
@@ -241,16 +243,16 @@ def test_only_the_wanted_gradients(cuda, T):
 @pytest.mark.parametrize("dtype", [BF, F16])
 @pytest.mark.parametrize("T,H,I,N", [(1, 520, 264, 520), (2, 280, 64, 280), (7, 1416, 1000, 1416), (16, 128, 1000, 72), (16, 2048, 768, 2048)])
 def test_few_tokens_are_rounded_once(cuda, T, H, I, N, dtype, kind):
-    """Of up to 16 tokens out alone is rounded: to half a step and what its sums are off."""
+    """Of up to 16 tokens out and the weights' gradients alone are rounded: to half a step and what their sums are off."""
     case = _case(cuda, T, H, I, N, dtype, seed=T)
+    got, want, eps = _run(*case, kind), _reference(*case, kind, two=True), torch.finfo(dtype).eps
+    for k in (0, 2, 3):
+        (v, tol), off = want[k], (got[k].double() - want[k][0]).abs()
+        assert (off <= tol * 1.0001).all(), k
+        # one rounding, of root mean square at most eps / sqrt(12) of its values, and what the sums are off
+        assert off.norm() <= eps / math.sqrt(12) * v.norm() + (tol - v.abs() * eps / 2).clamp(min=0).norm(), k
     with torch.no_grad():
-        out = placemoe_amd.gated_ffn(*case[:3], activation=kind)
-    (v, tol), *_ = _reference(*case, kind, two=True)
-    assert ((out.double() - v).abs() <= tol * 1.0001).all()
-    eps = torch.finfo(dtype).eps
-    # one rounding, of root mean square at most eps / sqrt(12) of its values, and what the sums are off
-    assert (out.double() - v).norm() <= eps / math.sqrt(12) * v.norm() + (tol - v.abs() * eps / 2).clamp(min=0).norm()
-    assert_exact(_run(*case, kind)[0], out, "with gradients")
+        assert_exact(placemoe_amd.gated_ffn(*case[:3], activation=kind), got[0], "without gradients")
 
 
 @pytest.mark.parametrize("T", [3, 120])
