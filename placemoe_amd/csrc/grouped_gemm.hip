@@ -566,15 +566,18 @@ __device__ __forceinline__ void activate2([[maybe_unused]] const GemmParams& P, 
 struct GatesWin {
   __amdgpu_buffer_rsrc_t r;
   uint32_t rowb;
-  // The lane's four columns from j on, of row `row`; `rows` further on (uniform).
+  // The lane's four columns from j on, of row `row`; `rows` further on.  All in the vector offset: a scalar one may pass the
+  // whole descriptor (a short last tile; no rows), and a check against the size less that offset would wrap.
   __device__ __forceinline__ uint32_t at(int row, int64_t j, int64_t I) const { return j < I ? (uint32_t)row * rowb + (uint32_t)j * 8u : kOOB; }
   __device__ __forceinline__ void store(uint32_t o, int rows, const f32x4_t& g, const f32x4_t& u) const {
-    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, g), r, o, (uint32_t)rows * rowb, 0);
-    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, u), r, o + 16u, (uint32_t)rows * rowb, 0);
+    const uint32_t at = o + (uint32_t)rows * rowb;
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, g), r, at, 0, 0);
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, u), r, at + 16u, 0, 0);
   }
   __device__ __forceinline__ void load(uint32_t o, int rows, f32x4_t& g, f32x4_t& u) const {
-    g = __builtin_bit_cast(f32x4_t, __builtin_amdgcn_raw_buffer_load_b128(r, o, (uint32_t)rows * rowb, 0));
-    u = __builtin_bit_cast(f32x4_t, __builtin_amdgcn_raw_buffer_load_b128(r, o + 16u, (uint32_t)rows * rowb, 0));
+    const uint32_t at = o + (uint32_t)rows * rowb;
+    g = __builtin_bit_cast(f32x4_t, __builtin_amdgcn_raw_buffer_load_b128(r, at, 0, 0));
+    u = __builtin_bit_cast(f32x4_t, __builtin_amdgcn_raw_buffer_load_b128(r, at + 16u, 0, 0));
   }
 };
 __device__ __forceinline__ GatesWin gates_window(const GemmParams& P, int64_t row0, int64_t row_end) {
