@@ -48,7 +48,8 @@ __device__ __forceinline__ f32x4_t mfma16(const uint4& w, const uint4& x, const 
 // tokens 0 .. 16 FT - 1 of x [T, K]: red[wave][weight row][token], after a barrier.
 // K a multiple of 8.  Lanes past K, and past T, multiply zeros.  A wave has
 // kSteps steps of 32 columns on their way; a token's sum is the same however many there are.
-// PLANES 2: x [2, T, K], whose two planes add up to the tokens.
+// PLANES 2: x [2, T, K], whose two planes add up to the tokens, summed apart: of an infinite weight the second,
+// of either sign, is left out.
 template <class E, int FT, int PLANES>
 __device__ __forceinline__ void few_products(const bf16_t* wrow, const bf16_t* x, int64_t T, int64_t K, int lane, int wave,
                                              float (*red)[16][16 * FT]) {
@@ -62,7 +63,7 @@ __device__ __forceinline__ void few_products(const bf16_t* wrow, const bf16_t* x
     xrow[f] = x + (token[f] ? f * 16 + t : 0) * K;
   }
   const int64_t chunks = K / 8;
-  f32x4_t acc[FT] = {};
+  f32x4_t acc[PLANES][FT] = {};
   for (int64_t c0 = (int64_t)wave * 4; c0 < chunks; c0 += 4 * kFewWaves * kSteps) {
     uint4 w[kSteps], v[kSteps][PLANES][FT];
 #pragma unroll
@@ -81,13 +82,17 @@ __device__ __forceinline__ void few_products(const bf16_t* wrow, const bf16_t* x
 #pragma unroll
       for (int p = 0; p < PLANES; ++p)
 #pragma unroll
-        for (int f = 0; f < FT; ++f) acc[f] = mfma16<E>(w[s], v[s][p][f], acc[f]);
+        for (int f = 0; f < FT; ++f) acc[p][f] = mfma16<E>(w[s], v[s][p][f], acc[p][f]);
   }
   // lane: token lane % 16, weight rows 4 (lane / 16) .. + 3
 #pragma unroll
   for (int f = 0; f < FT; ++f)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) red[wave][quarter * 4 + e][f * 16 + t] = acc[f][e];
+    for (int e = 0; e < 4; ++e) {
+      float sum = acc[0][f][e];
+      if constexpr (PLANES == 2) sum += __builtin_isfinite(sum) ? acc[1][f][e] : 0.f;
+      red[wave][quarter * 4 + e][f * 16 + t] = sum;
+    }
   __syncthreads();
 }
 
@@ -169,14 +174,26 @@ __global__ __launch_bounds__(256) void sum_parts_kernel(const float* __restrict_
   *reinterpret_cast<uint2*>(out + i) = make_uint2(E::pack2(sum[0], sum[1]), E::pack2(sum[2], sum[3]));
 }
 
-// Two copies, one behind the other, of a (na chunks of 16 bytes) and of b.
+// Eight values, zeros in the place of infinities and NaN.
+template <class E>
+__device__ __forceinline__ uint4 finite8(const uint4 v) {
+  constexpr uint32_t kInf = E::kCode == EltF16::kCode ? 0x7c00u : 0x7f80u;
+  const auto two = [](uint32_t w) {
+    return ((w & kInf) == kInf ? 0u : w & 0xffffu) | ((w >> 16 & kInf) == kInf ? 0u : w & 0xffff0000u);
+  };
+  return make_uint4(two(v.x), two(v.y), two(v.z), two(v.w));
+}
+
+// Two copies, one behind the other, of a (na chunks of 16 bytes) and of b: the second is multiplied with what a
+// rounding left, of either sign, and has what is finite alone.
+template <class E>
 __global__ __launch_bounds__(256) void two_copies_kernel(const uint4* __restrict__ a, int64_t na, uint4* __restrict__ a2,
                                                          const uint4* __restrict__ b, int64_t nb, uint4* __restrict__ b2) {
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (i < na) {
-    a2[i] = a2[na + i] = a[i];
+    a2[i] = a[i], a2[na + i] = finite8<E>(a[i]);
   } else if (i - na < nb) {
-    b2[i - na] = b2[nb + i - na] = b[i - na];
+    b2[i - na] = b[i - na], b2[nb + i - na] = finite8<E>(b[i - na]);
   }
 }
 
@@ -313,8 +330,8 @@ int backward_t(const void* dout, const void* x, const void* gate_up, const void*
   const bool two = T <= kTwoValues;
   if (two && (ddown || dgate_up)) {
     const int64_t na = ddown ? T * N / 8 : 0, nb = dgate_up ? T * H / 8 : 0;
-    two_copies_kernel<<<(unsigned)((na + nb + 255) / 256), 256, 0, stream>>>((const uint4*)dout, na, (uint4*)dout2, (const uint4*)x, nb,
-                                                                            (uint4*)x2);
+    two_copies_kernel<E><<<(unsigned)((na + nb + 255) / 256), 256, 0, stream>>>((const uint4*)dout, na, (uint4*)dout2, (const uint4*)x,
+                                                                               nb, (uint4*)x2);
     PMX_LAUNCH_CHECK();
   }
   int rc = PMX_OK;
