@@ -15,9 +15,8 @@ int launch_rows(const GemmParams& P, hipStream_t stream) {
   if (tiling == Few64::BM) return launch_few<KIND, Few64>(P, grid, stream);
   if (tiling == Few128::BM) return launch_few<KIND, Few128>(P, grid, stream);
   const bool fast = P.K % BK == 0;
-  if constexpr (use_w4<KIND>()) {
-    if (fast) w4::grouped_gemm_w4_kernel<KIND><<<grid, w4::NT, 0, stream>>>(P);
-    else grouped_gemm_kernel<KIND, kBM><<<grid, NTHREADS, 0, stream>>>(P);
+  if constexpr (KIND == KIND_FC1 || KIND == KIND_NNS) {  // whole K-tiles: the rule takes smaller tiles otherwise
+    w4::grouped_gemm_w4_kernel<KIND><<<grid, w4::NT, 0, stream>>>(P);
   } else if (!fast) {
     grouped_gemm_kernel<KIND, kBM><<<grid, NTHREADS, 0, stream>>>(P);
   } else if constexpr (KIND == KIND_NT) {  // the kernels of few copies with many rows, as in grouped_gemm.hip

@@ -27,7 +27,8 @@ constexpr double kGated64[4][4] = {  // K-tile with two blocks on a CU, with one
     {0.63, 0.342, 5.04, 0.2}, {0.645, 0.328, 3.78, 1.6}, {0.624, 0.344, 4.45, 1.0}, {0.662, 0.349, 7.44, 0.0}};
 constexpr GatedRound kGated128[4] = {{0.711, 7.44}, {0.636, 7.49}, {0.656, 7.85}, {0.725, 12.4}};
 constexpr GatedRound kGated256[4] = {{1.196, 13.8}, {1.056, 9.6}, {1.109, 9.5}, {1.371, 20.9}};
-// 256 x 256 tiles whose depth is not a multiple of 64: the kernel whose loads are masked.
+// 256 x 256 tiles whose depth is not a multiple of 64: fc2 and fc1's dgrad, on the kernel whose loads are masked.  (fc1 and
+// fc2's dgrad: at 1.45 times the figures above, twice as many 128-row tiles take less at every depth.)
 constexpr double kGatedMasked = 1.45;
 
 // The m-tile height of a product of `rows` rows, N columns (fc1: 2 I) and depth K on `cus` CUs.
@@ -46,6 +47,7 @@ inline GatedTiling gated_fastest(int kind, int64_t rows, int64_t N, int64_t K, i
     return (double)div_up(div_up(rows, height) * div_up(N, 256), cus) * (nk * r.ktile + r.fixed);
   };
   const double t128 = rounds(128, kGated128[kind]), t256 = rounds(256, kGated256[kind]) * (K % 64 ? kGatedMasked : 1.0);
+  if (K % 64 && (kind == 0 || kind == 3)) return t64 <= t128 ? GatedTiling{64, t64} : GatedTiling{128, t128};
   if (t64 <= t128 && t64 <= t256) return {64, t64};
   return t128 <= t256 ? GatedTiling{128, t128} : GatedTiling{256, t256};
 }

@@ -669,19 +669,6 @@ __device__ __forceinline__ void epilogue(const GemmParams& P, const TileInfo& ti
       const int64_t j0 = (int64_t)ti.ntile * 128 + wn * 32;
       float rw[4];  // the act stores' rows, loaded before the first store
       if (P.row_w != nullptr) row_weights(P, ti.row0 + rb, ti.row_end, lane >> 2, 16, rw);
-#ifdef PMX_GATED
-      {
-        const GatesWin w = gates_window(P, ti.row0 + rb, ti.row_end);
-#pragma unroll
-        for (int mtl = 0; mtl < 2; ++mtl)
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const f32x16_t &g = acc[2 * half + mtl][0], &u = acc[2 * half + mtl][1];
-            w.store(w.at(lane & 31, j0 + 8 * q + 4 * (lane >> 5), I), mtl * 32, f32x4_t{g[4 * q], g[4 * q + 1], g[4 * q + 2], g[4 * q + 3]},
-                    f32x4_t{u[4 * q], u[4 * q + 1], u[4 * q + 2], u[4 * q + 3]});
-          }
-      }
-#else
       stage_half<2>(stage, wave, lane, half, [&](int mt, int nt, int i) { return acc4(acc[mt][nt], i); });
       const int cc = lane & 7;
       {
@@ -691,7 +678,6 @@ __device__ __forceinline__ void epilogue(const GemmParams& P, const TileInfo& ti
 #pragma unroll
         for (int q = 0; q < 8; ++q) win_store(w, voff, q * 8, staged_chunk(stage, wave, q * 8 + (lane >> 3), cc));
       }
-#endif
       stage_half<1>(stage, wave, lane, half, [&](int mt, int, int i) {
         float g[4], u[4];
 #pragma unroll
@@ -721,26 +707,6 @@ __device__ __forceinline__ void epilogue(const GemmParams& P, const TileInfo& ti
       // that their latency overlaps the staging.
       // gate/up (gin) and [d_gate | d_up] (c0) share one row layout.
       const int64_t I = P.I;
-#ifdef PMX_GATED
-      const GatesWin wi = gates_window(P, ti.row0 + rb, ti.row_end);
-      const OutWin wo = out_window(P.c0, ti.row0 + rb, ti.row_end, 2 * I);
-#pragma unroll
-      for (int mtl = 0; mtl < 2; ++mtl)
-#pragma unroll
-        for (int nt = 0; nt < NTT; ++nt) {
-          const int row = mtl * 32 + (lane & 31);
-          const int64_t j = (int64_t)ti.ntile * BN + wn * WCOLS + nt * 32 + 4 * (lane >> 5);
-          f32x4_t g[4], u[4];
-#pragma unroll
-          for (int q = 0; q < 4; ++q) wi.load(wi.at(lane & 31, j + 8 * q, I), mtl * 32, g[q], u[q]);
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const f32x16_t& d = acc[2 * half + mtl][nt];
-            gradients4(P, wo, row, j + 8 * q, I, f32x4_t{d[4 * q], d[4 * q + 1], d[4 * q + 2], d[4 * q + 3]}, g[q], u[q]);
-          }
-          __builtin_amdgcn_sched_barrier(0);
-        }
-#else
       const int cc = lane & 7;
       const int64_t j = (int64_t)ti.ntile * BN + wn * WCOLS + cc * 8;
       const OutWin wi = out_window(P.gin, ti.row0 + rb, ti.row_end, 2 * I);
@@ -765,7 +731,6 @@ __device__ __forceinline__ void epilogue(const GemmParams& P, const TileInfo& ti
         win_store(wo, vg, q * 8, pack8e<Elt>(dg));
         win_store(wo, vu, q * 8, pack8e<Elt>(du));
       }
-#endif
     } else if constexpr (KIND == KIND_TN) {
       stage_half<NTT>(stage, wave, lane, half, [&](int mt, int nt, int i) { return acc4(acc[mt][nt], i); });
       const int cc = lane & 7;  // 16-byte chunk (8 columns) of the wave's 64

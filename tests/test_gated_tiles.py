@@ -41,3 +41,27 @@ def test_tiles_of_the_sizes(rule):
     assert run >= {(k, 256, True) for k in range(4)} | {(1, 256, False), (2, 256, False)}
     for kind in (0, 3):  # the four-wave kernel: 1, 15, 17 and 33 rows in the last 64
         assert {s[0] % 64 for s, h in TILES.items() if h[kind] == 256} == {1, 15, 17, 33}
+
+
+def test_no_256_rows_with_a_short_last_k_tile_for_fc1_and_fc2_dgrad(rule):
+    """Their 256-row kernel takes whole K-tiles alone."""
+    import random
+
+    rng = random.Random(7)
+    calls = [(rng.choice((0, 3)), int(2 ** rng.uniform(5, 24)), 8 * int(2 ** rng.uniform(0, 11)), 8 * int(2 ** rng.uniform(0, 11)))
+             for _ in range(4000)]
+    calls = [(k, r, n, d + 8 if d % 64 == 0 else d) for k, r, n, d in calls]
+    assert set(rule(calls)) == {64, 128}
+    whole = [(k, r, n, (d + 63) // 64 * 64) for k, r, n, d in calls]
+    assert set(rule(whole)) == {64, 128, 256}
+
+
+def test_no_kernel_is_built_that_no_call_reaches(tmp_path):
+    """The gated build has the eight-wave kernel for fc2, fc1's dgrad and the weight gradients, not for the other two."""
+    from placemoe_amd import build
+    from tests.test_build_resources import _compile_remarks
+
+    names = [r["name"] for r in _compile_remarks(build.CSRC / "grouped_gemm.hip", tmp_path, build.EXTRA_OBJECTS["grouped_gemm.gated"][1])]
+    eight = {n.split("grouped_gemm_kernelILi")[1][0] for n in names if "119grouped_gemm_kernelILi" in n}
+    four = {n.split("grouped_gemm_w4_kernelILi")[1][0] for n in names if "grouped_gemm_w4_kernelILi" in n}
+    assert (eight, four) == ({"1", "2", "4"}, {"0", "3", "4"}), names
