@@ -65,3 +65,15 @@ def test_no_kernel_is_built_that_no_call_reaches(tmp_path):
     eight = {n.split("grouped_gemm_kernelILi")[1][0] for n in names if "119grouped_gemm_kernelILi" in n}
     four = {n.split("grouped_gemm_w4_kernelILi")[1][0] for n in names if "grouped_gemm_w4_kernelILi" in n}
     assert (eight, four) == ({"1", "2", "4"}, {"0", "3", "4"}), names
+
+
+def test_kernels_for_few_tokens_are_held_to_registers(tmp_path):
+    """fc1 and fc2 of up to 16, 32 and 64 tokens in both types; the build refuses one that spills."""
+    from placemoe_amd import build
+    from tests.test_build_resources import _compile_remarks
+
+    few = [r for r in _compile_remarks(build.CSRC / "gated_ffn.hip", tmp_path) if build.RESOURCE_CHECKED["gated_ffn.hip"].search(r["name"])]
+    assert len(few) == 12
+    build.check_no_scratch(few, build.RESOURCE_CHECKED["gated_ffn.hip"], "gated_ffn.hip")
+    with pytest.raises(RuntimeError, match="spill"):
+        build.check_no_scratch([dict(few[0], vgpr_spill=1), *few[1:]], build.RESOURCE_CHECKED["gated_ffn.hip"], "gated_ffn.hip")
