@@ -58,9 +58,13 @@ class Rows4:
         return Rows4(self.codes.to(device), self.scales.to(device), self.columns, self.dtype)
 
 
+def _kind(name: str, q, *kinds: type) -> None:
+    assert isinstance(q, kinds), f"{name} must be {' or '.join(k.__name__ for k in kinds)}, got {type(q).__name__}"
+
+
 def _rows4(name: str, q: Rows4, dims: int, like: torch.dtype | None = None) -> torch.dtype:
     """Check an operand's parts against each other; returns its dtype."""
-    assert isinstance(q, Rows4), f"{name} must be Rows4, got {type(q).__name__}"
+    _kind(name, q, Rows4)
     assert q.codes.dtype == torch.uint8, f"{name} codes must be uint8, got {q.codes.dtype}"
     assert q.dtype in HALF, f"{name} must stand for bfloat16 or float16 rows, got {q.dtype}"
     assert like is None or q.dtype == like, f"{name} must stand for {like} like the other operands, got {q.dtype}"
@@ -121,6 +125,7 @@ def group_gemm_nt_rows4(a: Rows8 | Rows4, b: Rows4, offsets: torch.Tensor) -> to
     ``group_gemm_nt_rows8``: off by less than 7 * 2^-13 of the largest product
     of each eight neighbouring columns.
     """
+    _kind("a", a, Rows8, Rows4), _kind("b", b, Rows4)
     _check_dev(a.codes, a.scales, b.codes, b.scales, offsets)
     dev = offsets.device
     bits = 4 if isinstance(a, Rows4) else 8
@@ -142,6 +147,7 @@ def gemm_fc1_swiglu_rows4(x: Rows8, w: Rows4, offsets: torch.Tensor, row_token: 
     x[row_token[r]] @ w[g]^T: x [T, H] in e4m3, w [G, 2I, H] in 4 bits (gate rows
     first); row_token int32 [A] (None: row r is x[r]), row_w [A] (None: ones).
     fp32 up to the rounding to 8 bits.  H a multiple of 32, I of 16."""
+    _kind("x", x, Rows8), _kind("w", w, Rows4)
     dev = _check_dev(x.codes, x.scales, w.codes, w.scales, offsets, row_token, row_w)
     dt = _e4m3("x", x, 2)
     _rows4("w", w, 3, dt)
@@ -191,6 +197,6 @@ def expert_layer_rows4(hidden: torch.Tensor, routing_weights: torch.Tensor, sele
     ``Experts4.quantize``.  The steps and what is held between them are those of
     ``expert_layer_rows8``.  H and I multiples of 32.
     """
-    assert isinstance(weights, Experts4), f"weights must be Experts4, got {type(weights).__name__}"
+    _kind("weights", weights, Experts4), _kind("gate_up", weights.gate_up, Rows4), _kind("down", weights.down, Rows4)
     return _serving_layer("expert_layer_rows4", "pmx_rows4_layer", 32, _rows4, hidden, routing_weights, selected_experts, weights,
                           mapping, sources, source, recorder)
