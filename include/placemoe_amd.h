@@ -624,7 +624,9 @@ int pmx_rows4_layer(const void* hidden, const void* w, const int64_t* sel, const
  *   gate(g) = g sigmoid(g)                       PMX_GATE_SILU
  *             g (1 + tanh(sqrt(2/pi) (g + 0.044715 g^3))) / 2   PMX_GATE_GELU_TANH
  *             g sigmoid(1.702 g)                 PMX_GATE_QUICK_GELU
- * fp32 sums; act is rounded to bf16, fc2's operand (up to 16 tokens: to two of them).  Any other gate: PMX_ERR_ARG.  H, I and N
+ * fp32 sums; act is rounded to bf16, fc2's operand (up to 16 tokens: to two of them).  fp16 tensors: act, and in the
+ * backward the gradients of g and u, are infinite beyond 65504 and lost below 2^-25, whatever the outputs' size.
+ * Any other gate: PMX_ERR_ARG.  H, I and N
  * multiples of 8, tensors contiguous and 16-byte aligned, each weight matrix and 256 rows of each
  * operand below 2 GiB, else PMX_ERR_SHAPE.  T = 0: nothing is written. */
 #define PMX_GATE_SILU 0

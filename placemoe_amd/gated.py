@@ -101,9 +101,11 @@ def gated_ffn(x: torch.Tensor, gate_up: torch.Tensor, down: torch.Tensor, activa
     Sums are held in fp32; the gated products, and in the backward the gradients
     of gate and up, are rounded to the tensors' dtype, being operands of
     products (up to 16 tokens, for fc2 and the weights' gradients, to two such
-    values each).  For the backward x, the gate and up sums [tokens, 2I] in fp32 and
-    their products [tokens, I] are kept, as far as the gradients that are
-    wanted read them.
+    values each).  In float16 those beyond 65504 are infinite, and what is below
+    2^-25 is lost, also where an output or a gradient itself would be in range:
+    scale the loss as for any float16 training; bfloat16 has fp32's range.  For
+    the backward x, the gate and up sums [tokens, 2I] in fp32 and their products
+    [tokens, I] are kept, as far as the gradients that are wanted read them.
     """
     if activation not in GATES:
         raise ValueError(f"activation must be one of {sorted(GATES)}, got {activation!r}")

@@ -48,3 +48,27 @@ def test_infinities_and_nan(cuda, where, T, dtype):
         kinds = _kinds(v)
         assert torch.equal(_kinds(a), kinds), f"{name}: {(_kinds(a) != kinds).sum().item()} of {v.numel()} of another kind"
         assert_exact(a[kinds == 0], c[kinds == 0], f"{name}: the others")
+
+
+@pytest.mark.parametrize("T", [3, 16, 17, 200])
+def test_the_range_between_the_products_is_the_types(cuda, T):
+    """Gated products of 300 * 300 and of 2^-14 * 2^-13 beside weights that bring them back."""
+    I = H = N = 8
+    for dtype, keeps in ((BF, True), (F16, False)):
+        for size, back in ((300.0, 2.0**-10), (2.0**-13, 2.0**10)):
+            x = torch.full((T, H), 0.0, dtype=dtype)
+            x[:, 0] = 1
+            up = torch.zeros((2 * I, H), dtype=dtype)
+            up[:, 0] = size  # g = u = size
+            down = torch.full((N, I), back, dtype=dtype)
+            print(f"gated range {T} {dtype} {size}", flush=True)
+            got = _run(*(t.to(cuda) for t in (x, up, down, torch.ones((T, N), dtype=dtype))), "silu")
+            g = torch.tensor(size, dtype=dtype).double()
+            h = _gate(g, "silu")[0] * g
+            if keeps:
+                want = (I * h * back).expand(T, N)
+                # act's rounding and out's
+                assert ((got[0].double().cpu() - want).abs() <= want.abs() * (2.0**-7 + 2.0**-15)).all()
+            else:  # fp16: the product alone is past the type's range
+                assert h > 65504 or h < 2.0**-25
+                assert (got[0] == (math.inf if h > 1 else 0)).all() and (got[3] == (math.inf if h > 1 else 0)).all()
