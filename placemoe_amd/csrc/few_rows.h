@@ -167,7 +167,7 @@ __device__ __forceinline__ void epilogue(const GemmParams& P, const TileInfo& ti
     if (r >= ti.row_end) continue;
     if constexpr (KIND == KIND_FC1) {
       const int64_t I = P.I;
-      const float wt = P.row_w != nullptr ? Elt::to_f32(P.row_w[r]) : 0.f;
+      [[maybe_unused]] const float wt = kRowMaps && P.row_w != nullptr ? Elt::to_f32(P.row_w[r]) : 0.f;
 #pragma unroll
       for (int nt = 0; nt < CF::FN; nt += 2) {
         const int64_t j = (int64_t)ti.ntile * (CF::BN / 2) + (wn * CF::FN + nt) * 8 + c4;
@@ -190,7 +190,7 @@ __device__ __forceinline__ void epilogue(const GemmParams& P, const TileInfo& ti
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e) g[e] *= u[e];
-        if (P.row_w != nullptr) {  // the weight on the rounded activation (non-EP fc2 input)
+        if (kRowMaps && P.row_w != nullptr) {  // the weight on the rounded activation (non-EP fc2 input)
 #pragma unroll
           for (int e = 0; e < 4; e += 2) {
             Elt::round2(g[e], g[e + 1]);
@@ -242,7 +242,7 @@ __device__ __forceinline__ void epilogue(const GemmParams& P, const TileInfo& ti
 #endif
       }
     } else {
-      const bool mapped = P.row_tok != nullptr;
+      const bool mapped = kRowMaps && P.row_tok != nullptr;
       const int32_t tok = mapped ? P.row_tok[r] : -1;
       const bool to = mapped && (uint32_t)tok < (uint32_t)P.M;
       const float wt = KIND == KIND_NT && mapped ? Elt::to_f32(P.row_w[r]) : 0.f;

@@ -161,6 +161,13 @@ struct GemmParams {
 #endif
 };
 
+// Whether rows may have weights and targets of their own (row_w, row_tok); the gated block's have none.
+#ifdef PMX_GATED
+constexpr bool kRowMaps = false;
+#else
+constexpr bool kRowMaps = true;
+#endif
+
 // First row of group g; of g = G: the rows' end.
 __device__ __forceinline__ int32_t group_row(const GemmParams& P, int64_t g) {
 #ifdef PMX_GATED
@@ -640,7 +647,7 @@ __device__ __forceinline__ void epilogue(const GemmParams& P, const TileInfo& ti
   // One counter tracks this wave's loads and stores in issue order, so a load
   // issued after the first round's stores would wait for them as well.
   // Targets outside [0, M) are not written.
-  const bool mapped = (KIND == KIND_NT || KIND == KIND_NN) && P.row_tok != nullptr;
+  const bool mapped = kRowMaps && (KIND == KIND_NT || KIND == KIND_NN) && P.row_tok != nullptr;
   int32_t dst[16];
   float wt[16];
   if constexpr (KIND == KIND_NT || KIND == KIND_NN) {
@@ -1780,7 +1787,7 @@ __device__ __forceinline__ void epilogue(const GemmParams& P, const TileInfo& ti
   // counter tracks this wave's loads and stores in issue order: lane l holds
   // those of rows l and 64 + l, and a store's lanes fetch theirs with a
   // cross-lane read.  Targets outside [0, M) are not written.
-  const bool mapped = (KIND == KIND_NT || KIND == KIND_NN) && P.row_tok != nullptr;
+  const bool mapped = kRowMaps && (KIND == KIND_NT || KIND == KIND_NN) && P.row_tok != nullptr;
   [[maybe_unused]] uint4 nns_g[KIND == KIND_NNS ? 2 : 1][4], nns_u[KIND == KIND_NNS ? 2 : 1][4];  // KIND_NNS: two quarters of gate/up
   int32_t tok2[2] = {-1, -1};
   uint32_t wt2[2] = {0, 0};
