@@ -42,19 +42,24 @@ def test_short_last_tiles(cuda, size, dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF, F16])
-@pytest.mark.parametrize("size", [*TILES, (1, 72, 40, 24), (17, 264, 136, 520), (65, 128, 520, 128)], ids=str)
-def test_nothing_is_written_behind_a_tensor(cuda, size, dtype):
-    """Through the C ABI, every output with bytes behind it that have to stay."""
+@pytest.mark.parametrize("size", [*TILES, (1, 72, 40, 24), (17, 264, 136, 520), (65, 128, 520, 128), (1531, 520, 328, 520),
+                                  (3001, 264, 520, 264)], ids=str)
+def test_what_lies_behind_a_tensor_is_left_alone(cuda, size, dtype):
+    """Through the C ABI, every tensor with NaN behind it: outputs' have to stay, inputs' reach no result."""
     print(f"gated canaries {size} {dtype}", flush=True)
     T, H, I, N = size
-    x, up, down, dout = _case(cuda, *size, dtype)
+    case = _case(cuda, *size, dtype)
     planes = 2 if T <= 16 else 1
     lib, suffix = _capi.load(), "_f16" if dtype == F16 else ""
     stream = torch.cuda.current_stream().cuda_stream
     behind = 64 * 8 * max(H, 2 * I, N) + 4096  # more than 64 rows of anything
     need = {"gates": T * I * 8, "act": planes * T * I * 2, "out": T * N * 2, "dx": T * H * 2, "dup": 4 * I * H, "ddown": 2 * N * I,
             "ws": lib.pmx_gated_ffn_workspace_bytes(T, H, I, N)}
-    buf = {k: torch.full((n + behind,), 0xA5, dtype=torch.uint8, device=cuda) for k, n in need.items()}
+    # 0xff throughout is NaN in 16 and in 32 bits
+    buf = {k: torch.full((n + behind,), 0xFF, dtype=torch.uint8, device=cuda) for k, n in need.items()}
+    x, up, down, dout = (torch.full((t.numel() + behind,), float("nan"), dtype=dtype, device=cuda) for t in case)
+    for wide, t in zip((x, up, down, dout), case):
+        wide[:t.numel()] = t.flatten()
     at = {k: b.data_ptr() for k, b in buf.items()}
 
     def forward(gates):
@@ -64,7 +69,7 @@ def test_nothing_is_written_behind_a_tensor(cuda, size, dtype):
         return buf["act"][:need["act"]].clone(), buf["out"][:need["out"]].clone()
 
     first = forward(None)
-    assert (buf["gates"] == 0xA5).all()
+    assert (buf["gates"] == 0xFF).all()
     for a, b in zip(forward(at["gates"]), first):
         assert torch.equal(a, b), "with the sums kept"
     rc = getattr(lib, "pmx_gated_ffn_bwd" + suffix)(
@@ -72,7 +77,10 @@ def test_nothing_is_written_behind_a_tensor(cuda, size, dtype):
         at["ddown"], at["ws"], need["ws"], stream)
     assert rc == _capi.PMX_OK
     for k, b in buf.items():
-        assert (b[need[k]:] == 0xA5).all(), f"behind {k}"
-    want = _run(x, up, down, dout, "silu")
+        assert (b[need[k]:] == 0xFF).all(), f"behind {k}"
+    for wide, t in zip((x, up, down, dout), case):
+        assert_exact(wide[:t.numel()].view(t.shape), t, "an input")
+        assert wide[t.numel():].isnan().all()
+    want = _run(*case, "silu")
     for k, w in zip(("out", "dx", "dup", "ddown"), want):
         assert_exact(buf[k][:need[k]].view(dtype).view(w.shape), w, k)
