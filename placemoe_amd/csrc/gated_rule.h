@@ -13,7 +13,8 @@ namespace pmx {
 // tile is faster through it than one with two.  Fitted to 105 calls of each kind
 // (7 layers from 512 x 264 to 7168 x 2048, 17 to 8192 rows), of which the tiling
 // that this rule takes is within 0.3% of the best one's time in geometric mean, 1.20
-// at worst (64 / 128 / 256):
+// at worst.  (Single times lie further from the formula: a round of 256-row tiles of fc2's dgrad over 2048 columns counts as
+// 65, and is 80-85 at 8192 rows, 88 at 16384, whose sums are more bytes.)  Measured, operands at hand (64 / 128 / 256):
 //   rows   H     I      fc1                fc2                fc1 dgrad          fc2 dgrad
 //   256    2048  768     17 /  30 /  52      9 /  15 /  20     14 /  24 /  34     19 /  37 /  72
 //   2048   2048  768     27 /  35 /  58     15 /  18 /  29     23 /  27 /  45     22 /  41 /  74
