@@ -599,7 +599,8 @@ int pmx_rows4_group_gemm_nt(const void* a, const void* a_scales, int32_t a_bits,
                             int64_t K, void* c, pmx_stream_t stream);
 
 /* fc1 + SwiGLU as pmx_rows8_gemm_fc1_swiglu (X and act in e4m3), w [G, 2I, H] in
- * 4 bits: codes [G, 2I, H / 2].  fp32 sums as there.  H a multiple of 32, I of 16. */
+ * 4 bits: codes [G, 2I, H / 2].  fp32 sums as there (a weight that 4 bits round to 2^128 counts as infinite too).
+ * H a multiple of 32, I of 16. */
 int pmx_rows4_gemm_fc1_swiglu(const void* x, const void* x_scales, int64_t T, const int32_t* row_token,
                               const void* w, const void* w_scales, const int32_t* offsets, int32_t G,
                               int64_t A, int64_t H, int64_t I, const void* row_w, void* act, void* act_scales,

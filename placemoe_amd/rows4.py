@@ -146,7 +146,9 @@ def gemm_fc1_swiglu_rows4(x: Rows8, w: Rows4, offsets: torch.Tensor, row_token: 
     """act[r] = silu(gate) * up * row_w[r], in e4m3 again, with (gate | up) =
     x[row_token[r]] @ w[g]^T: x [T, H] in e4m3, w [G, 2I, H] in 4 bits (gate rows
     first); row_token int32 [A] (None: row r is x[r]), row_w [A] (None: ones).
-    fp32 up to the rounding to 8 bits.  H a multiple of 32, I of 16."""
+    fp32 up to the rounding to 8 bits (2^128, to which 4 bits round the topmost
+    eighth of bfloat16's range and 8 bits its topmost 3%, counts as infinite).
+    H a multiple of 32, I of 16."""
     _kind("x", x, Rows8), _kind("w", w, Rows4)
     dev = _check_dev(x.codes, x.scales, w.codes, w.scales, offsets, row_token, row_w)
     dt = _e4m3("x", x, 2)
